@@ -901,6 +901,62 @@ int mirl_seq_logprob_errors(const float* policy, int64_t p_sb, int64_t p_ss,
                             const float* sample_mask, int64_t s_sb, int64_t B, int64_t S,
                             float* errors, uint8_t* valid, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* The policy head: final norm, 8-bit rows, dropout                         */
+/* ---------------------------------------------------------------------- */
+
+/*
+ * Root-mean-square norm of R rows of H elements with the residual's addition:
+ *   h    = round(x + residual) to the residual's type   (h = x without a residual)
+ *   rstd = 1 / sqrt(mean(h^2) + eps),  y = (h * rstd) * weight
+ * x and y are of x_dtype (F32, BF16 or F16), the residual and h of res_dtype
+ * (x_dtype or F32), the weight of w_dtype (x_dtype or F32).  Rows have unit
+ * stride and the given row strides (any alignment); h and y are [R, H]
+ * contiguous.  With y_scale ([R]) y is e4m3 instead, one byte an element:
+ *   s = max|y| / 448 (at least 2^-126; 1 for a row of zeros), y8 = e4m3(y * (1 / s))
+ * from the unrounded y; a row that holds a NaN or an infinity has a scale that
+ * is none and NaN in those places.  rstd ([R], or NULL) is kept for the backward.
+ * Without a residual h is not written (may be NULL).
+ */
+int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* residual,
+                          int res_dtype, int64_t ldr, const void* weight, int w_dtype,
+                          int64_t R, int64_t H, double eps, void* h, void* y,
+                          float* y_scale, float* rstd, void* stream);
+
+/*
+ * Its backward, from the stored h and rstd: with n = h * rstd,
+ *   dh = rstd * (w dy - n * mean(w dy n)) + dh_out,   dw = sum over rows of dy * n.
+ * dh_out (the gradient of the returned h, of h_dtype) may be NULL.  dx (x_dtype)
+ * and dres (h_dtype) receive dh, either may be NULL; dw (w_dtype, [H]) may be
+ * NULL and otherwise needs a workspace of mirl_add_rms_norm_bwd_workspace_elems
+ * floats and at least one row.  Sums are fp32 in an order that depends on the
+ * sizes only.
+ */
+int64_t mirl_add_rms_norm_bwd_workspace_elems(int64_t R, int64_t H);
+int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, const void* dh_out,
+                          int64_t ldd, const void* h, int h_dtype, int64_t ldh,
+                          const float* rstd, const void* weight, int w_dtype, int64_t R,
+                          int64_t H, void* dx, void* dres, void* dw, float* workspace,
+                          void* stream);
+
+/*
+ * Rows in 8 bits: scale[r] and e4m3 rows of x as for the norm's y ([R, H]
+ * contiguous bytes).  An output weight's rows for the 8-bit hidden-state path.
+ */
+int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, void* y,
+                       float* scale, void* stream);
+
+/*
+ * Dropout of n contiguous elements (F32, BF16 or F16): element i takes the
+ * 16-bit piece i % 8 (low pieces first) of the Philox4x32-10 block with key
+ * `seed` and counter (i / 8, offset), is kept where the piece is at least
+ * T = floor(p * 65536 + 1/2) and multiplied by 65536 / (65536 - T); the others
+ * are 0 (also infinities and NaN).  With seed_dev the seed is read from the
+ * device.  The same call on the upstream gradient is the backward.  y may be x.
+ */
+int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
+                 const int64_t* seed_dev, int64_t offset, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -255,6 +255,15 @@ SIGNATURES = {
     ),
     "mirl_unpack_rows_fwd": (_I, [_P, _I64, _P, _I64, _I64, _P, _P]),
     "mirl_unpack_rows_bwd": (_I, [_P, _I64, _I64, _P, _I64, _P, _P]),
+    "mirl_add_rms_norm_fwd": (
+        _I, [_P, _I, _I64, _P, _I, _I64, _P, _I, _I64, _I64, ctypes.c_double, _P, _P, _P, _P, _P]
+    ),
+    "mirl_add_rms_norm_bwd_workspace_elems": (_I64, [_I64, _I64]),
+    "mirl_add_rms_norm_bwd": (
+        _I, [_P, _I, _I64, _P, _I64, _P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]
+    ),
+    "mirl_quantize_rows": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
 FILTER_KEEP_CAP = 1024  # MIRL_FILTER_KEEP_CAP
@@ -1459,3 +1468,114 @@ def seq_logprob_errors(policy: torch.Tensor, generation: torch.Tensor, token_mas
     )
     _check(st, "mirl_seq_logprob_errors")
     return errors, valid
+
+
+# ---------------------------------------------------------------------------
+# the policy head: final norm, 8-bit rows, dropout
+# ---------------------------------------------------------------------------
+def _rows2(t: torch.Tensor) -> torch.Tensor:
+    """``t [..., H]`` as ``[R, H]`` rows of unit stride and one row stride of at least H
+    (a copy where its layout is another)."""
+    t2 = t.reshape(-1, t.shape[-1])
+    ok = (t2.stride(1) == 1 or t2.shape[1] == 1) and (t2.stride(0) >= t2.shape[1] or t2.shape[0] <= 1)
+    return t2 if ok else t2.contiguous()
+
+
+def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
+                     want_rstd: bool, out8: bool):
+    """(y, h, rstd or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
+    itself without a residual, rstd and scale have a row's shape."""
+    dev = _require_gpu(x, residual, weight)
+    H = x.shape[-1]
+    _require(weight.dim() == 1 and weight.shape[0] == H, "a weight per element of a row")
+    x2 = _rows2(x)
+    r2 = None if residual is None else _rows2(residual)
+    R = x2.shape[0]
+    weight = weight.contiguous()
+    h = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if out8 else x.dtype, device=dev)
+    lead = x.shape[:-1]
+    scale = torch.empty(lead, dtype=torch.float32, device=dev) if out8 else None
+    rstd = torch.empty(lead, dtype=torch.float32, device=dev) if want_rstd else None
+    st = _launch(
+        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), _dtype_code(x), x2.stride(0), _ptr(r2),
+        _dtype_code(x if residual is None else residual), 0 if r2 is None else r2.stride(0), weight.data_ptr(),
+        _dtype_code(weight), R, H, float(eps), None if residual is None else h.data_ptr(), y.data_ptr(),
+        _ptr(scale), _ptr(rstd), _stream(dev),
+    )
+    _check(st, "mirl_add_rms_norm_fwd")
+    return y, h, rstd, scale
+
+
+def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.Tensor, rstd: torch.Tensor,
+                     weight: torch.Tensor, need_x: bool, need_res: bool, need_w: bool):
+    """(dx, dres, dw), None where not needed; dx and dres are one tensor where their types are
+    the same (see mirl_add_rms_norm_bwd)."""
+    dev = _require_gpu(dy, dh_out, h, rstd, weight)
+    H = h.shape[-1]
+    _require(dy.shape == h.shape and rstd.is_contiguous() and rstd.dtype == torch.float32
+             and rstd.numel() * H == h.numel(), "gradients and row statistics of the rows")
+    _require(dh_out is None or (dh_out.shape == h.shape and dh_out.dtype == h.dtype), "the stream's gradient has its type")
+    dy2, h2 = _rows2(dy), _rows2(h)
+    g2 = None if dh_out is None else _rows2(dh_out)
+    R = h2.shape[0]
+    weight = weight.contiguous()
+    one = need_x and need_res and dy.dtype == h.dtype
+    dx = torch.empty(h.shape, dtype=dy.dtype, device=dev) if need_x else None
+    dres = torch.empty(h.shape, dtype=h.dtype, device=dev) if need_res and not one else None
+    dw = ws = None
+    if need_w:
+        if R == 0:
+            dw = torch.zeros_like(weight)
+        else:
+            dw = torch.empty_like(weight)
+            lib = _lib if _lib is not None else load()
+            ws = torch.empty(int(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)), dtype=torch.float32, device=dev)
+    st = _launch(
+        "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), dy2.stride(0), _ptr(g2),
+        0 if g2 is None else g2.stride(0), h2.data_ptr(), _dtype_code(h), h2.stride(0), rstd.data_ptr(),
+        weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres), None if ws is None else dw.data_ptr(),
+        _ptr(ws), _stream(dev),
+    )
+    _check(st, "mirl_add_rms_norm_bwd")
+    return dx, (dx if one else dres), dw
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 rows, fp32 scales) of ``x [..., H]`` (see mirl_quantize_rows)."""
+    dev = _require_gpu(x)
+    x2 = _rows2(x)
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    st = _launch("mirl_quantize_rows", dev, x2.data_ptr(), _dtype_code(x), x2.stride(0), x2.shape[0], x2.shape[1],
+                 y.data_ptr(), scale.data_ptr(), _stream(dev))
+    _check(st, "mirl_quantize_rows")
+    return y, scale
+
+
+def _signed64(v: int) -> int:
+    """The 64 bits of ``v`` as a signed number (seeds are given signed or unsigned)."""
+    v = int(v)
+    _require(-(1 << 63) <= v < 1 << 64, "seeds and offsets have 64 bits")
+    return v - (1 << 64) if v >= 1 << 63 else v
+
+
+def _seed_args(seed, dev: torch.device) -> tuple[int, Optional[int]]:
+    """(value, device pointer) of a seed given as a number or a one-element int64 tensor."""
+    if isinstance(seed, torch.Tensor):
+        _require(seed.dtype == torch.int64 and seed.numel() == 1 and seed.device == dev,
+                 "a seed tensor holds one int64 on the input's device")
+        return 0, seed.data_ptr()
+    return _signed64(seed), None
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
+    """Dropout of ``x`` in its logical element order (see mirl_dropout); a new contiguous tensor."""
+    dev = _require_gpu(x)
+    x = x.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    value, ptr = _seed_args(seed, dev)
+    st = _launch("mirl_dropout", dev, x.data_ptr(), _dtype_code(x), x.numel(), float(p), value, ptr,
+                 _signed64(offset), y.data_ptr(), _stream(dev))
+    _check(st, "mirl_dropout")
+    return y

@@ -32,6 +32,8 @@ SOURCES = [
     "packing.hip",
     "temperature.hip",
     "seq_errors.hip",
+    "norm.hip",
+    "dropout.hip",
 ]
 
 ARCH = "gfx950"

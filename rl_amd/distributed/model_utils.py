@@ -31,6 +31,8 @@ from rl_amd.algorithms.logits_sampling_utils import (
 )
 
 __all__ = [
+    "add_rms_norm",
+    "add_rms_norm_8bit",
     "ChunkedDistributedCrossEntropyToFixedLogits",
     "ChunkedDistributedEntropy",
     "ChunkedDistributedGatherLogprob",
@@ -41,13 +43,18 @@ __all__ = [
     "DistributedLogprob",
     "distributed_vocab_topk",
     "DistributedLogprobWithSampling",
+    "dropout",
     "from_parallel_hidden_states_to_logprobs",
     "from_parallel_logits_to_logprobs",
     "from_parallel_logits_to_logprobs_packed_sequences",
     "get_next_token_logprobs_from_logits",
     "get_policy_logprobs_at_sampler_topk",
+    "quantize_rows_8bit",
+    "rms_norm",
     "set_early_backward",
 ]
+
+_NORMS = ("add_rms_norm", "add_rms_norm_8bit", "quantize_rows_8bit", "rms_norm")
 
 _VOCAB_REDUCTIONS = (
     "ChunkedDistributedGatherLogprob",
@@ -71,6 +78,14 @@ def __getattr__(name: str):
         from rl_amd.distributed import linear_ce
 
         return getattr(linear_ce, name)
+    if name in _NORMS:
+        from rl_amd.distributed import final_norm
+
+        return getattr(final_norm, name)
+    if name == "dropout":
+        from rl_amd.distributed.counter_dropout import dropout
+
+        return dropout
     if name in _VOCAB_REDUCTIONS:
         from rl_amd.distributed import vocab_reductions
 
