@@ -957,6 +957,26 @@ int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t R, int64_t
 int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
                  const int64_t* seed_dev, int64_t offset, void* y, void* stream);
 
+/*
+ * Selected-token logprobs from 8-bit hidden states and an 8-bit output weight
+ * (e4m3 bytes, one fp32 scale per row of either; see mirl_add_rms_norm_fwd and
+ * mirl_quantize_rows), the logits in fp32 and never written:
+ *   x[r, v] = hidden_scale[r] * weight_scale[v] * sum_k hidden8[r, k] weight8[v, k]
+ *   out     = log_softmax(x[r])[target - vocab_start], 0 for targets outside
+ *             [vocab_start, vocab_end)
+ * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, Hd]; Hd a
+ * multiple of 256, row strides multiples of 16, 16-byte-aligned starts (zero
+ * padding adds nothing).  out is [bsz, T / bsz] by strides; workspace as
+ * mirl_linear_ce_workspace_elems(T, V).
+ */
+int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int64_t T,
+                            int64_t Hd, int64_t ldh, const void* weight8,
+                            const float* weight_scale, int64_t V, int64_t ldw, int64_t bsz,
+                            const int64_t* target, int64_t t_stride_b, int64_t t_stride_s,
+                            int64_t vocab_start, int64_t vocab_end, float* out,
+                            int64_t o_stride_b, int64_t o_stride_s, float* workspace,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -263,6 +263,9 @@ SIGNATURES = {
         _I, [_P, _I, _I64, _P, _I64, _P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]
     ),
     "mirl_quantize_rows": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "mirl_linear_ce_8bit_fwd": (
+        _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
+    ),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
@@ -1579,3 +1582,32 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
                  _signed64(offset), y.data_ptr(), _stream(dev))
     _check(st, "mirl_dropout")
     return y
+
+
+def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight8: torch.Tensor,
+                       weight_scale: torch.Tensor, bsz: int, target: torch.Tensor, vocab_start: int,
+                       vocab_end: int, out: torch.Tensor) -> None:
+    """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd).
+
+    hidden8 [T, H] and weight8 [V, H] e4m3 (H a multiple of 256, rows multiples of 16 bytes),
+    scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
+    dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
+    T, H = hidden8.shape
+    V = weight8.shape[0]
+    _require(hidden8.dtype == torch.float8_e4m3fn and weight8.dtype == torch.float8_e4m3fn, "e4m3 operands")
+    _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and weight8.shape[1] == H,
+             "operands of one hidden size with unit stride")
+    _require(hidden_scale.is_contiguous() and hidden_scale.numel() == T and hidden_scale.dtype == torch.float32
+             and weight_scale.is_contiguous() and weight_scale.numel() == V and weight_scale.dtype == torch.float32,
+             "a contiguous fp32 scale per row")
+    _require(target.dtype == torch.int64 and out.dtype == torch.float32
+             and tuple(target.shape) == tuple(out.shape) == (bsz, T // bsz), "int64 targets and fp32 logprobs [B, S]")
+    lib = _lib if _lib is not None else load()
+    ws = torch.empty(max(1, int(lib.mirl_linear_ce_workspace_elems(T, V))), dtype=torch.float32, device=dev)
+    st = _launch(
+        "mirl_linear_ce_8bit_fwd", dev, hidden8.data_ptr(), hidden_scale.data_ptr(), T, H, hidden8.stride(0),
+        weight8.data_ptr(), weight_scale.data_ptr(), V, weight8.stride(0), int(bsz), target.data_ptr(), target.stride(0),
+        target.stride(1), int(vocab_start), int(vocab_end), out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
+        _stream(dev),
+    )
+    _check(st, "mirl_linear_ce_8bit_fwd")

@@ -34,6 +34,7 @@ SOURCES = [
     "seq_errors.hip",
     "norm.hip",
     "dropout.hip",
+    "linear_ce_8bit.hip",
 ]
 
 ARCH = "gfx950"

@@ -71,6 +71,22 @@ struct Mma<F32> {
     return c;
   }
 };
+// e4m3 operands (OCP, forward of the 8-bit path only): v_mfma_f32_32x32x64_f8f6f4, unscaled,
+// twice the bf16 rate.  A fragment is 32 bytes of a row per lane (two neighbouring 16-byte
+// chunks); which hidden elements a lane holds does not matter as long as both operands hold
+// the same ones.  The accumulator is laid out as for fp32.
+struct F8 {
+  using raw = uint8_t;
+};
+template <>
+struct Mma<F8> {
+  typedef int frag __attribute__((ext_vector_type(8)));
+  typedef f32x16 acc_t;
+  static constexpr int kT = 32;
+  __device__ __forceinline__ static f32x16 run(frag w, frag h, f32x16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, h, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+  }
+};
 
 // 16-bit element bits <-> fp32 for a dtype E (round to nearest even).
 template <class E>
@@ -171,7 +187,9 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_(std::make_integer_sequence<int, N>{}, f);
 }
 
-enum LceMode { kFwd = 0, kGrad = 1, kGemm = 2 };
+// kFwd, kGrad: logits rounded to the operand type.  kFwdX, kGradX: logits kept in fp32, with
+// adapters (16-bit operands) or row and column scales (e4m3, forward).
+enum LceMode { kFwd = 0, kGrad = 1, kGemm = 2, kFwdX = 3, kGradX = 4 };
 
 struct LceParams {
   const void* h;  // [T, Hd] of the kernel's E (bf16, fp16; fp32 for the plain GEMM), row stride ldh
@@ -213,6 +231,19 @@ struct LceParams {
   int64_t count_off;
   int count_axis;
   int64_t final_at;
+  // kFwdX and kGradX with adapters (or null): row r takes adapter aid[r] (rows of one
+  // adapter adjoin; negative: none), which adds U[r] . B[aid[r]]^T to its logits.  U is held as
+  // `planes` values of the operand type that add up to it: row r is [planes][r8], the planes
+  // r8 elements apart; B is [adapters, V, r8], r8 a multiple of 8.
+  const int32_t* aid;
+  const uint16_t* U;
+  const uint16_t* B;
+  int r8, planes;
+  // kGradX: G = (onehot - softmax) * g_scale in the operand type (rows past the end: 0)
+  float g_scale;
+  // kFwdX of e4m3: logits = products * col_scale[col] * row_scale[row]
+  const float* row_scale;
+  const float* col_scale;
 };
 
 template <int MODE, class E>
@@ -221,9 +252,12 @@ void lce_tile_kernel(LceParams P) {
   using frag = typename Mma<E>::frag;
   using acc_t = typename Mma<E>::acc_t;
   constexpr int kT = Mma<E>::kT, kTM = kWM / kT, kTN = kWN / kT, kAV = kT * kT / kWave;
-  constexpr int kKK = kRowBytes / (kWave / kT * 16);  // fragment steps (MFMA blocks) per stage
-  static_assert(MODE == kGemm || sizeof(typename E::raw) == 2, "fp32 operands: plain GEMM only");
+  constexpr int kKK = kRowBytes / (kWave / kT * (int)sizeof(frag));  // fragment steps (MFMA blocks) per stage
   constexpr int kES = (int)sizeof(typename E::raw);  // bytes per element
+  static_assert(MODE == kGemm ? kES != 1 : MODE == kFwdX ? kES <= 2 : kES == 2,
+                "fp32 operands: plain GEMM only; e4m3: forward only");
+  constexpr bool kIsGrad = MODE == kGrad || MODE == kGradX;
+  constexpr bool kAdapters = (MODE == kFwdX || MODE == kGradX) && kES == 2;
   constexpr int kSKE = kRowBytes / kES;              // hidden elements per stage
   // Two arrays rather than one, so that the compiler tracks the direct loads
   // into each stage on their own and an LDS read waits only for its stage.
@@ -231,6 +265,7 @@ void lce_tile_kernel(LceParams P) {
   __shared__ __align__(1024) unsigned char st1[kStageBytes];
   __shared__ int s_tcol[kBM];
   __shared__ float s_m[kBM], s_ls[kBM], s_g[kBM];
+  __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_heads[kWaves];
   auto stage_ptr = [&](int s) -> unsigned char* { return s == 0 ? st0 : st1; };
 
   // Tile order.  Workgroups are dispatched to the 8 XCDs round-robin
@@ -301,17 +336,44 @@ void lce_tile_kernel(LceParams P) {
         const int64_t c = t - P.vs - n0;
         if (c >= 0 && c < kBN) tc = (int)c;
       }
-      if (MODE == kGrad) {
-        my_g = P.g[b * P.gsb + s * P.gss];
+      if (kIsGrad) {
+        my_g = MODE == kGradX ? P.g_scale : P.g[b * P.gsb + s * P.gss];
         lm = P.stats[2 * r];
         ll = P.stats[2 * r + 1];
       }
     }
     s_tcol[tid] = tc;
-    if (MODE == kGrad) {
+    if (kIsGrad) {
       s_g[tid] = my_g;
       s_m[tid] = lm;
       s_ls[tid] = ll;
+    }
+    if constexpr (MODE == kFwdX && kES == 1) {
+      s_m[tid] = r < row_end ? P.row_scale[r] : 0.f;
+      s_ls[tid] = n0 + tid < P.V ? P.col_scale[n0 + tid] : 0.f;
+    }
+  }
+  // The tile's adapters in row order: s_seg[q] is the q-th one, s_ord[row] the row's (-1: none).
+  int n_seg = 0;
+  if constexpr (kAdapters) {
+    if (P.aid != nullptr) {
+      const int64_t r = m0 + tid;
+      const int a = r < row_end ? P.aid[r] : -1;
+      const int before = tid > 0 && r < row_end ? P.aid[r - 1] : -1;
+      const bool head = a >= 0 && (tid == 0 || a != before);
+      const uint64_t heads = __ballot(head);
+      if (lane == 0) s_heads[wave] = (int)__popcll(heads);
+      __syncthreads();
+      int at = (int)__popcll(heads & (~0ull >> (63 - lane)));  // heads up to this row
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        at += w < wave ? s_heads[w] : 0;
+        n_seg += s_heads[w];
+      }
+      s_ord[tid] = a >= 0 ? at - 1 : -1;
+      if (head) s_seg[at - 1] = a;
+      __syncthreads();
+      n_seg = __builtin_amdgcn_readfirstlane(n_seg);
     }
   }
   if (MODE == kGrad) {
@@ -403,22 +465,28 @@ void lce_tile_kernel(LceParams P) {
   };
 
   // fragment read offsets: row (wm*128 | wn*128) + i*kT + lane % kT, the lane group's
-  // chunk of step kk
+  // chunk of step kk (e4m3: the first of two neighbouring chunks, the other at offset ^ 16)
   const int frow = lane & (kT - 1);
+  constexpr int kFC = (int)sizeof(frag) / 16;  // chunks of a fragment
   int frag_off[kKK];
 #pragma unroll
-  for (int kk = 0; kk < kKK; ++kk) frag_off[kk] = lds_off(frow, kk * (kWave / kT) + lane / kT);
+  for (int kk = 0; kk < kKK; ++kk) frag_off[kk] = lds_off(frow, (kk * (kWave / kT) + lane / kT) * kFC);
   frag fa[2][kTM], fb[2][kTN];
   // Reads go out in the order the MFMAs first need them: A0, all B, the other A (1% on
   // the forward against all A, all B).
   auto fread = [&](int set, const unsigned char* stage, int kk, int n) __attribute__((always_inline)) {
     // idx < kTM: A fragment idx; else B fragment idx - kTM
     const int idx = n == 0 ? 0 : n <= kTN ? kTM + n - 1 : n - kTN;
-    if (idx < kTM)
-      fa[set][idx] = *reinterpret_cast<const frag*>(stage + (wm * kWM + idx * kT) * kRowBytes + frag_off[kk]);
-    else
-      fb[set][idx - kTM] = *reinterpret_cast<const frag*>(
-          stage + kHalfBytes + (wn * kWN + (idx - kTM) * kT) * kRowBytes + frag_off[kk]);
+    const unsigned char* base = idx < kTM ? stage + (wm * kWM + idx * kT) * kRowBytes
+                                          : stage + kHalfBytes + (wn * kWN + (idx - kTM) * kT) * kRowBytes;
+    frag& f = idx < kTM ? fa[set][idx] : fb[set][idx - kTM];
+    if constexpr (kFC == 1) {
+      f = *reinterpret_cast<const frag*>(base + frag_off[kk]);
+    } else {
+      const vu4 a = *reinterpret_cast<const vu4*>(base + frag_off[kk]);
+      const vu4 b = *reinterpret_cast<const vu4*>(base + (frag_off[kk] ^ 16));
+      f = frag{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    }
   };
 
   acc_t acc[kTM][kTN];
@@ -485,10 +553,47 @@ void lce_tile_kernel(LceParams P) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // The adapters' part of the logits, through stage array 1 while stage data 0 is in flight:
+  // the reduction runs over the tile's adapters one after the other, `planes` * r8 elements
+  // each, eight 16-byte chunks a stage; a row's U is zero in the chunks of other adapters.
+  // (Every adapter of the tile costs planes * r8 / 64 of a stage; a step of 4 adapters of rank
+  // 16 over [16384, 4096] x [151936, 4096] has one in all but three tiles in 64.)
+  auto adapter_stages = [&]() __attribute__((always_inline)) {
+    const int cpp = P.r8 >> 3, cps = P.planes * cpp, chunk = tid & 7;
+    const int n_ext = (n_seg * cps + 7) >> 3;
+    for (int e = 0; e < n_ext; ++e) {
+      const int x = e * 8 + chunk, q = x / cps, rem = x - q * cps, cc = rem % cpp;
+      const bool any = q < n_seg;
+      const uint16_t* up = P.U + m0 * (int64_t)(P.planes * P.r8) + rem * 8;
+      const uint16_t* bp = P.B + ((int64_t)(any ? s_seg[q] : 0) * P.V + n0) * P.r8 + cc * 8;
+      __syncthreads();  // the last stage's reads are done
+#pragma unroll
+      for (int k = 0; k < kBM / 32; ++k) {
+        const int row = k * 32 + (tid >> 3);
+        vu4 u = {0u, 0u, 0u, 0u}, b = {0u, 0u, 0u, 0u};
+        if (any && s_ord[row] == q) u = *reinterpret_cast<const vu4*>(up + (int64_t)row * (P.planes * P.r8));
+        if (any && n0 + row < P.V) b = *reinterpret_cast<const vu4*>(bp + (int64_t)row * P.r8);
+        *reinterpret_cast<vu4*>(st1 + lds_off(row, chunk)) = u;
+        *reinterpret_cast<vu4*>(st1 + kHalfBytes + lds_off(row, chunk)) = b;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) {
+#pragma unroll
+        for (int n = 0; n < kTM + kTN; ++n) fread(0, st1, kk, n);
+#pragma unroll
+        for (int m = 0; m < kMB; ++m) mfma(0, m);
+      }
+    }
+    __syncthreads();
+  };
   auto run_stages = [&]() __attribute__((always_inline)) {
     // Prologue: stage data 0 and 1 in flight; wait for 0 and read its block-0 fragments.
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st0, 0, q);
+    if constexpr (kAdapters) {
+      if (n_seg > 0) adapter_stages();
+    }
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st1, 1, q);
     wait_vm_barrier<kL>();
@@ -752,6 +857,94 @@ void lce_tile_kernel(LceParams P) {
     else
       each([&](int64_t row, int64_t col, f32x4 o, bool full)
                __attribute__((always_inline)) { store_c(row, col, o, full); });
+  } else if constexpr (MODE == kFwdX) {
+    // ---- forward, logits in fp32: the rows are reduced in the registers ----
+    //
+    // A lane holds kTN groups of columns of kTM rows, the lanes that share a row are kT apart
+    // and the two waves of a row band exchange through LDS.
+    wait_vm_barrier<0>();
+    constexpr int kG = kAV / 4;  // groups of four consecutive columns per MFMA tile
+    const int col_lane = lane / kT * 4;
+    const int64_t ncols = P.V - n0;
+    if constexpr (kES == 1) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int g = 0; g < kG; ++g) {
+          const float4 cs = *reinterpret_cast<const float4*>(s_ls + wn * kWN + j * kT + g * 8 + col_lane);
+          const float c4[4] = {cs.x, cs.y, cs.z, cs.w};
+#pragma unroll
+          for (int i = 0; i < kTM; ++i) {
+            const float rs = s_m[wm * kWM + i * kT + frow];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * g + e] = (acc[i][j][4 * g + e] * c4[e]) * rs;
+          }
+        }
+      __syncthreads();  // s_m is written below
+    }
+    if (ncols < kBN) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int v = 0; v < kAV; ++v) {
+          const bool out = wn * kWN + j * kT + v / 4 * 8 + col_lane + v % 4 >= ncols;
+#pragma unroll
+          for (int i = 0; i < kTM; ++i) acc[i][j][v] = out ? -INFINITY : acc[i][j][v];
+        }
+    }
+    float rm[kTM], rsum[kTM];
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+      const int rl = wm * kWM + i * kT + frow;
+      // few tiles hold a row's target: looked for only where one does
+      const int tc = s_tcol[rl] - wn * kWN;
+      if (__ballot(tc >= 0 && tc < kWN) != 0) {
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int v = 0; v < kAV; ++v)
+            if (j * kT + v / 4 * 8 + col_lane + v % 4 == tc) P.xt[m0 + rl - P.row0] = acc[i][j][v];
+      }
+      float M = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int v = 0; v < kAV; ++v) M = fmaxf(M, acc[i][j][v]);
+#pragma unroll
+      for (int off = kT; off < kWave; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, kWave));
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      if (M != -INFINITY) {
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int v = 0; v < kAV; ++v) s4[v & 3] += fast_exp2((acc[i][j][v] - M) * kLog2e);
+      }
+      float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+#pragma unroll
+      for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+      rm[i] = M;
+      rsum[i] = sum;
+      if (wn == 1 && lane < kT) {
+        s_m[rl] = M;
+        s_g[rl] = sum;
+      }
+    }
+    __syncthreads();
+    if (wn == 0 && lane < kT) {
+#pragma unroll
+      for (int i = 0; i < kTM; ++i) {
+        const int rl = wm * kWM + i * kT + frow;
+        const int64_t r = m0 + rl;
+        if (r >= row_end) continue;
+        const float m1 = s_m[rl], M = fmaxf(rm[i], m1);
+        float sum = 0.f;
+        if (rm[i] != -INFINITY) sum += rsum[i] * fast_exp2((rm[i] - M) * kLog2e);
+        if (m1 != -INFINITY) sum += s_g[rl] * fast_exp2((m1 - M) * kLog2e);
+        float* dst = P.part + ((r - P.row0) * P.n_nt + nt) * 2;
+        dst[0] = M;
+        dst[1] = sum;
+      }
+    }
   } else {
   // ---- epilogue: the tile goes through LDS as bf16, one row per thread ----
   //
@@ -830,14 +1023,15 @@ void lce_tile_kernel(LceParams P) {
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           float x0 = acc[i][j][e], x1 = acc[i][j][e + 1];
-          round_trip2<E>(x0, x1);  // the logits in the operand dtype
+          if constexpr (MODE == kGrad) round_trip2<E>(x0, x1);  // the logits in the operand dtype
           o[e] = fast_exp2(((x0 - M) - LS) * kLog2e);
           o[e + 1] = fast_exp2(((x1 - M) - LS) * kLog2e);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (cl + e == tc) ? (1.f - o[e]) * gv : -o[e] * gv;
-        // G is bf16 for either operand dtype
-        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<BF16>(o);
+        // kGrad: G is bf16 for either operand dtype
+        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) =
+            pack4<typename std::conditional<MODE == kGradX, E, BF16>::type>(o);
       }
     }
     __syncthreads();
@@ -891,6 +1085,45 @@ void lce_tile_kernel(LceParams P) {
   }
   }  // the fused epilogues
 }
+
+// Per row: combine the column-tile partials into the row's max and log-sum-exp,
+// then logprob = (x_t - max) - logsum (0 for targets outside the slice).
+// One wave per row; with `perm` the partials' row r is row perm[r] of targets and results.
+__global__ __launch_bounds__(256) void lce_merge_kernel(
+    const float* __restrict__ part, const float* __restrict__ xt, int64_t row0, int64_t nrows,
+    int64_t n_nt, int64_t bsz, const int64_t* __restrict__ target, int64_t tsb, int64_t tss,
+    int64_t vs, int64_t ve, int64_t V, float* __restrict__ out, int64_t osb, int64_t oss,
+    float* __restrict__ stats, const int64_t* __restrict__ perm) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rl = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (rl >= nrows) return;
+  const float* p = part + rl * n_nt * 2;
+  float M = -INFINITY;
+  for (int64_t j = lane; j < n_nt; j += 64) M = fmaxf(M, p[2 * j]);
+  M = wave_max(M);
+  float s = 0.f;
+  if (M != -INFINITY) {
+    for (int64_t j = lane; j < n_nt; j += 64) {
+      const float mj = p[2 * j];
+      if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
+    }
+  }
+  s = wave_sum(s);
+  if (lane == 0) {
+    const int64_t r = perm != nullptr ? perm[row0 + rl] : row0 + rl;
+    const int64_t sq = r / bsz, b = r - sq * bsz;
+    const int64_t t = target[b * tsb + sq * tss];
+    const bool tmask = (t < vs) || (t >= ve) || (t - vs >= V);
+    const float logsum = logf(s);
+    out[b * osb + sq * oss] = tmask ? 0.f : (xt[rl] - M) - logsum;
+    if (stats != nullptr) {
+      stats[2 * r] = M;
+      stats[2 * r + 1] = logsum;
+    }
+  }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 }  // namespace mirl

@@ -300,45 +300,6 @@ __global__ __launch_bounds__(256) void lce_gather_rows_kernel(
   }
 }
 
-// Per row: combine the column-tile partials into the row's max and log-sum-exp,
-// then logprob = (x_t - max) - logsum (0 for targets outside the slice).
-// One wave per row.
-__global__ __launch_bounds__(256) void lce_merge_kernel(
-    const float* __restrict__ part, const float* __restrict__ xt, int64_t row0, int64_t nrows,
-    int64_t n_nt, int64_t bsz, const int64_t* __restrict__ target, int64_t tsb, int64_t tss,
-    int64_t vs, int64_t ve, int64_t V, float* __restrict__ out, int64_t osb, int64_t oss,
-    float* __restrict__ stats) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rl = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (rl >= nrows) return;
-  const float* p = part + rl * n_nt * 2;
-  float M = -INFINITY;
-  for (int64_t j = lane; j < n_nt; j += 64) M = fmaxf(M, p[2 * j]);
-  M = wave_max(M);
-  float s = 0.f;
-  if (M != -INFINITY) {
-    for (int64_t j = lane; j < n_nt; j += 64) {
-      const float mj = p[2 * j];
-      if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
-    }
-  }
-  s = wave_sum(s);
-  if (lane == 0) {
-    const int64_t r = row0 + rl;
-    const int64_t sq = r / bsz, b = r - sq * bsz;
-    const int64_t t = target[b * tsb + sq * tss];
-    const bool tmask = (t < vs) || (t >= ve) || (t - vs >= V);
-    const float logsum = logf(s);
-    out[b * osb + sq * oss] = tmask ? 0.f : (xt[rl] - M) - logsum;
-    if (stats != nullptr) {
-      stats[2 * r] = M;
-      stats[2 * r + 1] = logsum;
-    }
-  }
-}
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 int check_common(const void* hidden, int64_t T, int64_t Hd, int64_t ldh, const void* weight,
                  int64_t V, int64_t ldw, const int64_t* target, int64_t bsz) {
   MIRL_REQUIRE(hidden && weight && target, "null pointer argument");
@@ -412,7 +373,7 @@ extern "C" int mirl_linear_ce_fwd(const void* hidden, int dtype, int64_t T, int6
     hipLaunchKernelGGL((lce_tile_kernel<kFwd, F16>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
   hipLaunchKernelGGL(lce_merge_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P.part,
                      P.xt, (int64_t)0, T, P.n_nt, bsz, target, t_stride_b, t_stride_s,
-                     vocab_start, vocab_end, V, out, o_stride_b, o_stride_s, row_stats);
+                     vocab_start, vocab_end, V, out, o_stride_b, o_stride_s, row_stats, nullptr);
   return check_launch("mirl_linear_ce_fwd");
 }
 

@@ -1,0 +1,141 @@
+// Token logprobs from hidden states and an output weight in 8 bits (e4m3), one fp32 scale per
+// row of either:
+//   x[r, v]   = hs[r] * ws[v] * sum_k h8[r, k] w8[v, k]        (the logits, fp32, never written)
+//   logprob_t = (x_t - m) - log(sum_v exp(x_v - m)),  0 for targets outside [vs, ve)
+// on the tile loop of the 16-bit paths (lce_tile.h): the same 128-byte stages hold twice the
+// hidden elements and the MFMA runs at twice the rate.  Forward only: passes that score
+// (previous and reference policy) take no gradient.
+//
+// The matrix unit adds e4m3 products in groups of eight consecutive elements and keeps 13 bits
+// below each group's largest product (measured: a product 2^-14 of its neighbour within the
+// eight is lost, one of another group kept to fp32); a logit of 4096 terms is off by 1.4e-5
+// rms of the root of the sum of its squared products.  In the sum of exponentials these errors
+// average out, but the target's logit stands alone: the merge forms it again in fp32 and puts
+// it in the place of the tile's value, also under the sum.
+
+#include "lce_tile.h"
+
+#pragma clang fp contract(off)
+
+namespace mirl {
+namespace {
+
+// Four e4m3 values of a word, widened.
+__device__ __forceinline__ void unpack_e4m3(uint32_t w, float (&v)[4]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  v[0] = a[0];
+  v[1] = a[1];
+  v[2] = b[0];
+  v[3] = b[1];
+}
+
+// Per row, one wave: the column tiles' partials combined, the target's logit formed in fp32
+// (a dot product of two rows, 8 KB read at H = 4096: 1% of the forward), the logprob.
+__global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float* __restrict__ out, int64_t osb,
+                                                             int64_t oss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= P.nrows) return;
+  const int64_t sq = r / P.bsz, b = r - sq * P.bsz;
+  const int64_t t = P.target[b * P.tsb + sq * P.tss];
+  const bool tmask = (t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V);
+  if (tmask) {
+    if (lane == 0) out[b * osb + sq * oss] = 0.f;
+    return;
+  }
+  const float* p = P.part + r * P.n_nt * 2;
+  float M = -INFINITY;
+  for (int64_t j = lane; j < P.n_nt; j += 64) M = fmaxf(M, p[2 * j]);
+  M = wave_max(M);
+  float s = 0.f;
+  for (int64_t j = lane; j < P.n_nt; j += 64) {
+    const float mj = p[2 * j];
+    if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
+  }
+  s = wave_sum(s);
+  const uint8_t* hr = static_cast<const uint8_t*>(P.h) + r * P.ldh;
+  const uint8_t* wr = static_cast<const uint8_t*>(P.w) + (t - P.vs) * P.ldw;
+  float dot[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t k = lane * 16; k < P.Hd; k += 64 * 16) {
+    const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const vu4*>(wr + k);
+    const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w}, ww[4] = {wq.x, wq.y, wq.z, wq.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float hv[4], wv[4];
+      unpack_e4m3(hw[i], hv);
+      unpack_e4m3(ww[i], wv);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dot[e] = fmaf(hv[e], wv[e], dot[e]);
+    }
+  }
+  const float d = wave_sum((dot[0] + dot[1]) + (dot[2] + dot[3]));
+  if (lane == 0) {
+    const float x = (d * P.col_scale[t - P.vs]) * P.row_scale[r], xt = P.xt[r];
+    // Logits so large that the two differ by more than 1 (some 1e5) keep the tile's value:
+    // the other logits are as far off there.  (Also where one is not finite.)
+    float use = xt;
+    if (fabsf(x - xt) <= 1.f) {
+      s = (s - fast_exp2((xt - M) * kLog2e)) + fast_exp2((x - M) * kLog2e);
+      use = x;
+    }
+    out[b * osb + sq * oss] = (use - M) - logf(s);
+  }
+}
+
+}  // namespace
+}  // namespace mirl
+
+using namespace mirl;
+
+extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int64_t T, int64_t Hd,
+                                       int64_t ldh, const void* weight8, const float* weight_scale, int64_t V,
+                                       int64_t ldw, int64_t bsz, const int64_t* target, int64_t t_stride_b,
+                                       int64_t t_stride_s, int64_t vocab_start, int64_t vocab_end, float* out,
+                                       int64_t o_stride_b, int64_t o_stride_s, float* workspace, void* stream) {
+  clear_error();
+  MIRL_REQUIRE(T >= 0 && V > 0 && Hd > 0 && bsz > 0, "invalid shape T=%lld V=%lld H=%lld B=%lld", (long long)T,
+               (long long)V, (long long)Hd, (long long)bsz);
+  MIRL_REQUIRE(T % bsz == 0, "row count %lld is not a multiple of the batch size %lld", (long long)T, (long long)bsz);
+  MIRL_REQUIRE(Hd % (kStages * kRowBytes) == 0, "hidden size %lld must be a multiple of %d", (long long)Hd,
+               kStages * kRowBytes);
+  // buffer ranges of one 256-row tile are 32-bit byte counts
+  MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22),
+               "row strides (%lld, %lld) must be below 2^22 elements", (long long)ldh, (long long)ldw);
+  MIRL_REQUIRE(ldh % 16 == 0 && ldw % 16 == 0 && ldh >= Hd && ldw >= Hd,
+               "row strides (%lld, %lld) must be multiples of 16 elements and >= the hidden size", (long long)ldh,
+               (long long)ldw);
+  MIRL_REQUIRE(V < (int64_t(1) << 31) && T < (int64_t(1) << 31), "sizes exceed 2^31-1");
+  if (T == 0) return MIRL_OK;
+  MIRL_REQUIRE(hidden8 && hidden_scale && weight8 && weight_scale && target && out && workspace,
+               "null pointer argument");
+  MIRL_REQUIRE((reinterpret_cast<uintptr_t>(hidden8) & 15u) == 0 && (reinterpret_cast<uintptr_t>(weight8) & 15u) == 0,
+               "hidden states and weight must be 16-byte aligned");
+  LceParams P{};
+  P.h = hidden8;
+  P.w = weight8;
+  P.ldh = ldh;
+  P.ldw = ldw;
+  P.V = V;
+  P.Hd = Hd;
+  P.nrows = T;
+  P.bsz = bsz;
+  P.target = target;
+  P.tsb = t_stride_b;
+  P.tss = t_stride_s;
+  P.vs = vocab_start;
+  P.ve = vocab_end;
+  P.n_mt = ceil_div(T, kBM);
+  P.n_nt = ceil_div(V, kBN);
+  P.part = workspace;
+  P.xt = workspace + T * P.n_nt * 2;
+  P.row_scale = hidden_scale;
+  P.col_scale = weight_scale;
+  const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
+  MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL((lce_tile_kernel<kFwdX, F8>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  hipLaunchKernelGGL(lce_merge_8bit_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P, out, o_stride_b,
+                     o_stride_s);
+  return check_launch("mirl_linear_ce_8bit_fwd");
+}

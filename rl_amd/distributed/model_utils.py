@@ -44,6 +44,7 @@ __all__ = [
     "distributed_vocab_topk",
     "DistributedLogprobWithSampling",
     "dropout",
+    "from_parallel_8bit_hidden_states_to_logprobs",
     "from_parallel_hidden_states_to_logprobs",
     "from_parallel_logits_to_logprobs",
     "from_parallel_logits_to_logprobs_packed_sequences",
@@ -82,6 +83,10 @@ def __getattr__(name: str):
         from rl_amd.distributed import final_norm
 
         return getattr(final_norm, name)
+    if name == "from_parallel_8bit_hidden_states_to_logprobs":
+        from rl_amd.distributed import linear_ce_8bit
+
+        return getattr(linear_ce_8bit, name)
     if name == "dropout":
         from rl_amd.distributed.counter_dropout import dropout
 
