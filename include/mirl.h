@@ -977,6 +977,104 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
                             int64_t o_stride_b, int64_t o_stride_s, float* workspace,
                             void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Logprobs from hidden states with low-rank adapters beside the weight     */
+/* ---------------------------------------------------------------------- */
+/* Rows r = s * B + b (position s of sample b), sample b under adapter ids[b] in
+ * [0, N), or the base model for any other id:
+ *   d = dropout(h_r),  U = scaling[a] * (d . A_a^T),  x = h_r . W^T + U . B_a^T
+ *   logprob = log_softmax(x)[target - vocab_start], 0 outside [vocab_start, vocab_end)
+ * h, W [V, H], A [N, r, H] and B [N, V, r] are bf16 or fp16 of one type; x, U and every sum
+ * are fp32 and x is never written.  Element k of row r is dropped as element r * H + k by
+ * mirl_dropout with the same p, seed and offset.  r8 is r rounded up to a multiple of 8 (at
+ * most 1024); B is read as [N, V, r8] (zeros past r), A as [N, r, lda] (zeros past H), both
+ * 16-byte aligned.  An adapter that holds an infinity or a NaN makes its own rows NaN, no
+ * others.
+ */
+
+/* The rows in order of adapter (the base model's first), then sample, then position: all of
+ * them, or with grad_out [B, R] those whose gradient is not zero.  Row m's original row
+ * perm[m], adapter (-1: none), target, gradient and statistics; seg[a] the first row of adapter
+ * a, seg[N] = *count their number.  workspace: 2 B int32. */
+int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64_t R, const float* grad_out,
+                      int64_t g_stride_b, int64_t g_stride_s, const int64_t* target,
+                      int64_t t_stride_b, int64_t t_stride_s, const float* row_stats,
+                      int64_t* perm, int32_t* adapter, int64_t* target_out, float* grad_rows,
+                      float* stats_out, int32_t* seg, int64_t* count, int32_t* workspace,
+                      void* stream);
+
+/* The T sorted rows' hidden states (zero padded to ldo) and their U: as two values of the
+ * operand type that add up to it (u_planes [T, 2, r8]) and, unless NULL, in fp32 by original row
+ * (u_rows [*, r8]).  Rows of the base model leave U as it is. */
+int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const int64_t* perm,
+                      const int32_t* adapter, int64_t T, const void* a, int64_t r, int64_t lda,
+                      const float* scaling, double p, int64_t seed, const int64_t* seed_dev,
+                      int64_t offset, void* hidden_out, int64_t ldo, void* u_planes, int64_t r8,
+                      float* u_rows, void* stream);
+
+/* The logprobs of the T sorted rows (hidden, u_planes as mirl_adapter_down writes them; Hd a
+ * multiple of 128) at their original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
+ * (or NULL).  target_rows: the sorted rows' targets; target [bsz, T / bsz] the original ones.
+ * workspace: mirl_linear_ce_workspace_elems(T, V). */
+int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, int64_t ldh,
+                        const void* weight, int64_t V, int64_t ldw, const int32_t* adapter,
+                        const void* u_planes, const void* b, int64_t r8, const int64_t* perm,
+                        const int64_t* target_rows, int64_t bsz, const int64_t* target,
+                        int64_t t_stride_b, int64_t t_stride_s, int64_t vocab_start,
+                        int64_t vocab_end, float* out, int64_t o_stride_b, int64_t o_stride_s,
+                        float* row_stats, float* workspace, void* stream);
+
+/* Backward operands: rows m < *count (of at most T): hidden rows (zero padded to ldo) and the
+ * planes of U from the forward's u_rows. */
+int mirl_adapter_gather(const int64_t* perm, const int32_t* adapter, const int64_t* count,
+                        int64_t T, const void* hidden, int dtype, int64_t Hd, int64_t ldh,
+                        const float* u_rows, int64_t r8, void* hidden_out, int64_t ldo,
+                        void* u_planes, void* stream);
+
+/* dst[z][c][r] = src[z][r][c] of 16-bit elements for r < R (lowered to *count with one), zeros
+ * for R <= r < R_pad (with a count, as far as the 64-row tile that holds the last row).  With
+ * perm, element c of row r is dropped as element perm[r] * C + c.  R_pad, ldd and dst_z are
+ * multiples of 8, dst is 16-byte aligned. */
+int mirl_transpose16(const void* src, int64_t Z, int64_t src_z, int64_t R, int64_t C, int64_t lds,
+                     void* dst, int64_t dst_z, int64_t ldd, int64_t R_pad, const int64_t* count,
+                     const int64_t* perm, double p, int64_t seed, const int64_t* seed_dev,
+                     int64_t offset, void* stream);
+
+/* G = onehot - softmax of the sorted rows row0 .. row0 + nrows as far as *row_count, in the
+ * operand type (fp16: times 2^15), without the rows' gradients, and its transpose [V, ldgt]
+ * (zeros past the last row in its 256-row tile). */
+int mirl_adapter_ce_grad(const void* hidden, int dtype, int64_t Hd, int64_t ldh,
+                         const void* weight, int64_t V, int64_t ldw, const int32_t* adapter,
+                         const void* u_planes, const void* b, int64_t r8,
+                         const int64_t* target_rows, int64_t vocab_start, int64_t vocab_end,
+                         const float* row_stats, int64_t row0, int64_t nrows, void* grad_logits,
+                         int64_t ldg, void* grad_logits_t, int64_t ldgt, const int64_t* row_count,
+                         void* stream);
+
+/* As mirl_gemm_bf16_abt for fp16 operands, fp32 partial products [k_splits][M][ldc] and a count
+ * of rows (or NULL). */
+int mirl_gemm_f16_abt(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,
+                      int64_t K, int64_t k_splits, float* C, int64_t ldc, const int64_t* count,
+                      int64_t count_off, void* stream);
+
+/* The gradients of one block of sorted rows from its G [n, ldg] (columns V .. ldbt zero), G^T, B^T
+ * [N, r8, ldbt] (zeros past V), A, the dropped hidden rows transposed (hidden_t [Hd, ldht], column
+ * m is sorted row m) and h_part = G . W [h_splits, n, Hd] fp32:
+ *   dh[perm[m]] = g (sum of h_part) + dropout'(dU . A_a)   (rows of the block, rounded once)
+ *   da += dU^T . d,  db += G^T . U                          (fp32 [N, r, Hd], [N, V, r])
+ * each may be NULL.  Sums run in an order that depends on the rows and sizes only. */
+int64_t mirl_adapter_block_workspace_bytes(int64_t n, int64_t r8, int64_t splits);
+int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, const int64_t* count,
+                             const int64_t* perm, const int32_t* adapter, const int32_t* seg,
+                             int64_t N, int64_t V, int64_t Hd, int64_t r, int64_t r8,
+                             const float* grad_rows, const float* scaling, const void* grad_logits,
+                             int64_t ldg, const void* grad_logits_t, int64_t ldgt, const void* b_t,
+                             int64_t ldbt, const void* a, int64_t lda, const void* hidden_t,
+                             int64_t ldht, const float* u_rows, double p, int64_t seed,
+                             const int64_t* seed_dev, int64_t offset, int64_t splits,
+                             const float* h_part, int64_t h_splits, void* dh, int64_t lddh,
+                             float* da, float* db, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

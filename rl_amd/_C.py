@@ -266,6 +266,35 @@ SIGNATURES = {
     "mirl_linear_ce_8bit_fwd": (
         _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
     ),
+    "mirl_adapter_rows": (
+        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+    ),
+    "mirl_adapter_down": (
+        _I,
+        [_P, _I, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _P, ctypes.c_double, _I64, _P, _I64, _P, _I64, _P, _I64, _P,
+         _P],
+    ),
+    "mirl_adapter_ce_fwd": (
+        _I,
+        [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64,
+         _I64, _P, _P, _P],
+    ),
+    "mirl_adapter_gather": (_I, [_P, _P, _P, _I64, _P, _I, _I64, _I64, _P, _I64, _P, _I64, _P, _P]),
+    "mirl_transpose16": (
+        _I, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, ctypes.c_double, _I64, _P, _I64, _P]
+    ),
+    "mirl_adapter_ce_grad": (
+        _I,
+        [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P,
+         _P],
+    ),
+    "mirl_gemm_f16_abt": (_I, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "mirl_adapter_block_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "mirl_adapter_block_grads": (
+        _I,
+        [_I, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
+         _P, _I64, _P, ctypes.c_double, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P],
+    ),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
@@ -1611,3 +1640,173 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
         _stream(dev),
     )
     _check(st, "mirl_linear_ce_8bit_fwd")
+
+
+# ---------------------------------------------------------------------------
+# logprobs from hidden states with low-rank adapters beside the weight
+# ---------------------------------------------------------------------------
+class Dropped:
+    """What names the adapters' dropped inputs: (p, seed, offset), the seed a number or a
+    one-element int64 tensor on ``dev``."""
+
+    def __init__(self, p: float, seed, offset: int, dev: torch.device):
+        self.p = float(p)
+        self.value, self.ptr = _seed_args(seed, dev)
+        self.offset = _signed64(offset)
+
+    def args(self) -> tuple:
+        return self.p, self.value, self.ptr, self.offset
+
+
+class AdapterRows:
+    """Rows sorted by adapter (see mirl_adapter_rows): perm, adapter, target, and with an upstream
+    gradient g and stats, as [rows] tensors; seg [N + 1], count [1]."""
+
+    def __init__(self, ids: torch.Tensor, N: int, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
+                 stats: Optional[torch.Tensor] = None):
+        dev = _require_gpu(ids, target, grad, stats)
+        B, R = target.shape
+        T = B * R
+        _require(ids.dtype == torch.int64 and ids.is_contiguous() and ids.numel() == B, "an int64 adapter id per sample")
+        _require(target.dtype == torch.int64 and (grad is None or (grad.dtype == torch.float32 and grad.shape == target.shape)),
+                 "int64 targets and fp32 gradients [B, R]")
+        _require((grad is None) == (stats is None) and (stats is None or (stats.is_contiguous() and stats.numel() == 2 * T)),
+                 "statistics of the rows go with their gradients")
+        i64 = torch.empty(2 * T + 1, dtype=torch.int64, device=dev)
+        i32 = torch.empty(T + N + 1 + 2 * B, dtype=torch.int32, device=dev)
+        self.perm, self.target, self.count = i64[:T], i64[T : 2 * T], i64[2 * T :]
+        self.adapter, self.seg, ws = i32[:T], i32[T : T + N + 1], i32[T + N + 1 :]
+        self.g = self.stats = None
+        if grad is not None:
+            f32 = torch.empty(3 * T, dtype=torch.float32, device=dev)
+            self.stats, self.g = f32[: 2 * T], f32[2 * T :]
+        st = _launch(
+            "mirl_adapter_rows", dev, ids.data_ptr(), B, N, R, _ptr(grad), 0 if grad is None else grad.stride(0),
+            0 if grad is None else grad.stride(1), target.data_ptr(), target.stride(0), target.stride(1), _ptr(stats),
+            self.perm.data_ptr(), self.adapter.data_ptr(), self.target.data_ptr(), _ptr(self.g), _ptr(self.stats),
+            self.seg.data_ptr(), self.count.data_ptr(), ws.data_ptr(), _stream(dev),
+        )
+        _check(st, "mirl_adapter_rows")
+
+
+def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, scaling: torch.Tensor, drop: Dropped,
+                 width: int, r8: int, want_u: bool):
+    """(hidden rows [T, width], U planes [T, 2, r8], U fp32 [T, r8] by original row or None)."""
+    dev = _require_gpu(hidden2d, a, scaling)
+    T, H, r = rows.perm.numel(), hidden2d.shape[1], a.shape[1]
+    _require(a.is_contiguous() and a.dtype == hidden2d.dtype and a.shape[2] >= H and hidden2d.stride(1) == 1
+             and scaling.dtype == torch.float32 and scaling.numel() == a.shape[0] and scaling.is_contiguous(),
+             "contiguous adapters of the hidden states' type, an fp32 scaling each")
+    h = torch.empty((T, width), dtype=hidden2d.dtype, device=dev)
+    planes = torch.empty((T, 2, r8), dtype=hidden2d.dtype, device=dev)
+    u = torch.empty((T, r8), dtype=torch.float32, device=dev) if want_u else None
+    st = _launch(
+        "mirl_adapter_down", dev, hidden2d.data_ptr(), _dtype_code(hidden2d), H, hidden2d.stride(0), rows.perm.data_ptr(),
+        rows.adapter.data_ptr(), T, a.data_ptr(), r, a.shape[2], scaling.data_ptr(), *drop.args(), h.data_ptr(), width,
+        planes.data_ptr(), r8, _ptr(u), _stream(dev),
+    )
+    _check(st, "mirl_adapter_down")
+    return h, planes, u
+
+
+def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, planes: torch.Tensor, b: torch.Tensor,
+                   target: torch.Tensor, vocab_start: int, vocab_end: int, out: torch.Tensor,
+                   stats: Optional[torch.Tensor]) -> None:
+    """Logprobs [B, R] of the sorted rows at their own places, and their statistics [T, 2]."""
+    dev = _require_gpu(h, weight, planes, b, target, out, stats)
+    T, H = h.shape
+    V = weight.shape[0]
+    _check_linear_ce(h, weight)
+    _require(weight.shape[1] == H and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
+             and planes.shape == (T, 2, b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
+    lib = _lib if _lib is not None else load()
+    ws = torch.empty(int(lib.mirl_linear_ce_workspace_elems(T, V)), dtype=torch.float32, device=dev)
+    st = _launch(
+        "mirl_adapter_ce_fwd", dev, h.data_ptr(), _dtype_code(h), T, H, h.stride(0), weight.data_ptr(), V, weight.stride(0),
+        rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2], rows.perm.data_ptr(), rows.target.data_ptr(),
+        target.shape[0], target.data_ptr(), target.stride(0), target.stride(1), int(vocab_start), int(vocab_end),
+        out.data_ptr(), out.stride(0), out.stride(1), _ptr(stats), ws.data_ptr(), _stream(dev),
+    )
+    _check(st, "mirl_adapter_ce_fwd")
+
+
+def adapter_gather(hidden2d: torch.Tensor, rows: AdapterRows, u: torch.Tensor, width: int):
+    """(hidden rows [T, width], U planes [T, 2, r8]) of the sorted rows below the count."""
+    dev = _require_gpu(hidden2d, u)
+    T, r8 = u.shape
+    h = torch.empty((T, width), dtype=hidden2d.dtype, device=dev)
+    planes = torch.empty((T, 2, r8), dtype=hidden2d.dtype, device=dev)
+    st = _launch(
+        "mirl_adapter_gather", dev, rows.perm.data_ptr(), rows.adapter.data_ptr(), rows.count.data_ptr(), T,
+        hidden2d.data_ptr(), _dtype_code(hidden2d), hidden2d.shape[1], hidden2d.stride(0), u.data_ptr(), r8, h.data_ptr(),
+        width, planes.data_ptr(), _stream(dev),
+    )
+    _check(st, "mirl_adapter_gather")
+    return h, planes
+
+
+def transpose16(src: torch.Tensor, rows: int, cols: int, dst: torch.Tensor, count: Optional[torch.Tensor] = None,
+                perm: Optional[torch.Tensor] = None, drop: Optional[Dropped] = None) -> None:
+    """dst [Z, cols, >= rows] = src [Z, rows, >= cols] transposed (16-bit elements; see
+    mirl_transpose16)."""
+    dev = _require_gpu(src, dst)
+    _check_count(count, dev)
+    Z = src.shape[0]
+    _require(src.element_size() == 2 and dst.dtype == src.dtype and src.stride(2) == 1 and dst.stride(2) == 1
+             and dst.shape[0] == Z and dst.shape[1] >= cols and src.shape[1] >= rows and src.shape[2] >= cols,
+             "16-bit operands of matching shapes")
+    st = _launch(
+        "mirl_transpose16", dev, src.data_ptr(), Z, src.stride(0), int(rows), int(cols), src.stride(1), dst.data_ptr(),
+        dst.stride(0), dst.stride(1), dst.shape[2], _ptr(count), _ptr(perm),
+        *(drop.args() if drop is not None else (0.0, 0, None, 0)), _stream(dev),
+    )
+    _check(st, "mirl_transpose16")
+
+
+def adapter_ce_grad(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, planes: torch.Tensor, b: torch.Tensor,
+                    vocab_start: int, vocab_end: int, row0: int, G: torch.Tensor, Gt: torch.Tensor) -> None:
+    """G [n, >= V] and its transpose of sorted rows row0 .. row0 + n (see mirl_adapter_ce_grad)."""
+    dev = _require_gpu(h, weight, planes, b, G, Gt)
+    _check_linear_ce(h, weight)
+    _require(G.dtype == h.dtype and Gt.dtype == h.dtype and G.stride(1) == 1 and Gt.stride(1) == 1, "G of the operand type")
+    st = _launch(
+        "mirl_adapter_ce_grad", dev, h.data_ptr(), _dtype_code(h), h.shape[1], h.stride(0), weight.data_ptr(),
+        weight.shape[0], weight.stride(0), rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2],
+        rows.target.data_ptr(), int(vocab_start), int(vocab_end), rows.stats.data_ptr(), int(row0), G.shape[0],
+        G.data_ptr(), G.stride(0), Gt.data_ptr(), Gt.stride(0), rows.count.data_ptr(), _stream(dev),
+    )
+    _check(st, "mirl_adapter_ce_grad")
+
+
+def gemm_f16_abt(a: torch.Tensor, b: torch.Tensor, k: int, out: torch.Tensor, count: Optional[torch.Tensor] = None,
+                 count_off: int = 0) -> None:
+    """out [k_splits, M, N] fp32 = partial products of fp16 a [M, >= k] . b [N, >= k]^T; rows of a
+    at or past count - count_off are absent."""
+    dev = _require_gpu(a, b, out)
+    _check_count(count, dev)
+    _require(a.dtype == torch.float16 and b.dtype == torch.float16 and out.dtype == torch.float32
+             and a.stride(1) == 1 and b.stride(1) == 1 and out.is_contiguous() and out.dim() == 3, "fp16 operands, fp32 partials")
+    st = _launch("mirl_gemm_f16_abt", dev, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), a.shape[0], b.shape[0],
+                 int(k), out.shape[0], out.data_ptr(), out.stride(1), _ptr(count), int(count_off), _stream(dev))
+    _check(st, "mirl_gemm_f16_abt")
+
+
+def adapter_block_grads(rows: AdapterRows, row0: int, V: int, H: int, r: int, scaling: torch.Tensor, G: torch.Tensor,
+                        Gt: torch.Tensor, bT: torch.Tensor, a: torch.Tensor, hT: Optional[torch.Tensor],
+                        u: torch.Tensor, drop: Dropped, splits: int, h_part: Optional[torch.Tensor],
+                        dh: Optional[torch.Tensor], da: Optional[torch.Tensor], db: Optional[torch.Tensor]) -> None:
+    """The gradients of sorted rows row0 .. row0 + n (see mirl_adapter_block_grads)."""
+    dev = _require_gpu(G, Gt, bT, a, hT, u, h_part, dh, da, db)
+    n, r8 = G.shape[0], u.shape[1]
+    _require(h_part is None or (h_part.is_contiguous() and h_part.shape[1:] == (n, H)), "h_part [splits, n, H]")
+    lib = _lib if _lib is not None else load()
+    ws = torch.empty(int(lib.mirl_adapter_block_workspace_bytes(n, r8, splits)), dtype=torch.uint8, device=dev)
+    st = _launch(
+        "mirl_adapter_block_grads", dev, _dtype_code(G), int(row0), n, rows.count.data_ptr(), rows.perm.data_ptr(),
+        rows.adapter.data_ptr(), rows.seg.data_ptr(), a.shape[0], V, H, r, r8, rows.g.data_ptr(), scaling.data_ptr(),
+        G.data_ptr(), G.stride(0), Gt.data_ptr(), Gt.stride(0), bT.data_ptr(), bT.shape[2], a.data_ptr(), a.shape[2],
+        _ptr(hT), 0 if hT is None else hT.stride(-2), u.data_ptr(), *drop.args(), int(splits), _ptr(h_part),
+        0 if h_part is None else h_part.shape[0], _ptr(dh), 0 if dh is None else dh.stride(0), _ptr(da), _ptr(db),
+        ws.data_ptr(), _stream(dev),
+    )
+    _check(st, "mirl_adapter_block_grads")

@@ -265,7 +265,8 @@ void lce_tile_kernel(LceParams P) {
   __shared__ __align__(1024) unsigned char st1[kStageBytes];
   __shared__ int s_tcol[kBM];
   __shared__ float s_m[kBM], s_ls[kBM], s_g[kBM];
-  __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_heads[kWaves];
+  __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_bad[kAdapters ? kBM : 1],
+      s_heads[kWaves];
   auto stage_ptr = [&](int s) -> unsigned char* { return s == 0 ? st0 : st1; };
 
   // Tile order.  Workgroups are dispatched to the 8 XCDs round-robin
@@ -372,6 +373,7 @@ void lce_tile_kernel(LceParams P) {
       }
       s_ord[tid] = a >= 0 ? at - 1 : -1;
       if (head) s_seg[at - 1] = a;
+      s_bad[tid] = 0;
       __syncthreads();
       n_seg = __builtin_amdgcn_readfirstlane(n_seg);
     }
@@ -558,6 +560,18 @@ void lce_tile_kernel(LceParams P) {
   // each, eight 16-byte chunks a stage; a row's U is zero in the chunks of other adapters.
   // (Every adapter of the tile costs planes * r8 / 64 of a stage; a step of 4 adapters of rank
   // 16 over [16384, 4096] x [151936, 4096] has one in all but three tiles in 64.)
+  // An infinity or a NaN of one adapter's B must not meet the other rows' zeros: it is taken
+  // out, and that adapter's rows of the tile become NaN afterwards (s_bad).
+  auto nonfinite = [](vu4 q) __attribute__((always_inline)) {
+    constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+      bad |= (w & ex) == ex || ((w >> 16) & ex) == ex;
+    }
+    return bad;
+  };
   auto adapter_stages = [&]() __attribute__((always_inline)) {
     const int cpp = P.r8 >> 3, cps = P.planes * cpp, chunk = tid & 7;
     const int n_ext = (n_seg * cps + 7) >> 3;
@@ -573,6 +587,10 @@ void lce_tile_kernel(LceParams P) {
         vu4 u = {0u, 0u, 0u, 0u}, b = {0u, 0u, 0u, 0u};
         if (any && s_ord[row] == q) u = *reinterpret_cast<const vu4*>(up + (int64_t)row * (P.planes * P.r8));
         if (any && n0 + row < P.V) b = *reinterpret_cast<const vu4*>(bp + (int64_t)row * P.r8);
+        if (nonfinite(b)) {
+          b = vu4{0u, 0u, 0u, 0u};
+          s_bad[q] = 1;
+        }
         *reinterpret_cast<vu4*>(st1 + lds_off(row, chunk)) = u;
         *reinterpret_cast<vu4*>(st1 + kHalfBytes + lds_off(row, chunk)) = b;
       }
@@ -586,6 +604,9 @@ void lce_tile_kernel(LceParams P) {
       }
     }
     __syncthreads();
+    if constexpr (MODE == kGradX) {
+      if (s_ord[tid] >= 0 && s_bad[s_ord[tid]] != 0) s_g[tid] = __builtin_nanf("");
+    }
   };
   auto run_stages = [&]() __attribute__((always_inline)) {
     // Prologue: stage data 0 and 1 in flight; wait for 0 and read its block-0 fragments.
@@ -940,6 +961,9 @@ void lce_tile_kernel(LceParams P) {
         float sum = 0.f;
         if (rm[i] != -INFINITY) sum += rsum[i] * fast_exp2((rm[i] - M) * kLog2e);
         if (m1 != -INFINITY) sum += s_g[rl] * fast_exp2((m1 - M) * kLog2e);
+        if constexpr (kAdapters) {
+          if (n_seg > 0 && s_ord[rl] >= 0 && s_bad[s_ord[rl]] != 0) sum = __builtin_nanf("");
+        }
         float* dst = P.part + ((r - P.row0) * P.n_nt + nt) * 2;
         dst[0] = M;
         dst[1] = sum;

@@ -46,6 +46,7 @@ __all__ = [
     "dropout",
     "from_parallel_8bit_hidden_states_to_logprobs",
     "from_parallel_hidden_states_to_logprobs",
+    "from_parallel_hidden_states_to_logprobs_with_adapters",
     "from_parallel_logits_to_logprobs",
     "from_parallel_logits_to_logprobs_packed_sequences",
     "get_next_token_logprobs_from_logits",
@@ -87,6 +88,10 @@ def __getattr__(name: str):
         from rl_amd.distributed import linear_ce_8bit
 
         return getattr(linear_ce_8bit, name)
+    if name == "from_parallel_hidden_states_to_logprobs_with_adapters":
+        from rl_amd.distributed import linear_ce_adapters
+
+        return getattr(linear_ce_adapters, name)
     if name == "dropout":
         from rl_amd.distributed.counter_dropout import dropout
 
