@@ -267,17 +267,17 @@ SIGNATURES = {
         _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
     ),
     "mirl_adapter_rows": (
-        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _P, _P, _P]
     ),
     "mirl_adapter_down": (
         _I,
-        [_P, _I, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _P, ctypes.c_double, _I64, _P, _I64, _P, _I64, _P, _I64, _P,
+        [_P, _I, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, ctypes.c_double, _I64, _P, _I64, _P, _I64, _P, _I64, _P,
          _P],
     ),
     "mirl_adapter_ce_fwd": (
         _I,
-        [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64,
-         _I64, _P, _P, _P],
+        [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64,
+         _P, _I64, _I64, _P, _P, _P],
     ),
     "mirl_adapter_gather": (_I, [_P, _P, _P, _I64, _P, _I, _I64, _I64, _P, _I64, _P, _I64, _P, _P]),
     "mirl_transpose16": (
@@ -285,8 +285,8 @@ SIGNATURES = {
     ),
     "mirl_adapter_ce_grad": (
         _I,
-        [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P,
-         _P],
+        [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P,
+         _I64, _P, _P],
     ),
     "mirl_gemm_f16_abt": (_I, [_P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
     "mirl_adapter_block_workspace_bytes": (_I64, [_I64, _I64, _I64]),
@@ -1660,11 +1660,17 @@ class Dropped:
 
 class AdapterRows:
     """Rows sorted by adapter (see mirl_adapter_rows): perm, adapter, target, and with an upstream
-    gradient g and stats, as [rows] tensors; seg [N + 1], count [1]."""
+    gradient g and stats, as [rows] tensors; seg [N + 1], count [1].  ``b [N, V, r8]`` is looked
+    through for values that are none (``bad [N]``), unless ``bad`` is given."""
 
-    def __init__(self, ids: torch.Tensor, N: int, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
-                 stats: Optional[torch.Tensor] = None):
-        dev = _require_gpu(ids, target, grad, stats)
+    def __init__(self, ids: torch.Tensor, b: torch.Tensor, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
+                 stats: Optional[torch.Tensor] = None, bad: Optional[torch.Tensor] = None):
+        dev = _require_gpu(ids, target, grad, stats, b)
+        N = b.shape[0]
+        _require(b.is_contiguous(), "contiguous adapters")
+        self.bad, look = bad, bad is None
+        if look:
+            self.bad = torch.empty(N, dtype=torch.int32, device=dev)
         B, R = target.shape
         T = B * R
         _require(ids.dtype == torch.int64 and ids.is_contiguous() and ids.numel() == B, "an int64 adapter id per sample")
@@ -1684,7 +1690,8 @@ class AdapterRows:
             "mirl_adapter_rows", dev, ids.data_ptr(), B, N, R, _ptr(grad), 0 if grad is None else grad.stride(0),
             0 if grad is None else grad.stride(1), target.data_ptr(), target.stride(0), target.stride(1), _ptr(stats),
             self.perm.data_ptr(), self.adapter.data_ptr(), self.target.data_ptr(), _ptr(self.g), _ptr(self.stats),
-            self.seg.data_ptr(), self.count.data_ptr(), ws.data_ptr(), _stream(dev),
+            self.seg.data_ptr(), self.count.data_ptr(), b.data_ptr(), _dtype_code(b), b.shape[1] * b.shape[2],
+            self.bad.data_ptr() if look else None, ws.data_ptr(), _stream(dev),
         )
         _check(st, "mirl_adapter_rows")
 
@@ -1702,7 +1709,7 @@ def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, sca
     u = torch.empty((T, r8), dtype=torch.float32, device=dev) if want_u else None
     st = _launch(
         "mirl_adapter_down", dev, hidden2d.data_ptr(), _dtype_code(hidden2d), H, hidden2d.stride(0), rows.perm.data_ptr(),
-        rows.adapter.data_ptr(), T, a.data_ptr(), r, a.shape[2], scaling.data_ptr(), *drop.args(), h.data_ptr(), width,
+        rows.adapter.data_ptr(), T, a.data_ptr(), a.shape[0], r, a.shape[2], scaling.data_ptr(), *drop.args(), h.data_ptr(), width,
         planes.data_ptr(), r8, _ptr(u), _stream(dev),
     )
     _check(st, "mirl_adapter_down")
@@ -1723,7 +1730,7 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
     ws = torch.empty(int(lib.mirl_linear_ce_workspace_elems(T, V)), dtype=torch.float32, device=dev)
     st = _launch(
         "mirl_adapter_ce_fwd", dev, h.data_ptr(), _dtype_code(h), T, H, h.stride(0), weight.data_ptr(), V, weight.stride(0),
-        rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2], rows.perm.data_ptr(), rows.target.data_ptr(),
+        rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2], b.shape[0], rows.bad.data_ptr(), rows.perm.data_ptr(), rows.target.data_ptr(),
         target.shape[0], target.data_ptr(), target.stride(0), target.stride(1), int(vocab_start), int(vocab_end),
         out.data_ptr(), out.stride(0), out.stride(1), _ptr(stats), ws.data_ptr(), _stream(dev),
     )
@@ -1772,6 +1779,7 @@ def adapter_ce_grad(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pl
     st = _launch(
         "mirl_adapter_ce_grad", dev, h.data_ptr(), _dtype_code(h), h.shape[1], h.stride(0), weight.data_ptr(),
         weight.shape[0], weight.stride(0), rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2],
+        b.shape[0], rows.bad.data_ptr(),
         rows.target.data_ptr(), int(vocab_start), int(vocab_end), rows.stats.data_ptr(), int(row0), G.shape[0],
         G.data_ptr(), G.stride(0), Gt.data_ptr(), Gt.stride(0), rows.count.data_ptr(), _stream(dev),
     )

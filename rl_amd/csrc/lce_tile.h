@@ -239,6 +239,8 @@ struct LceParams {
   const uint16_t* U;
   const uint16_t* B;
   int r8, planes;
+  const int32_t* bad;   // [adapters]: B holds an infinity or a NaN
+  int64_t b_bytes;      // size of B
   // kGradX: G = (onehot - softmax) * g_scale in the operand type (rows past the end: 0)
   float g_scale;
   // kFwdX of e4m3: logits = products * col_scale[col] * row_scale[row]
@@ -356,6 +358,7 @@ void lce_tile_kernel(LceParams P) {
   }
   // The tile's adapters in row order: s_seg[q] is the q-th one, s_ord[row] the row's (-1: none).
   int n_seg = 0;
+  bool apart = false;  // their part is formed by itself (adapter_stages)
   if constexpr (kAdapters) {
     if (P.aid != nullptr) {
       const int64_t r = m0 + tid;
@@ -372,9 +375,13 @@ void lce_tile_kernel(LceParams P) {
         n_seg += s_heads[w];
       }
       s_ord[tid] = a >= 0 ? at - 1 : -1;
-      if (head) s_seg[at - 1] = a;
-      s_bad[tid] = 0;
-      __syncthreads();
+      const int bad = head ? P.bad[a] : 0;
+      if (head) {
+        s_seg[at - 1] = a;
+        s_bad[at - 1] = bad;
+      }
+      // (32-bit offsets reach 2 GiB of B)
+      apart = __syncthreads_or(bad) != 0 || P.b_bytes >= (int64_t(1) << 31);
       n_seg = __builtin_amdgcn_readfirstlane(n_seg);
     }
   }
@@ -437,10 +444,10 @@ void lce_tile_kernel(LceParams P) {
   }
   const int64_t a_rows = (row_end - m0 < kBM) ? (row_end - m0) : kBM;
   const int64_t b_rows = (P.V - n0 < kBN) ? (P.V - n0) : kBN;
-  const __amdgpu_buffer_rsrc_t rsrc_a = __builtin_amdgcn_make_buffer_rsrc(
+  __amdgpu_buffer_rsrc_t rsrc_a = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(P.h) + (m0 * P.ldh + kbase) * kES), 0,
       (int)((a_rows * P.ldh - kbase) * kES), 0x00020000);
-  const __amdgpu_buffer_rsrc_t rsrc_b = __builtin_amdgcn_make_buffer_rsrc(
+  __amdgpu_buffer_rsrc_t rsrc_b = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(P.w) + (n0 * P.ldw + kbase) * kES), 0,
       (int)((b_rows * P.ldw - kbase) * kES), 0x00020000);
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -454,7 +461,7 @@ void lce_tile_kernel(LceParams P) {
   }
   // load q of stage data t: q < kDmaPerWave is an H block, else a W block
   auto dma = [&](unsigned char* stage, int t, int q) {
-    const int soff = t * kRowBytes;
+    const int soff = kAdapters && t >= nst ? 0 : t * kRowBytes;
     if (q < kDmaPerWave) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc_a, (lds_ptr_t)(stage + (wave_u * kDmaPerWave + q) * kDmaBytes), 16, voff_a[q], soff, 0, 0);
@@ -463,6 +470,38 @@ void lce_tile_kernel(LceParams P) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc_b, (lds_ptr_t)(stage + kHalfBytes + (wave_u * kDmaPerWave + qb) * kDmaBytes), 16,
           voff_b[qb], soff, 0, 0);
+    }
+  };
+
+  // Adapter stages: stage data nst + e continues the reduction over the tile's adapters one after
+  // the other, `planes` * r8 elements each, eight 16-byte chunks a stage; a row's U is zero in the
+  // chunks of other adapters (an offset out of range reads as zero).  One adapter of rank up to 16
+  // takes one of the two stages added to 64 at a hidden size of 4096, several share them.
+  const int cpp = kAdapters ? P.r8 >> 3 : 1, cps = kAdapters ? P.planes * cpp : 1;
+  const int n_ext = (n_seg * cps + 7) >> 3;
+  const int total = kAdapters && !apart ? nst + (n_ext + 1) / 2 * 2 : nst;
+  auto prepare = [&](int t) __attribute__((always_inline)) {
+    constexpr int kOut = -0x7fffffff - 1;
+    // opaque here, or everything that follows from it is formed ahead of the main loop and
+    // kept in registers that it lacks
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(P.planes * P.r8)), 0,
+                                               (int)(a_rows * P.planes * P.r8 * 2), 0x00020000);
+    rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.B + n0 * P.r8), 0,
+                                               (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      // a load's rows start at a multiple of 8, so its chunks depend on its parity only
+      const int x = (t - nst) * 8 + ((ln & 7) ^ (((ln >> 4) + 4 * odd) & 7));
+      const int seg = x / cps, rem = x - seg * cps, cc = rem % cpp;
+      const int b0 = (s_seg[seg < n_seg ? seg : 0] * (int)P.V * P.r8 + cc * 8) * 2;
+#pragma unroll
+      for (int i = odd; i < kDmaPerWave; i += 2) {
+        const int row = (wave * kDmaPerWave + i) * kDmaRows + (ln >> 3);
+        voff_a[i] = s_ord[row] == seg ? (row * P.planes * P.r8 + rem * 8) * 2 : kOut;
+        voff_b[i] = ((seg < n_seg) & (row < (int)b_rows)) ? b0 + row * P.r8 * 2 : kOut;
+      }
     }
   };
 
@@ -555,13 +594,10 @@ void lce_tile_kernel(LceParams P) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // The adapters' part of the logits, through stage array 1 while stage data 0 is in flight:
-  // the reduction runs over the tile's adapters one after the other, `planes` * r8 elements
-  // each, eight 16-byte chunks a stage; a row's U is zero in the chunks of other adapters.
-  // (Every adapter of the tile costs planes * r8 / 64 of a stage; a step of 4 adapters of rank
-  // 16 over [16384, 4096] x [151936, 4096] has one in all but three tiles in 64.)
-  // An infinity or a NaN of one adapter's B must not meet the other rows' zeros: it is taken
-  // out, and that adapter's rows of the tile become NaN afterwards (s_bad).
+  // The adapters' part by itself, stage by stage through stage array 1, where a value of an adapter
+  // is none or B passes 2 GiB:
+  // an infinity or a NaN of one adapter's B must not meet the other rows' zeros, so it is taken
+  // out, and that adapter's rows become NaN afterwards (s_bad).
   auto nonfinite = [](vu4 q) __attribute__((always_inline)) {
     constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
     bool bad = false;
@@ -573,24 +609,20 @@ void lce_tile_kernel(LceParams P) {
     return bad;
   };
   auto adapter_stages = [&]() __attribute__((always_inline)) {
-    const int cpp = P.r8 >> 3, cps = P.planes * cpp, chunk = tid & 7;
-    const int n_ext = (n_seg * cps + 7) >> 3;
+    const int chunk = tid & 7;
     for (int e = 0; e < n_ext; ++e) {
       const int x = e * 8 + chunk, q = x / cps, rem = x - q * cps, cc = rem % cpp;
       const bool any = q < n_seg;
       const uint16_t* up = P.U + m0 * (int64_t)(P.planes * P.r8) + rem * 8;
       const uint16_t* bp = P.B + ((int64_t)(any ? s_seg[q] : 0) * P.V + n0) * P.r8 + cc * 8;
       __syncthreads();  // the last stage's reads are done
-#pragma unroll
+#pragma unroll 1
       for (int k = 0; k < kBM / 32; ++k) {
         const int row = k * 32 + (tid >> 3);
         vu4 u = {0u, 0u, 0u, 0u}, b = {0u, 0u, 0u, 0u};
         if (any && s_ord[row] == q) u = *reinterpret_cast<const vu4*>(up + (int64_t)row * (P.planes * P.r8));
         if (any && n0 + row < P.V) b = *reinterpret_cast<const vu4*>(bp + (int64_t)row * P.r8);
-        if (nonfinite(b)) {
-          b = vu4{0u, 0u, 0u, 0u};
-          s_bad[q] = 1;
-        }
+        if (nonfinite(b)) b = vu4{0u, 0u, 0u, 0u};
         *reinterpret_cast<vu4*>(st1 + lds_off(row, chunk)) = u;
         *reinterpret_cast<vu4*>(st1 + kHalfBytes + lds_off(row, chunk)) = b;
       }
@@ -612,9 +644,6 @@ void lce_tile_kernel(LceParams P) {
     // Prologue: stage data 0 and 1 in flight; wait for 0 and read its block-0 fragments.
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st0, 0, q);
-    if constexpr (kAdapters) {
-      if (n_seg > 0) adapter_stages();
-    }
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st1, 1, q);
     wait_vm_barrier<kL>();
@@ -624,6 +653,14 @@ void lce_tile_kernel(LceParams P) {
     for (; t < nst - kStages; t += kStages) {
       step(t, S0{}, T_{}, T_{});
       step(t + 1, S1{}, T_{}, T_{});
+    }
+    if constexpr (kAdapters) {
+      for (; t < total - kStages; t += kStages) {
+        prepare(t + kStages);
+        step(t, S0{}, T_{}, T_{});
+        prepare(t + 1 + kStages);
+        step(t + 1, S1{}, T_{}, T_{});
+      }
     }
     step(t, S0{}, T_{}, F_{});
     step(t + 1, S1{}, F_{}, F_{});
@@ -792,6 +829,9 @@ void lce_tile_kernel(LceParams P) {
     }
   } else {
     run_stages();
+    if constexpr (kAdapters) {
+      if (apart) adapter_stages();
+    }
   }
 
   if constexpr (MODE == kGemm) {

@@ -35,6 +35,15 @@ constexpr float g_scale_of() {
 
 int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
+// A launch holds fewer than 2^32 threads.
+constexpr int64_t kMaxRows = int64_t(1) << 26, kMaxBlocks = int64_t(1) << 23;
+constexpr int64_t kMaxRank = 1024;  // a workgroup of adapter_dh_kernel holds eight rows of dU in LDS
+// Ranks of the plane arrays: whole tiles of those that with_rank chooses.
+int64_t padded_rank(int64_t r8) { return r8 <= 16 ? 16 : r8 <= 32 ? 32 : round_up(r8, kRankTile); }
+
+bool is16(int dtype) { return dtype == MIRL_DTYPE_BF16 || dtype == MIRL_DTYPE_F16; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 // -------------------------------------------------------------------------------------------
 // rows sorted by adapter
 // -------------------------------------------------------------------------------------------
@@ -66,7 +75,7 @@ __global__ __launch_bounds__(1024) void adapter_count_kernel(const float* __rest
 __global__ __launch_bounds__(1024) void adapter_starts_kernel(const int64_t* __restrict__ ids, int64_t B, int64_t N,
                                                               int32_t R, const int32_t* __restrict__ cnt,
                                                               int32_t* __restrict__ start, int32_t* __restrict__ seg,
-                                                              int64_t* __restrict__ count) {
+                                                              int64_t* __restrict__ count, int32_t* __restrict__ bad) {
   __shared__ int w[2][16];
   const int64_t k = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -78,7 +87,10 @@ __global__ __launch_bounds__(1024) void adapter_starts_kernel(const int64_t* __r
   __syncthreads();
   int at = 0;
   for (int i = 0; i < 16; ++i) at += w[0][i];
-  if (tid == 0 && k > 0) seg[k - 1] = at;
+  if (tid == 0 && k > 0) {
+    seg[k - 1] = at;
+    if (bad != nullptr) bad[k - 1] = 0;
+  }
   int turn = 1;
   for (int64_t b0 = 0; b0 < B; b0 += 1024) {
     const int64_t b = b0 + tid;
@@ -151,6 +163,31 @@ __global__ __launch_bounds__(1024) void adapter_fill_kernel(const int64_t* __res
       }
     }
   }
+}
+
+// bad[a] = 1 for the adapters with rows whose B holds an infinity or a NaN (from 0): 32 KB a
+// workgroup.
+constexpr int kScanVecs = 8;
+template <class E>
+__global__ __launch_bounds__(256) void adapter_scan_kernel(const vu4* __restrict__ b, int64_t vecs, int64_t per,
+                                                           const int32_t* __restrict__ seg,
+                                                           int32_t* __restrict__ bad) {
+  const int64_t a = blockIdx.x / per, part = blockIdx.x - a * per;
+  if (seg[a] >= seg[a + 1]) return;
+  constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
+  const vu4* src = b + a * vecs;
+  vu4 q[kScanVecs];
+#pragma unroll
+  for (int u = 0; u < kScanVecs; ++u) {
+    const int64_t i = (part * kScanVecs + u) * 256 + threadIdx.x;
+    q[u] = i < vecs ? src[i] : vu4{0u, 0u, 0u, 0u};
+  }
+  bool none = false;
+#pragma unroll
+  for (int u = 0; u < kScanVecs; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) none |= (q[u][j] & ex) == ex || ((q[u][j] >> 16) & ex) == ex;
+  if (none) bad[a] = 1;
 }
 
 // -------------------------------------------------------------------------------------------
@@ -229,12 +266,13 @@ struct DownParams {
   float* U32;              // [rows, r8] by original row, or null
 };
 
-// 16 sorted rows a workgroup, the hidden dimension split over its four waves 64 elements at a
+// 16 sorted rows a workgroup, the hidden dimension split over its NW waves 64 elements at a
 // time.  An MFMA takes 16 ranks of the adapter against the 16 rows.  Rows of several adapters
-// are read once per adapter (from the cache after the first time).
-template <class E, int NT>
-__global__ __launch_bounds__(256) void adapter_down_kernel(DownParams P) {
-  __shared__ float red[4][16][NT * 16 + 4];
+// are read once per adapter (from the cache after the first time); the gridDim.z workgroups of
+// the same rows take every gridDim.z-th adapter.
+template <class E, int NT, int NW>
+__global__ __launch_bounds__(NW * 64) void adapter_down_kernel(DownParams P) {
+  __shared__ float red[NW][16][NT * 16 + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 15, lg = lane >> 4;
   const int64_t m0 = (int64_t)blockIdx.x * 16, rho0 = (int64_t)blockIdx.y * kRankTile;
@@ -244,9 +282,10 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(DownParams P) {
   const int32_t my_aid = live ? P.aid[m] : -1;
   const uint16_t* hr = P.hidden + row * P.ldh;
   const uint64_t seed = P.drop.threshold > 0 ? P.drop.seed_of() : 0;
-  if (blockIdx.y == 0) {
+  if (blockIdx.y == 0 && blockIdx.z == 0) {
     uint16_t* ho = P.h_out + m * P.ldo;
-    for (int64_t k0 = (int64_t)wave * 64; k0 < P.ldo; k0 += 256) {
+#pragma unroll 4
+    for (int64_t k0 = (int64_t)wave * 64; k0 < P.ldo; k0 += NW * 64) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int64_t k = k0 + u * 32 + lg * 8;
@@ -255,7 +294,7 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(DownParams P) {
     }
   }
   int done = -1;  // adapters up to this one are done (rows are sorted: ids ascend)
-  for (;;) {
+  for (int nth = 0;; ++nth) {
     // the smallest adapter of the 16 rows that is still to do
     int a = my_aid > done ? my_aid : 0x7fffffff;
 #pragma unroll
@@ -266,15 +305,40 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(DownParams P) {
     a = __builtin_amdgcn_readfirstlane(a);
     if (a == 0x7fffffff) break;
     done = a;
+    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
     const uint16_t* Aa = P.A + ((int64_t)a * P.r + rho0) * P.lda;
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int64_t k0 = (int64_t)wave * 64; k0 < P.H; k0 += 256) {
+    const bool mine = my_aid == a;
+    int64_t k0 = (int64_t)wave * 64;
+    // two steps at a time while they end inside the row: their loads in flight together
+    constexpr int KU = NT < 4 ? 4 : 2;
+    for (; k0 + (KU / 2 - 1) * NW * 64 + 64 <= P.H; k0 += KU / 2 * NW * 64) {
+      vu4 h[KU], w[KU][NT];
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const int64_t k = k0 + (u / 2) * NW * 64 + (u & 1) * 32 + lg * 8;
+        h[u] = mine ? load_raw8(hr + k) : zero4();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int64_t rho = t * 16 + lr;
+          w[u][t] = rho0 + rho < P.r ? *reinterpret_cast<const vu4*>(Aa + rho * P.lda + k) : zero4();
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const int64_t k = k0 + (u / 2) * NW * 64 + (u & 1) * 32 + lg * 8;
+        if (P.drop.threshold > 0) h[u] = mask8(h[u], keep8_at(seed, P.drop, row * P.H + k));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = mfma16<E>(w[u][t], h[u], acc[t]);
+      }
+    }
+    for (; k0 < P.H; k0 += NW * 64) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int64_t k = k0 + u * 32 + lg * 8;
-        vu4 h = my_aid == a && k < P.H ? load_raw8_to(hr, k, P.H) : zero4();
+        vu4 h = mine && k < P.H ? load_raw8_to(hr, k, P.H) : zero4();
         if (P.drop.threshold > 0) h = mask8(h, keep8_at(seed, P.drop, row * P.H + k));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -291,11 +355,14 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(DownParams P) {
       for (int e = 0; e < 4; ++e) red[wave][lr][t * 16 + lg * 4 + e] = acc[t][e];
     __syncthreads();
     const float s = P.scaling[a] * (P.drop.threshold > 0 ? P.drop.scale : 1.f);
-    for (int q = tid; q < 16 * NT * 16; q += 256) {
+    for (int q = tid; q < 16 * NT * 16; q += NW * 64) {
       const int rl = q / (NT * 16), rho = q - rl * (NT * 16);
       const int64_t mm = m0 + rl;
       if (mm >= P.T || P.aid[mm] != a || rho0 + rho >= P.r8) continue;
-      const float v = ((red[0][rl][rho] + red[1][rl][rho]) + (red[2][rl][rho] + red[3][rl][rho])) * s;
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) v += red[i][rl][rho];
+      v *= s;
       uint16_t p[kPlanes];
       split_planes<E>(v, p);
 #pragma unroll
@@ -468,19 +535,29 @@ __global__ __launch_bounds__(256) void adapter_du_kernel(BlockParams P) {
       // rows past the block's are read as its last one
       const int64_t ra = w0 + lr < n ? w0 + lr : n - 1, rb = w0 + 16 + lr < n ? w0 + 16 + lr : n - 1;
       const uint16_t *ga = P.G + ra * P.ldg, *gb = P.G + rb * P.ldg;
-      for (int64_t k0 = split * P.k_len; k0 < k_end; k0 += 64) {
+      // KU steps of 32 columns at a time, their loads in flight together (k_len and the rows'
+      // padded length are multiples of 128)
+      constexpr int KU = NT < 4 ? 4 : 2;
+      for (int64_t k0 = split * P.k_len; k0 < k_end; k0 += KU * 32) {
+        vu4 q0[KU], q1[KU], b[KU][NT];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < KU; ++u) {
           const int64_t k = k0 + u * 32 + lg * 8;
-          const vu4 q0 = *reinterpret_cast<const vu4*>(ga + k), q1 = *reinterpret_cast<const vu4*>(gb + k);
+          q0[u] = *reinterpret_cast<const vu4*>(ga + k);
+          q1[u] = *reinterpret_cast<const vu4*>(gb + k);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             const int64_t rho = t * 16 + lr;
-            const vu4 b = rho0 + rho < P.r8 ? *reinterpret_cast<const vu4*>(Ba + rho * P.ldbt + k) : zero4();
-            acc[0][t] = mfma16<E>(b, q0, acc[0][t]);
-            acc[1][t] = mfma16<E>(b, q1, acc[1][t]);
+            b[u][t] = rho0 + rho < P.r8 ? *reinterpret_cast<const vu4*>(Ba + rho * P.ldbt + k) : zero4();
           }
         }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            acc[0][t] = mfma16<E>(b[u][t], q0[u], acc[0][t]);
+            acc[1][t] = mfma16<E>(b[u][t], q1[u], acc[1][t]);
+          }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -577,38 +654,64 @@ __device__ __forceinline__ uint32_t inside8(int64_t m, int64_t lo, int64_t hi) {
   return from & to;
 }
 
-// Two 16-row tiles of X [rows, ldx] against the planes Y [kPlanes, r16, ldn], summed over
-// columns k0, k0 + step, ... of 64 each as far as [lo, hi).  Columns outside are zero in both
-// operands (a row of another adapter may hold infinities or NaN).
+// 64 columns from k0 on of the product below; those outside [lo, hi) are zero in both operands (a
+// row of another adapter may hold infinities or NaN).
+template <class E, int NT, int MT>
+__device__ __forceinline__ void thin_piece(const uint16_t* const (&x)[MT], const uint16_t* y, int64_t plane,
+                                           int64_t ldn, int64_t k0, int64_t lo, int64_t hi, int lg,
+                                           f32x4 (&acc)[MT][NT]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int64_t k = k0 + u * 32 + lg * 8;
+    const uint32_t in = inside8(k, lo, hi);
+    vu4 q[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) q[i] = mask8(*reinterpret_cast<const vu4*>(x[i] + k), in);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p) {
+        const vu4 b = mask8(*reinterpret_cast<const vu4*>(y + p * plane + (int64_t)t * 16 * ldn + k), in);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][t] = mfma16<E>(q[i], b, acc[i][t]);
+      }
+  }
+}
+
+// MT 16-row tiles of X against the planes Y [kPlanes, r16, ldn], summed over the columns [lo, hi)
+// in pieces of 64 from k0 on, every step-th column.
 template <class E, int NT, int MT>
 __device__ __forceinline__ void thin_product(const uint16_t* const (&x)[MT], const uint16_t* y, int64_t plane,
                                              int64_t ldn, int64_t k0, int64_t step, int64_t lo, int64_t hi, int lg,
                                              f32x4 (&acc)[MT][NT]) {
-  for (; k0 < hi; k0 += step) {
-    const bool whole = k0 >= lo && k0 + 64 <= hi;
+  // whole pieces two at a time, their loads in flight together
+  while (k0 < lo) {
+    thin_piece<E, NT, MT>(x, y, plane, ldn, k0, lo, hi, lg, acc);
+    k0 += step;
+  }
+  for (; k0 + step + 64 <= hi; k0 += 2 * step) {
+    vu4 q[4][MT], b[4][NT][kPlanes];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t k = k0 + u * 32 + lg * 8;
-      vu4 q[MT];
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = k0 + (u >> 1) * step + (u & 1) * 32 + lg * 8;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) q[i] = *reinterpret_cast<const vu4*>(x[i] + k);
-      uint32_t in = 0xffu;
-      if (!whole) {
-        in = inside8(k, lo, hi);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) q[i] = mask8(q[i], in);
-      }
+      for (int i = 0; i < MT; ++i) q[u][i] = *reinterpret_cast<const vu4*>(x[i] + k);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int p = 0; p < kPlanes; ++p) {
-          vu4 b = *reinterpret_cast<const vu4*>(y + p * plane + (int64_t)t * 16 * ldn + k);
-          if (!whole) b = mask8(b, in);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][t] = mfma16<E>(q[i], b, acc[i][t]);
-        }
+        for (int p = 0; p < kPlanes; ++p)
+          b[u][t][p] = *reinterpret_cast<const vu4*>(y + p * plane + (int64_t)t * 16 * ldn + k);
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][t] = mfma16<E>(q[u][i], b[u][t][p], acc[i][t]);
   }
+  for (; k0 < hi; k0 += step) thin_piece<E, NT, MT>(x, y, plane, ldn, k0, lo, hi, lg, acc);
 }
 
 // dB_a += G^T . (g U): 32 vocabulary rows a wave, once per adapter with rows in the block.
@@ -779,15 +882,6 @@ __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
   }
 }
 
-// A launch holds fewer than 2^32 threads.
-constexpr int64_t kMaxRows = int64_t(1) << 26, kMaxBlocks = int64_t(1) << 23;
-constexpr int64_t kMaxRank = 1024;  // a workgroup of adapter_dh_kernel holds eight rows of dU in LDS
-// Ranks of the plane arrays: whole tiles of those that with_rank chooses.
-int64_t padded_rank(int64_t r8) { return r8 <= 16 ? 16 : r8 <= 32 ? 32 : round_up(r8, kRankTile); }
-
-bool is16(int dtype) { return dtype == MIRL_DTYPE_BF16 || dtype == MIRL_DTYPE_F16; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 // f(E, NT) for the operand type and the rank tiles of min(r, 64) ranks.
 template <class F>
 void with_rank(int dtype, int64_t r8, F&& f) {
@@ -826,7 +920,8 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
                                  int64_t g_stride_b, int64_t g_stride_s, const int64_t* target, int64_t t_stride_b,
                                  int64_t t_stride_s, const float* row_stats, int64_t* perm, int32_t* adapter,
                                  int64_t* target_out, float* grad_rows, float* stats_out, int32_t* seg, int64_t* count,
-                                 int32_t* workspace, void* stream) {
+                                 const void* b, int dtype, int64_t b_elems, int32_t* bad, int32_t* workspace,
+                                 void* stream) {
   clear_error();
   MIRL_REQUIRE(B > 0 && N > 0 && R > 0, "invalid shape B=%lld N=%lld R=%lld", (long long)B, (long long)N, (long long)R);
   MIRL_REQUIRE(B < (int64_t(1) << 22) && N < (int64_t(1) << 22) && R < kMaxRows && B * R < kMaxRows,
@@ -834,12 +929,26 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
   MIRL_REQUIRE(ids && target && perm && adapter && target_out && seg && count && workspace, "null pointer argument");
   MIRL_REQUIRE((row_stats == nullptr) == (stats_out == nullptr) && (grad_out == nullptr) == (grad_rows == nullptr),
                "null pointer argument");
+  MIRL_REQUIRE(bad == nullptr || (b != nullptr && is16(dtype) && b_elems > 0 && b_elems % 8 == 0 && aligned16(b) &&
+                                  N * ceil_div(b_elems, 2048 * kScanVecs) < kMaxBlocks),
+               "adapters of %lld elements (dtype code %d) cannot be looked through", (long long)b_elems, dtype);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int32_t *cnt = workspace, *start = workspace + B;
   if (grad_out != nullptr)
     hipLaunchKernelGGL(adapter_count_kernel, dim3((unsigned)B), dim3(1024), 0, st, grad_out, g_stride_b, g_stride_s, R, cnt);
   hipLaunchKernelGGL(adapter_starts_kernel, dim3((unsigned)(N + 1)), dim3(1024), 0, st, ids, B, N, (int32_t)R,
-                     grad_out != nullptr ? cnt : nullptr, start, seg, count);
+                     grad_out != nullptr ? cnt : nullptr, start, seg, count, bad);
+  if (bad != nullptr) {
+    const int64_t vecs = b_elems / 8, per = ceil_div(vecs, 256 * kScanVecs);
+    auto scan = [&](auto e) {
+      hipLaunchKernelGGL(adapter_scan_kernel<decltype(e)>, dim3((unsigned)(N * per)), dim3(256), 0, st,
+                         static_cast<const vu4*>(b), vecs, per, seg, bad);
+    };
+    if (dtype == MIRL_DTYPE_BF16)
+      scan(BF16{});
+    else
+      scan(F16{});
+  }
   hipLaunchKernelGGL(adapter_fill_kernel, dim3((unsigned)B), dim3(1024), 0, st, ids, B, N, R, grad_out, g_stride_b,
                      g_stride_s, target, t_stride_b, t_stride_s, row_stats, start,
                      RowsOut{perm, adapter, target_out, grad_rows, stats_out});
@@ -847,12 +956,12 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
 }
 
 extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const int64_t* perm,
-                                 const int32_t* adapter, int64_t T, const void* a, int64_t r, int64_t lda, const float* scaling,
+                                 const int32_t* adapter, int64_t T, const void* a, int64_t N, int64_t r, int64_t lda, const float* scaling,
                                  double p, int64_t seed, const int64_t* seed_dev, int64_t offset, void* hidden_out,
                                  int64_t ldo, void* u_planes, int64_t r8, float* u_rows, void* stream) {
   clear_error();
   MIRL_REQUIRE(is16(dtype), "hidden states and adapters must be bf16 or fp16 (dtype code %d)", dtype);
-  MIRL_REQUIRE(T > 0 && T < kMaxRows && Hd > 0 && r > 0 && r8 >= r && r8 % 8 == 0 && r8 <= kMaxRank && ldh >= Hd &&
+  MIRL_REQUIRE(T > 0 && T < kMaxRows && Hd > 0 && N > 0 && r > 0 && r8 >= r && r8 % 8 == 0 && r8 <= kMaxRank && ldh >= Hd &&
                    ldo >= Hd && ldo % 8 == 0,
                "invalid shape T=%lld H=%lld r=%lld r8=%lld ldo=%lld", (long long)T, (long long)Hd, (long long)r,
                (long long)r8, (long long)ldo);
@@ -865,16 +974,22 @@ extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int6
                      static_cast<uint16_t*>(u_planes), r8, u_rows};
   with_rank(dtype, r8, [&](auto e, auto nt) {
     using E = decltype(e);
-    hipLaunchKernelGGL((adapter_down_kernel<E, decltype(nt)::value>),
-                       dim3((unsigned)ceil_div(T, 16), (unsigned)ceil_div(r8, kRankTile)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), P);
+    constexpr int NT = decltype(nt)::value;
+    // few rows: 16 waves share them, and workgroups their adapters, to have the loads of all in
+    // flight (64 rows of 16 adapters, H = 4096: 91 -> 13 us); many: four waves (113 us against
+    // 130 of [16384, 4096])
+    const dim3 grid((unsigned)ceil_div(T, 16), (unsigned)ceil_div(r8, kRankTile), T <= 2048 ? (unsigned)std::min(N, int64_t(16)) : 1u);
+    if (T <= 2048)
+      hipLaunchKernelGGL((adapter_down_kernel<E, NT, 16>), grid, dim3(1024), 0, static_cast<hipStream_t>(stream), P);
+    else
+      hipLaunchKernelGGL((adapter_down_kernel<E, NT, 4>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), P);
   });
   return check_launch("mirl_adapter_down");
 }
 
 extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, int64_t ldh, const void* weight,
                                    int64_t V, int64_t ldw, const int32_t* adapter, const void* u_planes, const void* b,
-                                   int64_t r8, const int64_t* perm, const int64_t* target_rows, int64_t bsz,
+                                   int64_t r8, int64_t N, const int32_t* bad, const int64_t* perm, const int64_t* target_rows, int64_t bsz,
                                    const int64_t* target, int64_t t_stride_b, int64_t t_stride_s, int64_t vocab_start,
                                    int64_t vocab_end, float* out, int64_t o_stride_b, int64_t o_stride_s,
                                    float* row_stats, float* workspace, void* stream) {
@@ -882,7 +997,7 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   if (int e = check_operands(dtype, hidden, Hd, ldh, weight, V, ldw)) return e;
   MIRL_REQUIRE(T > 0 && T < kMaxRows && bsz > 0 && r8 > 0 && r8 % 8 == 0 && r8 <= kMaxRank,
                "invalid shape T=%lld B=%lld r8=%lld", (long long)T, (long long)bsz, (long long)r8);
-  MIRL_REQUIRE(hidden && weight && adapter && u_planes && b && perm && target_rows && target && out && workspace,
+  MIRL_REQUIRE(N > 0 && hidden && weight && adapter && u_planes && b && bad && perm && target_rows && target && out && workspace,
                "null pointer argument");
   MIRL_REQUIRE(aligned16(u_planes) && aligned16(b), "the adapters must be 16-byte aligned");
   LceParams P{};
@@ -907,6 +1022,8 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   P.B = static_cast<const uint16_t*>(b);
   P.r8 = (int)r8;
   P.planes = kPlanes;
+  P.bad = bad;
+  P.b_bytes = N * V * r8 * 2;
   const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
   MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -961,14 +1078,14 @@ extern "C" int mirl_transpose16(const void* src, int64_t Z, int64_t src_z, int64
 
 extern "C" int mirl_adapter_ce_grad(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const void* weight, int64_t V,
                                     int64_t ldw, const int32_t* adapter, const void* u_planes, const void* b, int64_t r8,
-                                    const int64_t* target_rows, int64_t vocab_start, int64_t vocab_end,
+                                    int64_t N, const int32_t* bad, const int64_t* target_rows, int64_t vocab_start, int64_t vocab_end,
                                     const float* row_stats, int64_t row0, int64_t nrows, void* grad_logits, int64_t ldg,
                                     void* grad_logits_t, int64_t ldgt, const int64_t* row_count, void* stream) {
   clear_error();
   if (int e = check_operands(dtype, hidden, Hd, ldh, weight, V, ldw)) return e;
   MIRL_REQUIRE(row0 >= 0 && nrows > 0 && row0 + nrows < kMaxRows && r8 > 0 && r8 % 8 == 0 && r8 <= kMaxRank,
                "invalid shape row0=%lld rows=%lld r8=%lld", (long long)row0, (long long)nrows, (long long)r8);
-  MIRL_REQUIRE(hidden && weight && adapter && u_planes && b && target_rows && row_stats && grad_logits && grad_logits_t &&
+  MIRL_REQUIRE(N > 0 && hidden && weight && adapter && u_planes && b && bad && target_rows && row_stats && grad_logits && grad_logits_t &&
                    row_count,
                "null pointer argument");
   MIRL_REQUIRE(ldg >= V, "gradient row stride %lld is smaller than V=%lld", (long long)ldg, (long long)V);
@@ -1004,6 +1121,8 @@ extern "C" int mirl_adapter_ce_grad(const void* hidden, int dtype, int64_t Hd, i
   P.B = static_cast<const uint16_t*>(b);
   P.r8 = (int)r8;
   P.planes = kPlanes;
+  P.bad = bad;
+  P.b_bytes = N * V * r8 * 2;
   const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
   MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
   if (dtype == MIRL_DTYPE_BF16) {
@@ -1090,7 +1209,7 @@ extern "C" int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, cons
   MIRL_REQUIRE(count && perm && adapter && seg && grad_rows && scaling && grad_logits && b_t && a && u_rows && workspace &&
                    (db == nullptr || grad_logits_t) && (da == nullptr || hidden_t) && (dh == nullptr || h_part),
                "null pointer argument");
-  MIRL_REQUIRE(ldbt % 64 == 0 && ldg >= ldbt && ldbt >= V && ldg % 8 == 0 && aligned16(grad_logits) && aligned16(b_t) &&
+  MIRL_REQUIRE(ldbt % 128 == 0 && ldg >= ldbt && ldbt >= V && ldg % 8 == 0 && aligned16(grad_logits) && aligned16(b_t) &&
                    (db == nullptr || (ldgt >= round_up(n, 64) && ldgt % 8 == 0 && aligned16(grad_logits_t))) &&
                    (da == nullptr || (ldht >= row0 + round_up(n, 64) && ldht % 8 == 0 && row0 % 8 == 0 && aligned16(hidden_t))),
                "operand rows must be whole 16-byte pieces that cover the padded block");
@@ -1123,7 +1242,7 @@ extern "C" int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, cons
   P.U32 = u_rows;
   P.drop = dropout_args(p, seed, seed_dev, offset);
   P.splits = splits;
-  P.k_len = round_up(ceil_div(ldbt, splits), 64);
+  P.k_len = round_up(ceil_div(ldbt, splits), 128);
   P.du_part = static_cast<float*>(workspace);
   P.du = P.du_part + splits * n * r8;
   P.duT = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + round_up(block_floats(n, r8, splits) * 4, 256));

@@ -63,8 +63,8 @@ class _AdapterLogprobs(torch.autograd.Function):
         dev = hidden.device
         h2 = hidden.view(S * B, H)
         drop = _C.Dropped(*drop_args, dev)
-        rows = _C.AdapterRows(ids, a.shape[0], target)
         bk = _padded_last(b)
+        rows = _C.AdapterRows(ids, bk, target)
         h, planes, u = _C.adapter_down(h2, rows, _padded_last(a), scaling, drop, _round_up(H, _H_ALIGN), bk.shape[2], keep)
         out = torch.empty((B, R), dtype=torch.float32, device=dev)
         stats = torch.empty((R * B, 2), dtype=torch.float32, device=dev) if keep else None
@@ -72,14 +72,14 @@ class _AdapterLogprobs(torch.autograd.Function):
         if keep:
             p, seed, offset = drop_args
             seed_t = seed if isinstance(seed, torch.Tensor) else None
-            ctx.save_for_backward(hidden, a, b, weight, ids, scaling, target, stats, u, seed_t)
+            ctx.save_for_backward(hidden, a, b, weight, ids, scaling, target, stats, u, rows.bad, seed_t)
             ctx.rest = (vs, ve, chunk_size, (p, None if seed_t is not None else seed, offset))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad):  # type: ignore[override]
-        hidden, a, b, weight, ids, scaling, target, stats, u, seed_t = ctx.saved_tensors
+        hidden, a, b, weight, ids, scaling, target, stats, u, bad, seed_t = ctx.saved_tensors
         vs, ve, chunk_size, (p, seed, offset) = ctx.rest
         need_h, need_a, need_b = ctx.needs_input_grad[:3]
         S, B, H = hidden.shape
@@ -88,10 +88,10 @@ class _AdapterLogprobs(torch.autograd.Function):
         V = weight.shape[0]
         dev = hidden.device
         drop = _C.Dropped(p, seed if seed_t is None else seed_t, offset, dev)
-        rows = _C.AdapterRows(ids, N, target, grad, stats)
+        ak, bk, wk = _padded_last(a), _padded_last(b), _kernel_operand(weight)
+        rows = _C.AdapterRows(ids, bk, target, grad, stats, bad)
         h2 = hidden.view(S * B, H)
         h, planes = _C.adapter_gather(h2, rows, u, _round_up(H, _H_ALIGN))
-        ak, bk, wk = _padded_last(a), _padded_last(b), _kernel_operand(weight)
         Vp = _round_up(V, _K_ALIGN)
         n_rows = _block_rows(T, chunk_size, _BLOCK_CHUNKS * B, V)
         bT = torch.empty((N, bk.shape[2], Vp), dtype=b.dtype, device=dev)
