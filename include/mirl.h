@@ -964,9 +964,10 @@ int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
  *   x[r, v] = hidden_scale[r] * weight_scale[v] * sum_k hidden8[r, k] weight8[v, k]
  *   out     = log_softmax(x[r])[target - vocab_start], 0 for targets outside
  *             [vocab_start, vocab_end)
- * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, Hd]; Hd a
- * multiple of 256, row strides multiples of 16, 16-byte-aligned starts (zero
- * padding adds nothing).  out is [bsz, T / bsz] by strides; workspace as
+ * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, <= Hd]; Hd a
+ * multiple of 256, row strides multiples of 16, 16-byte-aligned starts.  Hidden
+ * rows are zero past the true size; the weight's need no padding (a row stride
+ * below Hd is allowed).  out is [bsz, T / bsz] by strides; workspace as
  * mirl_linear_ce_workspace_elems(T, V).
  */
 int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int64_t T,
@@ -1015,7 +1016,8 @@ int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, co
                       float* u_rows, void* stream);
 
 /* The logprobs of the T sorted rows (hidden, u_planes as mirl_adapter_down writes them; Hd a
- * multiple of 128) at their original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
+ * multiple of 128, zeros past the true size; the weight's row stride may be below Hd) at their
+ * original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
  * (or NULL).  target_rows: the sorted rows' targets; target [bsz, T / bsz] the original ones.
  * workspace: mirl_linear_ce_workspace_elems(T, V). */
 int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, int64_t ldh,

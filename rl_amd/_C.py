@@ -1618,14 +1618,15 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
                        vocab_end: int, out: torch.Tensor) -> None:
     """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd).
 
-    hidden8 [T, H] and weight8 [V, H] e4m3 (H a multiple of 256, rows multiples of 16 bytes),
+    hidden8 [T, H] and weight8 [V, H] e4m3 (H a multiple of 256, row strides of 16; the weight's rows may be
+    shorter where the hidden rows are zero past them),
     scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
     dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
     T, H = hidden8.shape
     V = weight8.shape[0]
     _require(hidden8.dtype == torch.float8_e4m3fn and weight8.dtype == torch.float8_e4m3fn, "e4m3 operands")
-    _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and weight8.shape[1] == H,
-             "operands of one hidden size with unit stride")
+    _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and weight8.shape[1] <= H,
+             "hidden rows that cover the weight's, with unit stride")
     _require(hidden_scale.is_contiguous() and hidden_scale.numel() == T and hidden_scale.dtype == torch.float32
              and weight_scale.is_contiguous() and weight_scale.numel() == V and weight_scale.dtype == torch.float32,
              "a contiguous fp32 scale per row")
@@ -1724,7 +1725,7 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
     T, H = h.shape
     V = weight.shape[0]
     _check_linear_ce(h, weight)
-    _require(weight.shape[1] == H and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
+    _require(weight.shape[1] <= H and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
              and planes.shape == (T, 2, b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
     lib = _lib if _lib is not None else load()
     ws = torch.empty(int(lib.mirl_linear_ce_workspace_elems(T, V)), dtype=torch.float32, device=dev)

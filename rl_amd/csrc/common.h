@@ -17,6 +17,18 @@ namespace mirl {
 // Native 16-byte vector (clang ext vector, usable with the nontemporal builtins).
 typedef uint32_t vu4 __attribute__((ext_vector_type(4)));
 
+// The same at any multiple of A bytes (the hardware takes 16-byte accesses unaligned).
+template <int A>
+struct Piece;
+template <>
+struct Piece<2> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct Piece<4> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+
 // ---------------------------------------------------------------------------
 // host-side error state
 // ---------------------------------------------------------------------------

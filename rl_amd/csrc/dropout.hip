@@ -17,24 +17,27 @@ constexpr int kV = 8;
 constexpr int kThreads = 256;
 
 template <class E>
-struct __attribute__((packed, aligned(alignof(typename E::raw)))) Pack {
-  typename E::raw e[kV];
-};
-
-template <class E>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const typename E::raw* x, int64_t n,
                                                            DropoutArgs D, typename E::raw* y) {
   const uint64_t seed = D.seed_of();
   for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q * kV < n; q += (int64_t)gridDim.x * kThreads) {
     const int64_t i = q * kV;
     if (i + kV <= n) {
-      const Pack<E> in = *reinterpret_cast<const Pack<E>*>(x + i);
-      const uint32_t keep = dropout_keep8(seed, D.offset, (uint64_t)q, D.threshold);
-      Pack<E> out;
+      // any alignment of an element, each used once
+      using piece = typename Piece<alignof(typename E::raw)>::type;
+      constexpr int kP = kV / E::kVec;
+      vu4 q4[kP];
 #pragma unroll
-      for (int e = 0; e < kV; ++e)
-        out.e[e] = E::from_float((keep >> e) & 1u ? E::load_raw(in.e[e]) * D.scale : 0.f);
-      *reinterpret_cast<Pack<E>*>(y + i) = out;
+      for (int k = 0; k < kP; ++k) q4[k] = __builtin_nontemporal_load(reinterpret_cast<const piece*>(x + i) + k);
+      const uint32_t keep = dropout_keep8(seed, D.offset, (uint64_t)q, D.threshold);
+#pragma unroll
+      for (int k = 0; k < kP; ++k) {
+        float v[E::kVec];
+        E::unpack(q4[k], v);
+#pragma unroll
+        for (int e = 0; e < E::kVec; ++e) v[e] = (keep >> (k * E::kVec + e)) & 1u ? v[e] * D.scale : 0.f;
+        __builtin_nontemporal_store((piece)E::pack(v), reinterpret_cast<piece*>(y + i) + k);
+      }
     } else {
       const uint32_t keep = dropout_keep8(seed, D.offset, (uint64_t)q, D.threshold);
       for (int e = 0; i + e < n; ++e)

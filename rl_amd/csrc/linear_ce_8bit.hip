@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float*
   const uint8_t* hr = static_cast<const uint8_t*>(P.h) + r * P.ldh;
   const uint8_t* wr = static_cast<const uint8_t*>(P.w) + (t - P.vs) * P.ldw;
   float dot[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t k = lane * 16; k < P.Hd; k += 64 * 16) {
+  for (int64_t k = lane * 16; k < (P.Hd < P.ldw ? P.Hd : P.ldw); k += 64 * 16) {
     const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const vu4*>(wr + k);
     const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w}, ww[4] = {wq.x, wq.y, wq.z, wq.w};
 #pragma unroll
@@ -102,9 +102,12 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   // buffer ranges of one 256-row tile are 32-bit byte counts
   MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22),
                "row strides (%lld, %lld) must be below 2^22 elements", (long long)ldh, (long long)ldw);
-  MIRL_REQUIRE(ldh % 16 == 0 && ldw % 16 == 0 && ldh >= Hd && ldw >= Hd,
-               "row strides (%lld, %lld) must be multiples of 16 elements and >= the hidden size", (long long)ldh,
-               (long long)ldw);
+  // The weight's rows may be shorter than Hd: what is read past a row's end is the next row's
+  // beginning, and zero past the last row's, against zeros of the hidden rows.  A NaN there
+  // stands in the next column's logits as well, so it changes no logprob.
+  MIRL_REQUIRE(ldh % 16 == 0 && ldw % 16 == 0 && ldh >= Hd && ldw > 0,
+               "row strides (%lld, %lld) must be multiples of 16 elements, the hidden states' >= the hidden size",
+               (long long)ldh, (long long)ldw);
   MIRL_REQUIRE(V < (int64_t(1) << 31) && T < (int64_t(1) << 31), "sizes exceed 2^31-1");
   if (T == 0) return MIRL_OK;
   MIRL_REQUIRE(hidden8 && hidden_scale && weight8 && weight_scale && target && out && workspace,

@@ -37,7 +37,7 @@ int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // A launch holds fewer than 2^32 threads.
 constexpr int64_t kMaxRows = int64_t(1) << 26, kMaxBlocks = int64_t(1) << 23;
-constexpr int64_t kMaxRank = 1024;  // a workgroup of adapter_dh_kernel holds eight rows of dU in LDS
+constexpr int64_t kMaxRank = 1024;  // a workgroup of adapter_dh_kernel holds its rows of dU in LDS
 // Ranks of the plane arrays: whole tiles of those that with_rank chooses.
 int64_t padded_rank(int64_t r8) { return r8 <= 16 ? 16 : r8 <= 32 ? 32 : round_up(r8, kRankTile); }
 
@@ -585,6 +585,7 @@ __global__ __launch_bounds__(256) void adapter_du_sum_kernel(BlockParams P) {
     float v = 0.f;
     const float g = P.g[P.row0 + m];
     if (a >= 0) {
+#pragma unroll 8
       for (int64_t s = 0; s < P.splits; ++s) v += P.du_part[(s * P.n + m) * P.r8 + rho];
       v *= (1.f / g_scale_of<E>()) * P.scaling[a];
       v *= g;
@@ -796,9 +797,9 @@ __global__ __launch_bounds__(kDaWaves * 64) void adapter_da_kernel(BlockParams P
   }
 }
 
-// dH of the block's rows: g (sum of the splits of G . W) + dropout'(dU . A_a), rounded once.  Eight
+// dH of the block's rows: g (sum of the splits of G . W) + dropout'(dU . A_a), rounded once.  Four
 // rows a workgroup, eight columns a thread; the rows' adapters one after the other.
-constexpr int kDhRows = 8;
+constexpr int kDhRows = 4;
 template <class E>
 __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
   extern __shared__ float du_s[];  // [kDhRows][r8]
@@ -839,26 +840,43 @@ __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
     cur = next;
   }
   const uint64_t seed = P.drop.threshold > 0 ? P.drop.seed_of() : 0;
+  // the splits' sums of all rows, their loads in flight together (rows past the block's end
+  // read its last one)
+  float sum[kDhRows][8];
+#pragma unroll
+  for (int i = 0; i < kDhRows; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[i][e] = 0.f;
+  const bool vec = full && P.H % 4 == 0;
+  for (int64_t s = 0; s < P.h_splits; ++s) {
+    const float* src = P.h_part + (s * P.n + m0) * P.H + c;
+    if (vec) {
+      float4 q[kDhRows][2];
+#pragma unroll
+      for (int i = 0; i < kDhRows; ++i) {
+        const float4* row = reinterpret_cast<const float4*>(src + (i < rows ? i : rows - 1) * P.H);
+        q[i][0] = row[0];
+        q[i][1] = row[1];
+      }
+#pragma unroll
+      for (int i = 0; i < kDhRows; ++i) {
+        sum[i][0] += q[i][0].x; sum[i][1] += q[i][0].y; sum[i][2] += q[i][0].z; sum[i][3] += q[i][0].w;
+        sum[i][4] += q[i][1].x; sum[i][5] += q[i][1].y; sum[i][6] += q[i][1].z; sum[i][7] += q[i][1].w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDhRows; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i < rows && c + e < P.H) sum[i][e] += src[i * P.H + e];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kDhRows; ++i) {
     if (i >= rows) break;
     const int64_t m = m0 + i, row = P.perm[P.row0 + m];
     const float g = P.g[P.row0 + m] * (1.f / g_scale_of<E>());
-    float o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    for (int64_t s = 0; s < P.h_splits; ++s) {
-      const float* src = P.h_part + (s * P.n + m) * P.H + c;
-      if (full && P.H % 4 == 0) {
-        const float4 q0 = *reinterpret_cast<const float4*>(src), q1 = *reinterpret_cast<const float4*>(src + 4);
-        o[0] += q0.x; o[1] += q0.y; o[2] += q0.z; o[3] += q0.w;
-        o[4] += q1.x; o[5] += q1.y; o[6] += q1.z; o[7] += q1.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < P.H) o[e] += src[e];
-      }
-    }
+    float (&o)[8] = sum[i];
     uint32_t keep = 0xffu;
     float ds = 1.f;
     if (P.drop.threshold > 0) {
@@ -899,13 +917,16 @@ void with_rank(int dtype, int64_t r8, F&& f) {
     go(F16{});
 }
 
+// (The weight's rows may be shorter than Hd: what the tile loop reads past a row's end is the next
+// row's beginning, and zero past the last row's, against zeros of the hidden rows.  An infinity or
+// a NaN there stands in the next column's logits as well, so it changes no logprob.)
 int check_operands(int dtype, const void* hidden, int64_t Hd, int64_t ldh, const void* weight, int64_t V, int64_t ldw) {
   MIRL_REQUIRE(is16(dtype), "hidden states, weight and adapters must be bf16 or fp16 (dtype code %d)", dtype);
   MIRL_REQUIRE(V > 0 && Hd > 0 && V < (int64_t(1) << 31), "invalid shape V=%lld H=%lld", (long long)V, (long long)Hd);
   MIRL_REQUIRE(Hd % (kStages * kSK) == 0, "hidden size %lld must be a multiple of %d", (long long)Hd, kStages * kSK);
   MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22) && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= Hd &&
-                   ldw >= Hd,
-               "row strides (%lld, %lld) must be multiples of 8 elements, >= the hidden size and below 2^22",
+                   ldw > 0,
+               "row strides (%lld, %lld) must be multiples of 8 elements, the hidden states' >= the hidden size, and below 2^22",
                (long long)ldh, (long long)ldw);
   MIRL_REQUIRE(aligned16(hidden) && aligned16(weight), "hidden states and weight must be 16-byte aligned");
   return MIRL_OK;

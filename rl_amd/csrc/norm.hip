@@ -20,26 +20,33 @@
 namespace mirl {
 namespace {
 
-// N elements of E from p, which is aligned to one element only (odd hidden sizes put rows
-// anywhere): one to two wide loads, the hardware takes them unaligned.
-template <class E, int N>
-struct __attribute__((packed, aligned(alignof(typename E::raw)))) Pack {
-  typename E::raw e[N];
-};
 constexpr int kV = 8;  // elements a lane handles together
 
+// Eight elements at p, which is aligned to one element only (odd hidden sizes put rows
+// anywhere): one or two 16-byte pieces, which the hardware takes unaligned.  Nontemporal:
+// each is used once.
 template <class E>
 __device__ __forceinline__ void load8(const typename E::raw* p, float (&v)[kV]) {
-  const Pack<E, kV> q = *reinterpret_cast<const Pack<E, kV>*>(p);
 #pragma unroll
-  for (int e = 0; e < kV; ++e) v[e] = E::load_raw(q.e[e]);
+  for (int i = 0; i < kV / E::kVec; ++i) {
+    using piece = typename Piece<alignof(typename E::raw)>::type;
+    const vu4 q = __builtin_nontemporal_load(reinterpret_cast<const piece*>(p) + i);
+    float w[E::kVec];
+    E::unpack(q, w);
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) v[i * E::kVec + e] = w[e];
+  }
 }
 template <class E>
 __device__ __forceinline__ void store8(typename E::raw* p, const float (&v)[kV]) {
-  Pack<E, kV> q;
 #pragma unroll
-  for (int e = 0; e < kV; ++e) q.e[e] = E::from_float(v[e]);
-  *reinterpret_cast<Pack<E, kV>*>(p) = q;
+  for (int i = 0; i < kV / E::kVec; ++i) {
+    using piece = typename Piece<alignof(typename E::raw)>::type;
+    float w[E::kVec];
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) w[e] = v[i * E::kVec + e];
+    __builtin_nontemporal_store((piece)E::pack(w), reinterpret_cast<piece*>(p) + i);
+  }
 }
 // Elements c .. c + 7 of a row of H, zeros past its end.
 template <class E>

@@ -21,11 +21,12 @@ __all__ = ["from_parallel_8bit_hidden_states_to_logprobs"]
 _H_ALIGN = 256  # the kernel steps through the hidden dimension 256 elements at a time
 
 
-def _operand8(x: torch.Tensor) -> torch.Tensor:
-    """``x [N, H]`` e4m3 as the kernel reads it: ``H`` a multiple of 256, row strides multiples of
-    16, a 16-byte-aligned start; otherwise a zero-padded copy (the padding adds exact zeros)."""
+def _operand8(x: torch.Tensor, whole: bool) -> torch.Tensor:
+    """``x [N, H]`` e4m3 as the kernel reads it: row strides multiples of 16, a 16-byte-aligned
+    start, and with ``whole`` (the hidden states) ``H`` a multiple of 256; otherwise a zero-padded
+    copy (the padding adds exact zeros)."""
     N, H = x.shape
-    if (H % _H_ALIGN == 0 and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
+    if ((not whole or H % _H_ALIGN == 0) and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
             and x.data_ptr() % 16 == 0):
         return x
     out = torch.zeros((N, -(-H // _H_ALIGN) * _H_ALIGN), dtype=torch.uint8, device=x.device)
@@ -49,8 +50,9 @@ def from_parallel_8bit_hidden_states_to_logprobs(
 
     ``target`` ``[B, S]`` is shifted by one position, as in the 16-bit form; the last position,
     which has no next token, is not computed.  Targets outside ``[vocab_start_index,
-    vocab_end_index)`` give 0.  There is no gradient.  Hidden sizes that are not a multiple of
-    256 (or unaligned rows) are copied into padded buffers in every call."""
+    vocab_end_index)`` give 0.  There is no gradient.  Hidden states whose size is not a
+    multiple of 256, and a weight whose rows are not 16-byte aligned, are copied into padded
+    buffers in every call."""
     from rl_amd.distributed.model_utils import _group_size, _require_single_rank
 
     _require_single_rank(tp_group)
@@ -77,8 +79,8 @@ def from_parallel_8bit_hidden_states_to_logprobs(
         return out
     if target.dtype != torch.int64:
         target = target.long()
-    rows = _operand8(h8[:R].reshape(R * B, H))
-    _C.linear_ce_8bit_fwd(rows, hidden_scales[:R].reshape(-1).contiguous(), _operand8(w8),
+    rows = _operand8(h8[:R].reshape(R * B, H), True)
+    _C.linear_ce_8bit_fwd(rows, hidden_scales[:R].reshape(-1).contiguous(), _operand8(w8, False),
                           output_weight_scales.contiguous(), B, target[:, 1:], vocab_start_index,
                           vocab_end_index, out)
     return out

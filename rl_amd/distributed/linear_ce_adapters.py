@@ -41,7 +41,7 @@ from rl_amd.distributed.linear_ce import (
 __all__ = ["from_parallel_hidden_states_to_logprobs_with_adapters"]
 
 _MAX_RANK = 1024
-_DU_WAVES = 4096  # waves that dU's product is split into: four per SIMD
+_DU_WAVES = 16384  # waves that dU's product is split into (half of them past the active rows)
 
 
 def _padded_last(x: torch.Tensor) -> torch.Tensor:
@@ -51,6 +51,12 @@ def _padded_last(x: torch.Tensor) -> torch.Tensor:
     out = torch.zeros((*x.shape[:2], _round_up(x.shape[2], 8)), dtype=x.dtype, device=x.device)
     out[:, :, : x.shape[2]].copy_(x)
     return out
+
+
+def _weight_operand(w: torch.Tensor) -> torch.Tensor:
+    """``w [V, H]`` as the tile loop reads it against zero-padded hidden rows: row strides multiples
+    of 8 and a 16-byte-aligned start, or a padded copy."""
+    return w if w.stride(0) % 8 == 0 and w.stride(0) >= w.shape[1] and w.data_ptr() % 16 == 0 else _kernel_operand(w)
 
 
 class _AdapterLogprobs(torch.autograd.Function):
@@ -68,7 +74,7 @@ class _AdapterLogprobs(torch.autograd.Function):
         h, planes, u = _C.adapter_down(h2, rows, _padded_last(a), scaling, drop, _round_up(H, _H_ALIGN), bk.shape[2], keep)
         out = torch.empty((B, R), dtype=torch.float32, device=dev)
         stats = torch.empty((R * B, 2), dtype=torch.float32, device=dev) if keep else None
-        _C.adapter_ce_fwd(h, _kernel_operand(weight), rows, planes, bk, target, vs, ve, out, stats)
+        _C.adapter_ce_fwd(h, _weight_operand(weight), rows, planes, bk, target, vs, ve, out, stats)
         if keep:
             p, seed, offset = drop_args
             seed_t = seed if isinstance(seed, torch.Tensor) else None
@@ -88,7 +94,7 @@ class _AdapterLogprobs(torch.autograd.Function):
         V = weight.shape[0]
         dev = hidden.device
         drop = _C.Dropped(p, seed if seed_t is None else seed_t, offset, dev)
-        ak, bk, wk = _padded_last(a), _padded_last(b), _kernel_operand(weight)
+        ak, bk, wk = _padded_last(a), _padded_last(b), _weight_operand(weight)
         rows = _C.AdapterRows(ids, bk, target, grad, stats, bad)
         h2 = hidden.view(S * B, H)
         h, planes = _C.adapter_gather(h2, rows, u, _round_up(H, _H_ALIGN))
