@@ -1505,12 +1505,21 @@ def seq_logprob_errors(policy: torch.Tensor, generation: torch.Tensor, token_mas
 # ---------------------------------------------------------------------------
 # the policy head: final norm, 8-bit rows, dropout
 # ---------------------------------------------------------------------------
-def _rows2(t: torch.Tensor) -> torch.Tensor:
-    """``t [..., H]`` as ``[R, H]`` rows of unit stride and one row stride of at least H
-    (a copy where its layout is another)."""
+def _rows2(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [..., H]`` as rows of unit stride and one row stride of at least H (a copy where its
+    layout is another), and that row stride."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     t2 = t.reshape(-1, t.shape[-1])
     ok = (t2.stride(1) == 1 or t2.shape[1] == 1) and (t2.stride(0) >= t2.shape[1] or t2.shape[0] <= 1)
-    return t2 if ok else t2.contiguous()
+    return (t2, t2.stride(0)) if ok else (t2.contiguous(), t2.shape[1])
+
+
+def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of t's shape."""
+    if t.dtype == dtype and t.is_contiguous():
+        return torch.empty_like(t)
+    return t.new_empty(t.shape, dtype=dtype)
 
 
 def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
@@ -1518,22 +1527,24 @@ def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     """(y, h, rstd or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
     itself without a residual, rstd and scale have a row's shape."""
     dev = _require_gpu(x, residual, weight)
-    H = x.shape[-1]
+    shape = x.shape
+    H = shape[-1]
     _require(weight.dim() == 1 and weight.shape[0] == H, "a weight per element of a row")
-    x2 = _rows2(x)
-    r2 = None if residual is None else _rows2(residual)
-    R = x2.shape[0]
+    x2, ldx = _rows2(x)
     weight = weight.contiguous()
-    h = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=dev)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if out8 else x.dtype, device=dev)
-    lead = x.shape[:-1]
-    scale = torch.empty(lead, dtype=torch.float32, device=dev) if out8 else None
-    rstd = torch.empty(lead, dtype=torch.float32, device=dev) if want_rstd else None
+    if residual is None:
+        h, r_ptr, ldr, h_ptr, h_code = x, None, 0, None, _dtype_code(x)
+    else:
+        _require(residual.shape == shape, "a residual of the rows' shape")
+        r2, ldr = _rows2(residual)
+        h = _new_like(residual, residual.dtype)
+        r_ptr, h_ptr, h_code = r2.data_ptr(), h.data_ptr(), _dtype_code(residual)
+    y = _new_like(x, torch.float8_e4m3fn if out8 else x.dtype)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32) if out8 else None
+    rstd = x.new_empty(shape[:-1], dtype=torch.float32) if want_rstd else None
     st = _launch(
-        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), _dtype_code(x), x2.stride(0), _ptr(r2),
-        _dtype_code(x if residual is None else residual), 0 if r2 is None else r2.stride(0), weight.data_ptr(),
-        _dtype_code(weight), R, H, float(eps), None if residual is None else h.data_ptr(), y.data_ptr(),
-        _ptr(scale), _ptr(rstd), _stream(dev),
+        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), _dtype_code(x), ldx, r_ptr, h_code, ldr, weight.data_ptr(),
+        _dtype_code(weight), x.numel() // H, H, float(eps), h_ptr, y.data_ptr(), _ptr(scale), _ptr(rstd), _stream(dev),
     )
     _check(st, "mirl_add_rms_norm_fwd")
     return y, h, rstd, scale
@@ -1545,16 +1556,17 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
     the same (see mirl_add_rms_norm_bwd)."""
     dev = _require_gpu(dy, dh_out, h, rstd, weight)
     H = h.shape[-1]
+    R = h.numel() // H
     _require(dy.shape == h.shape and rstd.is_contiguous() and rstd.dtype == torch.float32
-             and rstd.numel() * H == h.numel(), "gradients and row statistics of the rows")
+             and rstd.numel() == R and weight.numel() == H, "gradients and row statistics of the rows")
     _require(dh_out is None or (dh_out.shape == h.shape and dh_out.dtype == h.dtype), "the stream's gradient has its type")
-    dy2, h2 = _rows2(dy), _rows2(h)
-    g2 = None if dh_out is None else _rows2(dh_out)
-    R = h2.shape[0]
+    dy2, lddy = _rows2(dy)
+    h2, ldh = _rows2(h)
+    g2, ldg = (None, 0) if dh_out is None else _rows2(dh_out)
     weight = weight.contiguous()
     one = need_x and need_res and dy.dtype == h.dtype
-    dx = torch.empty(h.shape, dtype=dy.dtype, device=dev) if need_x else None
-    dres = torch.empty(h.shape, dtype=h.dtype, device=dev) if need_res and not one else None
+    dx = _new_like(h, dy.dtype) if need_x else None
+    dres = _new_like(h, h.dtype) if need_res and not one else None
     dw = ws = None
     if need_w:
         if R == 0:
@@ -1562,12 +1574,11 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
         else:
             dw = torch.empty_like(weight)
             lib = _lib if _lib is not None else load()
-            ws = torch.empty(int(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)), dtype=torch.float32, device=dev)
+            ws = h.new_empty(int(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)), dtype=torch.float32)
     st = _launch(
-        "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), dy2.stride(0), _ptr(g2),
-        0 if g2 is None else g2.stride(0), h2.data_ptr(), _dtype_code(h), h2.stride(0), rstd.data_ptr(),
-        weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres), None if ws is None else dw.data_ptr(),
-        _ptr(ws), _stream(dev),
+        "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), lddy, _ptr(g2), ldg, h2.data_ptr(), _dtype_code(h),
+        ldh, rstd.data_ptr(), weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres),
+        None if ws is None else dw.data_ptr(), _ptr(ws), _stream(dev),
     )
     _check(st, "mirl_add_rms_norm_bwd")
     return dx, (dx if one else dres), dw
@@ -1576,11 +1587,12 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(e4m3 rows, fp32 scales) of ``x [..., H]`` (see mirl_quantize_rows)."""
     dev = _require_gpu(x)
-    x2 = _rows2(x)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    st = _launch("mirl_quantize_rows", dev, x2.data_ptr(), _dtype_code(x), x2.stride(0), x2.shape[0], x2.shape[1],
-                 y.data_ptr(), scale.data_ptr(), _stream(dev))
+    H = x.shape[-1]
+    x2, ldx = _rows2(x)
+    y = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    st = _launch("mirl_quantize_rows", dev, x2.data_ptr(), _dtype_code(x), ldx, x.numel() // H, H, y.data_ptr(),
+                 scale.data_ptr(), _stream(dev))
     _check(st, "mirl_quantize_rows")
     return y, scale
 
@@ -1605,7 +1617,7 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
     """Dropout of ``x`` in its logical element order (see mirl_dropout); a new contiguous tensor."""
     dev = _require_gpu(x)
     x = x.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x)
     value, ptr = _seed_args(seed, dev)
     st = _launch("mirl_dropout", dev, x.data_ptr(), _dtype_code(x), x.numel(), float(p), value, ptr,
                  _signed64(offset), y.data_ptr(), _stream(dev))
