@@ -967,9 +967,10 @@ int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
  * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, <= Hd]; Hd a
  * multiple of 256, row strides multiples of 16, 16-byte-aligned starts.  Hidden
  * rows are zero past the true size; the weight's need no padding (a row stride
- * below Hd is allowed).  out is [bsz, T / bsz] by strides; workspace as
- * mirl_linear_ce_workspace_elems(T, V).
+ * below Hd is allowed).  out is [bsz, T / bsz] by strides; workspace:
+ * mirl_lce_x_workspace_elems(T, V) floats.
  */
+int64_t mirl_lce_x_workspace_elems(int64_t T, int64_t V);
 int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int64_t T,
                             int64_t Hd, int64_t ldh, const void* weight8,
                             const float* weight_scale, int64_t V, int64_t ldw, int64_t bsz,
@@ -1019,7 +1020,7 @@ int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, co
  * multiple of 128, zeros past the true size; the weight's row stride may be below Hd) at their
  * original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
  * (or NULL).  target_rows: the sorted rows' targets; target [bsz, T / bsz] the original ones.
- * workspace: mirl_linear_ce_workspace_elems(T, V). */
+ * workspace: mirl_lce_x_workspace_elems(T, V) floats. */
 int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, int64_t ldh,
                         const void* weight, int64_t V, int64_t ldw, const int32_t* adapter,
                         const void* u_planes, const void* b, int64_t r8, int64_t N,

@@ -263,6 +263,7 @@ SIGNATURES = {
         _I, [_P, _I, _I64, _P, _I64, _P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]
     ),
     "mirl_quantize_rows": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "mirl_lce_x_workspace_elems": (_I64, [_I64, _I64]),
     "mirl_linear_ce_8bit_fwd": (
         _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
     ),
@@ -1645,7 +1646,7 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
     _require(target.dtype == torch.int64 and out.dtype == torch.float32
              and tuple(target.shape) == tuple(out.shape) == (bsz, T // bsz), "int64 targets and fp32 logprobs [B, S]")
     lib = _lib if _lib is not None else load()
-    ws = torch.empty(max(1, int(lib.mirl_linear_ce_workspace_elems(T, V))), dtype=torch.float32, device=dev)
+    ws = torch.empty(max(1, int(lib.mirl_lce_x_workspace_elems(T, V))), dtype=torch.float32, device=dev)
     st = _launch(
         "mirl_linear_ce_8bit_fwd", dev, hidden8.data_ptr(), hidden_scale.data_ptr(), T, H, hidden8.stride(0),
         weight8.data_ptr(), weight_scale.data_ptr(), V, weight8.stride(0), int(bsz), target.data_ptr(), target.stride(0),
@@ -1740,7 +1741,7 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
     _require(weight.shape[1] <= H and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
              and planes.shape == (T, 2, b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
     lib = _lib if _lib is not None else load()
-    ws = torch.empty(int(lib.mirl_linear_ce_workspace_elems(T, V)), dtype=torch.float32, device=dev)
+    ws = torch.empty(int(lib.mirl_lce_x_workspace_elems(T, V)), dtype=torch.float32, device=dev)
     st = _launch(
         "mirl_adapter_ce_fwd", dev, h.data_ptr(), _dtype_code(h), T, H, h.stride(0), weight.data_ptr(), V, weight.stride(0),
         rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2], b.shape[0], rows.bad.data_ptr(), rows.perm.data_ptr(), rows.target.data_ptr(),

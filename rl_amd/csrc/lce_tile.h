@@ -1150,6 +1150,284 @@ void lce_tile_kernel(LceParams P) {
   }  // the fused epilogues
 }
 
+// ---------------------------------------------------------------------------
+// few rows (kFwdX): 64 rows x 128 columns per workgroup
+// ---------------------------------------------------------------------------
+// With few rows the forward is bound by reading W once, and a 256-row tile spends its time on
+// rows that are not there.  Here a stage is 64 rows of H (from L2) and 128 of W, three stages
+// of 24 KB in a ring with two in flight, two workgroups a CU: 64 KB of W on the way to each CU.
+// Wave w owns columns 32 w .. 32 w + 31 of the 64 rows.  Logits of 64 rows, H = 4096, V = 151936:
+// (measured below)
+constexpr int kRM = 64, kRN = 128, kRStages = 3;
+constexpr int kRStageBytes = (kRM + kRN) * kRowBytes;          // 24 KB: the H rows, then W's
+constexpr int kRLoadsA = kRM / kDmaRows / kWaves, kRLoadsB = kRN / kDmaRows / kWaves;  // per wave and stage
+
+template <class E>
+__global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
+  using frag = typename Mma<E>::frag;
+  using acc_t = typename Mma<E>::acc_t;
+  constexpr int kT = Mma<E>::kT, kTM = kRM / kT, kTN = kRN / kWaves / kT, kAV = kT * kT / kWave;
+  constexpr int kES = (int)sizeof(typename E::raw), kSKE = kRowBytes / kES;
+  constexpr int kFC = (int)sizeof(frag) / 16;
+  constexpr int kKK = kRowBytes / (kWave / kT * (int)sizeof(frag));
+  constexpr bool kAdapters = kES == 2;
+  constexpr int kOut = -0x7fffffff - 1;  // an offset out of range: reads as zero
+  __shared__ __align__(1024) unsigned char st0[kRStageBytes];
+  __shared__ __align__(1024) unsigned char st1[kRStageBytes];
+  __shared__ __align__(1024) unsigned char st2[kRStageBytes];
+  __shared__ int s_tcol[kRM], s_ord[kRM], s_seg[kRM], s_bad[kRM];
+  __shared__ float s_rs[kRM], s_m[kWaves][kRM], s_sum[kWaves][kRM];
+  __shared__ __align__(16) float s_cs[kES == 1 ? kRN : 4];
+  auto stage_ptr = [&](int s) -> unsigned char* { return s == 0 ? st0 : s == 1 ? st1 : st2; };
+
+  // one XCD takes neighbouring column tiles, all row tiles of one after the other
+  const int64_t n_mt = (P.nrows + kRM - 1) / kRM, n_nt = (P.V + kRN - 1) / kRN, ntiles = n_mt * n_nt;
+  const int64_t per_xcd = (ntiles + kXcds - 1) / kXcds;
+  const int64_t gi = (int64_t)(blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds;
+  if ((int64_t)(blockIdx.x / kXcds) >= per_xcd || gi >= ntiles) return;
+  const int64_t nt = uniform(gi / n_mt), mt = uniform(gi - gi / n_mt * n_mt);
+  const int64_t m0 = mt * kRM, n0 = nt * kRN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const int a_rows = (int)(P.nrows - m0 < kRM ? P.nrows - m0 : kRM);
+  const int b_rows = (int)(P.V - n0 < kRN ? P.V - n0 : kRN);
+
+  int n_seg = 0;
+  bool apart = false;
+  if (wave == 0) {
+    const int64_t r = m0 + lane;
+    int tc = -1, a = -1, before = -1;
+    if (lane < a_rows) {
+      const int64_t s = r / P.bsz, b = r - s * P.bsz;
+      const int64_t t = P.target[b * P.tsb + s * P.tss];
+      if (!((t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V))) {
+        const int64_t c = t - P.vs - n0;
+        if (c >= 0 && c < kRN) tc = (int)c;
+      }
+      if constexpr (kAdapters) {
+        a = P.aid[r];
+        before = lane > 0 ? P.aid[r - 1] : -1;
+      }
+      if constexpr (kES == 1) s_rs[lane] = P.row_scale[r];
+    } else if constexpr (kES == 1) {
+      s_rs[lane] = 0.f;
+    }
+    s_tcol[lane] = tc;
+    if constexpr (kAdapters) {
+      const bool head = a >= 0 && (lane == 0 || a != before);
+      const uint64_t heads = __ballot(head);
+      const int at = (int)__popcll(heads & (~0ull >> (63 - lane)));  // heads up to this row
+      s_ord[lane] = a >= 0 ? at - 1 : -1;
+      if (head) {
+        s_seg[at - 1] = a;
+        s_bad[at - 1] = P.bad[a];
+      }
+      if (lane == 0) s_m[0][0] = __int_as_float((int)__popcll(heads));
+    }
+  }
+  if constexpr (kES == 1) {
+    if (tid >= kWave && tid - kWave < kRN) s_cs[tid - kWave] = tid - kWave < b_rows ? P.col_scale[n0 + tid - kWave] : 0.f;
+  }
+  __syncthreads();
+  if constexpr (kAdapters) {
+    n_seg = __builtin_amdgcn_readfirstlane(__float_as_int(s_m[0][0]));
+    apart = __syncthreads_or(tid < n_seg && s_bad[tid] != 0) != 0 || P.b_bytes >= (int64_t(1) << 31);
+  }
+
+  const int nst = (int)(P.Hd / kSKE);
+  const int cpp = kAdapters ? P.r8 >> 3 : 1, cps = kAdapters ? P.planes * cpp : 1;
+  const int n_ext = (n_seg * cps + 7) >> 3;
+  const int total = apart ? nst : nst + n_ext;
+  __amdgpu_buffer_rsrc_t rsrc_a = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(P.h) + m0 * P.ldh * kES), 0, (int)(a_rows * P.ldh * kES), 0x00020000);
+  __amdgpu_buffer_rsrc_t rsrc_b = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(P.w) + n0 * P.ldw * kES), 0, (int)(b_rows * P.ldw * kES), 0x00020000);
+  int voff_a[kRLoadsA], voff_b[kRLoadsB];
+#pragma unroll
+  for (int i = 0; i < kRLoadsA; ++i) {
+    const int row = (wave * kRLoadsA + i) * kDmaRows + (lane >> 3);
+    voff_a[i] = (int)(row * P.ldh * kES) + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < kRLoadsB; ++i) {
+    const int row = (wave * kRLoadsB + i) * kDmaRows + (lane >> 3);
+    voff_b[i] = (int)(row * P.ldw * kES) + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+  }
+  // the loads of stage data t (past the last one: zeros, so that the count in flight stays)
+  auto dma = [&](unsigned char* stage, int t) __attribute__((always_inline)) {
+    const int soff = t < nst ? t * kRowBytes : 0;
+#pragma unroll
+    for (int i = 0; i < kRLoadsA; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(stage + (wave_u * kRLoadsA + i) * kDmaBytes), 16,
+                                               voff_a[i], soff, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kRLoadsB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc_b, (lds_ptr_t)(stage + kRM * kRowBytes + (wave_u * kRLoadsB + i) * kDmaBytes), 16, voff_b[i], soff, 0, 0);
+  };
+  // offsets of stage data t >= nst (see lce_tile_kernel)
+  auto prepare = [&](int t) __attribute__((always_inline)) {
+    if constexpr (kAdapters) {
+      rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(P.planes * P.r8)), 0,
+                                                 a_rows * P.planes * P.r8 * 2, 0x00020000);
+      rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.B + n0 * P.r8), 0,
+                                                 (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
+    }
+    auto place = [&](int row, int& seg, int& rem) {
+      const int x = (t - nst) * 8 + ((lane & 7) ^ ((row >> 1) & 7));
+      seg = x / cps;
+      rem = x - seg * cps;
+    };
+#pragma unroll
+    for (int i = 0; i < kRLoadsA; ++i) {
+      const int row = (wave * kRLoadsA + i) * kDmaRows + (lane >> 3);
+      int seg, rem;
+      place(row, seg, rem);
+      voff_a[i] = kAdapters && t < total && s_ord[row] == seg ? (row * P.planes * P.r8 + rem * 8) * 2 : kOut;
+    }
+#pragma unroll
+    for (int i = 0; i < kRLoadsB; ++i) {
+      const int row = (wave * kRLoadsB + i) * kDmaRows + (lane >> 3);
+      int seg, rem;
+      place(row, seg, rem);
+      voff_b[i] = kAdapters && t < total && seg < n_seg && row < b_rows
+                      ? (s_seg[seg] * (int)P.V * P.r8 + rem % cpp * 8 + row * P.r8) * 2
+                      : kOut;
+    }
+  };
+
+  const int frow = lane & (kT - 1);
+  int frag_off[kKK];
+#pragma unroll
+  for (int kk = 0; kk < kKK; ++kk) frag_off[kk] = lds_off(frow, (kk * (kWave / kT) + lane / kT) * kFC);
+  acc_t acc[kTM][kTN];
+#pragma unroll
+  for (int i = 0; i < kTM; ++i)
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+#pragma unroll
+      for (int v = 0; v < kAV; ++v) acc[i][j][v] = 0.f;
+  auto fread = [&](const unsigned char* base, int kk) __attribute__((always_inline)) {
+    if constexpr (kFC == 1) {
+      return *reinterpret_cast<const frag*>(base + frag_off[kk]);
+    } else {
+      const vu4 a = *reinterpret_cast<const vu4*>(base + frag_off[kk]);
+      const vu4 b = *reinterpret_cast<const vu4*>(base + (frag_off[kk] ^ 16));
+      return frag{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+    }
+  };
+  auto compute = [&](const unsigned char* stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) {
+      frag fa[kTM], fb[kTN];
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) fb[j] = fread(stage + (kRM + wave * (kRN / kWaves) + j * kT) * kRowBytes, kk);
+#pragma unroll
+      for (int i = 0; i < kTM; ++i) fa[i] = fread(stage + i * kT * kRowBytes, kk);
+#pragma unroll
+      for (int i = 0; i < kTM; ++i)
+#pragma unroll
+        for (int j = 0; j < kTN; ++j) acc[i][j] = Mma<E>::run(fb[j], fa[i], acc[i][j]);
+    }
+  };
+  // Stage t: this wave's loads of it have landed when only those of t + 1 are in flight; past
+  // the barrier everyone's have, and everyone has read stage t - 1, whose place t + 2 takes.
+  auto step = [&](int t, auto s_c) __attribute__((always_inline)) {
+    constexpr int S = decltype(s_c)::value;
+    if (t + 2 >= nst) prepare(t + 2);
+    wait_vm_barrier<kRLoadsA + kRLoadsB>();
+    dma(stage_ptr((S + 2) % kRStages), t + 2);
+    compute(stage_ptr(S));
+  };
+  dma(st0, 0);
+  dma(st1, 1);
+  for (int t = 0; t < total; t += kRStages) {
+    step(t, std::integral_constant<int, 0>{});
+    step(t + 1, std::integral_constant<int, 1>{});
+    step(t + 2, std::integral_constant<int, 2>{});
+  }
+  wait_vm_barrier<0>();
+  if constexpr (kAdapters) {
+    // an adapter holds a value that is none (its rows become NaN, the others must not meet it),
+    // or B passes 2 GiB: the adapters' part by itself
+    if (apart) {
+      for (int e = 0; e < n_ext; ++e) {
+        const int chunk = tid & 7, x = e * 8 + chunk, q = x / cps, rem = x - q * cps;
+        const bool any = q < n_seg;
+        const uint16_t* bp = P.B + ((int64_t)(any ? s_seg[q] : 0) * P.V + n0) * P.r8 + rem % cpp * 8;
+        constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
+        for (int row = tid >> 3; row < kRN; row += kThreads / 8) {
+          vu4 u = {0u, 0u, 0u, 0u}, b = {0u, 0u, 0u, 0u};
+          if (any && row < b_rows) b = *reinterpret_cast<const vu4*>(bp + (int64_t)row * P.r8);
+          bool none = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) none |= (b[j] & ex) == ex || ((b[j] >> 16) & ex) == ex;
+          if (none) b = vu4{0u, 0u, 0u, 0u};
+          *reinterpret_cast<vu4*>(st0 + kRM * kRowBytes + lds_off(row, chunk)) = b;
+          if (row < kRM) {
+            if (any && s_ord[row] == q)
+              u = *reinterpret_cast<const vu4*>(P.U + (m0 + row) * (int64_t)(P.planes * P.r8) + rem * 8);
+            *reinterpret_cast<vu4*>(st0 + lds_off(row, chunk)) = u;
+          }
+        }
+        __syncthreads();
+        compute(st0);
+        __syncthreads();
+      }
+    }
+  }
+
+  // ---- epilogue: the rows reduced in the registers, the four waves joined through LDS ----
+  const int col_lane = lane / kT * 4;
+#pragma unroll
+  for (int i = 0; i < kTM; ++i) {
+    const int rl = i * kT + frow, tc = s_tcol[rl] - wave * (kRN / kWaves);
+    float M = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+#pragma unroll
+      for (int v = 0; v < kAV; ++v) {
+        const int c = j * kT + v / 4 * 8 + col_lane + v % 4;
+        float x = acc[i][j][v];
+        if constexpr (kES == 1) x = (x * s_cs[wave * (kRN / kWaves) + c]) * s_rs[rl];
+        if (wave * (kRN / kWaves) + c >= b_rows) x = -INFINITY;
+        if (c == tc) P.xt[m0 + rl] = x;
+        acc[i][j][v] = x;
+        M = fmaxf(M, x);
+      }
+#pragma unroll
+    for (int off = kT; off < kWave; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, kWave));
+    float sum = 0.f;
+    if (M != -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int v = 0; v < kAV; ++v) sum += fast_exp2((acc[i][j][v] - M) * kLog2e);
+    }
+#pragma unroll
+    for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+    if (lane < kT) {
+      s_m[wave][rl] = M;
+      s_sum[wave][rl] = sum;
+    }
+  }
+  __syncthreads();
+  if (tid < a_rows) {
+    float M = s_m[0][tid], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][tid]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      if (s_m[w][tid] != -INFINITY) sum += s_sum[w][tid] * fast_exp2((s_m[w][tid] - M) * kLog2e);
+    if constexpr (kAdapters) {
+      if (s_ord[tid] >= 0 && s_bad[s_ord[tid]] != 0) sum = __builtin_nanf("");
+    }
+    float* dst = P.part + ((m0 + tid) * n_nt + nt) * 2;
+    dst[0] = M;
+    dst[1] = sum;
+  }
+}
+
 // Per row: combine the column-tile partials into the row's max and log-sum-exp,
 // then logprob = (x_t - max) - logsum (0 for targets outside the slice).
 // One wave per row; with `perm` the partials' row r is row perm[r] of targets and results.
@@ -1188,6 +1466,25 @@ __global__ __launch_bounds__(256) void lce_merge_kernel(
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The forward kernel with fp32 logits for T rows (P.part, P.xt not set yet: `workspace` holds
+// mirl_lce_x_workspace_elems(T, V) floats).  Returns the number of tiles.
+constexpr int64_t kFewRows = 128;  // rows up to which lce_rows_kernel is taken
+template <class E>
+int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
+  const bool few = P.nrows <= kFewRows;
+  P.n_mt = ceil_div(P.nrows, few ? kRM : kBM);
+  P.n_nt = ceil_div(P.V, few ? kRN : kBN);
+  P.part = workspace;
+  P.xt = workspace + P.nrows * P.n_nt * 2;
+  const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
+  if (grid >= (int64_t(1) << 24)) return grid;  // a launch holds fewer than 2^32 threads
+  if (few)
+    hipLaunchKernelGGL(lce_rows_kernel<E>, dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  else
+    hipLaunchKernelGGL((lce_tile_kernel<kFwdX, E>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  return grid;
+}
 
 }  // namespace
 }  // namespace mirl

@@ -88,6 +88,11 @@ __global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float*
 
 using namespace mirl;
 
+extern "C" int64_t mirl_lce_x_workspace_elems(int64_t T, int64_t V) {
+  if (T <= 0 || V <= 0) return 0;
+  return T * ceil_div(V, T <= kFewRows ? kRN : kBN) * 2 + T;
+}
+
 extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int64_t T, int64_t Hd,
                                        int64_t ldh, const void* weight8, const float* weight_scale, int64_t V,
                                        int64_t ldw, int64_t bsz, const int64_t* target, int64_t t_stride_b,
@@ -128,16 +133,11 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   P.tss = t_stride_s;
   P.vs = vocab_start;
   P.ve = vocab_end;
-  P.n_mt = ceil_div(T, kBM);
-  P.n_nt = ceil_div(V, kBN);
-  P.part = workspace;
-  P.xt = workspace + T * P.n_nt * 2;
   P.row_scale = hidden_scale;
   P.col_scale = weight_scale;
-  const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
-  MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL((lce_tile_kernel<kFwdX, F8>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  const int64_t tiles = launch_fwd_x<F8>(P, workspace, st);
+  MIRL_REQUIRE(tiles < (int64_t(1) << 24), "too many tiles");
   hipLaunchKernelGGL(lce_merge_8bit_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P, out, o_stride_b,
                      o_stride_s);
   return check_launch("mirl_linear_ce_8bit_fwd");

@@ -1034,10 +1034,6 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   P.tss = 1;
   P.vs = vocab_start;
   P.ve = vocab_end;
-  P.n_mt = ceil_div(T, kBM);
-  P.n_nt = ceil_div(V, kBN);
-  P.part = workspace;
-  P.xt = workspace + T * P.n_nt * 2;
   P.aid = adapter;
   P.U = static_cast<const uint16_t*>(u_planes);
   P.B = static_cast<const uint16_t*>(b);
@@ -1045,13 +1041,9 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   P.planes = kPlanes;
   P.bad = bad;
   P.b_bytes = N * V * r8 * 2;
-  const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
-  MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == MIRL_DTYPE_BF16)
-    hipLaunchKernelGGL((lce_tile_kernel<kFwdX, BF16>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
-  else
-    hipLaunchKernelGGL((lce_tile_kernel<kFwdX, F16>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  const int64_t tiles = dtype == MIRL_DTYPE_BF16 ? launch_fwd_x<BF16>(P, workspace, st) : launch_fwd_x<F16>(P, workspace, st);
+  MIRL_REQUIRE(tiles < (int64_t(1) << 24), "too many tiles");
   hipLaunchKernelGGL(lce_merge_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P.part, P.xt, (int64_t)0, T,
                      P.n_nt, bsz, target, t_stride_b, t_stride_s, vocab_start, vocab_end, V, out, o_stride_b,
                      o_stride_s, row_stats, perm);
