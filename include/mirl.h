@@ -997,24 +997,25 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
 /* The rows in order of adapter (the base model's first), then sample, then position: all of
  * them, or with grad_out [B, R] those whose gradient is not zero.  Row m's original row
  * perm[m], adapter (-1: none), target, gradient and statistics; seg[a] the first row of adapter
- * a, seg[N] = *count their number.  With bad ([N], or NULL), bad[a] says whether adapter a has
- * rows and its B (b_elems elements of b each) holds an infinity or a NaN.  workspace: 2 B
- * int32. */
+ * a, seg[N] = *count their number.  bad ([N], or NULL) is zeroed.
+ * workspace: 2 B int32. */
 int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64_t R, const float* grad_out,
                       int64_t g_stride_b, int64_t g_stride_s, const int64_t* target,
                       int64_t t_stride_b, int64_t t_stride_s, const float* row_stats,
                       int64_t* perm, int32_t* adapter, int64_t* target_out, float* grad_rows,
-                      float* stats_out, int32_t* seg, int64_t* count, const void* b, int dtype,
-                      int64_t b_elems, int32_t* bad, int32_t* workspace, void* stream);
+                      float* stats_out, int32_t* seg, int64_t* count, int32_t* bad,
+                      int32_t* workspace, void* stream);
 
 /* The T sorted rows' hidden states (zero padded to ldo) and their U: as two values of the
  * operand type that add up to it (u_planes [T, 2, r8]) and, unless NULL, in fp32 by original row
- * (u_rows [*, r8]).  Rows of the base model leave U as it is. */
+ * (u_rows [*, r8]).  Rows of the base model leave U as it is.  bad[a] (zeroed before) becomes 1
+ * where adapter a has rows and its B (b_elems elements of b each) holds an infinity or a NaN. */
 int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const int64_t* perm,
                       const int32_t* adapter, int64_t T, const void* a, int64_t N, int64_t r,
                       int64_t lda, const float* scaling, double p, int64_t seed, const int64_t* seed_dev,
                       int64_t offset, void* hidden_out, int64_t ldo, void* u_planes, int64_t r8,
-                      float* u_rows, void* stream);
+                      float* u_rows, const void* b, int64_t b_elems, const int32_t* seg,
+                      int32_t* bad, void* stream);
 
 /* The logprobs of the T sorted rows (hidden, u_planes as mirl_adapter_down writes them; Hd a
  * multiple of 128, zeros past the true size; the weight's row stride may be below Hd) at their

@@ -268,12 +268,12 @@ SIGNATURES = {
         _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
     ),
     "mirl_adapter_rows": (
-        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _P, _P, _P]
+        _I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
     ),
     "mirl_adapter_down": (
         _I,
         [_P, _I, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, ctypes.c_double, _I64, _P, _I64, _P, _I64, _P, _I64, _P,
-         _P],
+         _P, _I64, _P, _P, _P],
     ),
     "mirl_adapter_ce_fwd": (
         _I,
@@ -1674,16 +1674,14 @@ class Dropped:
 
 class AdapterRows:
     """Rows sorted by adapter (see mirl_adapter_rows): perm, adapter, target, and with an upstream
-    gradient g and stats, as [rows] tensors; seg [N + 1], count [1].  ``b [N, V, r8]`` is looked
-    through for values that are none (``bad [N]``), unless ``bad`` is given."""
+    gradient g and stats, as [rows] tensors; seg [N + 1], count [1].  ``bad [N]``, zeroed here unless it is
+    given (a forward's), says which adapters hold values that are none."""
 
-    def __init__(self, ids: torch.Tensor, b: torch.Tensor, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
+    def __init__(self, ids: torch.Tensor, N: int, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
                  stats: Optional[torch.Tensor] = None, bad: Optional[torch.Tensor] = None):
-        dev = _require_gpu(ids, target, grad, stats, b)
-        N = b.shape[0]
-        _require(b.is_contiguous(), "contiguous adapters")
-        self.bad, look = bad, bad is None
-        if look:
+        dev = _require_gpu(ids, target, grad, stats)
+        self.bad, zero = bad, bad is None
+        if zero:
             self.bad = torch.empty(N, dtype=torch.int32, device=dev)
         B, R = target.shape
         T = B * R
@@ -1704,17 +1702,18 @@ class AdapterRows:
             "mirl_adapter_rows", dev, ids.data_ptr(), B, N, R, _ptr(grad), 0 if grad is None else grad.stride(0),
             0 if grad is None else grad.stride(1), target.data_ptr(), target.stride(0), target.stride(1), _ptr(stats),
             self.perm.data_ptr(), self.adapter.data_ptr(), self.target.data_ptr(), _ptr(self.g), _ptr(self.stats),
-            self.seg.data_ptr(), self.count.data_ptr(), b.data_ptr(), _dtype_code(b), b.shape[1] * b.shape[2],
-            self.bad.data_ptr() if look else None, ws.data_ptr(), _stream(dev),
+            self.seg.data_ptr(), self.count.data_ptr(), self.bad.data_ptr() if zero else None, ws.data_ptr(), _stream(dev),
         )
         _check(st, "mirl_adapter_rows")
 
 
-def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, scaling: torch.Tensor, drop: Dropped,
-                 width: int, r8: int, want_u: bool):
-    """(hidden rows [T, width], U planes [T, 2, r8], U fp32 [T, r8] by original row or None)."""
-    dev = _require_gpu(hidden2d, a, scaling)
-    T, H, r = rows.perm.numel(), hidden2d.shape[1], a.shape[1]
+def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                 drop: Dropped, width: int, want_u: bool):
+    """(hidden rows [T, width], U planes [T, 2, r8], U fp32 [T, r8] by original row or None); sets
+    rows.bad from b [N, V, r8]."""
+    dev = _require_gpu(hidden2d, a, b, scaling)
+    T, H, r, r8 = rows.perm.numel(), hidden2d.shape[1], a.shape[1], b.shape[2]
+    _require(b.is_contiguous() and b.dtype == hidden2d.dtype and b.shape[0] == a.shape[0], "contiguous adapters of one type")
     _require(a.is_contiguous() and a.dtype == hidden2d.dtype and a.shape[2] >= H and hidden2d.stride(1) == 1
              and scaling.dtype == torch.float32 and scaling.numel() == a.shape[0] and scaling.is_contiguous(),
              "contiguous adapters of the hidden states' type, an fp32 scaling each")
@@ -1724,7 +1723,7 @@ def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, sca
     st = _launch(
         "mirl_adapter_down", dev, hidden2d.data_ptr(), _dtype_code(hidden2d), H, hidden2d.stride(0), rows.perm.data_ptr(),
         rows.adapter.data_ptr(), T, a.data_ptr(), a.shape[0], r, a.shape[2], scaling.data_ptr(), *drop.args(), h.data_ptr(), width,
-        planes.data_ptr(), r8, _ptr(u), _stream(dev),
+        planes.data_ptr(), r8, _ptr(u), b.data_ptr(), b.shape[1] * r8, rows.seg.data_ptr(), rows.bad.data_ptr(), _stream(dev),
     )
     _check(st, "mirl_adapter_down")
     return h, planes, u

@@ -1428,30 +1428,58 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   }
 }
 
-// Per row: combine the column-tile partials into the row's max and log-sum-exp,
-// then logprob = (x_t - max) - logsum (0 for targets outside the slice).
-// One wave per row; with `perm` the partials' row r is row perm[r] of targets and results.
-__global__ __launch_bounds__(256) void lce_merge_kernel(
-    const float* __restrict__ part, const float* __restrict__ xt, int64_t row0, int64_t nrows,
-    int64_t n_nt, int64_t bsz, const int64_t* __restrict__ target, int64_t tsb, int64_t tss,
-    int64_t vs, int64_t ve, int64_t V, float* __restrict__ out, int64_t osb, int64_t oss,
-    float* __restrict__ stats, const int64_t* __restrict__ perm) {
-  const int lane = threadIdx.x & 63;
-  const int64_t rl = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (rl >= nrows) return;
-  const float* p = part + rl * n_nt * 2;
-  float M = -INFINITY;
-  for (int64_t j = lane; j < n_nt; j += 64) M = fmaxf(M, p[2 * j]);
+// The maximum M and the sum of exponentials s of a row from its n partial pairs, by the W waves
+// that share it (W == 1: all lanes of one wave; W == 4: the workgroup, which has one row).
+template <int W>
+__device__ __forceinline__ void join_partials(const float* __restrict__ p, int64_t n, float& M, float& s) {
+  __shared__ float s_j[2][W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = W == 1 ? lane : threadIdx.x;
+  M = -INFINITY;
+#pragma unroll 4
+  for (int64_t j = first; j < n; j += 64 * W) M = fmaxf(M, p[2 * j]);
   M = wave_max(M);
-  float s = 0.f;
+  if constexpr (W > 1) {
+    if (lane == 0) s_j[0][wave] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s_j[0][w]);
+  }
+  s = 0.f;
   if (M != -INFINITY) {
-    for (int64_t j = lane; j < n_nt; j += 64) {
+#pragma unroll 4
+    for (int64_t j = first; j < n; j += 64 * W) {
       const float mj = p[2 * j];
       if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
     }
   }
   s = wave_sum(s);
-  if (lane == 0) {
+  if constexpr (W > 1) {
+    if (lane == 0) s_j[1][wave] = s;
+    __syncthreads();
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += s_j[1][w];
+  }
+}
+// Rows up to which a workgroup joins one row's partials (17 us of [64, 1187] with one wave a
+// row, 8 with four); more rows have waves enough.
+constexpr int64_t kJoinRows = 2048;
+
+// Per row: combine the column-tile partials into the row's max and log-sum-exp,
+// then logprob = (x_t - max) - logsum (0 for targets outside the slice).
+// W waves per row; with `perm` the partials' row r is row perm[r] of targets and results.
+template <int W>
+__global__ __launch_bounds__(256) void lce_merge_kernel(
+    const float* __restrict__ part, const float* __restrict__ xt, int64_t row0, int64_t nrows,
+    int64_t n_nt, int64_t bsz, const int64_t* __restrict__ target, int64_t tsb, int64_t tss,
+    int64_t vs, int64_t ve, int64_t V, float* __restrict__ out, int64_t osb, int64_t oss,
+    float* __restrict__ stats, const int64_t* __restrict__ perm) {
+  const int64_t rl = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (rl >= nrows) return;
+  float M, s;
+  join_partials<W>(part + rl * n_nt * 2, n_nt, M, s);
+  if ((threadIdx.x & (64 * W - 1)) == 0) {
     const int64_t r = perm != nullptr ? perm[row0 + rl] : row0 + rl;
     const int64_t sq = r / bsz, b = r - sq * bsz;
     const int64_t t = target[b * tsb + sq * tss];

@@ -371,7 +371,7 @@ extern "C" int mirl_linear_ce_fwd(const void* hidden, int dtype, int64_t T, int6
     hipLaunchKernelGGL((lce_tile_kernel<kFwd, BF16>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
   else
     hipLaunchKernelGGL((lce_tile_kernel<kFwd, F16>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
-  hipLaunchKernelGGL(lce_merge_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P.part,
+  hipLaunchKernelGGL(lce_merge_kernel<1>, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P.part,
                      P.xt, (int64_t)0, T, P.n_nt, bsz, target, t_stride_b, t_stride_s,
                      vocab_start, vocab_end, V, out, o_stride_b, o_stride_s, row_stats, nullptr);
   return check_launch("mirl_linear_ce_fwd");

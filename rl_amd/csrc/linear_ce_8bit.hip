@@ -30,47 +30,50 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float (&v)[4]) {
   v[3] = b[1];
 }
 
-// Per row, one wave: the column tiles' partials combined, the target's logit formed in fp32
+// Per row, W waves: the column tiles' partials combined, the target's logit formed in fp32
 // (a dot product of two rows, 8 KB read at H = 4096: 1% of the forward), the logprob.
+template <int W>
 __global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float* __restrict__ out, int64_t osb,
                                                              int64_t oss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ float s_d[W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (r >= P.nrows) return;
   const int64_t sq = r / P.bsz, b = r - sq * P.bsz;
   const int64_t t = P.target[b * P.tsb + sq * P.tss];
   const bool tmask = (t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V);
-  if (tmask) {
-    if (lane == 0) out[b * osb + sq * oss] = 0.f;
+  const bool first = (threadIdx.x & (64 * W - 1)) == 0;
+  if (tmask) {  // all threads of the row
+    if (first) out[b * osb + sq * oss] = 0.f;
     return;
   }
-  const float* p = P.part + r * P.n_nt * 2;
-  float M = -INFINITY;
-  for (int64_t j = lane; j < P.n_nt; j += 64) M = fmaxf(M, p[2 * j]);
-  M = wave_max(M);
-  float s = 0.f;
-  for (int64_t j = lane; j < P.n_nt; j += 64) {
-    const float mj = p[2 * j];
-    if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
-  }
-  s = wave_sum(s);
+  float M, s;
+  join_partials<W>(P.part + r * P.n_nt * 2, P.n_nt, M, s);
   const uint8_t* hr = static_cast<const uint8_t*>(P.h) + r * P.ldh;
   const uint8_t* wr = static_cast<const uint8_t*>(P.w) + (t - P.vs) * P.ldw;
   float dot[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t k = lane * 16; k < (P.Hd < P.ldw ? P.Hd : P.ldw); k += 64 * 16) {
+  const int64_t width = P.Hd < P.ldw ? P.Hd : P.ldw;  // (multiples of 16)
+#pragma unroll 4
+  for (int64_t k = (W == 1 ? lane : threadIdx.x) * 16; k < width; k += 64 * W * 16) {
     const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const vu4*>(wr + k);
-    const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w}, ww[4] = {wq.x, wq.y, wq.z, wq.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float hv[4], wv[4];
-      unpack_e4m3(hw[i], hv);
-      unpack_e4m3(ww[i], wv);
+      unpack_e4m3(hq[i], hv);
+      unpack_e4m3(wq[i], wv);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dot[e] = fmaf(hv[e], wv[e], dot[e]);
     }
   }
-  const float d = wave_sum((dot[0] + dot[1]) + (dot[2] + dot[3]));
-  if (lane == 0) {
+  float d = wave_sum((dot[0] + dot[1]) + (dot[2] + dot[3]));
+  if constexpr (W > 1) {
+    if (lane == 0) s_d[wave] = d;
+    __syncthreads();
+    d = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) d += s_d[w];
+  }
+  if (first) {
     const float x = (d * P.col_scale[t - P.vs]) * P.row_scale[r], xt = P.xt[r];
     // Logits so large that the two differ by more than 1 (some 1e5) keep the tile's value:
     // the other logits are as far off there.  (Also where one is not finite.)
@@ -138,7 +141,10 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t tiles = launch_fwd_x<F8>(P, workspace, st);
   MIRL_REQUIRE(tiles < (int64_t(1) << 24), "too many tiles");
-  hipLaunchKernelGGL(lce_merge_8bit_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P, out, o_stride_b,
-                     o_stride_s);
+  if (T <= kJoinRows)
+    hipLaunchKernelGGL(lce_merge_8bit_kernel<4>, dim3((unsigned)T), dim3(256), 0, st, P, out, o_stride_b, o_stride_s);
+  else
+    hipLaunchKernelGGL(lce_merge_8bit_kernel<1>, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P, out, o_stride_b,
+                       o_stride_s);
   return check_launch("mirl_linear_ce_8bit_fwd");
 }

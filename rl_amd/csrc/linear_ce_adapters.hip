@@ -165,31 +165,6 @@ __global__ __launch_bounds__(1024) void adapter_fill_kernel(const int64_t* __res
   }
 }
 
-// bad[a] = 1 for the adapters with rows whose B holds an infinity or a NaN (from 0): 32 KB a
-// workgroup.
-constexpr int kScanVecs = 8;
-template <class E>
-__global__ __launch_bounds__(256) void adapter_scan_kernel(const vu4* __restrict__ b, int64_t vecs, int64_t per,
-                                                           const int32_t* __restrict__ seg,
-                                                           int32_t* __restrict__ bad) {
-  const int64_t a = blockIdx.x / per, part = blockIdx.x - a * per;
-  if (seg[a] >= seg[a + 1]) return;
-  constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
-  const vu4* src = b + a * vecs;
-  vu4 q[kScanVecs];
-#pragma unroll
-  for (int u = 0; u < kScanVecs; ++u) {
-    const int64_t i = (part * kScanVecs + u) * 256 + threadIdx.x;
-    q[u] = i < vecs ? src[i] : vu4{0u, 0u, 0u, 0u};
-  }
-  bool none = false;
-#pragma unroll
-  for (int u = 0; u < kScanVecs; ++u)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) none |= (q[u][j] & ex) == ex || ((q[u][j] >> 16) & ex) == ex;
-  if (none) bad[a] = 1;
-}
-
 // -------------------------------------------------------------------------------------------
 // small pieces shared by the kernels below
 // -------------------------------------------------------------------------------------------
@@ -264,7 +239,35 @@ struct DownParams {
   uint16_t* U;             // [T, kPlanes, r8]
   int64_t r8;
   float* U32;              // [rows, r8] by original row, or null
+  // and beside it, by workgroups past n_tiles: which adapters with rows hold an infinity or a
+  // NaN in B ([N, b_vecs] 16-byte pieces, `per` workgroups an adapter)
+  int64_t n_tiles;
+  const vu4* B;
+  int64_t b_vecs, per;
+  const int32_t* seg;
+  int32_t* bad;            // [N], zeros before
 };
+
+constexpr int kScanVecs = 8;  // pieces a thread looks at
+template <class E>
+__device__ __forceinline__ void look_through(const DownParams& P, int64_t block) {
+  const int64_t a = block / P.per, part = block - a * P.per;
+  if (P.seg[a] >= P.seg[a + 1]) return;
+  constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
+  const vu4* src = P.B + a * P.b_vecs;
+  vu4 q[kScanVecs];
+#pragma unroll
+  for (int u = 0; u < kScanVecs; ++u) {
+    const int64_t i = (part * kScanVecs + u) * blockDim.x + threadIdx.x;
+    q[u] = i < P.b_vecs ? src[i] : zero4();
+  }
+  bool none = false;
+#pragma unroll
+  for (int u = 0; u < kScanVecs; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) none |= (q[u][j] & ex) == ex || ((q[u][j] >> 16) & ex) == ex;
+  if (none) P.bad[a] = 1;
+}
 
 // 16 sorted rows a workgroup, the hidden dimension split over its NW waves 64 elements at a
 // time.  An MFMA takes 16 ranks of the adapter against the 16 rows.  Rows of several adapters
@@ -275,6 +278,10 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(DownParams P) {
   __shared__ float red[NW][16][NT * 16 + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 15, lg = lane >> 4;
+  if ((int64_t)blockIdx.x >= P.n_tiles) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) look_through<E>(P, blockIdx.x - P.n_tiles);
+    return;
+  }
   const int64_t m0 = (int64_t)blockIdx.x * 16, rho0 = (int64_t)blockIdx.y * kRankTile;
   const int64_t m = m0 + lr;
   const bool live = m < P.T;
@@ -941,8 +948,7 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
                                  int64_t g_stride_b, int64_t g_stride_s, const int64_t* target, int64_t t_stride_b,
                                  int64_t t_stride_s, const float* row_stats, int64_t* perm, int32_t* adapter,
                                  int64_t* target_out, float* grad_rows, float* stats_out, int32_t* seg, int64_t* count,
-                                 const void* b, int dtype, int64_t b_elems, int32_t* bad, int32_t* workspace,
-                                 void* stream) {
+                                 int32_t* bad, int32_t* workspace, void* stream) {
   clear_error();
   MIRL_REQUIRE(B > 0 && N > 0 && R > 0, "invalid shape B=%lld N=%lld R=%lld", (long long)B, (long long)N, (long long)R);
   MIRL_REQUIRE(B < (int64_t(1) << 22) && N < (int64_t(1) << 22) && R < kMaxRows && B * R < kMaxRows,
@@ -950,26 +956,12 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
   MIRL_REQUIRE(ids && target && perm && adapter && target_out && seg && count && workspace, "null pointer argument");
   MIRL_REQUIRE((row_stats == nullptr) == (stats_out == nullptr) && (grad_out == nullptr) == (grad_rows == nullptr),
                "null pointer argument");
-  MIRL_REQUIRE(bad == nullptr || (b != nullptr && is16(dtype) && b_elems > 0 && b_elems % 8 == 0 && aligned16(b) &&
-                                  N * ceil_div(b_elems, 2048 * kScanVecs) < kMaxBlocks),
-               "adapters of %lld elements (dtype code %d) cannot be looked through", (long long)b_elems, dtype);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int32_t *cnt = workspace, *start = workspace + B;
   if (grad_out != nullptr)
     hipLaunchKernelGGL(adapter_count_kernel, dim3((unsigned)B), dim3(1024), 0, st, grad_out, g_stride_b, g_stride_s, R, cnt);
   hipLaunchKernelGGL(adapter_starts_kernel, dim3((unsigned)(N + 1)), dim3(1024), 0, st, ids, B, N, (int32_t)R,
                      grad_out != nullptr ? cnt : nullptr, start, seg, count, bad);
-  if (bad != nullptr) {
-    const int64_t vecs = b_elems / 8, per = ceil_div(vecs, 256 * kScanVecs);
-    auto scan = [&](auto e) {
-      hipLaunchKernelGGL(adapter_scan_kernel<decltype(e)>, dim3((unsigned)(N * per)), dim3(256), 0, st,
-                         static_cast<const vu4*>(b), vecs, per, seg, bad);
-    };
-    if (dtype == MIRL_DTYPE_BF16)
-      scan(BF16{});
-    else
-      scan(F16{});
-  }
   hipLaunchKernelGGL(adapter_fill_kernel, dim3((unsigned)B), dim3(1024), 0, st, ids, B, N, R, grad_out, g_stride_b,
                      g_stride_s, target, t_stride_b, t_stride_s, row_stats, start,
                      RowsOut{perm, adapter, target_out, grad_rows, stats_out});
@@ -979,7 +971,8 @@ extern "C" int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64
 extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const int64_t* perm,
                                  const int32_t* adapter, int64_t T, const void* a, int64_t N, int64_t r, int64_t lda, const float* scaling,
                                  double p, int64_t seed, const int64_t* seed_dev, int64_t offset, void* hidden_out,
-                                 int64_t ldo, void* u_planes, int64_t r8, float* u_rows, void* stream) {
+                                 int64_t ldo, void* u_planes, int64_t r8, float* u_rows, const void* b,
+                                 int64_t b_elems, const int32_t* seg, int32_t* bad, void* stream) {
   clear_error();
   MIRL_REQUIRE(is16(dtype), "hidden states and adapters must be bf16 or fp16 (dtype code %d)", dtype);
   MIRL_REQUIRE(T > 0 && T < kMaxRows && Hd > 0 && N > 0 && r > 0 && r8 >= r && r8 % 8 == 0 && r8 <= kMaxRank && ldh >= Hd &&
@@ -987,20 +980,45 @@ extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int6
                "invalid shape T=%lld H=%lld r=%lld r8=%lld ldo=%lld", (long long)T, (long long)Hd, (long long)r,
                (long long)r8, (long long)ldo);
   MIRL_REQUIRE(p >= 0.0 && p <= 1.0, "dropout probability %g is outside [0, 1]", p);
-  MIRL_REQUIRE(hidden && perm && adapter && a && scaling && hidden_out && u_planes, "null pointer argument");
+  MIRL_REQUIRE(hidden && perm && adapter && a && scaling && hidden_out && u_planes && b && seg && bad,
+               "null pointer argument");
+  MIRL_REQUIRE(b_elems > 0 && b_elems % 8 == 0 && aligned16(b), "adapters of %lld elements", (long long)b_elems);
   MIRL_REQUIRE(lda >= Hd && lda % 8 == 0 && aligned16(a) && aligned16(hidden_out) && aligned16(u_planes),
                "the adapters' rows must be 16-byte aligned (row stride %lld)", (long long)lda);
-  const DownParams P{static_cast<const uint16_t*>(hidden), Hd, ldh, perm, adapter, T, static_cast<const uint16_t*>(a), r,
-                     lda, scaling, dropout_args(p, seed, seed_dev, offset), static_cast<uint16_t*>(hidden_out), ldo,
-                     static_cast<uint16_t*>(u_planes), r8, u_rows};
+  // few rows: 16 waves share them, and workgroups their adapters, to have the loads of all in
+  // flight (64 rows of 16 adapters, H = 4096: 91 -> 18 us); many: four waves (104 us of
+  // [16384, 4096])
+  const bool few = T <= 2048;
+  DownParams P{};
+  P.hidden = static_cast<const uint16_t*>(hidden);
+  P.H = Hd;
+  P.ldh = ldh;
+  P.perm = perm;
+  P.aid = adapter;
+  P.T = T;
+  P.A = static_cast<const uint16_t*>(a);
+  P.r = r;
+  P.lda = lda;
+  P.scaling = scaling;
+  P.drop = dropout_args(p, seed, seed_dev, offset);
+  P.h_out = static_cast<uint16_t*>(hidden_out);
+  P.ldo = ldo;
+  P.U = static_cast<uint16_t*>(u_planes);
+  P.r8 = r8;
+  P.U32 = u_rows;
+  P.n_tiles = ceil_div(T, 16);
+  P.B = static_cast<const vu4*>(b);
+  P.b_vecs = b_elems / 8;
+  P.per = ceil_div(P.b_vecs, (few ? 1024 : 256) * kScanVecs);
+  P.seg = seg;
+  P.bad = bad;
+  const int64_t ny = ceil_div(r8, kRankTile), nz = few ? std::min(N, int64_t(16)) : 1;
+  MIRL_REQUIRE((P.n_tiles + N * P.per) * ny * nz < kMaxBlocks / 4 * (few ? 1 : 4), "too many rows or adapters");
+  const dim3 grid((unsigned)(P.n_tiles + N * P.per), (unsigned)ny, (unsigned)nz);
   with_rank(dtype, r8, [&](auto e, auto nt) {
     using E = decltype(e);
     constexpr int NT = decltype(nt)::value;
-    // few rows: 16 waves share them, and workgroups their adapters, to have the loads of all in
-    // flight (64 rows of 16 adapters, H = 4096: 91 -> 13 us); many: four waves (113 us against
-    // 130 of [16384, 4096])
-    const dim3 grid((unsigned)ceil_div(T, 16), (unsigned)ceil_div(r8, kRankTile), T <= 2048 ? (unsigned)std::min(N, int64_t(16)) : 1u);
-    if (T <= 2048)
+    if (few)
       hipLaunchKernelGGL((adapter_down_kernel<E, NT, 16>), grid, dim3(1024), 0, static_cast<hipStream_t>(stream), P);
     else
       hipLaunchKernelGGL((adapter_down_kernel<E, NT, 4>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), P);
@@ -1044,9 +1062,14 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t tiles = dtype == MIRL_DTYPE_BF16 ? launch_fwd_x<BF16>(P, workspace, st) : launch_fwd_x<F16>(P, workspace, st);
   MIRL_REQUIRE(tiles < (int64_t(1) << 24), "too many tiles");
-  hipLaunchKernelGGL(lce_merge_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), 0, st, P.part, P.xt, (int64_t)0, T,
-                     P.n_nt, bsz, target, t_stride_b, t_stride_s, vocab_start, vocab_end, V, out, o_stride_b,
-                     o_stride_s, row_stats, perm);
+  auto merge = [&](auto kernel, int64_t blocks) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, P.part, P.xt, (int64_t)0, T, P.n_nt, bsz, target,
+                       t_stride_b, t_stride_s, vocab_start, vocab_end, V, out, o_stride_b, o_stride_s, row_stats, perm);
+  };
+  if (T <= kJoinRows)
+    merge(lce_merge_kernel<4>, T);
+  else
+    merge(lce_merge_kernel<1>, ceil_div(T, 4));
   return check_launch("mirl_adapter_ce_fwd");
 }
 

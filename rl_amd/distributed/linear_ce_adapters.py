@@ -70,8 +70,8 @@ class _AdapterLogprobs(torch.autograd.Function):
         h2 = hidden.view(S * B, H)
         drop = _C.Dropped(*drop_args, dev)
         bk = _padded_last(b)
-        rows = _C.AdapterRows(ids, bk, target)
-        h, planes, u = _C.adapter_down(h2, rows, _padded_last(a), scaling, drop, _round_up(H, _H_ALIGN), bk.shape[2], keep)
+        rows = _C.AdapterRows(ids, a.shape[0], target)
+        h, planes, u = _C.adapter_down(h2, rows, _padded_last(a), bk, scaling, drop, _round_up(H, _H_ALIGN), keep)
         out = torch.empty((B, R), dtype=torch.float32, device=dev)
         stats = torch.empty((R * B, 2), dtype=torch.float32, device=dev) if keep else None
         _C.adapter_ce_fwd(h, _weight_operand(weight), rows, planes, bk, target, vs, ve, out, stats)
@@ -95,7 +95,7 @@ class _AdapterLogprobs(torch.autograd.Function):
         dev = hidden.device
         drop = _C.Dropped(p, seed if seed_t is None else seed_t, offset, dev)
         ak, bk, wk = _padded_last(a), _padded_last(b), _weight_operand(weight)
-        rows = _C.AdapterRows(ids, bk, target, grad, stats, bad)
+        rows = _C.AdapterRows(ids, N, target, grad, stats, bad)
         h2 = hidden.view(S * B, H)
         h, planes = _C.adapter_gather(h2, rows, u, _round_up(H, _H_ALIGN))
         Vp = _round_up(V, _K_ALIGN)
