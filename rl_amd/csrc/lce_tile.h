@@ -266,7 +266,7 @@ void lce_tile_kernel(LceParams P) {
   __shared__ __align__(1024) unsigned char st0[kStageBytes];
   __shared__ __align__(1024) unsigned char st1[kStageBytes];
   __shared__ int s_tcol[kBM];
-  __shared__ float s_m[kBM], s_ls[kBM], s_g[kBM];
+  __shared__ __align__(16) float s_m[kBM], s_ls[kBM], s_g[kBM], s_rs[MODE == kFwdX && kES == 1 ? kBM : 1];
   __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_bad[kAdapters ? kBM : 1],
       s_heads[kWaves];
   auto stage_ptr = [&](int s) -> unsigned char* { return s == 0 ? st0 : st1; };
@@ -327,7 +327,9 @@ void lce_tile_kernel(LceParams P) {
 
   // per-row metadata of the tile (kThreads == kBM: one row per thread)
   float my_g = 0.f;
-  if constexpr (MODE != kGemm) {
+  int n_seg = 0;
+  bool apart = false;  // the adapters' part is formed by itself (adapter_stages)
+  auto metadata = [&]() __attribute__((always_inline)) {
     const int64_t r = m0 + tid;
     int tc = -1;
     float lm = 0.f, ll = 0.f;
@@ -352,16 +354,11 @@ void lce_tile_kernel(LceParams P) {
       s_ls[tid] = ll;
     }
     if constexpr (MODE == kFwdX && kES == 1) {
-      s_m[tid] = r < row_end ? P.row_scale[r] : 0.f;
+      s_rs[tid] = r < row_end ? P.row_scale[r] : 0.f;
       s_ls[tid] = n0 + tid < P.V ? P.col_scale[n0 + tid] : 0.f;
     }
-  }
-  // The tile's adapters in row order: s_seg[q] is the q-th one, s_ord[row] the row's (-1: none).
-  int n_seg = 0;
-  bool apart = false;  // their part is formed by itself (adapter_stages)
-  if constexpr (kAdapters) {
-    if (P.aid != nullptr) {
-      const int64_t r = m0 + tid;
+    // The tile's adapters in row order: s_seg[q] is the q-th one, s_ord[row] the row's (-1: none).
+    if constexpr (kAdapters) {
       const int a = r < row_end ? P.aid[r] : -1;
       const int before = tid > 0 && r < row_end ? P.aid[r - 1] : -1;
       const bool head = a >= 0 && (tid == 0 || a != before);
@@ -384,7 +381,8 @@ void lce_tile_kernel(LceParams P) {
       apart = __syncthreads_or(bad) != 0 || P.b_bytes >= (int64_t(1) << 31);
       n_seg = __builtin_amdgcn_readfirstlane(n_seg);
     }
-  }
+  };
+  if constexpr (MODE != kGemm) metadata();
   if (MODE == kGrad) {
     // (onehot - p) * 0 == 0: a tile whose rows all have a zero upstream
     // gradient is written as zeros without the GEMM.
@@ -924,71 +922,94 @@ void lce_tile_kernel(LceParams P) {
     // A lane holds kTN groups of columns of kTM rows, the lanes that share a row are kT apart
     // and the two waves of a row band exchange through LDS.
     wait_vm_barrier<0>();
+    // (the accumulators are complete here: without this the compiler moves MFMAs of the last
+    // stage down between the rows' reductions, and they wait for each other)
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) asm volatile("" : "+a"(acc[i][j]));
     constexpr int kG = kAV / 4;  // groups of four consecutive columns per MFMA tile
     const int col_lane = lane / kT * 4;
     const int64_t ncols = P.V - n0;
-    if constexpr (kES == 1) {
-#pragma unroll
-      for (int j = 0; j < kTN; ++j)
-#pragma unroll
-        for (int g = 0; g < kG; ++g) {
-          const float4 cs = *reinterpret_cast<const float4*>(s_ls + wn * kWN + j * kT + g * 8 + col_lane);
-          const float c4[4] = {cs.x, cs.y, cs.z, cs.w};
-#pragma unroll
-          for (int i = 0; i < kTM; ++i) {
-            const float rs = s_m[wm * kWM + i * kT + frow];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][4 * g + e] = (acc[i][j][4 * g + e] * c4[e]) * rs;
-          }
-        }
-      __syncthreads();  // s_m is written below
-    }
-    if (ncols < kBN) {
-#pragma unroll
-      for (int j = 0; j < kTN; ++j)
-#pragma unroll
-        for (int v = 0; v < kAV; ++v) {
-          const bool out = wn * kWN + j * kT + v / 4 * 8 + col_lane + v % 4 >= ncols;
-#pragma unroll
-          for (int i = 0; i < kTM; ++i) acc[i][j][v] = out ? -INFINITY : acc[i][j][v];
-        }
-    }
+    // A value is y with the logit x = y * rs: e4m3 products come with the column's scale, and the
+    // row's goes into the exponent's factor, 2^(y c - M c) with c = rs log2(e), one fma a value.  The
+    // rounding of M c is undone at the end.  (c is kept above 0, so that the columns past the end,
+    // -inf, stay that under a row scale of 0; a negative row scale goes into the values.)
+    // Row by row of MFMA tiles, so that each accumulator is read once.
     float rm[kTM], rsum[kTM];
 #pragma unroll
     for (int i = 0; i < kTM; ++i) {
       const int rl = wm * kWM + i * kT + frow;
+      float rs = kES == 1 ? s_rs[rl] : 1.f;
+      const float f = rs < 0.f ? rs : 1.f;
+      rs = rs < 0.f ? 1.f : rs;
+      const bool negative = kES == 1 && __ballot(f != 1.f) != 0;
       // few tiles hold a row's target: looked for only where one does
       const int tc = s_tcol[rl] - wn * kWN;
-      if (__ballot(tc >= 0 && tc < kWN) != 0) {
+      const bool held = __ballot(tc >= 0 && tc < kWN) != 0;
+      float y[kTN][kAV];
+      float M = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int g = 0; g < kG; ++g) {
+          float c4[4] = {1.f, 1.f, 1.f, 1.f};
+          if constexpr (kES == 1) {
+            const float4 cs = *reinterpret_cast<const float4*>(s_ls + wn * kWN + j * kT + g * 8 + col_lane);
+            c4[0] = cs.x;
+            c4[1] = cs.y;
+            c4[2] = cs.z;
+            c4[3] = cs.w;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[j][4 * g + e] = kES == 1 ? acc[i][j][4 * g + e] * c4[e] : acc[i][j][4 * g + e];
+        }
+      if (negative) {
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int v = 0; v < kAV; ++v) y[j][v] *= f;
+      }
+      if (ncols < kBN) {
 #pragma unroll
         for (int j = 0; j < kTN; ++j)
 #pragma unroll
           for (int v = 0; v < kAV; ++v)
-            if (j * kT + v / 4 * 8 + col_lane + v % 4 == tc) P.xt[m0 + rl - P.row0] = acc[i][j][v];
+            if (wn * kWN + j * kT + v / 4 * 8 + col_lane + v % 4 >= ncols) y[j][v] = -INFINITY;
       }
-      float M = acc[i][0][0];
+      if (held) {
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int v = 0; v < kAV; ++v)
+            if (j * kT + v / 4 * 8 + col_lane + v % 4 == tc) P.xt[m0 + rl - P.row0] = y[j][v] * rs;
+      }
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int v = 0; v < kAV; ++v) M = fmaxf(M, acc[i][j][v]);
+        for (int v = 0; v < kAV; ++v) M = fmaxf(M, y[j][v]);
 #pragma unroll
       for (int off = kT; off < kWave; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, kWave));
+      const float c = kES == 1 ? fmaxf(rs * kLog2e, 0x1p-126f) : kLog2e, Mc = M * c;
       float s4[4] = {0.f, 0.f, 0.f, 0.f};
       if (M != -INFINITY) {
 #pragma unroll
         for (int j = 0; j < kTN; ++j)
 #pragma unroll
-          for (int v = 0; v < kAV; ++v) s4[v & 3] += fast_exp2((acc[i][j][v] - M) * kLog2e);
+          for (int v = 0; v < kAV; ++v) s4[v & 3] += fast_exp2(fmaf(y[j][v], c, -Mc));
       }
       float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
       for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+      if (M != -INFINITY) sum *= fast_exp2(-fmaf(M, c, -Mc));
+      M = kES == 1 ? M * rs : M;
       rm[i] = M;
       rsum[i] = sum;
       if (wn == 1 && lane < kT) {
         s_m[rl] = M;
         s_g[rl] = sum;
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     if (wn == 0 && lane < kT) {
@@ -1079,6 +1100,7 @@ void lce_tile_kernel(LceParams P) {
     for (int i = 0; i < kTM; ++i) {
       const int rl = wm * kWM + i * kT + frow;
       const float gv = s_g[rl], M = s_m[rl], LS = s_ls[rl];
+      const float off = (M + LS) * kLog2e;
       const int tc = s_tcol[rl];
 #pragma unroll
       for (int j = 0; j < kTN; ++j) {
@@ -1087,9 +1109,15 @@ void lce_tile_kernel(LceParams P) {
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           float x0 = acc[i][j][e], x1 = acc[i][j][e + 1];
-          if constexpr (MODE == kGrad) round_trip2<E>(x0, x1);  // the logits in the operand dtype
-          o[e] = fast_exp2(((x0 - M) - LS) * kLog2e);
-          o[e + 1] = fast_exp2(((x1 - M) - LS) * kLog2e);
+          if constexpr (MODE == kGradX) {
+            // (the offset's rounding moves a row's probabilities by 2^-24 |M + LS|, relatively)
+            o[e] = fast_exp2(fmaf(x0, kLog2e, -off));
+            o[e + 1] = fast_exp2(fmaf(x1, kLog2e, -off));
+          } else {
+            round_trip2<E>(x0, x1);  // the logits in the operand dtype
+            o[e] = fast_exp2(((x0 - M) - LS) * kLog2e);
+            o[e + 1] = fast_exp2(((x1 - M) - LS) * kLog2e);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (cl + e == tc) ? (1.f - o[e]) * gv : -o[e] * gv;
