@@ -1001,8 +1001,10 @@ void lce_tile_kernel(LceParams P) {
       float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
       for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-      if (M != -INFINITY) sum *= fast_exp2(-fmaf(M, c, -Mc));
-      M = kES == 1 ? M * rs : M;
+      if (M != -INFINITY) {  // (else no column is there)
+        sum *= fast_exp2(-fmaf(M, c, -Mc));
+        M = kES == 1 ? M * rs : M;
+      }
       rm[i] = M;
       rsum[i] = sum;
       if (wn == 1 && lane < kT) {

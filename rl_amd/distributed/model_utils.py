@@ -49,8 +49,10 @@ __all__ = [
     "from_parallel_hidden_states_to_logprobs_with_adapters",
     "from_parallel_logits_to_logprobs",
     "from_parallel_logits_to_logprobs_packed_sequences",
+    "from_residual_stream_to_logprobs",
     "get_next_token_logprobs_from_logits",
     "get_policy_logprobs_at_sampler_topk",
+    "HeadAdapters",
     "quantize_rows_8bit",
     "rms_norm",
     "set_early_backward",
@@ -92,6 +94,10 @@ def __getattr__(name: str):
         from rl_amd.distributed import linear_ce_adapters
 
         return getattr(linear_ce_adapters, name)
+    if name in ("HeadAdapters", "from_residual_stream_to_logprobs"):
+        from rl_amd.distributed import policy_head
+
+        return getattr(policy_head, name)
     if name == "dropout":
         from rl_amd.distributed.counter_dropout import dropout
 

@@ -112,6 +112,22 @@ def test_typical_error():
     assert torch.all((got - want).abs() <= tol)
 
 
+@pytest.mark.parametrize("S", [3, 90])  # few rows, and whole 256-row tiles
+def test_scales_of_any_sign(S):
+    """Row and column scales of zero or below it, over a vocabulary that ends inside a tile."""
+    h8, hs, w8, ws, target = inputs(S, 2, 256, 600, seed=8)
+    hs, ws = hs.clone(), ws.clone()
+    hs[0, 0], hs[0, 1] = 0.0, -hs[0, 1]
+    hs[-2, 0] = -2 * hs[-2, 0]
+    ws[5], ws[300:400] = 0.0, -ws[300:400]
+    got = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 600)
+    want, tol = oracle(h8, hs, w8, ws, target, 0, 600)
+    assert torch.all((got.cpu().double() - want).abs() <= tol)
+    hs[0, 1] = float("nan")
+    got = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 600)
+    assert torch.isnan(got[1, 0]) and torch.isnan(got).sum() == 1
+
+
 def test_layouts_empty_and_streams():
     h8, hs, w8, ws, target = inputs(21, 4, 512, 900)
     want = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 900)
