@@ -470,6 +470,8 @@ _pinned: dict = {}
 _fetch_streams: dict = {}
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
 try:  # raw handle of the current stream without building a Stream object
     _raw_stream = torch._C._cuda_getCurrentRawStream  # type: ignore[attr-defined]
 except AttributeError:  # pragma: no cover - older torch
@@ -508,7 +510,8 @@ class _OnDevice:
 def _launch(name: str, dev: torch.device, *args):
     """Call entry point `name` with `dev` current (and timed when launch timing is on)."""
     fn = getattr(_lib if _lib is not None else load(), name)
-    if _timer is None and (dev.index is None or dev.index == torch.cuda.current_device()):
+    # (the device is initialised: there is a tensor on it)
+    if _timer is None and (dev.index is None or dev.index == _current_device()):
         return fn(*args)
     with _OnDevice(dev), _Timed(name, dev):
         return fn(*args)
@@ -1526,17 +1529,18 @@ def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
                      want_rstd: bool, out8: bool):
     """(y, h, rstd or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
-    itself without a residual, rstd and scale have a row's shape."""
+    itself without a residual, rstd and scale have a row's shape.  Shapes and types are the
+    caller's to check."""
     dev = _require_gpu(x, residual, weight)
     shape = x.shape
     H = shape[-1]
-    _require(weight.dim() == 1 and weight.shape[0] == H, "a weight per element of a row")
     x2, ldx = _rows2(x)
-    weight = weight.contiguous()
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    x_code = _dtype_code(x)
     if residual is None:
-        h, r_ptr, ldr, h_ptr, h_code = x, None, 0, None, _dtype_code(x)
+        h, r_ptr, ldr, h_ptr, h_code = x, None, 0, None, x_code
     else:
-        _require(residual.shape == shape, "a residual of the rows' shape")
         r2, ldr = _rows2(residual)
         h = _new_like(residual, residual.dtype)
         r_ptr, h_ptr, h_code = r2.data_ptr(), h.data_ptr(), _dtype_code(residual)
@@ -1544,30 +1548,30 @@ def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     scale = x.new_empty(shape[:-1], dtype=torch.float32) if out8 else None
     rstd = x.new_empty(shape[:-1], dtype=torch.float32) if want_rstd else None
     st = _launch(
-        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), _dtype_code(x), ldx, r_ptr, h_code, ldr, weight.data_ptr(),
-        _dtype_code(weight), x.numel() // H, H, float(eps), h_ptr, y.data_ptr(), _ptr(scale), _ptr(rstd), _stream(dev),
+        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), x_code, ldx, r_ptr, h_code, ldr, weight.data_ptr(),
+        _dtype_code(weight), x.numel() // H, H, eps, h_ptr, y.data_ptr(), _ptr(scale), _ptr(rstd), _stream(dev),
     )
-    _check(st, "mirl_add_rms_norm_fwd")
+    if st != 0:
+        _check(st, "mirl_add_rms_norm_fwd")
     return y, h, rstd, scale
 
 
 def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.Tensor, rstd: torch.Tensor,
                      weight: torch.Tensor, need_x: bool, need_res: bool, need_w: bool):
     """(dx, dres, dw), None where not needed; dx and dres are one tensor where their types are
-    the same (see mirl_add_rms_norm_bwd)."""
+    the same (see mirl_add_rms_norm_bwd).  The operands are a forward's and its gradients."""
     dev = _require_gpu(dy, dh_out, h, rstd, weight)
     H = h.shape[-1]
     R = h.numel() // H
-    _require(dy.shape == h.shape and rstd.is_contiguous() and rstd.dtype == torch.float32
-             and rstd.numel() == R and weight.numel() == H, "gradients and row statistics of the rows")
-    _require(dh_out is None or (dh_out.shape == h.shape and dh_out.dtype == h.dtype), "the stream's gradient has its type")
     dy2, lddy = _rows2(dy)
     h2, ldh = _rows2(h)
     g2, ldg = (None, 0) if dh_out is None else _rows2(dh_out)
-    weight = weight.contiguous()
-    one = need_x and need_res and dy.dtype == h.dtype
-    dx = _new_like(h, dy.dtype) if need_x else None
-    dres = _new_like(h, h.dtype) if need_res and not one else None
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    dtype, h_dtype = dy.dtype, h.dtype
+    one = need_x and need_res and dtype == h_dtype
+    dx = _new_like(h, dtype) if need_x else None
+    dres = _new_like(h, h_dtype) if need_res and not one else None
     dw = ws = None
     if need_w:
         if R == 0:
@@ -1575,13 +1579,14 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
         else:
             dw = torch.empty_like(weight)
             lib = _lib if _lib is not None else load()
-            ws = h.new_empty(int(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)), dtype=torch.float32)
+            ws = rstd.new_empty(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H))
     st = _launch(
         "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), lddy, _ptr(g2), ldg, h2.data_ptr(), _dtype_code(h),
         ldh, rstd.data_ptr(), weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres),
         None if ws is None else dw.data_ptr(), _ptr(ws), _stream(dev),
     )
-    _check(st, "mirl_add_rms_norm_bwd")
+    if st != 0:
+        _check(st, "mirl_add_rms_norm_bwd")
     return dx, (dx if one else dres), dw
 
 

@@ -29,12 +29,18 @@ class _Dropout(torch.autograd.Function):
         return _C.dropout(x, p, seed, offset)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, dy):  # type: ignore[override]
+        # the decorator only where a graph of the backward is asked for: it costs a small call 4 us
+        return (_Dropout._once if torch.is_grad_enabled() else _Dropout._grads)(ctx, dy)
+
+    @staticmethod
+    def _grads(ctx: Any, dy):
         p, seed, offset = ctx.args
         if seed is None:
             (seed,) = ctx.saved_tensors
         return _C.dropout(dy, p, seed, offset), None, None, None
+
+    _once = staticmethod(once_differentiable(_grads.__func__))
 
 
 def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: int = 0,

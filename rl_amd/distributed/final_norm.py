@@ -28,19 +28,20 @@ _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> None:
-    if x.dtype not in _ROW_DTYPES:
-        raise TypeError(f"the norm takes fp32, bf16 or fp16 rows, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"expected rows [..., H], got {tuple(x.shape)}")
-    if tuple(weight.shape) != (x.shape[-1],):
-        raise ValueError(f"weight shape {tuple(weight.shape)} does not match rows of {x.shape[-1]}")
-    if weight.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"the weight has the rows' type {x.dtype} or float32, got {weight.dtype}")
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _ROW_DTYPES:
+        raise TypeError(f"the norm takes fp32, bf16 or fp16 rows, got {dtype}")
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"expected rows [..., H], got {tuple(shape)}")
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight shape {tuple(weight.shape)} does not match rows of {shape[-1]}")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise TypeError(f"the weight has the rows' type {dtype} or float32, got {weight.dtype}")
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"residual shape {tuple(residual.shape)} does not match {tuple(x.shape)}")
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"the residual has the rows' type {x.dtype} or float32, got {residual.dtype}")
+        if residual.shape != shape:
+            raise ValueError(f"residual shape {tuple(residual.shape)} does not match {tuple(shape)}")
+        if residual.dtype != dtype and residual.dtype != torch.float32:
+            raise TypeError(f"the residual has the rows' type {dtype} or float32, got {residual.dtype}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
 
@@ -58,14 +59,20 @@ class _AddRmsNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, dy, dh):  # type: ignore[override]
+        # the decorator only where a graph of the backward is asked for: it costs a small call 4 us
+        return (_AddRmsNorm._once if torch.is_grad_enabled() else _AddRmsNorm._grads)(ctx, dy, dh)
+
+    @staticmethod
+    def _grads(ctx: Any, dy, dh):
         h, rstd, weight = ctx.saved_tensors
         need_x, need_res, need_w = ctx.needs_input_grad[:3]
         if dy is None:  # only the stream has a consumer
             return (dh.to(ctx.x_dtype) if need_x else None), (dh if need_res else None), None, None
         dx, dres, dw = _C.add_rms_norm_bwd(dy, dh, h, rstd, weight, need_x, need_res, need_w)
         return dx, dres, dw, None
+
+    _once = staticmethod(once_differentiable(_grads.__func__))
 
 
 class _RmsNorm(torch.autograd.Function):

@@ -219,3 +219,14 @@ def test_side_stream_graph_and_repeat():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_no_second_derivative():
+    from rl_amd.distributed.model_utils import dropout
+
+    x, w = rows((3, 40), FP, 1).requires_grad_(True), rows((40,), FP, 3).requires_grad_(True)
+    for y in (add_rms_norm(x, x, w)[0], rms_norm(x, w), dropout(x, 0.5, 3)):
+        dy = torch.ones_like(y).requires_grad_(True)
+        (g,) = torch.autograd.grad([y], [x], [dy], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
