@@ -274,3 +274,60 @@ def test_empty():
     lp, g = run(x)
     assert lp.shape == (3, 0) and not any(v.any() for v in g.values())
     assert with_adapters(x["hidden"], x["weight"], x["a"], x["b"], x["ids"], 1.0, x["target"], 0, 300).shape == (3, 0)
+
+
+@pytest.mark.parametrize("S,B,H,V,N,r", [(70, 2, 128, 300, 2, 200), (4, 3, 5, 90, 2, 8), (20, 2, 64, 130, 1, 1024),
+                                         (2, 1000, 64, 257, 1000, 8), (2, 128, 64, 300, 128, 16), (2, 129, 64, 300, 129, 12)])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+def test_ranks_sizes_and_many_adapters(S, B, H, V, N, r, dtype):
+    """Ranks over several tiles, a hidden size below a vector, an adapter for every row of a tile."""
+    print("[case]", S, B, H, V, N, r, flush=True)
+    x = inputs(S, B, H, V, N, r, dtype, seed=r, ids=[(7 * i) % N for i in range(B)], active=1.0)
+    check(*run(x), oracle(x))
+    check(*run(x, chunk_size=4), oracle(x))
+
+
+def test_few_rows_with_a_broken_adapter():
+    x = inputs(5, 6, 128, 600, 3, 8, BF, seed=7, ids=[0, 1, 2, -1, 1, 0], active=1.0)
+    ref_lp, ref = run(x)
+    y = dict(x, b=x["b"].clone())
+    y["b"][1, 599, 7] = float("-inf")
+    lp, g = run(y)
+    assert torch.isnan(lp[[1, 4]]).all() and torch.equal(lp[[0, 2, 3, 5]], ref_lp[[0, 2, 3, 5]])
+    assert torch.equal(g["hidden"][:, [0, 2, 3, 5]], ref["hidden"][:, [0, 2, 3, 5]])
+    # an adapter that no sample is under may hold anything
+    y = dict(x, b=x["b"].clone(), a=x["a"].clone(), ids=torch.tensor([0, 2, 2, -1, 2, 0], device=DEV))
+    clean = run(dict(x, ids=y["ids"]))
+    y["b"][1], y["a"][1] = float("nan"), float("inf")
+    lp, g = run(y)
+    assert torch.equal(lp, clean[0]) and all(torch.equal(g[k], clean[1][k]) for k in g)
+
+
+@pytest.mark.parametrize("S", [3, 100])
+def test_adapters_of_more_than_2_gib(S):
+    """9 adapters of rank 800 over 151936 tokens are 2.19 GB: past 32-bit byte offsets.  The one in use
+    alone takes the other route; both are fp32 sums of the same products, off by at most r u sum|U b|
+    each (and the logprob by twice that, its own and the log-sum-exp's)."""
+    V, H, r = 151936, 128, 800
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    hidden, weight = rnd(S, 2, H).to(BF), (rnd(V, H) * 0.1).to(BF)
+    a, b = (rnd(9, r, H) / H**0.5).to(BF), torch.empty(9, V, r, dtype=BF, device=DEV)
+    for i in range(9):
+        b[i] = (rnd(V, r) * 0.02).to(BF)
+    target = torch.randint(0, V, (2, S), generator=g, device=DEV)
+    grad = rnd(2, S - 1)
+
+    def go(a, b, ids):
+        h, a, b = (t.detach().requires_grad_(True) for t in (hidden, a, b))
+        lp = with_adapters(h, weight, a, b, torch.tensor(ids, device=DEV), 1.0, target, 0, V)
+        return (lp.detach(), *torch.autograd.grad([lp], [h, a, b], [grad]))
+
+    far = go(a, b, [8, -1])
+    near = go(a[8:], b[8:].contiguous(), [0, -1])
+    mag = r * 0.02 * 4  # sum|U b| of r terms of order 1 x 0.02, four standard deviations
+    assert (far[0] - near[0]).abs().max() <= 4 * r * U * mag
+    for p, q in zip(far[1:], (near[1], near[2], near[3])):
+        p = p if p.shape == q.shape else p[8:]
+        assert (p.float() - q.float()).norm() <= 2.0**-7 * q.float().norm()
+    assert not far[2][:8].any() and not far[3][:8].any()
