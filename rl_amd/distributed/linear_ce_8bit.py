@@ -29,8 +29,9 @@ def _operand8(x: torch.Tensor, whole: bool) -> torch.Tensor:
     if ((not whole or H % _H_ALIGN == 0) and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
             and x.data_ptr() % 16 == 0):
         return x
-    out = torch.zeros((N, -(-H // _H_ALIGN) * _H_ALIGN), dtype=torch.uint8, device=x.device)
+    out = torch.empty((N, -(-H // _H_ALIGN) * _H_ALIGN), dtype=torch.uint8, device=x.device)
     out[:, :H].copy_(x.view(torch.uint8))
+    out[:, H:].zero_()
     return out.view(torch.float8_e4m3fn)
 
 

@@ -48,8 +48,10 @@ def _padded_last(x: torch.Tensor) -> torch.Tensor:
     """``x [N, M, K]`` contiguous, 16-byte aligned and with K a multiple of 8 (zeros past K)."""
     if x.is_contiguous() and x.shape[2] % 8 == 0 and x.data_ptr() % 16 == 0:
         return x
-    out = torch.zeros((*x.shape[:2], _round_up(x.shape[2], 8)), dtype=x.dtype, device=x.device)
-    out[:, :, : x.shape[2]].copy_(x)
+    K = x.shape[2]
+    out = torch.empty((*x.shape[:2], _round_up(K, 8)), dtype=x.dtype, device=x.device)
+    out[:, :, :K].copy_(x)
+    out[:, :, K:].zero_()
     return out
 
 
