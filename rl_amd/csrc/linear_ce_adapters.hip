@@ -15,6 +15,15 @@
 // keeps probabilities down to 2^-40), and its transpose; dH = g (G . W) runs on the tile loop
 // as well, and the adapters' three thin products on kernels of their own below, which are bound
 // by reading G (dU), its transpose (dB) and the hidden states (dA) once.
+//
+// G is the one value on the way that is rounded to 16 bits: a gradient is then off by that
+// rounding and its own (1.1 times the rounding of the result alone, measured), and G in fp32
+// would double what dH's product reads.
+//
+// Step of 8 x 2048 tokens, 8200 of them active, 4 adapters of rank 16, H = 4096, V = 151936, bf16:
+// 32 ms, of which the forward tiles 14.3, the gradient tiles 8.1 and dH 7.25 (1400 TFLOP/s, the
+// library's product of the forward's operands 1495), dU 0.62 (2.5 GB of G, 4.0 TB/s), dB 0.49
+// (5.1 TB/s), the down projection 0.11, dH's sum 0.08, dA 0.03.
 
 #include "lce_tile.h"
 #include "philox.h"
@@ -986,8 +995,8 @@ extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int6
   MIRL_REQUIRE(lda >= Hd && lda % 8 == 0 && aligned16(a) && aligned16(hidden_out) && aligned16(u_planes),
                "the adapters' rows must be 16-byte aligned (row stride %lld)", (long long)lda);
   // few rows: 16 waves share them, and workgroups their adapters, to have the loads of all in
-  // flight (64 rows of 16 adapters, H = 4096: 91 -> 18 us); many: four waves (104 us of
-  // [16384, 4096])
+  // flight (64 rows of 16 adapters, H = 4096: 91 -> 18 us, 23 with the look at 78 MB of B beside
+  // it); many: four waves (108 us of [16384, 4096])
   const bool few = T <= 2048;
   DownParams P{};
   P.hidden = static_cast<const uint16_t*>(hidden);
