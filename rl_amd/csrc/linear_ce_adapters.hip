@@ -248,7 +248,8 @@ struct DownParams {
   uint16_t* U;             // [T, kPlanes, r8]
   int64_t r8;
   float* U32;              // [rows, r8] by original row, or null
-  // and beside it, by workgroups past n_tiles: which adapters with rows hold an infinity or a
+  int64_t ny, nz;          // rank tiles, workgroups that share a row tile's adapters
+  // and beside it, by workgroups past n_tiles * ny * nz: which adapters with rows hold an infinity or a
   // NaN in B ([N, b_vecs] 16-byte pieces, `per` workgroups an adapter)
   int64_t n_tiles;
   const vu4* B;
@@ -280,25 +281,28 @@ __device__ __forceinline__ void look_through(const DownParams& P, int64_t block)
 
 // 16 sorted rows a workgroup, the hidden dimension split over its NW waves 64 elements at a
 // time.  An MFMA takes 16 ranks of the adapter against the 16 rows.  Rows of several adapters
-// are read once per adapter (from the cache after the first time); the gridDim.z workgroups of
-// the same rows take every gridDim.z-th adapter.
+// are read once per adapter (from the cache after the first time); the nz workgroups of the same
+// rows take every nz-th adapter.
 template <class E, int NT, int NW>
 __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(DownParams P) {
   __shared__ float red[NW][16][NT * 16 + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lr = lane & 15, lg = lane >> 4;
-  if ((int64_t)blockIdx.x >= P.n_tiles) {
-    if (blockIdx.y == 0 && blockIdx.z == 0) look_through<E>(P, blockIdx.x - P.n_tiles);
+  const int64_t shares = P.ny * P.nz;
+  if ((int64_t)blockIdx.x >= P.n_tiles * shares) {
+    look_through<E>(P, blockIdx.x - P.n_tiles * shares);
     return;
   }
-  const int64_t m0 = (int64_t)blockIdx.x * 16, rho0 = (int64_t)blockIdx.y * kRankTile;
+  const int64_t tile = blockIdx.x / shares, share = blockIdx.x - tile * shares;
+  const int by = (int)(share / P.nz), bz = (int)(share - by * P.nz);
+  const int64_t m0 = tile * 16, rho0 = (int64_t)by * kRankTile;
   const int64_t m = m0 + lr;
   const bool live = m < P.T;
   const int64_t row = live ? P.perm[m] : 0;
   const int32_t my_aid = live ? P.aid[m] : -1;
   const uint16_t* hr = P.hidden + row * P.ldh;
   const uint64_t seed = P.drop.threshold > 0 ? P.drop.seed_of() : 0;
-  if (blockIdx.y == 0 && blockIdx.z == 0) {
+  if (share == 0) {
     uint16_t* ho = P.h_out + m * P.ldo;
 #pragma unroll 4
     for (int64_t k0 = (int64_t)wave * 64; k0 < P.ldo; k0 += NW * 64) {
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(DownParams P) {
     a = __builtin_amdgcn_readfirstlane(a);
     if (a == 0x7fffffff) break;
     done = a;
-    if (nth % (int)gridDim.z != (int)blockIdx.z) continue;
+    if (nth % (int)P.nz != bz) continue;
     const uint16_t* Aa = P.A + ((int64_t)a * P.r + rho0) * P.lda;
     f32x4 acc[NT];
 #pragma unroll
@@ -1021,9 +1025,11 @@ extern "C" int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int6
   P.per = ceil_div(P.b_vecs, (few ? 1024 : 256) * kScanVecs);
   P.seg = seg;
   P.bad = bad;
-  const int64_t ny = ceil_div(r8, kRankTile), nz = few ? std::min(N, int64_t(16)) : 1;
-  MIRL_REQUIRE((P.n_tiles + N * P.per) * ny * nz < kMaxBlocks / 4 * (few ? 1 : 4), "too many rows or adapters");
-  const dim3 grid((unsigned)(P.n_tiles + N * P.per), (unsigned)ny, (unsigned)nz);
+  P.ny = ceil_div(r8, kRankTile);
+  P.nz = few ? std::min(N, int64_t(16)) : 1;
+  const int64_t blocks = P.n_tiles * P.ny * P.nz + N * P.per;
+  MIRL_REQUIRE(blocks < (few ? kMaxBlocks / 4 : kMaxBlocks), "too many rows or adapters");
+  const dim3 grid((unsigned)blocks);
   with_rank(dtype, r8, [&](auto e, auto nt) {
     using E = decltype(e);
     constexpr int NT = decltype(nt)::value;
