@@ -1579,11 +1579,13 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
         else:
             dw = torch.empty_like(weight)
             lib = _lib if _lib is not None else load()
-            ws = rstd.new_empty(lib.mirl_add_rms_norm_bwd_workspace_elems(R, H))
+            elems = lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)
+            if elems:
+                ws = rstd.new_empty(elems)
     st = _launch(
         "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), lddy, _ptr(g2), ldg, h2.data_ptr(), _dtype_code(h),
         ldh, rstd.data_ptr(), weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres),
-        None if ws is None else dw.data_ptr(), _ptr(ws), _stream(dev),
+        None if dw is None or R == 0 else dw.data_ptr(), _ptr(ws), _stream(dev),
     )
     if st != 0:
         _check(st, "mirl_add_rms_norm_bwd")

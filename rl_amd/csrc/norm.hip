@@ -369,7 +369,36 @@ struct NormBwd {
   void* dres;          // [R, H] of EH, or null
   float* dw_part;      // [groups, H] or null
   int64_t groups;      // rows group, group + groups, ... belong to one partial sum of dw
+  void* dw;            // [H] of the weight's type, written by the workgroups from dw_first on, or null
+  int64_t dw_first;
 };
+
+// dw of 16 columns by one workgroup that reads them again: for rows few enough to lie in the
+// caches, beside the workgroups that form dh, in place of partial sums and a second launch.
+template <class EX, class EH>
+__device__ __forceinline__ void dw_columns(const NormBwd& P, int64_t block, float (*s)[17]) {
+  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, lanes = blockDim.x >> 4;
+  const int64_t c = block * 16 + cl;
+  float v = 0.f;
+  if (c < P.H) {
+#pragma unroll 8
+    for (int64_t r = rl; r < P.R; r += lanes) {
+      const float d = EX::load(static_cast<const typename EX::raw*>(P.dy) + r * P.lddy + c);
+      const float h = EH::load(static_cast<const typename EH::raw*>(P.h) + r * P.ldh + c);
+      v = fmaf(d, h * P.rstd[r], v);
+    }
+  }
+  s[rl][cl] = v;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < P.H) {
+    float sum = 0.f;
+    for (int i = 0; i < lanes; ++i) sum += s[i][cl];
+    if (std::is_same<EX, F32>::value || P.w.f32)
+      static_cast<float*>(P.dw)[c] = sum;
+    else
+      static_cast<typename EX::raw*>(P.dw)[c] = EX::from_float(sum);
+  }
+}
 
 // One wave (NW == 1) or workgroup per group of rows; the row's two operands stay in registers
 // between the reduction and the output, and the columns' sums of dy * n across the group.
@@ -377,6 +406,11 @@ template <class EX, class EH, int NW, int NV>
 __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_bwd_kernel(NormBwd P) {
   constexpr int kRowsPerWg = NW < 4 ? 4 / NW : 1;
   __shared__ float s[NW];
+  __shared__ float s_dw[(NW < 4 ? 256 : 64 * NW) / 16][17];
+  if (P.dw != nullptr && (int64_t)blockIdx.x >= P.dw_first) {
+    dw_columns<EX, EH>(P, blockIdx.x - P.dw_first, s_dw);
+    return;
+  }
   const int64_t g = (int64_t)blockIdx.x * kRowsPerWg + (NW == 1 ? threadIdx.x >> 6 : 0);
   if (g >= P.groups) return;
   const int t = NW == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -560,6 +594,8 @@ int check_weight(int x_dtype, int w_dtype) {
   return MIRL_OK;
 }
 constexpr int64_t kMaxSide = int64_t(1) << 31, kMaxWidth = int64_t(1) << 24;
+// Elements of a batch whose dw is formed from a second read, in the same launch.
+constexpr int64_t kFewElems = int64_t(1) << 20;
 // Partial sums of dw: four workgroups per CU (eight: 108 and 11 us of [16384, 4096] against 104
 // and 6; three: 6% more).
 constexpr int64_t kMaxGroups = 1024;
@@ -610,7 +646,7 @@ extern "C" int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, co
 }
 
 extern "C" int64_t mirl_add_rms_norm_bwd_workspace_elems(int64_t R, int64_t H) {
-  if (R <= 0 || H <= 0) return 0;
+  if (R <= 0 || H <= 0 || (H <= 16384 && R * H <= kFewElems)) return 0;
   return (R < kMaxGroups ? R : kMaxGroups) * H;
 }
 
@@ -628,13 +664,16 @@ extern "C" int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, 
       MIRL_REQUIRE(dw == nullptr, "a weight gradient of no rows");
       return MIRL_OK;
     }
-    MIRL_REQUIRE(dy && h && rstd && weight && (dw == nullptr || workspace != nullptr), "null pointer argument");
+    MIRL_REQUIRE(dy && h && rstd && weight, "null pointer argument");
     MIRL_REQUIRE(R == 1 || (lddy >= H && ldh >= H && (dh_out == nullptr || ldd >= H)),
                  "row strides (%lld, %lld, %lld) are below H=%lld", (long long)lddy, (long long)ldh, (long long)ldd,
                  (long long)H);
+    MIRL_REQUIRE(dw == nullptr || workspace != nullptr || mirl_add_rms_norm_bwd_workspace_elems(R, H) == 0,
+                 "null pointer argument");
     const int64_t groups = R < kMaxGroups ? R : kMaxGroups;
-    const NormBwd P{dy, lddy, dh_out, ldd, h, ldh, rstd, Weight{weight, w_dtype == MIRL_DTYPE_F32}, R, H, dx, dres,
-                    dw != nullptr ? workspace : nullptr, groups};
+    const bool few = dw != nullptr && H <= 16384 && R * H <= kFewElems;
+    NormBwd P{dy, lddy, dh_out, ldd, h, ldh, rstd, Weight{weight, w_dtype == MIRL_DTYPE_F32}, R, H, dx, dres,
+              dw != nullptr && !few ? workspace : nullptr, groups, few ? dw : nullptr, 0};
     hipStream_t st = static_cast<hipStream_t>(stream);
     with_layout(H, [&](auto layout) -> int {
       using L = decltype(layout);
@@ -646,12 +685,14 @@ extern "C" int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, 
                              0, st, P);
       } else {
         constexpr int per = L::kNW == 1 ? 4 : 1;
-        hipLaunchKernelGGL((norm_bwd_kernel<EX, EH, L::kNW, L::kNV>), dim3((unsigned)ceil_div(groups, per)),
+        P.dw_first = ceil_div(groups, per);
+        hipLaunchKernelGGL((norm_bwd_kernel<EX, EH, L::kNW, L::kNV>),
+                           dim3((unsigned)(P.dw_first + (few ? ceil_div(H, 16) : 0))),
                            dim3(L::kNW == 1 ? 256 : 64 * L::kNW), 0, st, P);
       }
       return MIRL_OK;
     });
-    if (dw != nullptr) {
+    if (dw != nullptr && !few) {
       auto sum = [&](auto ew) {
         using EW = decltype(ew);
         hipLaunchKernelGGL(norm_dw_sum_kernel<EW>, dim3((unsigned)ceil_div(H, 32)), dim3(1024), 0, st, workspace, groups, H,

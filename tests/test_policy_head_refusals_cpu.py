@@ -135,7 +135,8 @@ def test_c_entries_return_a_status():
     assert lib.mirl_add_rms_norm_fwd(None, 3, 8, None, 3, 8, None, 3, 4, 8, 1e-6, None, None, None, None, None) != 0
     assert lib.mirl_add_rms_norm_fwd(None, 1, 8, None, 1, 8, None, 1, 4, 0, 1e-6, None, None, None, None, None) != 0
     assert lib.mirl_add_rms_norm_bwd(None, 1, 8, None, 8, None, 1, 8, None, None, 1, 4, 8, None, None, None, None, None) != 0
-    assert lib.mirl_add_rms_norm_bwd_workspace_elems(5, 8) == 40
+    assert lib.mirl_add_rms_norm_bwd_workspace_elems(5, 8) == 0  # small: formed in the same launch
+    assert lib.mirl_add_rms_norm_bwd_workspace_elems(2048, 1024) == 1024 * 1024
     assert lib.mirl_add_rms_norm_bwd_workspace_elems(0, 8) == 0
     assert lib.mirl_quantize_rows(None, 0, 8, 4, 8, None, None, None) != 0
     assert lib.mirl_dropout(None, 0, 8, 1.5, 1, None, 0, None, None) != 0
