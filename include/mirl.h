@@ -964,10 +964,9 @@ int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
  *   x[r, v] = hidden_scale[r] * weight_scale[v] * sum_k hidden8[r, k] weight8[v, k]
  *   out     = log_softmax(x[r])[target - vocab_start], 0 for targets outside
  *             [vocab_start, vocab_end)
- * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, <= Hd]; Hd a
- * multiple of 256, row strides multiples of 16, 16-byte-aligned starts.  Hidden
- * rows are zero past the true size; the weight's need no padding (a row stride
- * below Hd is allowed).  out is [bsz, T / bsz] by strides; workspace:
+ * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, Hd]; Hd and the
+ * row strides multiples of 16, 16-byte-aligned starts.  Hidden rows go on with
+ * zeros up to a multiple of 256; what lies past the weight's rows is not read.  out is [bsz, T / bsz] by strides; workspace:
  * mirl_lce_x_workspace_elems(T, V) floats.
  */
 int64_t mirl_lce_x_workspace_elems(int64_t T, int64_t V);
@@ -1018,8 +1017,8 @@ int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, co
                       int32_t* bad, void* stream);
 
 /* The logprobs of the T sorted rows (hidden, u_planes as mirl_adapter_down writes them; Hd a
- * multiple of 128, zeros past the true size; the weight's row stride may be below Hd) at their
- * original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
+ * multiple of 8, the hidden rows zero past it up to a multiple of 128; what lies past the
+ * weight's rows is not read) at their original places: out [bsz, T / bsz] by strides, row_stats [T, 2]
  * (or NULL).  target_rows: the sorted rows' targets; target [bsz, T / bsz] the original ones.
  * workspace: mirl_lce_x_workspace_elems(T, V) floats. */
 int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, int64_t ldh,

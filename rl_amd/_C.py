@@ -1638,15 +1638,14 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
                        vocab_end: int, out: torch.Tensor) -> None:
     """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd).
 
-    hidden8 [T, H] and weight8 [V, H] e4m3 (H a multiple of 256, row strides of 16; the weight's rows may be
-    shorter where the hidden rows are zero past them),
-    scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
+    hidden8 [T, >= H] and weight8 [V, H] e4m3 (H and row strides multiples of 16; the hidden rows are zero past H,
+    up to a multiple of 256), scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
     dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
-    T, H = hidden8.shape
-    V = weight8.shape[0]
+    T = hidden8.shape[0]
+    V, H = weight8.shape
     _require(hidden8.dtype == torch.float8_e4m3fn and weight8.dtype == torch.float8_e4m3fn, "e4m3 operands")
-    _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and weight8.shape[1] <= H,
-             "hidden rows that cover the weight's, with unit stride")
+    _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and hidden8.shape[1] == -(-H // 256) * 256,
+             "hidden rows padded to 256 elements, with unit stride")
     _require(hidden_scale.is_contiguous() and hidden_scale.numel() == T and hidden_scale.dtype == torch.float32
              and weight_scale.is_contiguous() and weight_scale.numel() == V and weight_scale.dtype == torch.float32,
              "a contiguous fp32 scale per row")
@@ -1741,10 +1740,10 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
                    stats: Optional[torch.Tensor]) -> None:
     """Logprobs [B, R] of the sorted rows at their own places, and their statistics [T, 2]."""
     dev = _require_gpu(h, weight, planes, b, target, out, stats)
-    T, H = h.shape
-    V = weight.shape[0]
+    T = h.shape[0]
+    V, H = weight.shape
     _check_linear_ce(h, weight)
-    _require(weight.shape[1] <= H and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
+    _require(h.shape[1] == -(-H // 128) * 128 and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
              and planes.shape == (T, 2, b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
     lib = _lib if _lib is not None else load()
     ws = torch.empty(int(lib.mirl_lce_x_workspace_elems(T, V)), dtype=torch.float32, device=dev)
@@ -1795,9 +1794,10 @@ def adapter_ce_grad(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pl
     """G [n, >= V] and its transpose of sorted rows row0 .. row0 + n (see mirl_adapter_ce_grad)."""
     dev = _require_gpu(h, weight, planes, b, G, Gt)
     _check_linear_ce(h, weight)
+    _require(h.shape[1] == -(-weight.shape[1] // 128) * 128, "hidden rows padded to 128 elements")
     _require(G.dtype == h.dtype and Gt.dtype == h.dtype and G.stride(1) == 1 and Gt.stride(1) == 1, "G of the operand type")
     st = _launch(
-        "mirl_adapter_ce_grad", dev, h.data_ptr(), _dtype_code(h), h.shape[1], h.stride(0), weight.data_ptr(),
+        "mirl_adapter_ce_grad", dev, h.data_ptr(), _dtype_code(h), weight.shape[1], h.stride(0), weight.data_ptr(),
         weight.shape[0], weight.stride(0), rows.adapter.data_ptr(), planes.data_ptr(), b.data_ptr(), b.shape[2],
         b.shape[0], rows.bad.data_ptr(),
         rows.target.data_ptr(), int(vocab_start), int(vocab_end), rows.stats.data_ptr(), int(row0), G.shape[0],

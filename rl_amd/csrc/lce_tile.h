@@ -243,12 +243,17 @@ struct LceParams {
   int64_t b_bytes;      // size of B
   // kGradX: G = (onehot - softmax) * g_scale in the operand type (rows past the end: 0)
   float g_scale;
+  // kFwdX and kGradX: W's rows hold Hw elements (whole 16-byte chunks), H's Hd, zeros past Hw
+  int64_t Hw;
   // kFwdX of e4m3: logits = products * col_scale[col] * row_scale[row]
   const float* row_scale;
   const float* col_scale;
 };
 
-template <int MODE, class E>
+// RAGGED (kFwdX, kGradX): Hw is not a whole number of stage pairs.  What lies past a row of W is then
+// masked in the last two stages' loads: it is the next row's beginning, or no part of W, and an
+// infinity or a NaN there must not meet the zeros of H's rows.
+template <int MODE, class E, bool RAGGED = false>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void lce_tile_kernel(LceParams P) {
   using frag = typename Mma<E>::frag;
@@ -457,6 +462,19 @@ void lce_tile_kernel(LceParams P) {
     voff_a[i] = (int)(row * P.ldh * kES) + chunk * 16;
     voff_b[i] = (int)(row * P.ldw * kES) + chunk * 16;
   }
+  constexpr int kOut = -0x7fffffff - 1;  // an offset out of range: reads as zero
+  // RAGGED: from stage t on, one of the last two, the chunks past W's row are out of range.
+  auto end_w = [&](int t) __attribute__((always_inline)) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (see prepare)
+    const int left = (int)(P.Hw * kES) - t * kRowBytes;
+#pragma unroll
+    for (int i = 0; i < kDmaPerWave; ++i) {
+      // a load's rows start at a multiple of 8, so its chunks depend on its parity only
+      const int chunk = (ln & 7) ^ (((ln >> 4) + 4 * (i & 1)) & 7);
+      voff_b[i] = chunk * 16 >= left ? kOut : voff_b[i];
+    }
+  };
   // load q of stage data t: q < kDmaPerWave is an H block, else a W block
   auto dma = [&](unsigned char* stage, int t, int q) {
     const int soff = kAdapters && t >= nst ? 0 : t * kRowBytes;
@@ -482,7 +500,6 @@ void lce_tile_kernel(LceParams P) {
   const int n_ext = (n_seg * cps + 7) >> 3;
   const int total = kAdapters && !apart ? nst + (n_ext + 1) / 2 * 2 : nst;
   auto prepare = [&](int t) __attribute__((always_inline)) {
-    constexpr int kOut = -0x7fffffff - 1;
     // opaque here, or everything that follows from it is formed ahead of the main loop and
     // kept in registers that it lacks
     int ln = lane;
@@ -643,17 +660,27 @@ void lce_tile_kernel(LceParams P) {
   };
   auto run_stages = [&]() __attribute__((always_inline)) {
     // Prologue: stage data 0 and 1 in flight; wait for 0 and read its block-0 fragments.
+    if (RAGGED && nst == kStages) end_w(0);
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st0, 0, q);
+    if (RAGGED && nst == kStages) end_w(1);
 #pragma unroll
     for (int q = 0; q < kL; ++q) dma(st1, 1, q);
     wait_vm_barrier<kL>();
 #pragma unroll
     for (int idx = 0; idx < kTM + kTN; ++idx) fread(0, st0, 0, idx);
     int t = 0;
-    for (; t < nst - kStages; t += kStages) {
+    for (; t < nst - (RAGGED ? 2 : 1) * kStages; t += kStages) {
       step(t, S0{}, T_{}, T_{});
       step(t + 1, S1{}, T_{}, T_{});
+    }
+    if constexpr (RAGGED) {
+      for (; t < nst - kStages; t += kStages) {  // the last two stages' loads
+        end_w(t + kStages);
+        step(t, S0{}, T_{}, T_{});
+        end_w(t + 1 + kStages);
+        step(t + 1, S1{}, T_{}, T_{});
+      }
     }
     if constexpr (kAdapters) {
       for (; t < total - kStages; t += kStages) {
@@ -1199,8 +1226,9 @@ void lce_tile_kernel(LceParams P) {
 constexpr int kRM = 64, kRN = 128, kRStages = 3;
 constexpr int kRStageBytes = (kRM + kRN) * kRowBytes;          // 24 KB: the H rows, then W's
 constexpr int kRLoadsA = kRM / kDmaRows / kWaves, kRLoadsB = kRN / kDmaRows / kWaves;  // per wave and stage
+static_assert(kRLoadsB % 2 == 0 && kDmaPerWave % 2 == 0, "a load's parity among the wave's is that of its rows' eights");
 
-template <class E>
+template <class E, bool RAGGED>
 __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   using frag = typename Mma<E>::frag;
   using acc_t = typename Mma<E>::acc_t;
@@ -1299,9 +1327,15 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_a, (lds_ptr_t)(stage + (wave_u * kRLoadsA + i) * kDmaBytes), 16,
                                                voff_a[i], soff, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kRLoadsB; ++i)
+    for (int i = 0; i < kRLoadsB; ++i) {
+      int off = voff_b[i];
+      if constexpr (RAGGED) {  // past W's row (see lce_tile_kernel)
+        const int left = t < nst ? (int)(P.Hw * kES) - t * kRowBytes : kRowBytes;
+        off = ((lane & 7) ^ (((lane >> 4) + 4 * (i & 1)) & 7)) * 16 >= left ? kOut : off;
+      }
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc_b, (lds_ptr_t)(stage + kRM * kRowBytes + (wave_u * kRLoadsB + i) * kDmaBytes), 16, voff_b[i], soff, 0, 0);
+          rsrc_b, (lds_ptr_t)(stage + kRM * kRowBytes + (wave_u * kRLoadsB + i) * kDmaBytes), 16, off, soff, 0, 0);
+    }
   };
   // offsets of stage data t >= nst (see lce_tile_kernel)
   auto prepare = [&](int t) __attribute__((always_inline)) {
@@ -1532,6 +1566,11 @@ __global__ __launch_bounds__(256) void lce_merge_kernel(
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Hd of LceParams for a weight whose rows hold Hw elements of `bytes` bytes: whole pairs of stages.
+int64_t padded_hidden(int64_t Hw, int64_t bytes) {
+  const int64_t pair = kStages * kRowBytes / bytes;
+  return ceil_div(Hw, pair) * pair;
+}
 
 // The forward kernel with fp32 logits for T rows (P.part, P.xt not set yet: `workspace` holds
 // mirl_lce_x_workspace_elems(T, V) floats).  Returns the number of tiles.
@@ -1548,10 +1587,10 @@ int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
   P.xt = workspace + P.nrows * P.n_nt * 2;
   const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
   if (grid >= (int64_t(1) << 24)) return grid;  // a launch holds fewer than 2^32 threads
-  if (few)
-    hipLaunchKernelGGL(lce_rows_kernel<E>, dim3((unsigned)grid), dim3(kThreads), 0, st, P);
-  else
-    hipLaunchKernelGGL((lce_tile_kernel<kFwdX, E>), dim3((unsigned)grid), dim3(kThreads), 0, st, P);
+  const bool ragged = P.Hw != P.Hd;
+  const auto kernel = few ? ragged ? lce_rows_kernel<E, true> : lce_rows_kernel<E, false>
+                          : ragged ? lce_tile_kernel<kFwdX, E, true> : lce_tile_kernel<kFwdX, E, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, P);
   return grid;
 }
 

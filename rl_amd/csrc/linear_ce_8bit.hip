@@ -52,9 +52,8 @@ __global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float*
   const uint8_t* hr = static_cast<const uint8_t*>(P.h) + r * P.ldh;
   const uint8_t* wr = static_cast<const uint8_t*>(P.w) + (t - P.vs) * P.ldw;
   float dot[4] = {0.f, 0.f, 0.f, 0.f};
-  const int64_t width = P.Hd < P.ldw ? P.Hd : P.ldw;  // (multiples of 16)
 #pragma unroll 4
-  for (int64_t k = (W == 1 ? lane : threadIdx.x) * 16; k < width; k += 64 * W * 16) {
+  for (int64_t k = (W == 1 ? lane : threadIdx.x) * 16; k < P.Hw; k += 64 * W * 16) {
     const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const vu4*>(wr + k);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -105,17 +104,13 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   MIRL_REQUIRE(T >= 0 && V > 0 && Hd > 0 && bsz > 0, "invalid shape T=%lld V=%lld H=%lld B=%lld", (long long)T,
                (long long)V, (long long)Hd, (long long)bsz);
   MIRL_REQUIRE(T % bsz == 0, "row count %lld is not a multiple of the batch size %lld", (long long)T, (long long)bsz);
-  MIRL_REQUIRE(Hd % (kStages * kRowBytes) == 0, "hidden size %lld must be a multiple of %d", (long long)Hd,
-               kStages * kRowBytes);
   // buffer ranges of one 256-row tile are 32-bit byte counts
   MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22),
                "row strides (%lld, %lld) must be below 2^22 elements", (long long)ldh, (long long)ldw);
-  // The weight's rows may be shorter than Hd: what is read past a row's end is the next row's
-  // beginning, and zero past the last row's, against zeros of the hidden rows.  A NaN there
-  // stands in the next column's logits as well, so it changes no logprob.
-  MIRL_REQUIRE(ldh % 16 == 0 && ldw % 16 == 0 && ldh >= Hd && ldw > 0,
-               "row strides (%lld, %lld) must be multiples of 16 elements, the hidden states' >= the hidden size",
-               (long long)ldh, (long long)ldw);
+  const int64_t padded = padded_hidden(Hd, 1);
+  MIRL_REQUIRE(Hd % 16 == 0 && ldh % 16 == 0 && ldw % 16 == 0 && ldh >= padded && ldw >= Hd,
+               "hidden size %lld and row strides (%lld, %lld) must be multiples of 16, the hidden states' rows padded to %lld",
+               (long long)Hd, (long long)ldh, (long long)ldw, (long long)padded);
   MIRL_REQUIRE(V < (int64_t(1) << 31) && T < (int64_t(1) << 31), "sizes exceed 2^31-1");
   if (T == 0) return MIRL_OK;
   MIRL_REQUIRE(hidden8 && hidden_scale && weight8 && weight_scale && target && out && workspace,
@@ -128,7 +123,8 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   P.ldh = ldh;
   P.ldw = ldw;
   P.V = V;
-  P.Hd = Hd;
+  P.Hd = padded;
+  P.Hw = Hd;
   P.nrows = T;
   P.bsz = bsz;
   P.target = target;

@@ -937,17 +937,14 @@ void with_rank(int dtype, int64_t r8, F&& f) {
     go(F16{});
 }
 
-// (The weight's rows may be shorter than Hd: what the tile loop reads past a row's end is the next
-// row's beginning, and zero past the last row's, against zeros of the hidden rows.  An infinity or
-// a NaN there stands in the next column's logits as well, so it changes no logprob.)
 int check_operands(int dtype, const void* hidden, int64_t Hd, int64_t ldh, const void* weight, int64_t V, int64_t ldw) {
   MIRL_REQUIRE(is16(dtype), "hidden states, weight and adapters must be bf16 or fp16 (dtype code %d)", dtype);
   MIRL_REQUIRE(V > 0 && Hd > 0 && V < (int64_t(1) << 31), "invalid shape V=%lld H=%lld", (long long)V, (long long)Hd);
-  MIRL_REQUIRE(Hd % (kStages * kSK) == 0, "hidden size %lld must be a multiple of %d", (long long)Hd, kStages * kSK);
-  MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22) && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= Hd &&
-                   ldw > 0,
-               "row strides (%lld, %lld) must be multiples of 8 elements, the hidden states' >= the hidden size, and below 2^22",
-               (long long)ldh, (long long)ldw);
+  MIRL_REQUIRE(Hd % 8 == 0 && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= padded_hidden(Hd, 2) && ldw >= Hd &&
+                   ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22),
+               "hidden size %lld and row strides (%lld, %lld) must be multiples of 8, the hidden states' rows padded to %lld, "
+               "and the strides below 2^22",
+               (long long)Hd, (long long)ldh, (long long)ldw, (long long)padded_hidden(Hd, 2));
   MIRL_REQUIRE(aligned16(hidden) && aligned16(weight), "hidden states and weight must be 16-byte aligned");
   return MIRL_OK;
 }
@@ -1060,7 +1057,8 @@ extern "C" int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int
   P.ldh = ldh;
   P.ldw = ldw;
   P.V = V;
-  P.Hd = Hd;
+  P.Hd = padded_hidden(Hd, 2);
+  P.Hw = Hd;
   P.nrows = T;
   P.bsz = 1;
   P.target = target_rows;
@@ -1151,7 +1149,8 @@ extern "C" int mirl_adapter_ce_grad(const void* hidden, int dtype, int64_t Hd, i
   P.ldh = ldh;
   P.ldw = ldw;
   P.V = V;
-  P.Hd = Hd;
+  P.Hd = padded_hidden(Hd, 2);
+  P.Hw = Hd;
   P.row0 = row0;
   P.nrows = nrows;
   P.bsz = 1;
@@ -1176,15 +1175,16 @@ extern "C" int mirl_adapter_ce_grad(const void* hidden, int dtype, int64_t Hd, i
   P.b_bytes = N * V * r8 * 2;
   const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
   MIRL_REQUIRE(grid < (int64_t(1) << 24), "too many tiles");
-  if (dtype == MIRL_DTYPE_BF16) {
-    P.g_scale = g_scale_of<BF16>();
-    hipLaunchKernelGGL((lce_tile_kernel<kGradX, BF16>), dim3((unsigned)grid), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), P);
-  } else {
-    P.g_scale = g_scale_of<F16>();
-    hipLaunchKernelGGL((lce_tile_kernel<kGradX, F16>), dim3((unsigned)grid), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), P);
-  }
+  auto launch = [&](auto e) {
+    using E = decltype(e);
+    P.g_scale = g_scale_of<E>();
+    const auto kernel = P.Hw != P.Hd ? lce_tile_kernel<kGradX, E, true> : lce_tile_kernel<kGradX, E, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream), P);
+  };
+  if (dtype == MIRL_DTYPE_BF16)
+    launch(BF16{});
+  else
+    launch(F16{});
   return check_launch("mirl_adapter_ce_grad");
 }
 

@@ -22,11 +22,11 @@ _H_ALIGN = 256  # the kernel steps through the hidden dimension 256 elements at 
 
 
 def _operand8(x: torch.Tensor, whole: bool) -> torch.Tensor:
-    """``x [N, H]`` e4m3 as the kernel reads it: row strides multiples of 16, a 16-byte-aligned
+    """``x [N, H]`` e4m3 as the kernel reads it: ``H`` and row strides multiples of 16, a 16-byte-aligned
     start, and with ``whole`` (the hidden states) ``H`` a multiple of 256; otherwise a zero-padded
     copy (the padding adds exact zeros)."""
     N, H = x.shape
-    if ((not whole or H % _H_ALIGN == 0) and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
+    if (H % (_H_ALIGN if whole else 16) == 0 and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
             and x.data_ptr() % 16 == 0):
         return x
     out = torch.empty((N, -(-H // _H_ALIGN) * _H_ALIGN), dtype=torch.uint8, device=x.device)

@@ -56,9 +56,10 @@ def _padded_last(x: torch.Tensor) -> torch.Tensor:
 
 
 def _weight_operand(w: torch.Tensor) -> torch.Tensor:
-    """``w [V, H]`` as the tile loop reads it against zero-padded hidden rows: row strides multiples
-    of 8 and a 16-byte-aligned start, or a padded copy."""
-    return w if w.stride(0) % 8 == 0 and w.stride(0) >= w.shape[1] and w.data_ptr() % 16 == 0 else _kernel_operand(w)
+    """``w [V, H]`` as the tile loop reads it against zero-padded hidden rows: ``H`` and the row stride
+    multiples of 8 and a 16-byte-aligned start, or a padded copy."""
+    H, ld = w.shape[1], w.stride(0)
+    return w if H % 8 == 0 and ld % 8 == 0 and ld >= H and w.data_ptr() % 16 == 0 else _kernel_operand(w)
 
 
 class _AdapterLogprobs(torch.autograd.Function):

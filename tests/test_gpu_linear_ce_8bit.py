@@ -168,3 +168,20 @@ def test_norm_into_the_head():
     got = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 2000)
     want, tol = oracle(h8, hs, w8, ws, target, 0, 2000)
     assert torch.all((got.cpu().double() - want).abs() <= tol)
+
+
+@pytest.mark.parametrize("S", [9, 200])
+@pytest.mark.parametrize("H,left,wide", [(48, 16, 64), (256 + 16, 0, 512), (400, 112, 512), (1008, 16, 1024), (80, 16, 800)])
+def test_nothing_past_the_weights_rows_is_read(S, H, left, wide):
+    """The weight as columns of a wider tensor whose other bytes are NaN (its last row may end the
+    storage): what a contiguous copy gives, and what zero-padded rows give (the padding adds exact
+    zeros; the target's logit is formed over the same elements)."""
+    h8, hs, w8, ws, target = inputs(S, 2, H, 300, seed=H)
+    buf = torch.full((300, wide), 0x7F, dtype=torch.uint8, device=DEV)
+    buf[:, left : left + H] = w8.view(torch.uint8)
+    sliced = buf.view(torch.float8_e4m3fn)[:, left : left + H]
+    got = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, sliced, ws, target, 0, 300)
+    assert torch.equal(got, from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 300))
+    pad = -(-H // 256) * 256 - H
+    h8p, w8p = (torch.nn.functional.pad(t.view(torch.uint8), (0, pad)).view(torch.float8_e4m3fn) for t in (h8, w8))
+    assert torch.equal(got, from_parallel_8bit_hidden_states_to_logprobs(h8p, hs, w8p, ws, target, 0, 300))

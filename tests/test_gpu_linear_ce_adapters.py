@@ -331,3 +331,37 @@ def test_adapters_of_more_than_2_gib(S):
         p = p if p.shape == q.shape else p[8:]
         assert (p.float() - q.float()).norm() <= 2.0**-7 * q.float().norm()
     assert not far[2][:8].any() and not far[3][:8].any()
+
+
+@pytest.mark.parametrize("S", [9, 200])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("H,left,wide", [(40, 24, 64), (128 + 8, 0, 256), (200, 56, 256), (1000, 16, 1024), (72, 8, 400)])
+def test_nothing_past_the_weights_rows_is_read(S, dtype, H, left, wide):
+    """The weight as columns of a wider tensor whose other columns are NaN (its last row may end the
+    storage): what a contiguous copy gives, and what zero-padded hidden states, weight and
+    adapters give (the padding adds exact zeros)."""
+    x = inputs(S, 2, H, 300, 2, 8, dtype, seed=H, ids=[1, 0])
+    buf = torch.full((300, wide), float("nan"), dtype=dtype, device=DEV)
+    buf[:, left : left + H] = x["weight"]
+    pad = -(-H // 128) * 128 - H
+    zero_padded = {k: torch.nn.functional.pad(x[k], (0, pad)) for k in ("hidden", "weight", "a")}
+    lp, grads = run({**x, "weight": buf[:, left : left + H]})
+    lp2, grads2 = run(x)
+    assert torch.equal(lp, lp2) and all(torch.equal(grads[k], grads2[k]) for k in grads)
+    lp2, grads2 = run({**x, **zero_padded})  # (dH's sum over the vocabulary is split by the padded size)
+    assert torch.equal(lp, lp2) and torch.equal(grads["b"], grads2["b"])
+
+
+@pytest.mark.parametrize("S", [9, 200])
+def test_infinity_in_the_next_row_of_the_weight(S):
+    """A token that an infinity rules out (logit -inf) leaves the others as without it."""
+    H, V = 200, 300
+    x = inputs(S, 2, H, V, 2, 8, BF, ids=[1, 0])
+    x["hidden"][..., 0] = x["hidden"][..., 0].abs() + 0.5
+    x["target"] = x["target"] % 17
+    x["b"][:, 17:] = 0
+    weight = x["weight"].clone()
+    weight[17:, 0] = -float("inf")
+    got, _ = run({**x, "weight": weight}, grads=())
+    want = oracle({**x, "weight": weight[:17], "b": x["b"][:, :17].contiguous()})
+    assert bool(((got.double() - want["lp"]).abs() <= want["lp_tol"]).all())
