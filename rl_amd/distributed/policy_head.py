@@ -58,8 +58,14 @@ def from_residual_stream_to_logprobs(
 
     ``output_weight_layer`` is the weight ``[V, H]``, or the pair that
     :func:`~rl_amd.distributed.final_norm.quantize_rows_8bit` makes of it, with which the norm's rows
-    are 8-bit as well; that form has no gradient and takes no adapters.  The other arguments are those of the
+    are 8-bit as well; that form has no gradient and takes no adapters.  With ``inference_only`` no part
+    keeps anything for a backward and the result has none.  The other arguments are those of the
     functions named above."""
+    if inference_only and torch.is_grad_enabled():
+        with torch.no_grad():
+            return from_residual_stream_to_logprobs(
+                x, residual, norm_weight, output_weight_layer, target, vocab_start_index, vocab_end_index, eps, adapters,
+                tp_group, True, cp_group, chunk_size)
     if isinstance(output_weight_layer, (tuple, list)):
         if adapters is not None:
             raise NotImplementedError("adapters stand beside a 16-bit output weight")

@@ -131,3 +131,19 @@ def test_the_whole_step_captured_and_replayed():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
+@pytest.mark.parametrize("form", ["8 bits", "16 bits", "adapters"])
+def test_inference_only_of_a_policy_in_training(form):
+    """Parameters that ask for gradients, gradients on: the same logprobs as without, and no graph."""
+    x = inputs(5)
+    xs, res, nw, a, b, w = leaves(x, "x", "res", "nw", "a", "b", "w")
+    weight = quantize_rows_8bit(x["w"]) if form == "8 bits" else w
+    ids = torch.tensor([0, 1, -1, 2], device=DEV)
+    lp = from_residual_stream_to_logprobs(xs, res, nw, weight, x["target"], 0, V, inference_only=True,
+                                          adapters=HeadAdapters(a, b, ids) if form == "adapters" else None)
+    assert not lp.requires_grad
+    with torch.no_grad():
+        want = from_residual_stream_to_logprobs(x["x"], x["res"], x["nw"], weight, x["target"], 0, V,
+                                                adapters=HeadAdapters(x["a"], x["b"], ids) if form == "adapters" else None)
+    assert torch.equal(lp, want)
