@@ -929,8 +929,8 @@ int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* r
  * dh_out (the gradient of the returned h, of h_dtype) may be NULL.  dx (x_dtype)
  * and dres (h_dtype) receive dh, either may be NULL; dw (w_dtype, [H]) may be
  * NULL and otherwise needs a workspace of mirl_add_rms_norm_bwd_workspace_elems
- * floats (none for small batches) and at least one row.  Sums are fp32 in an order that depends on the
- * sizes only.
+ * floats (none for small batches) and at least one row.  Sums are fp32 in an
+ * order that depends on the sizes only.  No output may overlap an input.
  */
 int64_t mirl_add_rms_norm_bwd_workspace_elems(int64_t R, int64_t H);
 int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, const void* dh_out,
