@@ -522,12 +522,8 @@ __device__ __forceinline__ int64_t block_rows(const BlockParams& P) {
   return c < 0 ? 0 : c < P.n ? c : P.n;
 }
 
-__global__ void adapter_zero_kernel(uint32_t* p) {
-  if (threadIdx.x < 2) p[threadIdx.x] = 0;
-}
-
 // dU's partial sums: a wave takes 32 rows and a range of the vocabulary, once per adapter
-// among its rows.
+// among its rows.  (Also clears the maxima that the next kernel takes.)
 template <class E, int NT>
 __global__ __launch_bounds__(256) void adapter_du_kernel(BlockParams P) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -536,6 +532,7 @@ __global__ __launch_bounds__(256) void adapter_du_kernel(BlockParams P) {
   const int64_t n_rt = (P.n + 127) / 128;
   const int64_t split = blockIdx.x / n_rt, rt = blockIdx.x - split * n_rt;
   const int64_t w0 = rt * 128 + wave * 32, rho0 = (int64_t)blockIdx.y * kRankTile;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid < 2) P.peak[tid] = 0;
   if (w0 >= n) return;
   const int64_t w1 = w0 + 32 < n ? w0 + 32 : n;
   const int64_t k_end = (split + 1) * P.k_len < P.ldbt ? (split + 1) * P.k_len : P.ldbt;
@@ -735,7 +732,8 @@ __device__ __forceinline__ void thin_product(const uint16_t* const (&x)[MT], con
   for (; k0 < hi; k0 += step) thin_piece<E, NT, MT>(x, y, plane, ldn, k0, lo, hi, lg, acc);
 }
 
-// dB_a += G^T . (g U): 32 vocabulary rows a wave, once per adapter with rows in the block.
+// dB_a += G^T . (g U): 32 vocabulary rows a wave, once per adapter with rows in the block; with
+// few vocabulary rows gridDim.z workgroups share their adapters.
 template <class E, int NT>
 __global__ __launch_bounds__(256) void adapter_db_kernel(BlockParams P) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -750,11 +748,12 @@ __global__ __launch_bounds__(256) void adapter_db_kernel(BlockParams P) {
   const uint16_t* y = P.ugT + (rho0 + lr) * P.ldn;
   int64_t a = P.aid[P.row0] < 0 ? 0 : P.aid[P.row0];
   const int64_t a_last = P.aid[P.row0 + n - 1];
+  unsigned nth = 0;
   for (; a <= a_last; ++a) {
     int64_t lo = P.seg[a] - P.row0, hi = P.seg[a + 1] - P.row0;
     lo = lo < 0 ? 0 : lo;
     hi = hi > n ? n : hi;
-    if (lo >= hi) continue;
+    if (lo >= hi || nth++ % gridDim.z != blockIdx.z) continue;
     f32x4 acc[2][NT];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -817,25 +816,25 @@ __global__ __launch_bounds__(kDaWaves * 64) void adapter_da_kernel(BlockParams P
   }
 }
 
-// dH of the block's rows: g (sum of the splits of G . W) + dropout'(dU . A_a), rounded once.  Four
+// dH of the block's rows: g (sum of the splits of G . W) + dropout'(dU . A_a), rounded once.  ROWS
 // rows a workgroup, eight columns a thread; the rows' adapters one after the other.
 constexpr int kDhRows = 4;
-template <class E>
+template <class E, int ROWS>
 __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
-  extern __shared__ float du_s[];  // [kDhRows][r8]
+  extern __shared__ float du_s[];  // [ROWS][r8]
   const int64_t n = block_rows(P);
   const int64_t n_ct = (P.H + 2047) / 2048;
   const int64_t rt = blockIdx.x / n_ct, ct = blockIdx.x - rt * n_ct;
-  const int64_t m0 = rt * kDhRows, c = (ct * 256 + threadIdx.x) * 8;
+  const int64_t m0 = rt * ROWS, c = (ct * 256 + threadIdx.x) * 8;
   if (m0 >= n) return;
-  const int rows = n - m0 < kDhRows ? (int)(n - m0) : kDhRows;
+  const int rows = n - m0 < ROWS ? (int)(n - m0) : ROWS;
   for (int q = threadIdx.x; q < rows * (int)P.r8; q += 256) du_s[q] = P.du[m0 * P.r8 + q];
   __syncthreads();
   if (c >= P.H) return;
   const bool full = c + 8 <= P.H;
-  float add[kDhRows][8];
+  float add[ROWS][8];
 #pragma unroll
-  for (int i = 0; i < kDhRows; ++i)
+  for (int i = 0; i < ROWS; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) add[i][e] = 0.f;
   int cur = 0;
@@ -845,15 +844,22 @@ __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
     const int next = end < rows ? (int)end : rows;
     if (a >= 0) {
       const uint16_t* Aa = P.A + (int64_t)a * P.r * P.lda;
-      for (int64_t rho = 0; rho < P.r; ++rho) {
-        float w[8];
-        E::unpack(load_raw8_to(Aa + rho * P.lda, c, P.H), w);
+      // four ranks at a time, their loads in flight together (r8 holds a multiple of eight)
+      for (int64_t rho = 0; rho < P.r; rho += 4) {
+        vu4 q[4];
 #pragma unroll
-        for (int i = 0; i < kDhRows; ++i) {
-          if (i < cur || i >= next) continue;
-          const float d = du_s[i * P.r8 + rho];
+        for (int j = 0; j < 4; ++j) q[j] = rho + j < P.r ? load_raw8_to(Aa + (rho + j) * P.lda, c, P.H) : zero4();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) add[i][e] = fmaf(d, w[e], add[i][e]);
+        for (int j = 0; j < 4; ++j) {
+          float w[8];
+          E::unpack(q[j], w);
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            if (i < cur || i >= next) continue;
+            const float d = du_s[i * P.r8 + rho + j];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) add[i][e] = fmaf(d, w[e], add[i][e]);
+          }
         }
       }
     }
@@ -862,37 +868,39 @@ __global__ __launch_bounds__(256) void adapter_dh_kernel(BlockParams P) {
   const uint64_t seed = P.drop.threshold > 0 ? P.drop.seed_of() : 0;
   // the splits' sums of all rows, their loads in flight together (rows past the block's end
   // read its last one)
-  float sum[kDhRows][8];
+  float sum[ROWS][8];
 #pragma unroll
-  for (int i = 0; i < kDhRows; ++i)
+  for (int i = 0; i < ROWS; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[i][e] = 0.f;
   const bool vec = full && P.H % 4 == 0;
+  constexpr int kU = ROWS == 1 ? 4 : 1;
+#pragma unroll kU
   for (int64_t s = 0; s < P.h_splits; ++s) {
     const float* src = P.h_part + (s * P.n + m0) * P.H + c;
     if (vec) {
-      float4 q[kDhRows][2];
+      float4 q[ROWS][2];
 #pragma unroll
-      for (int i = 0; i < kDhRows; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         const float4* row = reinterpret_cast<const float4*>(src + (i < rows ? i : rows - 1) * P.H);
         q[i][0] = row[0];
         q[i][1] = row[1];
       }
 #pragma unroll
-      for (int i = 0; i < kDhRows; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         sum[i][0] += q[i][0].x; sum[i][1] += q[i][0].y; sum[i][2] += q[i][0].z; sum[i][3] += q[i][0].w;
         sum[i][4] += q[i][1].x; sum[i][5] += q[i][1].y; sum[i][6] += q[i][1].z; sum[i][7] += q[i][1].w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kDhRows; ++i)
+      for (int i = 0; i < ROWS; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (i < rows && c + e < P.H) sum[i][e] += src[i * P.H + e];
     }
   }
 #pragma unroll
-  for (int i = 0; i < kDhRows; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     if (i >= rows) break;
     const int64_t m = m0 + i, row = P.perm[P.row0 + m];
     const float g = P.g[P.row0 + m] * (1.f / g_scale_of<E>());
@@ -1309,10 +1317,15 @@ extern "C" int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, cons
   P.dB = db;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned ny = (unsigned)ceil_div(r8, kRankTile);
+  // dB: about four workgroups a CU (774 rows of 3 adapters, V = 32003: 31 -> 21 us)
+  const unsigned nz = (unsigned)std::min(N, std::max(int64_t(1), 1024 / (ceil_div(V, 128) * ny)));
+  // dH: four rows a workgroup read A once for them; one, where that leaves CUs idle (774 rows of
+  // H = 1000 with 16 splits: 24.6 -> 17.7 us)
+  const int64_t n_ct = ceil_div(Hd, 2048);
+  const bool few = ceil_div(n, kDhRows) * n_ct < 1024;
   MIRL_REQUIRE(ceil_div(n, 128) * splits * ny < kMaxBlocks && ceil_div(V, 128) * ny < kMaxBlocks &&
-                   ceil_div(Hd, 16) * ny < kMaxBlocks / 4 && ceil_div(n, kDhRows) * ceil_div(Hd, 2048) < kMaxBlocks,
+                   ceil_div(Hd, 16) * ny < kMaxBlocks / 4 && ceil_div(n, kDhRows) * n_ct < kMaxBlocks,
                "too many tiles");
-  if (dtype == MIRL_DTYPE_F16) hipLaunchKernelGGL(adapter_zero_kernel, dim3(1), dim3(64), 0, st, P.peak);
   with_rank(dtype, r8, [&](auto e, auto nt_c) {
     using E = decltype(e);
     constexpr int NT = decltype(nt_c)::value;
@@ -1321,11 +1334,13 @@ extern "C" int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, cons
     hipLaunchKernelGGL(adapter_du_sum_kernel<E>, flat, dim3(256), 0, st, P);
     if (da != nullptr || db != nullptr) hipLaunchKernelGGL(adapter_planes_kernel<E>, flat, dim3(256), 0, st, P);
     if (db != nullptr)
-      hipLaunchKernelGGL((adapter_db_kernel<E, NT>), dim3((unsigned)ceil_div(V, 128), ny), dim3(256), 0, st, P);
+      hipLaunchKernelGGL((adapter_db_kernel<E, NT>), dim3((unsigned)ceil_div(V, 128), ny, nz), dim3(256), 0, st, P);
     if (da != nullptr)
       hipLaunchKernelGGL((adapter_da_kernel<E, NT>), dim3((unsigned)ceil_div(Hd, 16), ny), dim3(kDaWaves * 64), 0, st, P);
-    if (dh != nullptr)
-      hipLaunchKernelGGL(adapter_dh_kernel<E>, dim3((unsigned)(ceil_div(n, kDhRows) * ceil_div(Hd, 2048))), dim3(256),
+    if (dh != nullptr && few)
+      hipLaunchKernelGGL((adapter_dh_kernel<E, 1>), dim3((unsigned)(n * n_ct)), dim3(256), (unsigned)(r8 * 4), st, P);
+    else if (dh != nullptr)
+      hipLaunchKernelGGL((adapter_dh_kernel<E, kDhRows>), dim3((unsigned)(ceil_div(n, kDhRows) * n_ct)), dim3(256),
                          (unsigned)(kDhRows * r8 * 4), st, P);
   });
   return check_launch("mirl_adapter_block_grads");
