@@ -10,6 +10,7 @@ fallback implementation.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 from typing import Optional
@@ -1526,67 +1527,97 @@ def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t.new_empty(t.shape, dtype=dtype)
 
 
+def _direct(dev: torch.device) -> bool:
+    """Whether a launch on ``dev`` can go straight to the loaded library: small calls of the norm and
+    dropout are host work, of which _launch and its stream object are 3 us."""
+    return _timer is None and _lib is not None and _raw_stream is not None and dev.index == _current_device()
+
+
 def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
                      want_rstd: bool, out8: bool):
-    """(y, h, rstd or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
-    itself without a residual, rstd and scale have a row's shape.  Shapes and types are the
-    caller's to check."""
-    dev = _require_gpu(x, residual, weight)
-    shape = x.shape
+    """(y, h, rstd [R] or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
+    itself without a residual, scale has a row's shape.  Shapes and types are the caller's to check."""
+    dev = x.device
+    if not x.is_cuda or weight.device != dev or (residual is not None and residual.device != dev):
+        _require_gpu(x, residual, weight)
+    shape, dtype = x.shape, x.dtype
     H = shape[-1]
-    x2, ldx = _rows2(x)
+    R = x.numel() // H
+    code = DTYPE_CODES[dtype]
+    if x.is_contiguous():
+        x2, ldx = x, H
+        y = torch.empty_like(x, dtype=torch.float8_e4m3fn) if out8 else torch.empty_like(x)
+    else:
+        x2, ldx = _rows2(x)
+        y = x.new_empty(shape, dtype=torch.float8_e4m3fn if out8 else dtype)
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    x_code = _dtype_code(x)
     if residual is None:
-        h, r_ptr, ldr, h_ptr, h_code = x, None, 0, None, x_code
+        h, r_ptr, ldr, h_ptr, h_code = x, None, 0, None, code
     else:
-        r2, ldr = _rows2(residual)
-        h = _new_like(residual, residual.dtype)
-        r_ptr, h_ptr, h_code = r2.data_ptr(), h.data_ptr(), _dtype_code(residual)
-    y = _new_like(x, torch.float8_e4m3fn if out8 else x.dtype)
+        if residual.is_contiguous():
+            r2, ldr, h = residual, H, torch.empty_like(residual)
+        else:
+            r2, ldr = _rows2(residual)
+            h = residual.new_empty(shape)
+        r_ptr, h_ptr, h_code = r2.data_ptr(), h.data_ptr(), DTYPE_CODES[residual.dtype]
     scale = x.new_empty(shape[:-1], dtype=torch.float32) if out8 else None
-    rstd = x.new_empty(shape[:-1], dtype=torch.float32) if want_rstd else None
-    st = _launch(
-        "mirl_add_rms_norm_fwd", dev, x2.data_ptr(), x_code, ldx, r_ptr, h_code, ldr, weight.data_ptr(),
-        _dtype_code(weight), x.numel() // H, H, eps, h_ptr, y.data_ptr(), _ptr(scale), _ptr(rstd), _stream(dev),
-    )
+    rstd = torch.empty(R, dtype=torch.float32, device=dev) if want_rstd else None
+    args = (x2.data_ptr(), code, ldx, r_ptr, h_code, ldr, weight.data_ptr(), DTYPE_CODES[weight.dtype], R, H, eps, h_ptr,
+            y.data_ptr(), None if scale is None else scale.data_ptr(), None if rstd is None else rstd.data_ptr())
+    if _direct(dev):
+        st = _lib.mirl_add_rms_norm_fwd(*args, _raw_stream(dev.index))
+    else:
+        st = _launch("mirl_add_rms_norm_fwd", dev, *args, _stream(dev))
     if st != 0:
         _check(st, "mirl_add_rms_norm_fwd")
     return y, h, rstd, scale
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_elems(R: int, H: int) -> int:
+    return load().mirl_add_rms_norm_bwd_workspace_elems(R, H)
 
 
 def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.Tensor, rstd: torch.Tensor,
                      weight: torch.Tensor, need_x: bool, need_res: bool, need_w: bool):
     """(dx, dres, dw), None where not needed; dx and dres are one tensor where their types are
     the same (see mirl_add_rms_norm_bwd).  The operands are a forward's and its gradients."""
-    dev = _require_gpu(dy, dh_out, h, rstd, weight)
+    dev = h.device
+    if dy.device != dev or (dh_out is not None and dh_out.device != dev):
+        _require_gpu(dy, dh_out, h, rstd, weight)
     H = h.shape[-1]
     R = h.numel() // H
-    dy2, lddy = _rows2(dy)
-    h2, ldh = _rows2(h)
-    g2, ldg = (None, 0) if dh_out is None else _rows2(dh_out)
+    dtype, h_dtype = dy.dtype, h.dtype
+    dy2, lddy = (dy, H) if dy.is_contiguous() else _rows2(dy)
+    h2, ldh = (h, H) if h.is_contiguous() else _rows2(h)
+    g_ptr, ldg = None, 0
+    if dh_out is not None:
+        g2, ldg = (dh_out, H) if dh_out.is_contiguous() else _rows2(dh_out)
+        g_ptr = g2.data_ptr()
     if not weight.is_contiguous():
         weight = weight.contiguous()
-    dtype, h_dtype = dy.dtype, h.dtype
     one = need_x and need_res and dtype == h_dtype
     dx = _new_like(h, dtype) if need_x else None
     dres = _new_like(h, h_dtype) if need_res and not one else None
-    dw = ws = None
+    dw = dw_ptr = ws_ptr = None
     if need_w:
         if R == 0:
             dw = torch.zeros_like(weight)
         else:
             dw = torch.empty_like(weight)
-            lib = _lib if _lib is not None else load()
-            elems = lib.mirl_add_rms_norm_bwd_workspace_elems(R, H)
+            dw_ptr = dw.data_ptr()
+            elems = _norm_workspace_elems(R, H)
             if elems:
                 ws = rstd.new_empty(elems)
-    st = _launch(
-        "mirl_add_rms_norm_bwd", dev, dy2.data_ptr(), _dtype_code(dy), lddy, _ptr(g2), ldg, h2.data_ptr(), _dtype_code(h),
-        ldh, rstd.data_ptr(), weight.data_ptr(), _dtype_code(weight), R, H, _ptr(dx), _ptr(dres),
-        None if dw is None or R == 0 else dw.data_ptr(), _ptr(ws), _stream(dev),
-    )
+                ws_ptr = ws.data_ptr()
+    args = (dy2.data_ptr(), DTYPE_CODES[dtype], lddy, g_ptr, ldg, h2.data_ptr(), DTYPE_CODES[h_dtype], ldh, rstd.data_ptr(),
+            weight.data_ptr(), DTYPE_CODES[weight.dtype], R, H, None if dx is None else dx.data_ptr(),
+            None if dres is None else dres.data_ptr(), dw_ptr, ws_ptr)
+    if _direct(dev):
+        st = _lib.mirl_add_rms_norm_bwd(*args, _raw_stream(dev.index))
+    else:
+        st = _launch("mirl_add_rms_norm_bwd", dev, *args, _stream(dev))
     if st != 0:
         _check(st, "mirl_add_rms_norm_bwd")
     return dx, (dx if one else dres), dw
@@ -1624,12 +1655,17 @@ def _seed_args(seed, dev: torch.device) -> tuple[int, Optional[int]]:
 def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
     """Dropout of ``x`` in its logical element order (see mirl_dropout); a new contiguous tensor."""
     dev = _require_gpu(x)
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     y = torch.empty_like(x)
     value, ptr = _seed_args(seed, dev)
-    st = _launch("mirl_dropout", dev, x.data_ptr(), _dtype_code(x), x.numel(), float(p), value, ptr,
-                 _signed64(offset), y.data_ptr(), _stream(dev))
-    _check(st, "mirl_dropout")
+    args = (x.data_ptr(), _dtype_code(x), x.numel(), p, value, ptr, _signed64(offset), y.data_ptr())
+    if _direct(dev):
+        st = _lib.mirl_dropout(*args, _raw_stream(dev.index))
+    else:
+        st = _launch("mirl_dropout", dev, *args, _stream(dev))
+    if st != 0:
+        _check(st, "mirl_dropout")
     return y
 
 
