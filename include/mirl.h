@@ -965,8 +965,9 @@ int mirl_dropout(const void* x, int dtype, int64_t n, double p, int64_t seed,
  *   out     = log_softmax(x[r])[target - vocab_start], 0 for targets outside
  *             [vocab_start, vocab_end)
  * hidden8 [T, Hd] (row r is position (r / bsz, r % bsz)), weight8 [V, Hd]; Hd and the
- * row strides multiples of 16, 16-byte-aligned starts.  Hidden rows go on with
- * zeros up to a multiple of 256; what lies past the weight's rows is not read.  out is [bsz, T / bsz] by strides; workspace:
+ * row strides multiples of 16, 16-byte-aligned starts, or, for the weight, Hd a multiple of
+ * 4, ldw = Hd and a 4-byte-aligned start.  Hidden rows go on with
+ * zeros up to a multiple of 256; what lies past the weight's rows has no influence.  out is [bsz, T / bsz] by strides; workspace:
  * mirl_lce_x_workspace_elems(T, V) floats.
  */
 int64_t mirl_lce_x_workspace_elems(int64_t T, int64_t V);

@@ -1674,7 +1674,8 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
                        vocab_end: int, out: torch.Tensor) -> None:
     """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd).
 
-    hidden8 [T, >= H] and weight8 [V, H] e4m3 (H and row strides multiples of 16; the hidden rows are zero past H,
+    hidden8 [T, >= H] and weight8 [V, H] e4m3 (H and row strides multiples of 16, or a contiguous weight with H a
+    multiple of 4; the hidden rows are zero past H,
     up to a multiple of 256), scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
     dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
     T = hidden8.shape[0]

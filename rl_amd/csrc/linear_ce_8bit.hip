@@ -52,9 +52,19 @@ __global__ __launch_bounds__(256) void lce_merge_8bit_kernel(LceParams P, float*
   const uint8_t* hr = static_cast<const uint8_t*>(P.h) + r * P.ldh;
   const uint8_t* wr = static_cast<const uint8_t*>(P.w) + (t - P.vs) * P.ldw;
   float dot[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t first_k = (W == 1 ? lane : threadIdx.x) * 16, whole = P.Hw / 16 * 16;
+  if (first_k == 0) {  // words past the whole pieces
+    for (int64_t k = whole; k < P.Hw; k += 4) {
+      float hv[4], wv[4];
+      unpack_e4m3(*reinterpret_cast<const uint32_t*>(hr + k), hv);
+      unpack_e4m3(*reinterpret_cast<const uint32_t*>(wr + k), wv);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dot[e] = fmaf(hv[e], wv[e], dot[e]);
+    }
+  }
 #pragma unroll 4
-  for (int64_t k = (W == 1 ? lane : threadIdx.x) * 16; k < P.Hw; k += 64 * W * 16) {
-    const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const vu4*>(wr + k);
+  for (int64_t k = first_k; k < whole; k += 64 * W * 16) {
+    const vu4 hq = *reinterpret_cast<const vu4*>(hr + k), wq = *reinterpret_cast<const Piece<4>::type*>(wr + k);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float hv[4], wv[4];
@@ -108,15 +118,21 @@ extern "C" int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_
   MIRL_REQUIRE(ldh < (int64_t(1) << 22) && ldw < (int64_t(1) << 22),
                "row strides (%lld, %lld) must be below 2^22 elements", (long long)ldh, (long long)ldw);
   const int64_t padded = padded_hidden(Hd, 1);
-  MIRL_REQUIRE(Hd % 16 == 0 && ldh % 16 == 0 && ldw % 16 == 0 && ldh >= padded && ldw >= Hd,
-               "hidden size %lld and row strides (%lld, %lld) must be multiples of 16, the hidden states' rows padded to %lld",
+  // A weight without gaps may have rows of any whole words: the piece that holds a row's end then goes
+  // on into the next row, whose NaN (e4m3 has no infinity) makes every logprob NaN by itself; the
+  // last row's is cut off word by word by the buffer's range.  ([387, 1000] x [32003, 1000]: 36 us,
+  // with a padded copy of the weight 60.)
+  const bool packed = Hd % 4 == 0 && ldw == Hd && (reinterpret_cast<uintptr_t>(weight8) & 3u) == 0;
+  const bool pieces = Hd % 16 == 0 && ldw % 16 == 0 && ldw >= Hd && (reinterpret_cast<uintptr_t>(weight8) & 15u) == 0;
+  MIRL_REQUIRE(ldh % 16 == 0 && ldh >= padded && (packed || pieces),
+               "hidden size %lld and row strides (%lld, %lld) must be multiples of 16 and the weight 16-byte aligned (or its "
+               "rows whole words without gaps), the hidden states' rows padded to %lld",
                (long long)Hd, (long long)ldh, (long long)ldw, (long long)padded);
   MIRL_REQUIRE(V < (int64_t(1) << 31) && T < (int64_t(1) << 31), "sizes exceed 2^31-1");
   if (T == 0) return MIRL_OK;
   MIRL_REQUIRE(hidden8 && hidden_scale && weight8 && weight_scale && target && out && workspace,
                "null pointer argument");
-  MIRL_REQUIRE((reinterpret_cast<uintptr_t>(hidden8) & 15u) == 0 && (reinterpret_cast<uintptr_t>(weight8) & 15u) == 0,
-               "hidden states and weight must be 16-byte aligned");
+  MIRL_REQUIRE((reinterpret_cast<uintptr_t>(hidden8) & 15u) == 0, "hidden states must be 16-byte aligned");
   LceParams P{};
   P.h = hidden8;
   P.w = weight8;

@@ -23,9 +23,11 @@ _H_ALIGN = 256  # the kernel steps through the hidden dimension 256 elements at 
 
 def _operand8(x: torch.Tensor, whole: bool) -> torch.Tensor:
     """``x [N, H]`` e4m3 as the kernel reads it: ``H`` and row strides multiples of 16, a 16-byte-aligned
-    start, and with ``whole`` (the hidden states) ``H`` a multiple of 256; otherwise a zero-padded
-    copy (the padding adds exact zeros)."""
+    start, and with ``whole`` (the hidden states) ``H`` a multiple of 256; the weight also contiguous
+    with rows of whole words; otherwise a zero-padded copy (the padding adds exact zeros)."""
     N, H = x.shape
+    if not whole and H % 4 == 0 and x.is_contiguous() and x.data_ptr() % 4 == 0:
+        return x
     if (H % (_H_ALIGN if whole else 16) == 0 and x.stride(-1) == 1 and x.stride(0) % 16 == 0 and x.stride(0) >= H
             and x.data_ptr() % 16 == 0):
         return x
@@ -52,8 +54,8 @@ def from_parallel_8bit_hidden_states_to_logprobs(
     ``target`` ``[B, S]`` is shifted by one position, as in the 16-bit form; the last position,
     which has no next token, is not computed.  Targets outside ``[vocab_start_index,
     vocab_end_index)`` give 0.  There is no gradient.  Hidden states whose size is not a
-    multiple of 256, and a weight whose rows are not 16-byte aligned, are copied into padded
-    buffers in every call."""
+    multiple of 256, and a weight whose rows are neither 16-byte aligned nor whole words without
+    gaps, are copied into padded buffers in every call."""
     from rl_amd.distributed.model_utils import _group_size, _require_single_rank
 
     _require_single_rank(tp_group)

@@ -185,3 +185,29 @@ def test_nothing_past_the_weights_rows_is_read(S, H, left, wide):
     pad = -(-H // 256) * 256 - H
     h8p, w8p = (torch.nn.functional.pad(t.view(torch.uint8), (0, pad)).view(torch.float8_e4m3fn) for t in (h8, w8))
     assert torch.equal(got, from_parallel_8bit_hidden_states_to_logprobs(h8p, hs, w8p, ws, target, 0, 300))
+
+
+@pytest.mark.parametrize("S", [9, 200])
+@pytest.mark.parametrize("H", [4, 20, 200, 252, 260, 1000, 1028])
+def test_packed_rows_of_whole_words(S, H):
+    """A contiguous weight whose rows start at any word, NaN right behind it: what zero-padded rows give
+    (they add the same products; the target's logit adds those of up to three words in another order:
+    a rounding each of 12 products more)."""
+    h8, hs, w8, ws, target = inputs(S, 2, H, 300, seed=H)
+    buf = torch.full((4 + 300 * H + 64,), 0x7F, dtype=torch.uint8, device=DEV)
+    buf[4 : 4 + 300 * H] = w8.view(torch.uint8).flatten()
+    packed = buf[4 : 4 + 300 * H].view(300, H).view(torch.float8_e4m3fn)
+    got = from_parallel_8bit_hidden_states_to_logprobs(h8, hs, packed, ws, target, 0, 300)
+    pad = -(-H // 256) * 256 - H
+    h8p, w8p = (torch.nn.functional.pad(t.view(torch.uint8), (0, pad)).view(torch.float8_e4m3fn) for t in (h8, w8))
+    same = from_parallel_8bit_hidden_states_to_logprobs(h8p, hs, w8p, ws, target, 0, 300)
+    want, tol = oracle(h8, hs, w8, ws, target, 0, 300)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    assert ((got - same).cpu().double().abs() <= 2 * tol).all()
+
+
+def test_packed_rows_with_a_nan():
+    """A NaN in a packed weight makes every logprob NaN, as it does in padded rows."""
+    h8, hs, w8, ws, target = inputs(9, 2, 20, 300, seed=1)
+    w8.view(torch.uint8)[7, 2] = 0x7F
+    assert from_parallel_8bit_hidden_states_to_logprobs(h8, hs, w8, ws, target, 0, 300).isnan().all()
