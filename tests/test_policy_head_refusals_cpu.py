@@ -155,3 +155,26 @@ def test_c_entries_return_a_status():
     # nothing to do
     assert lib.mirl_dropout(None, 0, 0, 0.5, 1, None, 0, None, None) == 0
     assert lib.mirl_quantize_rows(None, 0, 8, 0, 8, None, None, None) == 0
+
+
+def test_layouts_that_the_tile_loop_cannot_read():
+    """Refused for their layout, before the pointers are looked at."""
+    lib = _C.load()
+
+    def fwd8(Hd, ldh, ldw, w=None):
+        return lib.mirl_linear_ce_8bit_fwd(None, None, 4, Hd, ldh, w, None, 10, ldw, 2, None, 1, 1, 0, 10, None, 1, 1, None, None)
+
+    for args in ((250, 256, 250), (252, 256, 256), (252, 252, 252), (256, 264, 256), (272, 272, 272), (256, 256, 240), (252, 256, 252, 2),
+                 (256, 256, 272, 4), (256, 256, 256, 6)):
+        assert fwd8(*args) != 0 and "multiples of 16" in lib.mirl_last_error().decode(), args
+    for args in ((252, 256, 252), (256, 256, 272), (272, 512, 272), (4, 256, 4, 4)):  # readable: the null pointers are next
+        assert fwd8(*args) != 0 and "null" in lib.mirl_last_error().decode(), args
+
+    def adapters(Hd, ldh, ldw, w=None):
+        return lib.mirl_adapter_ce_fwd(None, 1, 4, Hd, ldh, w, 10, ldw, *[None] * 3, 8, 1, *[None] * 3, 2, None, 1, 1, 0, 10, None, 1, 1,
+                                       None, None, None)
+
+    for args in ((12, 128, 16), (16, 16, 16), (136, 136, 136), (128, 128, 120), (128, 132, 128), (128, 128, 132)):
+        assert adapters(*args) != 0 and "multiples of 8" in lib.mirl_last_error().decode(), args
+    assert adapters(128, 128, 128, 8) != 0 and "aligned" in lib.mirl_last_error().decode()
+    assert adapters(136, 256, 136) != 0 and "null" in lib.mirl_last_error().decode()
