@@ -1297,7 +1297,8 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   __syncthreads();
   if constexpr (kAdapters) {
     n_seg = __builtin_amdgcn_readfirstlane(__float_as_int(s_m[0][0]));
-    apart = __syncthreads_or(tid < n_seg && s_bad[tid] != 0) != 0 || P.b_bytes >= (int64_t(1) << 31);
+    apart = __builtin_amdgcn_readfirstlane(__syncthreads_or(tid < n_seg && s_bad[tid] != 0)) != 0 ||
+            P.b_bytes >= (int64_t(1) << 31);
   }
 
   const int nst = (int)(P.Hd / kSKE);
@@ -1342,8 +1343,9 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
     if constexpr (kAdapters) {
       rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(P.planes * P.r8)), 0,
                                                  a_rows * P.planes * P.r8 * 2, 0x00020000);
+      // (apart: the loop reads nothing of B, which may hold anything and, past 2 GiB, kOut too)
       rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.B + n0 * P.r8), 0,
-                                                 (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
+                                                 apart ? 0 : (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
     }
     auto place = [&](int row, int& seg, int& rem) {
       const int x = (t - nst) * 8 + ((lane & 7) ^ ((row >> 1) & 7));
