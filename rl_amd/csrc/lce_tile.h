@@ -88,6 +88,10 @@ struct Mma<F8> {
   }
 };
 
+// Whether a partial pair (maximum, sum of exponentials) has a share in its row: all columns of one
+// without are absent or -inf (a sum of 0).  A group of NaN has a maximum of -inf too, and NaN as its sum.
+__device__ __forceinline__ bool counts(float m, float s) { return m != -INFINITY || s != 0.f; }
+
 // 16-bit element bits <-> fp32 for a dtype E (round to nearest even).
 template <class E>
 __device__ __forceinline__ uint16_t bits_of(float f) {
@@ -1031,11 +1035,16 @@ void lce_tile_kernel(LceParams P) {
         for (int j = 0; j < kTN; ++j)
 #pragma unroll
           for (int v = 0; v < kAV; ++v) s4[v & 3] += fast_exp2(fmaf(y[j][v], c, -Mc));
+      } else {  // columns that are not there, -inf and NaN, which a maximum does not show
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int v = 0; v < kAV; ++v) s4[v & 3] = y[j][v] != y[j][v] ? y[j][v] : s4[v & 3];
       }
       float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
 #pragma unroll
       for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-      if (M != -INFINITY) {  // (else no column is there)
+      if (M != -INFINITY) {  // (else the sum is 0 or NaN)
         sum *= fast_exp2(-fmaf(M, c, -Mc));
         M = kES == 1 ? M * rs : M;
       }
@@ -1056,8 +1065,8 @@ void lce_tile_kernel(LceParams P) {
         if (r >= row_end) continue;
         const float m1 = s_m[rl], M = fmaxf(rm[i], m1);
         float sum = 0.f;
-        if (rm[i] != -INFINITY) sum += rsum[i] * fast_exp2((rm[i] - M) * kLog2e);
-        if (m1 != -INFINITY) sum += s_g[rl] * fast_exp2((m1 - M) * kLog2e);
+        if (counts(rm[i], rsum[i])) sum += rsum[i] * fast_exp2((rm[i] - M) * kLog2e);
+        if (counts(m1, s_g[rl])) sum += s_g[rl] * fast_exp2((m1 - M) * kLog2e);
         if constexpr (kAdapters) {
           if (n_seg > 0 && s_ord[rl] >= 0 && s_bad[s_ord[rl]] != 0) sum = __builtin_nanf("");
         }
@@ -1119,6 +1128,14 @@ void lce_tile_kernel(LceParams P) {
               if (FULL || c * 8 + e < ncols) s4[e & 3] += fast_exp2((w[e] - M) * kLog2e);
           }
           sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        } else {  // -inf and NaN, which a maximum does not show
+          for (int c = 0; c < kBN / 8; ++c) {
+            float w[8];
+            E::unpack(rowp[c ^ sw], w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if ((FULL || c * 8 + e < ncols) && w[e] != w[e]) sum = w[e];
+          }
         }
       };
       if (ncols == kBN)
@@ -1477,6 +1494,11 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
       for (int j = 0; j < kTN; ++j)
 #pragma unroll
         for (int v = 0; v < kAV; ++v) sum += fast_exp2((acc[i][j][v] - M) * kLog2e);
+    } else {  // (see lce_tile_kernel)
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int v = 0; v < kAV; ++v) sum = acc[i][j][v] != acc[i][j][v] ? acc[i][j][v] : sum;
     }
 #pragma unroll
     for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
@@ -1492,7 +1514,7 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
     for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][tid]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
-      if (s_m[w][tid] != -INFINITY) sum += s_sum[w][tid] * fast_exp2((s_m[w][tid] - M) * kLog2e);
+      if (counts(s_m[w][tid], s_sum[w][tid])) sum += s_sum[w][tid] * fast_exp2((s_m[w][tid] - M) * kLog2e);
     if constexpr (kAdapters) {
       if (s_ord[tid] >= 0 && s_bad[s_ord[tid]] != 0) sum = __builtin_nanf("");
     }
@@ -1520,12 +1542,10 @@ __device__ __forceinline__ void join_partials(const float* __restrict__ p, int64
     for (int w = 0; w < W; ++w) M = fmaxf(M, s_j[0][w]);
   }
   s = 0.f;
-  if (M != -INFINITY) {
 #pragma unroll 4
-    for (int64_t j = first; j < n; j += 64 * W) {
-      const float mj = p[2 * j];
-      if (mj != -INFINITY) s += p[2 * j + 1] * fast_exp2((mj - M) * kLog2e);
-    }
+  for (int64_t j = first; j < n; j += 64 * W) {
+    const float mj = p[2 * j], sj = p[2 * j + 1];
+    if (counts(mj, sj)) s += sj * fast_exp2((mj - M) * kLog2e);
   }
   s = wave_sum(s);
   if constexpr (W > 1) {
