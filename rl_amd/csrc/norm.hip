@@ -374,25 +374,54 @@ struct NormBwd {
 };
 
 // dw of 16 columns by one workgroup that reads them again: for rows few enough to lie in the
-// caches, beside the workgroups that form dh, in place of partial sums and a second launch.
+// caches, beside the workgroups that form dh, in place of partial sums and a second launch.  A
+// lane's rows go into eight sums and the lanes' sums into four: at most R / 128 + 10 additions in
+// sequence with 16 lanes a column, 22 with 64.
 template <class EX, class EH>
 __device__ __forceinline__ void dw_columns(const NormBwd& P, int64_t block, float (*s)[17]) {
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, lanes = blockDim.x >> 4;
   const int64_t c = block * 16 + cl;
-  float v = 0.f;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
   if (c < P.H) {
-#pragma unroll 8
-    for (int64_t r = rl; r < P.R; r += lanes) {
-      const float d = EX::load(static_cast<const typename EX::raw*>(P.dy) + r * P.lddy + c);
-      const float h = EH::load(static_cast<const typename EH::raw*>(P.h) + r * P.ldh + c);
-      v = fmaf(d, h * P.rstd[r], v);
+    const typename EX::raw* d = static_cast<const typename EX::raw*>(P.dy) + rl * P.lddy + c;
+    const typename EH::raw* h = static_cast<const typename EH::raw*>(P.h) + rl * P.ldh + c;
+    const int64_t sd = lanes * P.lddy, sh = lanes * P.ldh;
+    // n of the lane's rows from r on, the first `have` of them there (the others are read as the first)
+    auto rows = [&](auto n_c, int64_t r, int64_t have) __attribute__((always_inline)) {
+      constexpr int N = decltype(n_c)::value;
+      float dv[N], hv[N], rs[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t k = i < have ? i : 0;
+        dv[i] = EX::load(d + k * sd);
+        hv[i] = EH::load(h + k * sh);
+        rs[i] = P.rstd[r + k * lanes];
+      }
+      __builtin_amdgcn_sched_barrier(0);  // all loads in flight before the first sum waits
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = i < have ? fmaf(dv[i], hv[i] * rs[i], v[i]) : v[i];
+    };
+    int64_t r = rl;
+    for (; r + 7 * lanes < P.R; r += 8 * lanes) {
+      rows(std::integral_constant<int, 8>{}, r, 8);
+      d += 8 * sd;
+      h += 8 * sh;
     }
+    if (r + lanes < P.R)
+      rows(std::integral_constant<int, 7>{}, r, (P.R - r + lanes - 1) / lanes);
+    else if (r < P.R)
+      rows(std::integral_constant<int, 1>{}, r, 1);
   }
-  s[rl][cl] = v;
+  s[rl][cl] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
   __syncthreads();
   if (threadIdx.x < 16 && c < P.H) {
-    float sum = 0.f;
-    for (int i = 0; i < lanes; ++i) sum += s[i][cl];
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < lanes; i += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] += s[i + e][cl];
+    const float sum = (t[0] + t[1]) + (t[2] + t[3]);
     if (std::is_same<EX, F32>::value || P.w.f32)
       static_cast<float*>(P.dw)[c] = sum;
     else
@@ -594,9 +623,13 @@ int check_weight(int x_dtype, int w_dtype) {
   return MIRL_OK;
 }
 constexpr int64_t kMaxSide = int64_t(1) << 31, kMaxWidth = int64_t(1) << 24;
-// Elements of a batch whose dw is formed from a second read, in the same launch (forward and
-// backward of [257, 3, 1021] fp32 with autograd around them: 114 us with partial sums and a launch more, 106 so).
-constexpr int64_t kFewElems = int64_t(1) << 20;
+// Batches whose dw is formed from a second read, in the same launch: of few elements (forward and
+// backward of [257, 3, 1021] fp32 with autograd around them: 114 us with partial sums and a launch more,
+// 106 so) in few rows, which a column's 16 lanes share.  Kernels alone, second read against partial sums, us:
+// bf16 [771, 1021] 5.7 and 12.4, [2048, 512] 8.2 and 10.5, [2048, 64] 7.8 and 9.1, [2048, 17] 9.1 and 9.5,
+// [4096, 64] 13.3 and 11.2, [16384, 17] 57 and 28, [60000, 17] 303 and 83.
+constexpr int64_t kFewElems = int64_t(1) << 20, kFewRows = 2048;
+bool few_rows(int64_t R, int64_t H) { return H <= 16384 && R <= kFewRows && R * H <= kFewElems; }
 // Partial sums of dw: four workgroups per CU (eight: 108 and 11 us of [16384, 4096] against 104
 // and 6; three: 6% more).
 constexpr int64_t kMaxGroups = 1024;
@@ -647,7 +680,7 @@ extern "C" int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, co
 }
 
 extern "C" int64_t mirl_add_rms_norm_bwd_workspace_elems(int64_t R, int64_t H) {
-  if (R <= 0 || H <= 0 || (H <= 16384 && R * H <= kFewElems)) return 0;
+  if (R <= 0 || H <= 0 || few_rows(R, H)) return 0;
   return (R < kMaxGroups ? R : kMaxGroups) * H;
 }
 
@@ -672,7 +705,7 @@ extern "C" int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, 
     MIRL_REQUIRE(dw == nullptr || workspace != nullptr || mirl_add_rms_norm_bwd_workspace_elems(R, H) == 0,
                  "null pointer argument");
     const int64_t groups = R < kMaxGroups ? R : kMaxGroups;
-    const bool few = dw != nullptr && H <= 16384 && R * H <= kFewElems;
+    const bool few = dw != nullptr && few_rows(R, H);
     NormBwd P{dy, lddy, dh_out, ldd, h, ldh, rstd, Weight{weight, w_dtype == MIRL_DTYPE_F32}, R, H, dx, dres,
               dw != nullptr && !few ? workspace : nullptr, groups, few ? dw : nullptr, 0};
     hipStream_t st = static_cast<hipStream_t>(stream);
