@@ -1007,9 +1007,11 @@ int mirl_adapter_rows(const int64_t* ids, int64_t B, int64_t N, int64_t R, const
                       int32_t* workspace, void* stream);
 
 /* The T sorted rows' hidden states (zero padded to ldo) and their U: as two values of the
- * operand type that add up to it (u_planes [T, 2, r8]) and, unless NULL, in fp32 by original row
- * (u_rows [*, r8]).  Rows of the base model leave U as it is.  bad[a] (zeroed before) becomes 1
- * where adapter a has rows and its B (b_elems elements of b each) holds an infinity or a NaN. */
+ * operand type that add up to it (u_planes [T, 2, r8]; fp16: [T, 4, r8], a row's last two rows of r8
+ * hold its U in fp32) and, unless NULL, in fp32 by original row (u_rows [*, r8]).  Rows of the base
+ * model leave U as it is.  bad[a] (zeroed before) takes bit 0 where adapter a has rows and its B
+ * (b_elems elements of b each) holds an infinity or a NaN, and with fp16 bit 1 where a row's U is
+ * finite and past 65504: the functions below take such a row from its fp32 values. */
 int mirl_adapter_down(const void* hidden, int dtype, int64_t Hd, int64_t ldh, const int64_t* perm,
                       const int32_t* adapter, int64_t T, const void* a, int64_t N, int64_t r,
                       int64_t lda, const float* scaling, double p, int64_t seed, const int64_t* seed_dev,
@@ -1031,8 +1033,8 @@ int mirl_adapter_ce_fwd(const void* hidden, int dtype, int64_t T, int64_t Hd, in
                         int64_t vocab_end, float* out, int64_t o_stride_b, int64_t o_stride_s,
                         float* row_stats, float* workspace, void* stream);
 
-/* Backward operands: rows m < *count (of at most T): hidden rows (zero padded to ldo) and the
- * planes of U from the forward's u_rows. */
+/* Backward operands: rows m < *count (of at most T): hidden rows (zero padded to ldo) and u_planes as
+ * above from the forward's u_rows. */
 int mirl_adapter_gather(const int64_t* perm, const int32_t* adapter, const int64_t* count,
                         int64_t T, const void* hidden, int dtype, int64_t Hd, int64_t ldh,
                         const float* u_rows, int64_t r8, void* hidden_out, int64_t ldo,

@@ -1718,7 +1718,8 @@ class Dropped:
 class AdapterRows:
     """Rows sorted by adapter (see mirl_adapter_rows): perm, adapter, target, and with an upstream
     gradient g and stats, as [rows] tensors; seg [N + 1], count [1].  ``bad [N]``, zeroed here unless it is
-    given (a forward's), says which adapters hold values that are none."""
+    given (a forward's), says which adapters hold values that are none, and (fp16) which have a row whose U
+    passes the type's range."""
 
     def __init__(self, ids: torch.Tensor, N: int, target: torch.Tensor, grad: Optional[torch.Tensor] = None,
                  stats: Optional[torch.Tensor] = None, bad: Optional[torch.Tensor] = None):
@@ -1750,9 +1751,14 @@ class AdapterRows:
         _check(st, "mirl_adapter_rows")
 
 
+def _u_rows(t: torch.Tensor) -> int:
+    """16-bit rows that a row of U takes: two planes, and for fp16 its fp32 values."""
+    return 4 if t.dtype == torch.float16 else 2
+
+
 def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
                  drop: Dropped, width: int, want_u: bool):
-    """(hidden rows [T, width], U planes [T, 2, r8], U fp32 [T, r8] by original row or None); sets
+    """(hidden rows [T, width], U planes [T, 2 or (fp16) 4, r8], U fp32 [T, r8] by original row or None); sets
     rows.bad from b [N, V, r8]."""
     dev = _require_gpu(hidden2d, a, b, scaling)
     T, H, r, r8 = rows.perm.numel(), hidden2d.shape[1], a.shape[1], b.shape[2]
@@ -1761,7 +1767,7 @@ def adapter_down(hidden2d: torch.Tensor, rows: AdapterRows, a: torch.Tensor, b: 
              and scaling.dtype == torch.float32 and scaling.numel() == a.shape[0] and scaling.is_contiguous(),
              "contiguous adapters of the hidden states' type, an fp32 scaling each")
     h = torch.empty((T, width), dtype=hidden2d.dtype, device=dev)
-    planes = torch.empty((T, 2, r8), dtype=hidden2d.dtype, device=dev)
+    planes = torch.empty((T, _u_rows(hidden2d), r8), dtype=hidden2d.dtype, device=dev)
     u = torch.empty((T, r8), dtype=torch.float32, device=dev) if want_u else None
     st = _launch(
         "mirl_adapter_down", dev, hidden2d.data_ptr(), _dtype_code(hidden2d), H, hidden2d.stride(0), rows.perm.data_ptr(),
@@ -1781,7 +1787,7 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
     V, H = weight.shape
     _check_linear_ce(h, weight)
     _require(h.shape[1] == -(-H // 128) * 128 and b.is_contiguous() and b.dtype == h.dtype and b.shape[1] == V
-             and planes.shape == (T, 2, b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
+             and planes.shape == (T, _u_rows(h), b.shape[2]) and tuple(out.shape) == tuple(target.shape), "operands of one shape")
     lib = _lib if _lib is not None else load()
     ws = torch.empty(int(lib.mirl_lce_x_workspace_elems(T, V)), dtype=torch.float32, device=dev)
     st = _launch(
@@ -1794,11 +1800,11 @@ def adapter_ce_fwd(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pla
 
 
 def adapter_gather(hidden2d: torch.Tensor, rows: AdapterRows, u: torch.Tensor, width: int):
-    """(hidden rows [T, width], U planes [T, 2, r8]) of the sorted rows below the count."""
+    """(hidden rows [T, width], U planes as adapter_down's) of the sorted rows below the count."""
     dev = _require_gpu(hidden2d, u)
     T, r8 = u.shape
     h = torch.empty((T, width), dtype=hidden2d.dtype, device=dev)
-    planes = torch.empty((T, 2, r8), dtype=hidden2d.dtype, device=dev)
+    planes = torch.empty((T, _u_rows(hidden2d), r8), dtype=hidden2d.dtype, device=dev)
     st = _launch(
         "mirl_adapter_gather", dev, rows.perm.data_ptr(), rows.adapter.data_ptr(), rows.count.data_ptr(), T,
         hidden2d.data_ptr(), _dtype_code(hidden2d), hidden2d.shape[1], hidden2d.stride(0), u.data_ptr(), r8, h.data_ptr(),
@@ -1831,7 +1837,8 @@ def adapter_ce_grad(h: torch.Tensor, weight: torch.Tensor, rows: AdapterRows, pl
     """G [n, >= V] and its transpose of sorted rows row0 .. row0 + n (see mirl_adapter_ce_grad)."""
     dev = _require_gpu(h, weight, planes, b, G, Gt)
     _check_linear_ce(h, weight)
-    _require(h.shape[1] == -(-weight.shape[1] // 128) * 128, "hidden rows padded to 128 elements")
+    _require(h.shape[1] == -(-weight.shape[1] // 128) * 128 and planes.shape[1:] == (_u_rows(h), b.shape[2]),
+             "hidden rows padded to 128 elements, U planes of the operand type")
     _require(G.dtype == h.dtype and Gt.dtype == h.dtype and G.stride(1) == 1 and Gt.stride(1) == 1, "G of the operand type")
     st = _launch(
         "mirl_adapter_ce_grad", dev, h.data_ptr(), _dtype_code(h), weight.shape[1], h.stride(0), weight.data_ptr(),

@@ -110,6 +110,33 @@ __device__ __forceinline__ uint2 pack4(f32x4 o) {
     return uint2{(uint32_t)bits_of<E>(o[0]) | ((uint32_t)bits_of<E>(o[1]) << 16),
                  (uint32_t)bits_of<E>(o[2]) | ((uint32_t)bits_of<E>(o[3]) << 16)};
 }
+constexpr uint32_t kF16Past = 0x477ff000u;  // 65520, which fp16 rounds to infinity (bits of the fp32 value)
+// A row of U past fp16's range (r8 values) enters the reduction times this power of two, which takes its
+// largest finite magnitude to [2^14, 2^15); rows within the range times 1.
+__device__ __forceinline__ float wide_scale(const float* u, int r8) {
+  uint32_t peak = 0;
+  for (int i = 0; i < r8; i += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(u + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t b = __float_as_uint(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w) & 0x7fffffffu;
+      peak = b < 0x7f800000u && b > peak ? b : peak;
+    }
+  }
+  return peak < kF16Past ? 1.f : __uint_as_float((14 + 2 * 127 - (peak >> 23)) << 23);
+}
+// Eight values of u times `scale`: plane 0 of the two that add up to them, or plane 1.
+template <class E>
+__device__ __forceinline__ vu4 plane8(const float* u, float scale, int plane) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = u[i] * scale;
+    const float first = value_of<E>(bits_of<E>(v[i]));
+    v[i] = plane == 0 ? first : v[i] - first;
+  }
+  return E::pack(v);
+}
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr int kBM = 256;                 // rows per tile
@@ -191,6 +218,18 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_(std::make_integer_sequence<int, N>{}, f);
 }
 
+// Flags of an adapter: its B holds an infinity or a NaN; fp16: a row's U is finite and past fp16's range.
+constexpr int kBroken = 1, kWide = 2;
+constexpr int kPlanes = 2;
+// 16-bit rows of r8 that a row of U takes: its planes, and for fp16 its fp32 values (u_f32).
+template <class E>
+constexpr int kURow = std::is_same<E, F16>::value ? 4 : 2;
+template <class T>
+__device__ __forceinline__ auto u_f32(T* U, int64_t row, int r8) {
+  using F = typename std::conditional<std::is_const<T>::value, const float, float>::type;
+  return reinterpret_cast<F*>(U + (row * kURow<F16> + kPlanes) * r8);
+}
+
 // kFwd, kGrad: logits rounded to the operand type.  kFwdX, kGradX: logits kept in fp32, with
 // adapters (16-bit operands) or row and column scales (e4m3, forward).
 enum LceMode { kFwd = 0, kGrad = 1, kGemm = 2, kFwdX = 3, kGradX = 4 };
@@ -237,13 +276,13 @@ struct LceParams {
   int64_t final_at;
   // kFwdX and kGradX with adapters (or null): row r takes adapter aid[r] (rows of one
   // adapter adjoin; negative: none), which adds U[r] . B[aid[r]]^T to its logits.  U is held as
-  // `planes` values of the operand type that add up to it: row r is [planes][r8], the planes
-  // r8 elements apart; B is [adapters, V, r8], r8 a multiple of 8.
+  // `planes` values of the operand type that add up to it: row r is [kURow<E>][r8], the planes
+  // first (fp16: then U in fp32); B is [adapters, V, r8], r8 a multiple of 8.
   const int32_t* aid;
   const uint16_t* U;
   const uint16_t* B;
   int r8, planes;
-  const int32_t* bad;   // [adapters]: B holds an infinity or a NaN
+  const int32_t* bad;   // [adapters]: kBroken, kWide
   int64_t b_bytes;      // size of B
   // kGradX: G = (onehot - softmax) * g_scale in the operand type (rows past the end: 0)
   float g_scale;
@@ -278,6 +317,9 @@ void lce_tile_kernel(LceParams P) {
   __shared__ __align__(16) float s_m[kBM], s_ls[kBM], s_g[kBM], s_rs[MODE == kFwdX && kES == 1 ? kBM : 1];
   __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_bad[kAdapters ? kBM : 1],
       s_heads[kWaves];
+  constexpr bool kF16 = kAdapters && std::is_same<E, F16>::value;
+  const int ur = kF16 ? kURow<F16> : P.planes;
+  __shared__ float s_us[kF16 ? kBM : 1];
   auto stage_ptr = [&](int s) -> unsigned char* { return s == 0 ? st0 : st1; };
 
   // Tile order.  Workgroups are dispatched to the 8 XCDs round-robin
@@ -508,8 +550,8 @@ void lce_tile_kernel(LceParams P) {
     // kept in registers that it lacks
     int ln = lane;
     asm volatile("" : "+v"(ln));
-    rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(P.planes * P.r8)), 0,
-                                               (int)(a_rows * P.planes * P.r8 * 2), 0x00020000);
+    rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(ur * P.r8)), 0,
+                                               (int)(a_rows * ur * P.r8 * 2), 0x00020000);
     rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.B + n0 * P.r8), 0,
                                                (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
 #pragma unroll
@@ -521,7 +563,7 @@ void lce_tile_kernel(LceParams P) {
 #pragma unroll
       for (int i = odd; i < kDmaPerWave; i += 2) {
         const int row = (wave * kDmaPerWave + i) * kDmaRows + (ln >> 3);
-        voff_a[i] = s_ord[row] == seg ? (row * P.planes * P.r8 + rem * 8) * 2 : kOut;
+        voff_a[i] = s_ord[row] == seg ? (row * ur * P.r8 + rem * 8) * 2 : kOut;
         voff_b[i] = ((seg < n_seg) & (row < (int)b_rows)) ? b0 + row * P.r8 * 2 : kOut;
       }
     }
@@ -617,9 +659,10 @@ void lce_tile_kernel(LceParams P) {
     }
   };
   // The adapters' part by itself, stage by stage through stage array 1, where a value of an adapter
-  // is none or B passes 2 GiB:
+  // is none, B passes 2 GiB or (fp16) a row's U the type's range:
   // an infinity or a NaN of one adapter's B must not meet the other rows' zeros, so it is taken
-  // out, and that adapter's rows become NaN afterwards (s_bad).
+  // out, and that adapter's rows become NaN afterwards (s_bad).  A row of U past the range comes from
+  // fp32 times a power of two, and so does what the row has summed.
   auto nonfinite = [](vu4 q) __attribute__((always_inline)) {
     constexpr uint32_t ex = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
     bool bad = false;
@@ -630,19 +673,60 @@ void lce_tile_kernel(LceParams P) {
     }
     return bad;
   };
+  // The accumulators are complete here, in the registers that the MFMAs write.
+  auto keep_acc = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) asm volatile("" : "+a"(acc[i][j]));
+  };
+  auto scale_rows = [&](bool back) __attribute__((always_inline)) {
+    // One accumulator register at a time, by asm: left to itself the compiler moves all of them to other
+    // registers around this branch and spills 130.  The waits stand between MFMAs and these accesses.
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+      float f = s_us[kF16 ? wm * kWM + i * kT + frow : 0];
+      f = back ? 1.f / f : f;  // powers of two: exact
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) {
+#pragma unroll
+        for (int v = 0; v < kAV; ++v) {
+          float x;
+          asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(acc[i][j][v]));
+          x *= f;
+          asm volatile("v_accvgpr_write_b32 %0, %1" : "=a"(acc[i][j][v]) : "v"(x));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_nop 15" ::: "memory");
+  };
   auto adapter_stages = [&]() __attribute__((always_inline)) {
     const int chunk = tid & 7;
+    bool wide = false;
+    if constexpr (kF16) {
+      const bool mine = s_ord[tid] >= 0 && (s_bad[s_ord[tid]] & kWide) != 0;
+      s_us[tid] = mine ? wide_scale(u_f32(P.U, m0 + tid, P.r8), P.r8) : 1.f;
+      wide = __syncthreads_or(mine) != 0;
+      if (wide) scale_rows(false);
+    }
     for (int e = 0; e < n_ext; ++e) {
       const int x = e * 8 + chunk, q = x / cps, rem = x - q * cps, cc = rem % cpp;
       const bool any = q < n_seg;
-      const uint16_t* up = P.U + m0 * (int64_t)(P.planes * P.r8) + rem * 8;
+      const uint16_t* up = P.U + m0 * (int64_t)(ur * P.r8) + rem * 8;
       const uint16_t* bp = P.B + ((int64_t)(any ? s_seg[q] : 0) * P.V + n0) * P.r8 + cc * 8;
       __syncthreads();  // the last stage's reads are done
 #pragma unroll 1
       for (int k = 0; k < kBM / 32; ++k) {
         const int row = k * 32 + (tid >> 3);
         vu4 u = {0u, 0u, 0u, 0u}, b = {0u, 0u, 0u, 0u};
-        if (any && s_ord[row] == q) u = *reinterpret_cast<const vu4*>(up + (int64_t)row * (P.planes * P.r8));
+        if (any && s_ord[row] == q) {
+          u = *reinterpret_cast<const vu4*>(up + (int64_t)row * (ur * P.r8));
+          if constexpr (kF16) {
+            if (wide) u = plane8<E>(u_f32(P.U, m0 + row, P.r8) + cc * 8, s_us[row], rem / cpp);
+          }
+        }
         if (any && n0 + row < P.V) b = *reinterpret_cast<const vu4*>(bp + (int64_t)row * P.r8);
         if (nonfinite(b)) b = vu4{0u, 0u, 0u, 0u};
         *reinterpret_cast<vu4*>(st1 + lds_off(row, chunk)) = u;
@@ -658,8 +742,11 @@ void lce_tile_kernel(LceParams P) {
       }
     }
     __syncthreads();
+    if constexpr (kF16) {
+      if (wide) scale_rows(true);
+    }
     if constexpr (MODE == kGradX) {
-      if (s_ord[tid] >= 0 && s_bad[s_ord[tid]] != 0) s_g[tid] = __builtin_nanf("");
+      if (s_ord[tid] >= 0 && (s_bad[s_ord[tid]] & kBroken) != 0) s_g[tid] = __builtin_nanf("");
     }
   };
   auto run_stages = [&]() __attribute__((always_inline)) {
@@ -862,7 +949,9 @@ void lce_tile_kernel(LceParams P) {
   } else {
     run_stages();
     if constexpr (kAdapters) {
+      if constexpr (kF16) keep_acc();  // (on both sides of the branch, or 13 registers are spilled)
       if (apart) adapter_stages();
+      if constexpr (kF16) keep_acc();
     }
   }
 
@@ -1068,7 +1157,7 @@ void lce_tile_kernel(LceParams P) {
         if (counts(rm[i], rsum[i])) sum += rsum[i] * fast_exp2((rm[i] - M) * kLog2e);
         if (counts(m1, s_g[rl])) sum += s_g[rl] * fast_exp2((m1 - M) * kLog2e);
         if constexpr (kAdapters) {
-          if (n_seg > 0 && s_ord[rl] >= 0 && s_bad[s_ord[rl]] != 0) sum = __builtin_nanf("");
+          if (n_seg > 0 && s_ord[rl] >= 0 && (s_bad[s_ord[rl]] & kBroken) != 0) sum = __builtin_nanf("");
         }
         float* dst = P.part + ((r - P.row0) * P.n_nt + nt) * 2;
         dst[0] = M;
@@ -1253,7 +1342,8 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   constexpr int kES = (int)sizeof(typename E::raw), kSKE = kRowBytes / kES;
   constexpr int kFC = (int)sizeof(frag) / 16;
   constexpr int kKK = kRowBytes / (kWave / kT * (int)sizeof(frag));
-  constexpr bool kAdapters = kES == 2;
+  constexpr bool kAdapters = kES == 2, kF16 = std::is_same<E, F16>::value;
+  const int ur = kF16 ? kURow<F16> : P.planes;
   constexpr int kOut = -0x7fffffff - 1;  // an offset out of range: reads as zero
   __shared__ __align__(1024) unsigned char st0[kRStageBytes];
   __shared__ __align__(1024) unsigned char st1[kRStageBytes];
@@ -1358,8 +1448,8 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   // offsets of stage data t >= nst (see lce_tile_kernel)
   auto prepare = [&](int t) __attribute__((always_inline)) {
     if constexpr (kAdapters) {
-      rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(P.planes * P.r8)), 0,
-                                                 a_rows * P.planes * P.r8 * 2, 0x00020000);
+      rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.U + m0 * (int64_t)(ur * P.r8)), 0,
+                                                 a_rows * ur * P.r8 * 2, 0x00020000);
       // (apart: the loop reads nothing of B, which may hold anything and, past 2 GiB, kOut too)
       rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(P.B + n0 * P.r8), 0,
                                                  apart ? 0 : (int)(P.b_bytes - n0 * P.r8 * 2), 0x00020000);
@@ -1374,7 +1464,7 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
       const int row = (wave * kRLoadsA + i) * kDmaRows + (lane >> 3);
       int seg, rem;
       place(row, seg, rem);
-      voff_a[i] = kAdapters && t < total && s_ord[row] == seg ? (row * P.planes * P.r8 + rem * 8) * 2 : kOut;
+      voff_a[i] = kAdapters && t < total && s_ord[row] == seg ? (row * ur * P.r8 + rem * 8) * 2 : kOut;
     }
 #pragma unroll
     for (int i = 0; i < kRLoadsB; ++i) {
@@ -1440,8 +1530,26 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   wait_vm_barrier<0>();
   if constexpr (kAdapters) {
     // an adapter holds a value that is none (its rows become NaN, the others must not meet it),
-    // or B passes 2 GiB: the adapters' part by itself
+    // B passes 2 GiB or a row's U fp16's range: the adapters' part by itself (see lce_tile_kernel)
     if (apart) {
+      bool wide = false;
+      auto scale_rows = [&](bool back) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kTM; ++i) {
+          float f = s_rs[i * kT + frow];
+          f = back ? 1.f / f : f;
+#pragma unroll
+          for (int j = 0; j < kTN; ++j)
+#pragma unroll
+            for (int v = 0; v < kAV; ++v) acc[i][j][v] *= f;
+        }
+      };
+      if constexpr (kF16) {
+        const bool mine = tid < kRM && s_ord[tid] >= 0 && (s_bad[s_ord[tid]] & kWide) != 0;
+        if (tid < kRM) s_rs[tid] = mine ? wide_scale(u_f32(P.U, m0 + tid, P.r8), P.r8) : 1.f;
+        wide = __syncthreads_or(mine) != 0;
+        if (wide) scale_rows(false);
+      }
       for (int e = 0; e < n_ext; ++e) {
         const int chunk = tid & 7, x = e * 8 + chunk, q = x / cps, rem = x - q * cps;
         const bool any = q < n_seg;
@@ -1456,14 +1564,21 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
           if (none) b = vu4{0u, 0u, 0u, 0u};
           *reinterpret_cast<vu4*>(st0 + kRM * kRowBytes + lds_off(row, chunk)) = b;
           if (row < kRM) {
-            if (any && s_ord[row] == q)
-              u = *reinterpret_cast<const vu4*>(P.U + (m0 + row) * (int64_t)(P.planes * P.r8) + rem * 8);
+            if (any && s_ord[row] == q) {
+              u = *reinterpret_cast<const vu4*>(P.U + (m0 + row) * (int64_t)(ur * P.r8) + rem * 8);
+              if constexpr (kF16) {
+                if (wide) u = plane8<E>(u_f32(P.U, m0 + row, P.r8) + rem % cpp * 8, s_rs[row], rem / cpp);
+              }
+            }
             *reinterpret_cast<vu4*>(st0 + lds_off(row, chunk)) = u;
           }
         }
         __syncthreads();
         compute(st0);
         __syncthreads();
+      }
+      if constexpr (kF16) {
+        if (wide) scale_rows(true);
       }
     }
   }
@@ -1516,7 +1631,7 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
     for (int w = 0; w < kWaves; ++w)
       if (counts(s_m[w][tid], s_sum[w][tid])) sum += s_sum[w][tid] * fast_exp2((s_m[w][tid] - M) * kLog2e);
     if constexpr (kAdapters) {
-      if (s_ord[tid] >= 0 && s_bad[s_ord[tid]] != 0) sum = __builtin_nanf("");
+      if (s_ord[tid] >= 0 && (s_bad[s_ord[tid]] & kBroken) != 0) sum = __builtin_nanf("");
     }
     float* dst = P.part + ((m0 + tid) * n_nt + nt) * 2;
     dst[0] = M;

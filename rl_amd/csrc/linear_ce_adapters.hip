@@ -7,8 +7,9 @@
 //
 // The [rows, V] logits are never written.  The rows are sorted by adapter, so a 256-row tile of
 // the logits (lce_tile.h) meets few adapters; their part enters the tile's reduction as
-// planes * r more hidden elements (U as two 16-bit values that add up to it).  The logits stay
-// fp32, and U, dU and their sums are fp32.
+// planes * r more hidden elements (U as two 16-bit values that add up to it; fp16: rows of U past
+// its range from fp32 times a power of two, by themselves).  The logits stay fp32, and U, dU and
+// their sums are fp32.
 //
 // Backward: the rows with a non-zero upstream gradient, sorted by adapter, in blocks.  Per block
 // the tile loop writes G without its row factor g, in the operand type (fp16: times 2^15, which
@@ -33,7 +34,6 @@
 namespace mirl {
 namespace {
 
-constexpr int kPlanes = 2;
 constexpr int kRankTile = 64;  // ranks a kernel below handles together
 constexpr float kF16Scale = 32768.f;
 
@@ -245,7 +245,7 @@ struct DownParams {
   DropoutArgs drop;
   uint16_t* h_out;         // [T, ldo], zeros in columns H .. ldo
   int64_t ldo;
-  uint16_t* U;             // [T, kPlanes, r8]
+  uint16_t* U;             // [T, kURow<E>, r8]
   int64_t r8;
   float* U32;              // [rows, r8] by original row, or null
   int64_t ny, nz;          // rank tiles, workgroups that share a row tile's adapters
@@ -255,7 +255,7 @@ struct DownParams {
   const vu4* B;
   int64_t b_vecs, per;
   const int32_t* seg;
-  int32_t* bad;            // [N], zeros before
+  int32_t* bad;            // [N], zeros before: kBroken, and kWide from the rows themselves
 };
 
 constexpr int kScanVecs = 8;  // pieces a thread looks at
@@ -276,7 +276,7 @@ __device__ __forceinline__ void look_through(const DownParams& P, int64_t block)
   for (int u = 0; u < kScanVecs; ++u)
 #pragma unroll
     for (int j = 0; j < 4; ++j) none |= (q[u][j] & ex) == ex || ((q[u][j] >> 16) & ex) == ex;
-  if (none) P.bad[a] = 1;
+  if (none) atomicOr(P.bad + a, kBroken);
 }
 
 // 16 sorted rows a workgroup, the hidden dimension split over its NW waves 64 elements at a
@@ -383,10 +383,15 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(DownParams P) {
 #pragma unroll
       for (int i = 0; i < NW; ++i) v += red[i][rl][rho];
       v *= s;
+      if constexpr (std::is_same<E, F16>::value) {
+        const uint32_t mag = __float_as_uint(v) & 0x7fffffffu;
+        if (mag >= kF16Past && mag < 0x7f800000u) atomicOr(P.bad + a, kWide);  // (its planes are not used)
+        u_f32(P.U, mm, (int)P.r8)[rho0 + rho] = v;
+      }
       uint16_t p[kPlanes];
       split_planes<E>(v, p);
 #pragma unroll
-      for (int k = 0; k < kPlanes; ++k) P.U[(mm * kPlanes + k) * P.r8 + rho0 + rho] = p[k];
+      for (int k = 0; k < kPlanes; ++k) P.U[(mm * kURow<E> + k) * P.r8 + rho0 + rho] = p[k];
       if (P.U32 != nullptr) P.U32[P.perm[mm] * P.r8 + rho0 + rho] = v;
     }
     __syncthreads();
@@ -413,10 +418,12 @@ __global__ __launch_bounds__(256) void adapter_gather_kernel(const int64_t* __re
       *reinterpret_cast<vu4*>(h_out + m * ldo + k) = load_raw8_to(hr, k, H);
     if (aid[m] < 0) continue;
     for (int64_t rho = threadIdx.x; rho < r8; rho += 256) {
+      const float v = U32[row * r8 + rho];
       uint16_t p[kPlanes];
-      split_planes<E>(U32[row * r8 + rho], p);
+      split_planes<E>(v, p);
 #pragma unroll
-      for (int k = 0; k < kPlanes; ++k) U[(m * kPlanes + k) * r8 + rho] = p[k];
+      for (int k = 0; k < kPlanes; ++k) U[(m * kURow<E> + k) * r8 + rho] = p[k];
+      if constexpr (std::is_same<E, F16>::value) u_f32(U, m, (int)r8)[rho] = v;
     }
   }
 }
@@ -1101,7 +1108,7 @@ extern "C" int mirl_adapter_gather(const int64_t* perm, const int32_t* adapter, 
   MIRL_REQUIRE(is16(dtype), "hidden states must be bf16 or fp16 (dtype code %d)", dtype);
   MIRL_REQUIRE(T > 0 && Hd > 0 && ldh >= Hd && ldo >= Hd && ldo % 8 == 0 && r8 > 0, "invalid shape");
   MIRL_REQUIRE(perm && adapter && count && hidden && u_rows && hidden_out && u_planes, "null pointer argument");
-  MIRL_REQUIRE(aligned16(hidden_out), "the gathered rows must be 16-byte aligned");
+  MIRL_REQUIRE(r8 % 8 == 0 && aligned16(hidden_out) && aligned16(u_planes), "the gathered rows must be 16-byte aligned");
   auto launch = [&](auto e) {
     using E = decltype(e);
     hipLaunchKernelGGL(adapter_gather_kernel<E>, dim3((unsigned)std::min(T, int64_t(1) << 20)), dim3(256), 0,
