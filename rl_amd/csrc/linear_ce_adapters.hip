@@ -512,7 +512,7 @@ struct BlockParams {
   int64_t splits, k_len;   // dU's split of the vocabulary
   float* du_part;          // [splits, n, r8]
   float* du;               // [n, r8]: dU with s_a and g
-  uint32_t* peak;          // [2]: the largest |dU| and |g U| of the block (fp16), as bits
+  uint32_t* peak;          // [n, 2]: an adapter's largest |dU| and |g U| (fp16), as bits, at its first row (peak_of)
   uint16_t* duT;           // [kPlanes, r16, ldn]: dU transposed, scaled into range (fp16)
   uint16_t* ugT;           // [kPlanes, r16, ldn]: g U transposed, likewise
   int64_t ldn, r16;
@@ -529,6 +529,12 @@ __device__ __forceinline__ int64_t block_rows(const BlockParams& P) {
   return c < 0 ? 0 : c < P.n ? c : P.n;
 }
 
+// An adapter's maxima in the block: at the place of its first row there.
+__device__ __forceinline__ uint32_t* peak_of(const BlockParams& P, int64_t a) {
+  const int64_t first = P.seg[a] - P.row0;
+  return P.peak + 2 * (first > 0 ? first : 0);
+}
+
 // dU's partial sums: a wave takes 32 rows and a range of the vocabulary, once per adapter
 // among its rows.  (Also clears the maxima that the next kernel takes.)
 template <class E, int NT>
@@ -539,7 +545,10 @@ __global__ __launch_bounds__(256) void adapter_du_kernel(BlockParams P) {
   const int64_t n_rt = (P.n + 127) / 128;
   const int64_t split = blockIdx.x / n_rt, rt = blockIdx.x - split * n_rt;
   const int64_t w0 = rt * 128 + wave * 32, rho0 = (int64_t)blockIdx.y * kRankTile;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && tid < 2) P.peak[tid] = 0;
+  if (std::is_same<E, F16>::value && split == 0 && blockIdx.y == 0) {
+    const int64_t m = rt * 128 + (tid >> 1);
+    if (m < n) P.peak[2 * m + (tid & 1)] = 0;
+  }
   if (w0 >= n) return;
   const int64_t w1 = w0 + 32 < n ? w0 + 32 : n;
   const int64_t k_end = (split + 1) * P.k_len < P.ldbt ? (split + 1) * P.k_len : P.ldbt;
@@ -598,45 +607,59 @@ __global__ __launch_bounds__(256) void adapter_du_kernel(BlockParams P) {
   }
 }
 
-// dU = s_a g (sum of the splits), in split order; the largest magnitudes of dU and g U.
+// dU = s_a g (sum of the splits), in split order; each adapter's largest magnitudes of dU and g U.
 template <class E>
 __global__ __launch_bounds__(256) void adapter_du_sum_kernel(BlockParams P) {
-  const int64_t n = block_rows(P);
-  uint32_t pu = 0, pg = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n * P.r8; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / P.r8, rho = i - m * P.r8;
-    const int32_t a = P.aid[P.row0 + m];
-    float v = 0.f;
-    const float g = P.g[P.row0 + m];
-    if (a >= 0) {
+  const int64_t n = block_rows(P), total = n * P.r8;
+  const int lane = threadIdx.x & 63;
+  // (whole waves go round: 64 elements each)
+  for (int64_t i0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63); i0 < total; i0 += (int64_t)gridDim.x * 256) {
+    const int64_t i = i0 + lane;
+    int32_t a = -1;
+    uint32_t pu = 0, pg = 0;
+    if (i < total) {
+      const int64_t m = i / P.r8, rho = i - m * P.r8;
+      a = P.aid[P.row0 + m];
+      float v = 0.f;
+      const float g = P.g[P.row0 + m];
+      if (a >= 0) {
 #pragma unroll 8
-      for (int64_t s = 0; s < P.splits; ++s) v += P.du_part[(s * P.n + m) * P.r8 + rho];
-      v *= (1.f / g_scale_of<E>()) * P.scaling[a];
-      v *= g;
-      const uint32_t b = __float_as_uint(g * P.U32[P.perm[P.row0 + m] * P.r8 + rho]) & 0x7fffffffu;
-      const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-      // (values that are none do not set the scale)
-      pu = u < 0x7f800000u && u > pu ? u : pu;
-      pg = b < 0x7f800000u && b > pg ? b : pg;
+        for (int64_t s = 0; s < P.splits; ++s) v += P.du_part[(s * P.n + m) * P.r8 + rho];
+        v *= (1.f / g_scale_of<E>()) * P.scaling[a];
+        v *= g;
+        const uint32_t b = __float_as_uint(g * P.U32[P.perm[P.row0 + m] * P.r8 + rho]) & 0x7fffffffu;
+        const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+        // (values that are none do not set the scale)
+        pu = u < 0x7f800000u ? u : 0u;
+        pg = b < 0x7f800000u ? b : 0u;
+      }
+      P.du[i] = v;
     }
-    P.du[i] = v;
-  }
-  if constexpr (std::is_same<E, F16>::value) {
+    if constexpr (std::is_same<E, F16>::value) {
+      uint64_t todo = __ballot(a >= 0);
+      while (todo != 0) {  // the adapters of the wave's rows, one after the other
+        const int32_t at = __shfl(a, __ffsll((unsigned long long)todo) - 1, kWave);
+        const bool mine = a == at;
+        uint32_t mu = mine ? pu : 0u, mg = mine ? pg : 0u;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const uint32_t a = (uint32_t)__shfl_xor((int)pu, off, kWave), b = (uint32_t)__shfl_xor((int)pg, off, kWave);
-      pu = a > pu ? a : pu;
-      pg = b > pg ? b : pg;
-    }
-    if ((threadIdx.x & 63) == 0) {
-      atomicMax(P.peak, pu);  // maxima of whole numbers: any order gives the same
-      atomicMax(P.peak + 1, pg);
+        for (int off = 32; off > 0; off >>= 1) {
+          const uint32_t x = (uint32_t)__shfl_xor((int)mu, off, kWave), y = (uint32_t)__shfl_xor((int)mg, off, kWave);
+          mu = x > mu ? x : mu;
+          mg = y > mg ? y : mg;
+        }
+        if (lane == 0) {
+          uint32_t* peak = peak_of(P, at);
+          atomicMax(peak, mu);  // maxima of whole numbers: any order gives the same
+          atomicMax(peak + 1, mg);
+        }
+        todo &= ~__ballot(mine);
+      }
     }
   }
 }
 
 // The power of two that takes the largest magnitude (its bits) to [2^14, 2^15), for fp16
-// planes; 1 for bf16, which has fp32's range, and for a block of zeros.
+// planes; 1 for bf16, which has fp32's range, and for zeros.
 template <class E>
 __device__ __forceinline__ float plane_scale(const uint32_t* peak) {
   if constexpr (!std::is_same<E, F16>::value) return 1.f;
@@ -651,14 +674,15 @@ __device__ __forceinline__ float plane_scale(const uint32_t* peak) {
 template <class E>
 __global__ __launch_bounds__(256) void adapter_planes_kernel(BlockParams P) {
   const int64_t n = block_rows(P);
-  const float su = plane_scale<E>(P.peak), sg = plane_scale<E>(P.peak + 1);
   const int64_t width = (n + 63) / 64 * 64;  // what the products below read
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < width * P.r16; i += (int64_t)gridDim.x * 256) {
     const int64_t rho = i / width, m = i - rho * width;
     float u = 0.f, gu = 0.f;
-    if (m < n && rho < P.r8 && P.aid[P.row0 + m] >= 0) {
-      u = P.du[m * P.r8 + rho] * su;
-      gu = (P.g[P.row0 + m] * P.U32[P.perm[P.row0 + m] * P.r8 + rho]) * sg;
+    const int32_t a = m < n && rho < P.r8 ? P.aid[P.row0 + m] : -1;
+    if (a >= 0) {
+      const uint32_t* peak = peak_of(P, a);
+      u = P.du[m * P.r8 + rho] * plane_scale<E>(peak);
+      gu = (P.g[P.row0 + m] * P.U32[P.perm[P.row0 + m] * P.r8 + rho]) * plane_scale<E>(peak + 1);
     }
     uint16_t pu[kPlanes], pg[kPlanes];
     split_planes<E>(u, pu);
@@ -748,7 +772,6 @@ __global__ __launch_bounds__(256) void adapter_db_kernel(BlockParams P) {
   const int64_t n = block_rows(P);
   const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 32, rho0 = (int64_t)blockIdx.y * kRankTile;
   if (v0 >= P.V || n == 0) return;
-  const float scale = 1.f / (plane_scale<E>(P.peak + 1) * g_scale_of<E>());
   const uint16_t* x[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) x[i] = P.Gt + (v0 + i * 16 + lr < P.V ? v0 + i * 16 + lr : P.V - 1) * P.ldgt;
@@ -766,6 +789,7 @@ __global__ __launch_bounds__(256) void adapter_db_kernel(BlockParams P) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float scale = 1.f / (plane_scale<E>(P.peak + 2 * lo + 1) * g_scale_of<E>());
     thin_product<E, NT, 2>(x, y, P.r16 * P.ldn, P.ldn, lo / 64 * 64, 64, lo, hi, lg, acc);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -792,7 +816,6 @@ __global__ __launch_bounds__(kDaWaves * 64) void adapter_da_kernel(BlockParams P
   const int64_t n = block_rows(P);
   if (n == 0) return;
   const int64_t h0 = (int64_t)blockIdx.x * 16, rho0 = (int64_t)blockIdx.y * kRankTile;
-  const float scale = (P.drop.threshold > 0 ? P.drop.scale : 1.f) / plane_scale<E>(P.peak);
   const uint16_t* x[1] = {P.hT + (h0 + lr < P.H ? h0 + lr : P.H - 1) * P.ldht + P.row0};
   const uint16_t* y = P.duT + (rho0 + lr) * P.ldn;
   int64_t a = P.aid[P.row0] < 0 ? 0 : P.aid[P.row0];
@@ -805,6 +828,7 @@ __global__ __launch_bounds__(kDaWaves * 64) void adapter_da_kernel(BlockParams P
     f32x4 acc[1][NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float scale = (P.drop.threshold > 0 ? P.drop.scale : 1.f) / plane_scale<E>(P.peak + 2 * lo);
     thin_product<E, NT, 1>(x, y, P.r16 * P.ldn, P.ldn, lo / 64 * 64 + wave * 64, kDaWaves * 64, lo, hi, lg, acc);
     __syncthreads();  // the last adapter's sums are read
 #pragma unroll
@@ -1253,7 +1277,7 @@ static int64_t block_halves(int64_t n, int64_t r8) { return 2 * kPlanes * padded
 
 extern "C" int64_t mirl_adapter_block_workspace_bytes(int64_t n, int64_t r8, int64_t splits) {
   if (n <= 0 || r8 <= 0 || splits <= 0) return 0;
-  return round_up(block_floats(n, r8, splits) * 4, 256) + round_up(block_halves(n, r8) * 2, 256) + 256;
+  return round_up(block_floats(n, r8, splits) * 4, 256) + round_up(block_halves(n, r8) * 2, 256) + n * 8;
 }
 
 extern "C" int mirl_adapter_block_grads(int dtype, int64_t row0, int64_t n, const int64_t* count, const int64_t* perm,
