@@ -1692,7 +1692,7 @@ def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight
     ws = torch.empty(max(1, int(lib.mirl_lce_x_workspace_elems(T, V))), dtype=torch.float32, device=dev)
     st = _launch(
         "mirl_linear_ce_8bit_fwd", dev, hidden8.data_ptr(), hidden_scale.data_ptr(), T, H, hidden8.stride(0),
-        weight8.data_ptr(), weight_scale.data_ptr(), V, weight8.stride(0), int(bsz), target.data_ptr(), target.stride(0),
+        weight8.data_ptr(), weight_scale.data_ptr(), V, H if weight8.is_contiguous() else weight8.stride(0), int(bsz), target.data_ptr(), target.stride(0),
         target.stride(1), int(vocab_start), int(vocab_end), out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
         _stream(dev),
     )
@@ -1825,7 +1825,8 @@ def transpose16(src: torch.Tensor, rows: int, cols: int, dst: torch.Tensor, coun
              and dst.shape[0] == Z and dst.shape[1] >= cols and src.shape[1] >= rows and src.shape[2] >= cols,
              "16-bit operands of matching shapes")
     st = _launch(
-        "mirl_transpose16", dev, src.data_ptr(), Z, src.stride(0), int(rows), int(cols), src.stride(1), dst.data_ptr(),
+        "mirl_transpose16", dev, src.data_ptr(), Z, src.stride(0), int(rows), int(cols),
+        src.shape[2] if src.is_contiguous() else src.stride(1), dst.data_ptr(),
         dst.stride(0), dst.stride(1), dst.shape[2], _ptr(count), _ptr(perm),
         *(drop.args() if drop is not None else (0.0, 0, None, 0)), _stream(dev),
     )
