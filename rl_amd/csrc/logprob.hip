@@ -38,10 +38,14 @@ struct LseState {
 #pragma unroll
     for (int i = 1; i < N; ++i) bm = fmaxf(bm, v[i]);
     const float mn = fmaxf(m, bm);
-    if (mn == -INFINITY) return;  // nothing finite yet on this lane
+    if (mn == -INFINITY) {  // nothing finite yet on this lane: -inf, and NaN, which a maximum does not show
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[0] = v[i] != v[i] ? v[i] : s[0];
+      return;
+    }
     if (mn != m) {
       const float noff = mn * kLog2e;
-      // m == -inf gives 2^-inf = 0, which is the correct (empty) rescale.
+      // m == -inf gives 2^-inf = 0, which is the correct (empty) rescale (and keeps a NaN).
       const float sc = (m == -INFINITY) ? 0.f : fast_exp2(off - noff);
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[k] *= sc;
@@ -138,7 +142,7 @@ __device__ __forceinline__ void row_lse(const typename E::raw* x, int64_t V, int
   float M = wave_max(st.m);
   float s = st.s[0] + st.s[1] + st.s[2] + st.s[3];
   const float OFF = M * kLog2e;
-  s = (st.m == -INFINITY) ? 0.f : s * fast_exp2(st.off - OFF);
+  s = (st.m == -INFINITY) ? s : s * fast_exp2(st.off - OFF);  // (0 or NaN without a maximum)
   s = wave_sum(s);
   // one lane holds the picked value, every other lane 0: the sums are exact
   if (want) pv = wave_sum(pv);
@@ -159,7 +163,7 @@ __device__ __forceinline__ void row_lse(const typename E::raw* x, int64_t V, int
       float sb2 = 0.f;
 #pragma unroll
       for (int k = 0; k < W; ++k)
-        sb2 += (sm[k] == -INFINITY) ? 0.f : ss[k] * fast_exp2(sm[k] * kLog2e - OFFb);
+        sb2 += (sm[k] == -INFINITY) ? ss[k] : ss[k] * fast_exp2(sm[k] * kLog2e - OFFb);
       M = Mb;
       s = sb2;
       if (want) {
