@@ -1044,7 +1044,7 @@ void lce_tile_kernel(LceParams P) {
     //
     // e4m3 of [16384, 4096] x [151936, 4096]: 7.4 ms, 2.75 PFLOP/s (the library's product of
     // these operands, which writes the logits and has no log-sum-exp, 2.89); the MFMA units are
-    // busy 68% of the cycles at the 1.6 GHz that this load leaves: bound by power.
+    // busy 68 to 71% of the cycles at the 1.6 to 1.7 GHz that this load leaves: bound by power.
     //
     // A lane holds kTN groups of columns of kTM rows, the lanes that share a row are kT apart
     // and the two waves of a row band exchange through LDS.

@@ -3,7 +3,7 @@
 //
 //   h    = EH(x + res)                       the stream as it is stored (h = x without res)
 //   n    = h * rstd,  rstd = 1 / sqrt(mean(h^2) + eps)
-//   y    = EX(n * w)                         or, in 8 bits, e4m3(y / s) with s = max|y| / 448
+//   y    = EX(n * w)                         or, in 8 bits, e4m3(y * (1 / s)) with s = max|y| / 448
 //   dh   = rstd * (w dy - n * mean(w dy n)) + dh_out,   dw = sum over rows of dy * n
 //
 // Every sum is fp32; y, h, dx, dres and dw are rounded once, to the types of the tensors that
@@ -324,7 +324,9 @@ __global__ __launch_bounds__(kLongThreads) void norm_fwd_long_kernel(NormFwd P) 
 }
 
 // Rows in 8 bits without a norm (an output weight's): one workgroup per row, read twice (the
-// second time from the cache for rows of ordinary length).
+// second time from the cache for rows of ordinary length).  [151936, 4096] bf16 499 us, once per
+// set of weights: 3.7 TB/s with each element read and written once, 6.4 being what streams reach;
+// a workgroup's second pass waits for the row's maximum.
 template <class EX>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename EX::raw* __restrict__ x, int64_t ldx,
                                                             int64_t R, int64_t H, uint8_t* __restrict__ y,
