@@ -980,6 +980,83 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
                             void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* What a sampler does to logits ahead of top-k and top-p                   */
+/* ---------------------------------------------------------------------- */
+/* Row r of sample b follows the first n = lengths[b] + r (lengths NULL: 1 + r) of the
+ * sample's n_ids tokens (at most 2^20 - 1).  With c the occurrences of a token among those
+ * at positions prompt_lengths[b] (NULL: 0) and later, `seen` if it occurs at all:
+ *   z = x + bias,  z = seen ? (z > 0 ? z / repetition : z * repetition) : z
+ *   z = z - frequency * c - (c > 0 ? presence : 0)
+ *   y = z / temperature where the row's mask allows the token, -inf elsewhere
+ * in fp32.  Ids vocab_start .. vocab_end - 1 are columns 0, 1, ..; others concern no column.
+ * repetition, presence, frequency and temperature are [B], or NULL for one value of all
+ * samples.  bias_ids and bias hold n_bias entries (at most 2047) for each sample
+ * (bias_stride_b apart; 0: the same for all); of two entries of one id the later holds.  masks
+ * holds n_masks rows of at least ceil(V / 32) words, mask_stride words apart, token v being
+ * bit v % 32 of word v / 32 (1: allowed); mask_rows[b, r] names a row's mask, numbers
+ * outside [0, n_masks) none (n_masks 0: no masks, mask_rows not read).
+ */
+typedef struct mirl_logit_processors {
+  const int64_t* ids;
+  int64_t n_ids, ids_stride_b, ids_stride_s;
+  const int64_t* lengths;
+  const int64_t* prompt_lengths;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const float* temperature;
+  const int64_t* bias_ids;
+  const float* bias;
+  int64_t n_bias, bias_stride_b;
+  const int32_t* masks;
+  int64_t n_masks, mask_stride;
+  const int64_t* mask_rows;
+  int64_t mask_rows_stride_b, mask_rows_stride_r;
+  int64_t vocab_start, vocab_end;
+  float repetition_all, presence_all, frequency_all, temperature_all;
+} mirl_logit_processors;
+
+/*
+ * out[b, r] ([B, R] contiguous) = log_softmax(y[b, r]) at the token behind row r, ids[b, n]:
+ * 0 without one (n >= n_ids, or an id outside the columns), -inf in a row that allows
+ * nothing or not that token.  y is never written.  stats ([B, R, 2], or NULL) is
+ * kept for the backward.  workspace: mirl_processed_logprob_workspace_elems floats.
+ */
+int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V);
+int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
+                               int64_t stride_b, int64_t stride_r,
+                               const mirl_logit_processors* processors, float* out,
+                               float* stats, float* workspace, void* stream);
+
+/*
+ * Its backward: grad_in [B, Rt, V] in the logits' type, zeros in rows R .. Rt - 1, in rows
+ * whose upstream gradient (grad_out [B, R] by strides) is zero and in rows that allow
+ * nothing; those rows' logits are not read.
+ */
+int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t Rt,
+                               int64_t V, int64_t stride_b, int64_t stride_r,
+                               const mirl_logit_processors* processors, const float* stats,
+                               const float* grad_out, int64_t g_stride_b, int64_t g_stride_r,
+                               void* grad_in, int64_t gi_stride_b, int64_t gi_stride_r,
+                               void* stream);
+
+/*
+ * y written out in the logits' type, each value rounded once; out may be the logits (same
+ * strides), of which then only what changes is touched.  And the backward of that: grad_in =
+ * grad_out times what each logit was multiplied by (0 where a mask forbids it), logits being
+ * those of the forward.
+ */
+int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
+                        int64_t stride_b, int64_t stride_r,
+                        const mirl_logit_processors* processors, void* out,
+                        int64_t o_stride_b, int64_t o_stride_r, void* stream);
+int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
+                            int64_t stride_b, int64_t stride_r,
+                            const mirl_logit_processors* processors, const void* grad_out,
+                            int64_t g_stride_b, int64_t g_stride_r, void* grad_in,
+                            int64_t gi_stride_b, int64_t gi_stride_r, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Logprobs from hidden states with low-rank adapters beside the weight     */
 /* ---------------------------------------------------------------------- */
 /* Rows r = s * B + b (position s of sample b), sample b under adapter ids[b] in

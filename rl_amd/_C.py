@@ -122,6 +122,39 @@ class ScArgs(ctypes.Structure):
     ]
 
 
+class LogitProcessorArgs(ctypes.Structure):
+    """mirl_logit_processors."""
+
+    _fields_ = [
+        ("ids", ctypes.c_void_p),
+        ("n_ids", ctypes.c_int64),
+        ("ids_stride_b", ctypes.c_int64),
+        ("ids_stride_s", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("prompt_lengths", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("n_bias", ctypes.c_int64),
+        ("bias_stride_b", ctypes.c_int64),
+        ("masks", ctypes.c_void_p),
+        ("n_masks", ctypes.c_int64),
+        ("mask_stride", ctypes.c_int64),
+        ("mask_rows", ctypes.c_void_p),
+        ("mask_rows_stride_b", ctypes.c_int64),
+        ("mask_rows_stride_r", ctypes.c_int64),
+        ("vocab_start", ctypes.c_int64),
+        ("vocab_end", ctypes.c_int64),
+        ("repetition_all", ctypes.c_float),
+        ("presence_all", ctypes.c_float),
+        ("frequency_all", ctypes.c_float),
+        ("temperature_all", ctypes.c_float),
+    ]
+
+
 # exported symbol -> (restype, argtypes)
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -297,6 +330,13 @@ SIGNATURES = {
         [_I, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
          _P, _I64, _P, ctypes.c_double, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P],
     ),
+    "mirl_processed_logprob_workspace_elems": (_I64, [_I64, _I64, _I64]),
+    "mirl_processed_logprob_fwd": (_I, [_P, _I] + [_I64] * 5 + [_P] * 5),
+    "mirl_processed_logprob_bwd": (
+        _I, [_P, _I] + [_I64] * 6 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
+    "mirl_process_logits": (_I, [_P, _I] + [_I64] * 5 + [_P] * 2 + [_I64] * 2 + [_P]),
+    "mirl_process_logits_bwd": (
+        _I, [_P, _I] + [_I64] * 5 + [_P] * 2 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
@@ -1202,6 +1242,89 @@ def top_k_top_p_mask(x2d: torch.Tensor, top_k: int, top_p: float,
     )
     _check(st, "mirl_top_k_top_p_mask")
     return filt, keep
+
+
+# ---------------------------------------------------------------------------
+# penalties, biases and grammar masks on logits
+# ---------------------------------------------------------------------------
+def processor_args(ids: torch.Tensor, tensors: dict, scalars: dict, vocab: tuple) -> LogitProcessorArgs:
+    """The C struct of one call.  ``ids`` [B, n_ids] int64; ``tensors``: lengths and prompt_lengths
+    [B] int64, repetition, presence, frequency and temperature [B] fp32, bias_ids and bias [K] or [B, K]
+    (int64, fp32), masks [M, W] int32, mask_rows [B, R] int64, each contiguous in its last dimension or
+    None; ``scalars``: the value of each of the four that is None; ``vocab``: (start, end).  Sizes are
+    the caller's to check."""
+    A = LogitProcessorArgs()
+    A.ids, A.n_ids, A.ids_stride_b, A.ids_stride_s = ids.data_ptr(), ids.shape[1], ids.stride(0), ids.stride(1)
+    for name in ("lengths", "prompt_lengths", "repetition", "presence", "frequency", "temperature", "bias_ids", "bias", "masks", "mask_rows"):
+        t = tensors.get(name)
+        if t is not None:
+            setattr(A, name, t.data_ptr())
+    for name, value in scalars.items():
+        setattr(A, name + "_all", value)
+    bias = tensors.get("bias")
+    if bias is not None:
+        A.n_bias, A.bias_stride_b = bias.shape[-1], bias.shape[-1] if bias.dim() == 2 else 0
+    masks, rows = tensors.get("masks"), tensors.get("mask_rows")
+    if masks is not None:
+        A.n_masks, A.mask_stride = masks.shape[0], masks.stride(0)
+        A.mask_rows_stride_b, A.mask_rows_stride_r = rows.stride(0), rows.stride(1)
+    A.vocab_start, A.vocab_end = vocab
+    return A
+
+
+def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs, want_stats: bool):
+    """(logprobs [B, R] fp32, stats [B, R, 2] or None) of the first R rows (see mirl_processed_logprob_fwd)."""
+    dev = logits.device
+    B, _, V = logits.shape
+    out = torch.empty((B, R), dtype=torch.float32, device=dev)
+    stats = torch.empty((B, R, 2), dtype=torch.float32, device=dev) if want_stats else None
+    lib = _lib if _lib is not None else load()
+    ws = torch.empty(max(1, lib.mirl_processed_logprob_workspace_elems(B, R, V)), dtype=torch.float32, device=dev)
+    st = _launch("mirl_processed_logprob_fwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
+                 logits.stride(1), ctypes.byref(args), out.data_ptr(), _ptr(stats), ws.data_ptr(), _stream(dev))
+    _check(st, "mirl_processed_logprob_fwd")
+    return out, stats
+
+
+def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, stats: torch.Tensor,
+                          grad_out: torch.Tensor) -> torch.Tensor:
+    """The gradient of the logits, a new contiguous tensor (see mirl_processed_logprob_bwd)."""
+    dev = _require_gpu(logits, stats, grad_out)
+    B, Rt, V = logits.shape
+    R = stats.shape[1]
+    _require(grad_out.dtype == torch.float32 and tuple(grad_out.shape) == (B, R), "an fp32 gradient [B, R]")
+    grad = torch.empty((B, Rt, V), dtype=logits.dtype, device=dev)
+    st = _launch("mirl_processed_logprob_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, Rt, V, logits.stride(0),
+                 logits.stride(1), ctypes.byref(args), stats.data_ptr(), grad_out.data_ptr(), grad_out.stride(0),
+                 grad_out.stride(1), grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
+    _check(st, "mirl_processed_logprob_bwd")
+    return grad
+
+
+def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool) -> torch.Tensor:
+    """Processed logits, in place or as a new contiguous tensor (see mirl_process_logits)."""
+    dev = logits.device
+    B, R, V = logits.shape
+    out = logits if inplace else torch.empty((B, R, V), dtype=logits.dtype, device=dev)
+    st = _launch("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
+                 logits.stride(1), ctypes.byref(args), out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
+    _check(st, "mirl_process_logits")
+    return out
+
+
+def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, grad_out: torch.Tensor) -> torch.Tensor:
+    """The gradient of the logits, a new contiguous tensor (see mirl_process_logits_bwd)."""
+    dev = _require_gpu(logits, grad_out)
+    B, R, V = logits.shape
+    _require(grad_out.dtype == logits.dtype and grad_out.shape == logits.shape, "a gradient like the logits")
+    if grad_out.stride(-1) != 1:
+        grad_out = grad_out.contiguous()
+    grad = torch.empty((B, R, V), dtype=logits.dtype, device=dev)
+    st = _launch("mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
+                 logits.stride(1), ctypes.byref(args), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
+                 grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
+    _check(st, "mirl_process_logits_bwd")
+    return grad
 
 
 # ---------------------------------------------------------------------------

@@ -76,6 +76,54 @@ def apply_top_k_top_p(
     return apply_top_k_top_p_kernel(logits, top_k, top_p)
 
 
+@dataclass
+class LogitProcessors:
+    """What a sampler does to logits ahead of top-k and top-p, for training-side logprobs that match it.
+
+    Penalties and temperature are one number or a floating tensor ``[B]``.  A token of the prompt or the
+    response so far is under ``repetition_penalty`` (a logit above 0 is divided by it, others are
+    multiplied; 1.0: off); one of the response, the positions from ``prompt_lengths [B]`` on (None: all),
+    loses ``frequency_penalty`` for each occurrence and ``presence_penalty`` once.  ``bias_ids`` and ``bias``
+    (``[K]`` or ``[B, K]``, at most 2047 entries, unused ones with an id of -1; of two entries of one id the
+    later holds) are added to single tokens' logits ahead of the penalties; -inf rules a token out.
+    ``grammar_masks [M, W]`` (int32; token v is bit ``v % 32`` of word ``v // 32``, 1 allowed) holds the distinct
+    masks and ``grammar_rows [B, R]`` each row's, -1 for a row under no grammar.  ``temperature`` comes last:
+    with it here ``apply_temperature_scaling`` is not called as well.
+    """
+
+    repetition_penalty: float | torch.Tensor = 1.0
+    presence_penalty: float | torch.Tensor = 0.0
+    frequency_penalty: float | torch.Tensor = 0.0
+    temperature: float | torch.Tensor = 1.0
+    prompt_lengths: Optional[torch.Tensor] = None
+    bias_ids: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    grammar_masks: Optional[torch.Tensor] = None
+    grammar_rows: Optional[torch.Tensor] = None
+
+
+def apply_logit_processors(
+    logits: torch.Tensor,
+    input_ids: torch.Tensor,
+    processors: Optional[LogitProcessors],
+    history_lengths: Optional[torch.Tensor] = None,
+    inplace: bool = False,
+) -> torch.Tensor:
+    """Logits under penalties, biases, grammar masks and temperature, in their own type (each rounded
+    once from fp32); the logits themselves for None.
+
+    ``logits [B, R, V]``: row r follows tokens ``0 .. r`` of ``input_ids [B, L]``, or with
+    ``history_lengths [B]`` the first ``history_lengths[b] + r`` of them; ``logits [B, V]``: one row behind
+    each history.  Differentiable in the logits.  With ``inplace`` only what changes is read and written,
+    and there is no gradient.  The formulas are those of :mod:`rl_amd.distributed.logit_processing`.
+    """
+    if processors is None:
+        return logits
+    from rl_amd.distributed.logit_processing import process_logits
+
+    return process_logits(logits, input_ids, processors, history_lengths, inplace)
+
+
 def need_temperature_scaling(sampling_params: Optional[TrainingSamplingParams]) -> bool:
     """Whether apply_temperature_scaling will mutate the logits in place
     (reference nemo_rl/models/automodel/train.py:241-245)."""

@@ -36,6 +36,7 @@ SOURCES = [
     "dropout.hip",
     "linear_ce_8bit.hip",
     "linear_ce_adapters.hip",
+    "processors.hip",
 ]
 
 ARCH = "gfx950"

@@ -26,6 +26,7 @@ import torch
 from rl_amd import _C
 from rl_amd.distributed.early_backward import POLICY, set_early_backward
 from rl_amd.algorithms.logits_sampling_utils import (
+    LogitProcessors,
     TrainingSamplingParams,
     need_top_k_or_top_p_filtering,
 )
@@ -53,6 +54,7 @@ __all__ = [
     "get_next_token_logprobs_from_logits",
     "get_policy_logprobs_at_sampler_topk",
     "HeadAdapters",
+    "processed_next_token_logprobs",
     "quantize_rows_8bit",
     "rms_norm",
     "set_early_backward",
@@ -98,6 +100,10 @@ def __getattr__(name: str):
         from rl_amd.distributed import policy_head
 
         return getattr(policy_head, name)
+    if name == "processed_next_token_logprobs":
+        from rl_amd.distributed.logit_processing import processed_next_token_logprobs
+
+        return processed_next_token_logprobs
     if name == "dropout":
         from rl_amd.distributed.counter_dropout import dropout
 
@@ -430,6 +436,7 @@ def from_parallel_logits_to_logprobs(
     cp_group: Optional[Any] = None,
     chunk_size: Optional[int] = None,
     sampling_params: Optional[TrainingSamplingParams] = None,
+    logit_processors: Optional[LogitProcessors] = None,
 ) -> torch.Tensor:
     """Next-token logprobs ``[B, S-1]`` (fp32) from ``[B, S, V]`` logits and ``[B, S]`` targets.
 
@@ -439,17 +446,36 @@ def from_parallel_logits_to_logprobs(
     are computed; the backward writes zeros for the last row.  With
     ``sampling_params`` the filter decides top-p in the logits' own dtype, as
     the reference's DistributedLogprobWithSampling does on this tensor.
+    ``logit_processors`` (an extension: penalties, biases, grammar masks and temperature of the
+    sampler) come ahead of the filter; ``target`` is also the history that they count.  Without
+    a filter the processed logits are never written, with one they are, in the logits' type.
     """
     return _next_token_logprobs(vocab_parallel_logits, target, vocab_start_index,
                                 vocab_end_index, tp_group, inference_only, cp_group, chunk_size,
-                                sampling_params, None)
+                                sampling_params, None, logit_processors)
 
 
 def _next_token_logprobs(logits, target, vocab_start_index, vocab_end_index, tp_group,
-                         inference_only, cp_group, chunk_size, sampling_params, decision_dtype):
+                         inference_only, cp_group, chunk_size, sampling_params, decision_dtype,
+                         logit_processors=None):
     _require_single_rank(tp_group, cp_group)
     _check_chunk_size(chunk_size)
     logits = _check_logits(logits)
+    if logit_processors is not None:
+        from rl_amd.distributed.logit_processing import process_logits, processed_next_token_logprobs
+
+        tgt = _next_token_targets(target, logits.shape[1])  # (the checks of the plain path)
+        if not need_top_k_or_top_p_filtering(sampling_params):
+            return processed_next_token_logprobs(
+                logits, target, logit_processors, None, inference_only, vocab_start_index, vocab_end_index)
+        from rl_amd.distributed.sampling import filtered_row_logprobs
+
+        with torch.set_grad_enabled(torch.is_grad_enabled() and not inference_only):
+            rows = process_logits(logits[:, : tgt.shape[1]], target, logit_processors)
+        return filtered_row_logprobs(
+            rows, tgt, sampling_params.top_k, sampling_params.top_p,  # type: ignore[union-attr]
+            inference_only=inference_only, decision_dtype=decision_dtype,
+        )
     if need_top_k_or_top_p_filtering(sampling_params):
         from rl_amd.distributed.sampling import filtered_next_token_logprobs
 
@@ -599,6 +625,7 @@ def get_next_token_logprobs_from_logits(
     sampling_params: Optional[TrainingSamplingParams] = None,
     chunk_size: Optional[int] = None,
     cp_sharder: Optional[Any] = None,
+    logit_processors: Optional[LogitProcessors] = None,
 ) -> torch.Tensor:
     """Next-token logprobs ``[B, S-1]`` (reference model_utils.py:1624-1720).
 
@@ -626,7 +653,7 @@ def get_next_token_logprobs_from_logits(
     # filter decides top-p in fp32; the kernels read the logits dtype directly
     logprobs = _next_token_logprobs(
         next_token_logits, input_ids, 0, V, None, False, None,
-        chunk_size if use_chunking else None, sampling_params, torch.float32,
+        chunk_size if use_chunking else None, sampling_params, torch.float32, logit_processors,
     )
     if logprobs.shape[1] == input_ids.shape[1] - 1:
         return logprobs  # the slice below would be the whole tensor
