@@ -56,6 +56,8 @@ template <class E>
 using piece_t = typename Piece<alignof(typename E::raw)>::type;
 template <class E>
 constexpr int kP = kG / E::kVec;  // 16-byte pieces of a group
+template <class E>
+constexpr uint32_t kGroupBytes = kG * sizeof(typename E::raw);
 
 template <class E>
 __device__ __forceinline__ void unpack_group(const vu4 (&q)[kP<E>], float (&v)[kG]) {
@@ -67,33 +69,41 @@ __device__ __forceinline__ void unpack_group(const vu4 (&q)[kP<E>], float (&v)[k
     for (int e = 0; e < E::kVec; ++e) v[i * E::kVec + e] = w[e];
   }
 }
-// (rows start anywhere: the hardware takes 16-byte pieces at any element)
+// A group at `at` bytes into a row's slice (rows start anywhere: the hardware takes 16-byte pieces at
+// any element).
 template <class E>
-__device__ __forceinline__ void load_pieces(const typename E::raw* p, vu4 (&q)[kP<E>]) {
+__device__ __forceinline__ void load_group(const typename E::raw* slice, uint32_t at, vu4 (&q)[kP<E>]) {
 #pragma unroll
-  for (int i = 0; i < kP<E>; ++i) q[i] = __builtin_nontemporal_load(reinterpret_cast<const piece_t<E>*>(p) + i);
+  for (int i = 0; i < kP<E>; ++i)
+    q[i] = __builtin_nontemporal_load(reinterpret_cast<const piece_t<E>*>(reinterpret_cast<const char*>(slice) + at) + i);
 }
 template <class E>
-__device__ __forceinline__ void store_group(typename E::raw* row, int64_t c, int64_t V, const float (&v)[kG]) {
-  if (c + kG <= V) {
+__device__ __forceinline__ void store_group(typename E::raw* slice, uint32_t at, const float (&v)[kG]) {
 #pragma unroll
-    for (int i = 0; i < kP<E>; ++i) {
-      float w[E::kVec];
+  for (int i = 0; i < kP<E>; ++i) {
+    float w[E::kVec];
 #pragma unroll
-      for (int e = 0; e < E::kVec; ++e) w[e] = v[i * E::kVec + e];
-      __builtin_nontemporal_store((piece_t<E>)E::pack(w), reinterpret_cast<piece_t<E>*>(row + c) + i);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kG; ++e)
-      if (c + e < V) row[c + e] = E::from_float(v[e]);
+    for (int e = 0; e < E::kVec; ++e) w[e] = v[i * E::kVec + e];
+    __builtin_nontemporal_store((piece_t<E>)E::pack(w), reinterpret_cast<piece_t<E>*>(reinterpret_cast<char*>(slice) + at) + i);
   }
 }
-template <class E>
-__device__ __forceinline__ void load_tail(const typename E::raw* row, int64_t c, int64_t V, float fill, float (&v)[kG]) {
-#pragma unroll
-  for (int e = 0; e < kG; ++e) v[e] = c + e < V ? E::load(row + c + e) : fill;
+
+// The maximum and the sum over a wave by lane permutes within the VALU (64 lanes; in lane 63, given to all).
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float other, float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, 0xf, 0xf, false));
 }
+template <class F>
+__device__ __forceinline__ float wave_fold(float v, float none, F&& f) {
+  v = f(v, from_lane<0x111>(none, v));  // row_shr 1, 2, 4, 8
+  v = f(v, from_lane<0x112>(none, v));
+  v = f(v, from_lane<0x114>(none, v));
+  v = f(v, from_lane<0x118>(none, v));
+  v = f(v, from_lane<0x142>(none, v));  // row_bcast 15, 31
+  v = f(v, from_lane<0x143>(none, v));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float of_row(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
 
 // What holds for all rows of a sample.
 struct Sample {
@@ -101,16 +111,16 @@ struct Sample {
   const float* bias;
 };
 
-// Bias and penalties of the tokens of a group whose bit is set (a wave looks at a token only if one
-// of its lanes has it), and with SLOPE what each x was multiplied by.
+// Bias and penalties of a group's tokens: those of any lane of the wave (`any`, a scalar), in the
+// lanes that have them (`bits`); with SLOPE what each x was multiplied by.
 template <bool SLOPE>
-__device__ __forceinline__ void special(float (&v)[kG], float (&slope)[kG], uint32_t bits, const uint32_t* words, const Sample& S) {
+__device__ __forceinline__ void special(float (&v)[kG], float (&slope)[kG], uint32_t any, uint32_t bits, const vu4* words,
+                                        const Sample& S) {
 #pragma unroll
   for (int e = 0; e < kG; ++e) {
-    const bool mine = (bits >> e) & 1u;
-    if (__ballot(mine) == 0) continue;
-    if (mine) {
-      const uint32_t w = words[e];
+    if ((any & (1u << e)) == 0) continue;
+    if ((bits >> e) & 1u) {
+      const uint32_t w = words[e / 4][e % 4];
       float z = v[e];
       if (w >> kBiasShift) z += S.bias[(w >> kBiasShift) - 1];
       if (w & (kInPrompt | kCount)) {
@@ -129,17 +139,18 @@ __device__ __forceinline__ void special(float (&v)[kG], float (&slope)[kG], uint
 template <class E, int MODE, int NV>
 __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   using raw = typename E::raw;
-  constexpr int kSlice = kThreads * NV * kG;
-  constexpr bool kReads = MODE != kInPlace;  // every group of a row is read
+  constexpr int kWaveCols = kWave * NV * kG, kSlice = kWaves * kWaveCols;
   __shared__ __align__(16) uint32_t s_word[kSlice];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t slice = blockIdx.x % P.slices, rest = blockIdx.x / P.slices;
-  const int64_t chunk = rest % P.chunks, b = rest / P.chunks;
-  const int64_t n0 = slice * kSlice, V = P.V;
-  const int64_t r0 = chunk * P.rows, r1 = min(r0 + P.rows, P.Rt);
+  const uint32_t slices = (uint32_t)P.slices, chunks = (uint32_t)P.chunks;
+  const uint32_t slice = blockIdx.x % slices, rest = blockIdx.x / slices;
+  const uint32_t chunk = rest % chunks, b = rest / chunks;
+  const int64_t n0 = (int64_t)slice * kSlice;
+  const int64_t r0 = (int64_t)chunk * P.rows;
+  const int n_rows = (int)min((int64_t)P.rows, P.Rt - r0);
   const mirl_logit_processors& A = P.A;
-  const int64_t L = A.n_ids, vs = A.vocab_start;
+  const int64_t L = A.n_ids;
   const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1;
   const int64_t prompt = A.prompt_lengths != nullptr ? A.prompt_lengths[b] : 0;
   const int64_t* ids = A.ids + b * A.ids_stride_b;
@@ -156,259 +167,323 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 #pragma unroll
   for (int i = 0; i < kSlice / 4 / kThreads; ++i)
     reinterpret_cast<vu4*>(s_word)[i * kThreads + tid] = vu4{0u, 0u, 0u, 0u};
+  // an id's column in this slice, or -1
+  const int64_t first_id = A.vocab_start + n0;
+  const uint32_t here = (uint32_t)max(int64_t(0), min((int64_t)kSlice, P.n_vocab - n0));
+  auto column = [&](int64_t id) {
+    const uint64_t c = (uint64_t)id - (uint64_t)first_id;
+    return c < here ? (int)c : -1;
+  };
   __syncthreads();
-  // the column of an id in this slice, or a number outside it
-  auto column = [&](int64_t id) { return id >= vs && id - vs < P.n_vocab ? id - vs - n0 : -1; };
   if (A.n_bias > 0) {  // of two entries of a token the later holds
     for (int64_t k = tid; k < A.n_bias; k += kThreads) {
-      const int64_t c = column(A.bias_ids[b * A.bias_stride_b + k]);
-      if (c >= 0 && c < kSlice) atomicMax(&s_word[c], (uint32_t)(k + 1) << kBiasShift);
+      const int c = column(A.bias_ids[b * A.bias_stride_b + k]);
+      if (c >= 0) atomicMax(&s_word[c], (uint32_t)(k + 1) << kBiasShift);
     }
     __syncthreads();
   }
-  const int64_t ahead = min(max(n_b + r0, int64_t(0)), L);
-  for (int64_t p = tid; p < ahead; p += kThreads) {
-    const int64_t c = column(ids[p * A.ids_stride_s]);
-    if (c >= 0 && c < kSlice) {
-      if (p < prompt)
+  const int ahead = (int)min(max(n_b + r0, int64_t(0)), L);
+  const int in_prompt = (int)min(max(prompt, int64_t(0)), L);
+#pragma unroll 4
+  for (int p = tid; p < ahead; p += kThreads) {
+    const int c = column(ids[p * A.ids_stride_s]);
+    if (c >= 0) {
+      if (p < in_prompt)
         atomicOr(&s_word[c], kInPrompt);
       else
         atomicAdd(&s_word[c], 1u);
     }
   }
+  // What the rows need, row r0 + l in lane l: the token that is new ahead of it and the one behind it
+  // (columns of this wave, or -1), its mask, its gradient and statistics.
+  int m_new = -1, m_next = -1, m_mask = -1;
+  float m_g = 0.f, m_M = 0.f, m_ls = 0.f;
+  if (lane < n_rows) {
+    const int64_t r = r0 + lane, at = n_b + r;
+    auto of_wave = [&](int c) { return c >= 0 && c / kWaveCols == wave ? c - wave * kWaveCols : -1; };
+    if (lane > 0 && at > 0 && at <= L) {
+      m_new = of_wave(column(ids[(at - 1) * A.ids_stride_s]));
+      if (m_new >= 0 && at - 1 < prompt) m_new |= 1 << 30;
+    }
+    if constexpr (MODE == kFwd || MODE == kBwd) {
+      if (at >= 0 && at < L) m_next = of_wave(column(ids[at * A.ids_stride_s]));
+    }
+    if (A.n_masks > 0 && (MODE != kBwd || r < P.R)) {
+      const int64_t m = A.mask_rows[b * A.mask_rows_stride_b + r * A.mask_rows_stride_r];
+      m_mask = m >= 0 && m < A.n_masks ? (int)m : -1;
+    }
+    if constexpr (MODE == kBwd) {
+      if (r < P.R) {
+        m_g = P.g[b * P.gsb + r * P.gsr];
+        m_M = P.stats[(b * P.R + r) * 2];
+        m_ls = P.stats[(b * P.R + r) * 2 + 1];
+        if (m_M == -INFINITY && m_ls == -INFINITY) m_g = 0.f;  // nothing was left in the row
+      }
+    }
+  }
   __syncthreads();
 
-  // ---- from here on each lane by itself ----
+  // ---- from here on each wave by itself ----
   const int g0 = wave * NV * kWave + lane;  // group u of the lane: g0 + 64 u
-  uint32_t bits[(NV + 3) / 4] = {};
+  const vu4* words = reinterpret_cast<const vu4*>(s_word) + g0 * (kG / 4);
+  constexpr int kU = kWave * (kG / 4);  // between the lane's groups
+  uint32_t bits[(NV + 3) / 4] = {}, any[(NV + 3) / 4] = {};  // a byte per group: the lane's, the wave's
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    const vu4 a = *reinterpret_cast<const vu4*>(s_word + (g0 + u * kWave) * kG);
-    const vu4 c = *reinterpret_cast<const vu4*>(s_word + (g0 + u * kWave) * kG + 4);
-    uint32_t m = 0;
+    const vu4 lo = words[u * kU], hi = words[u * kU + 1];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m |= (a[e] != 0 ? 1u << e : 0u) | (c[e] != 0 ? 16u << e : 0u);
-    bits[u / 4] |= m << (8 * (u % 4));
+    for (int e = 0; e < kG; ++e) {
+      const bool set = (e < 4 ? lo[e & 3] : hi[e & 3]) != 0;
+      bits[u / 4] |= set ? 1u << (8 * (u % 4) + e) : 0u;
+      any[u / 4] |= __ballot(set) != 0 ? 1u << (8 * (u % 4) + e) : 0u;
+    }
   }
-  const raw* xb = static_cast<const raw*>(P.x) + b * P.xsb;
-  raw* yb = MODE == kFwd ? nullptr : static_cast<raw*>(P.y) + b * P.ysb;
-  // rows of the gradient without an upstream one are not read
-  auto upstream = [&](int64_t r) { return r < P.R ? P.g[b * P.gsb + r * P.gsr] : 0.f; };
-  auto dead_row = [&](int64_t r, float gv) {
-    if (gv == 0.f) return true;
-    const float* st = P.stats + (b * P.R + r) * 2;
-    return st[0] == -INFINITY && st[1] == -INFINITY;  // nothing was left in it
-  };
-  auto column_of = [&](int u) { return n0 + (int64_t)(g0 + u * kWave) * kG; };
-  vu4 q[NV][kP<E>];
-  auto issue = [&](int64_t r) {
-    const raw* row = MODE == kApplyGrad ? static_cast<const raw*>(P.dy) + b * P.gsb + r * P.gsr : xb + r * P.xsr;
-#pragma unroll
-    for (int u = 0; u < NV; ++u)
-      if (column_of(u) + kG <= V) load_pieces<E>(row + column_of(u), q[u]);
-  };
+  const raw* xr = static_cast<const raw*>(P.x) + b * P.xsb + r0 * P.xsr + n0;
+  const raw* dyr = MODE == kApplyGrad ? static_cast<const raw*>(P.dy) + b * P.gsb + r0 * P.gsr + n0 : nullptr;
+  raw* yr = MODE == kFwd ? nullptr : static_cast<raw*>(P.y) + b * P.ysb + r0 * P.ysr + n0;
+  const uint32_t left = (uint32_t)min((int64_t)kSlice, P.V - n0);  // columns of the slice
+  const uint32_t at0 = g0 * kGroupBytes<E>;
   const bool dense = S.inv_t != 1.f;  // kInPlace: every value changes
 
-  float gv = 0.f;
-  bool skip = false;
-  if constexpr (MODE == kBwd) {
-    gv = upstream(r0);
-    skip = dead_row(r0, gv);
-  }
-  if (kReads && !skip) issue(r0);
-  for (int64_t r = r0; r < r1; ++r) {
-    if (r > r0) {  // the token ahead of this row
-      const int64_t p = n_b + r - 1;
-      if (p >= 0 && p < L) {
-        const int64_t c = column(ids[p * A.ids_stride_s]);
-        if (c >= 0 && c < kSlice && (int)(c / (kG * kWave * NV)) == wave) {
-          const int in = (int)(c / kG) - wave * NV * kWave;  // 64 u + lane
-          if ((in & 63) == lane) {
-            s_word[c] = p < prompt ? s_word[c] | kInPrompt : s_word[c] + 1;
+  // WHOLE: the slice lies inside the row
+  auto rows = [&](auto whole_c) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole_c)::value;
+    constexpr bool kStreams = MODE != kInPlace;  // every group of a row is read
+    auto full = [&](int u) { return WHOLE || (uint32_t)(g0 + u * kWave + 1) * kG <= left; };
+    auto at = [&](int u) { return at0 + u * kWave * kGroupBytes<E>; };
+    auto tail = [&](const raw* row, int u, float fill, float (&v)[kG]) {
 #pragma unroll
-            for (int u = 0; u < NV; ++u)
-              if (u == in / 64) bits[u / 4] |= 1u << (8 * (u % 4) + (int)(c % kG));
+      for (int e = 0; e < kG; ++e) {
+        const uint32_t c = (uint32_t)(g0 + u * kWave) * kG + e;
+        v[e] = c < left ? E::load(row + c) : fill;
+      }
+    };
+    auto put = [&](int u, const float (&v)[kG]) {
+      if (full(u)) {
+        store_group<E>(yr, at(u), v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kG; ++e) {
+          const uint32_t c = (uint32_t)(g0 + u * kWave) * kG + e;
+          if (c < left) yr[c] = E::from_float(v[e]);
+        }
+      }
+    };
+    vu4 q[NV][kP<E>];
+    auto issue = [&](const raw* row, int u) {
+      if (full(u)) load_group<E>(row, at(u), q[u]);
+    };
+    bool read = true;  // whether this row's values are on their way
+    if constexpr (MODE == kBwd) read = of_row(m_g, 0) != 0.f;
+    if (kStreams && read) {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) issue(MODE == kApplyGrad ? dyr : xr, u);
+    }
+    for (int i = 0; i < n_rows; ++i) {
+      if (i > 0) {  // the token ahead of this row
+        const int t = __builtin_amdgcn_readlane(m_new, i);
+        if (t >= 0) {
+          const uint32_t c = (uint32_t)t & ((1u << 30) - 1), group = c / kG, e = c % kG;
+          const uint32_t bit = 1u << e;
+          if ((int)(group % kWave) == lane) {
+            uint32_t& w = s_word[wave * kWaveCols + c];
+            w = (uint32_t)t >> 30 ? w | kInPrompt : w + 1;
           }
-        }
-      }
-    }
-    // this row's values, and the next row's on their way
-    float v[NV][kG];
-    const float g_now = gv;
-    const bool skip_now = skip;
-    if (kReads && !skip_now) {
-      const raw* row = MODE == kApplyGrad ? static_cast<const raw*>(P.dy) + b * P.gsb + r * P.gsr : xb + r * P.xsr;
 #pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        if (column_of(u) + kG <= V)
-          unpack_group<E>(q[u], v[u]);
-        else
-          load_tail<E>(row, column_of(u), V, MODE == kFwd ? -INFINITY : 0.f, v[u]);
-      }
-    }
-    if (r + 1 < r1) {
-      if constexpr (MODE == kBwd) {
-        gv = upstream(r + 1);
-        skip = dead_row(r + 1, gv);
-      }
-      if (kReads && !skip) issue(r + 1);
-    }
-    raw* yr = MODE == kFwd ? nullptr : yb + r * P.ysr;
-    if constexpr (MODE == kBwd) {
-      if (skip_now) {
-        const float z[kG] = {};
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (column_of(u) < V) store_group<E>(yr, column_of(u), V, z);
-        continue;
-      }
-    }
-    const uint8_t* mask = nullptr;
-    if (A.n_masks > 0) {
-      const int64_t m = A.mask_rows[b * A.mask_rows_stride_b + r * A.mask_rows_stride_r];
-      if (m >= 0 && m < A.n_masks) mask = reinterpret_cast<const uint8_t*>(A.masks + m * A.mask_stride);
-    }
-    uint32_t allowed[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      allowed[u] = 0xffu;
-      if (mask != nullptr && column_of(u) < V) allowed[u] = mask[column_of(u) / kG];
-    }
-    // the next token's place in this wave: group of the lane, and which of its eight
-    int tu = -1, tlane = -1, te = -1;
-    if constexpr (MODE == kFwd || MODE == kBwd) {
-      const int64_t p = n_b + r;
-      const int64_t c = p >= 0 && p < L ? column(ids[p * A.ids_stride_s]) : -1;
-      if (c >= 0 && c < kSlice && (int)(c / (kG * kWave * NV)) == wave) {
-        const int in = (int)(c / kG) - wave * NV * kWave;
-        tu = in / 64;
-        tlane = in & 63;
-        te = (int)(c % kG);
-      }
-    }
-    float none[kG];
-    if constexpr (MODE == kFwd) {
-      float m = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        const uint32_t sp = (bits[u / 4] >> (8 * (u % 4))) & 0xffu;
-        if (__ballot(sp != 0)) special<false>(v[u], none, sp, s_word + (g0 + u * kWave) * kG, S);
-        if (__ballot(allowed[u] != 0xffu)) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) v[u][e] = (allowed[u] >> e) & 1u ? v[u][e] : -INFINITY;
-        }
-        if (u == tu && lane == tlane) {
-          float t = 0.f;
-#pragma unroll
-          for (int e = 0; e < kG; ++e) t = e == te ? v[u][e] : t;
-          P.xt[b * P.R + r] = t;
-        }
-#pragma unroll
-        for (int e = 0; e < kG; ++e) m = fmaxf(m, v[u][e]);
-      }
-      // the lane's sum, then the wave's: sums of 2^(y c - fl(m c)) with c = log2(e) / T
-      const float c = kLog2e * S.inv_t;
-      const float M = wave_max(m);
-      const float off = M * c;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool in_range = fabsf(off) < INFINITY;
-      if (in_range) {
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-          for (int e = 0; e < kG; ++e) s4[e & 3] += fast_exp2(fmaf(v[u][e], c, -off));
-      } else if (M != -INFINITY) {  // a row of nothing but the type's lowest values, or of an infinity
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-          for (int e = 0; e < kG; ++e) s4[e & 3] += fast_exp2((v[u][e] - M) * c);
-      } else {  // -inf, and NaN, which a maximum does not show
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-          for (int e = 0; e < kG; ++e) s4[e & 3] = v[u][e] != v[u][e] ? v[u][e] : s4[e & 3];
-      }
-      float s = wave_sum((s4[0] + s4[1]) + (s4[2] + s4[3]));
-      if (in_range) s *= fast_exp2(-fmaf(M, c, -off));  // the offset's rounding undone
-      if (lane == 0) {
-        float* dst = P.part + ((b * P.R + r) * (P.slices * kWaves) + slice * kWaves + wave) * 2;
-        dst[0] = M;
-        dst[1] = s;
-      }
-    } else if constexpr (MODE == kBwd) {
-      const float* st = P.stats + (b * P.R + r) * 2;
-      const float M = st[0], c = kLog2e * S.inv_t, ls = st[1] * kLog2e, gt = g_now * S.inv_t;
-#pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        if (column_of(u) >= V) continue;
-        const uint32_t sp = (bits[u / 4] >> (8 * (u % 4))) & 0xffu;
-        float slope[kG];
-        const bool any = __ballot(sp != 0) != 0;
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) slope[e] = 1.f;
-          special<true>(v[u], slope, sp, s_word + (g0 + u * kWave) * kG, S);
-        }
-        const bool masked = __ballot(allowed[u] != 0xffu) != 0;
-        float o[kG];
-#pragma unroll
-        for (int e = 0; e < kG; ++e) o[e] = -fast_exp2(fmaf(v[u][e] - M, c, -ls)) * gt;
-        if (u == tu && lane == tlane) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) o[e] = e == te ? (1.f - fast_exp2(fmaf(v[u][e] - M, c, -ls))) * gt : o[e];
-        }
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) o[e] *= slope[e];
-        }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) o[e] = (allowed[u] >> e) & 1u ? o[e] : 0.f;
-        }
-        store_group<E>(yr, column_of(u), V, o);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        const int64_t c = column_of(u);
-        if (c >= V) continue;
-        const uint32_t sp = (bits[u / 4] >> (8 * (u % 4))) & 0xffu;
-        if constexpr (MODE == kInPlace) {
-          if (!dense && sp == 0 && allowed[u] == 0xffu) continue;
-          if (c + kG <= V) {
-            vu4 w[kP<E>];
-            load_pieces<E>(xb + r * P.xsr + c, w);
-            unpack_group<E>(w, v[u]);
-          } else {
-            load_tail<E>(xb + r * P.xsr, c, V, 0.f, v[u]);
-          }
-        }
-        float slope[kG];
-        if constexpr (MODE == kApplyGrad) {
-#pragma unroll
-          for (int e = 0; e < kG; ++e) slope[e] = S.inv_t;
-          if (sp != 0) {
-            float xv[kG];
-            if (c + kG <= V) {
-              vu4 w[kP<E>];
-              load_pieces<E>(xb + r * P.xsr + c, w);
-              unpack_group<E>(w, xv);
-            } else {
-              load_tail<E>(xb + r * P.xsr, c, V, 0.f, xv);
+          for (int u = 0; u < NV; ++u)
+            if ((int)(group / kWave) == u) {
+              any[u / 4] |= bit << (8 * (u % 4));
+              if ((int)(group % kWave) == lane) bits[u / 4] |= bit << (8 * (u % 4));
             }
-            special<true>(xv, slope, sp, s_word + (g0 + u * kWave) * kG, S);
+        }
+      }
+      const bool more = i + 1 < n_rows;
+      const raw* next = MODE == kApplyGrad ? dyr + P.gsr : xr + P.xsr;
+      float g_now = 0.f, M_now = 0.f, ls_now = 0.f;
+      bool read_next = more;
+      if constexpr (MODE == kBwd) {
+        g_now = of_row(m_g, i);
+        M_now = of_row(m_M, i);
+        ls_now = of_row(m_ls, i);
+        read_next = more && of_row(m_g, more ? i + 1 : i) != 0.f;
+      }
+      // the next token's group of the lane, and which of its eight
+      int tu = -1, tlane = -1, te = -1;
+      if constexpr (MODE == kFwd || MODE == kBwd) {
+        const int t = __builtin_amdgcn_readlane(m_next, i);
+        if (t >= 0) {
+          tu = t / (kG * kWave);
+          tlane = t / kG % kWave;
+          te = t % kG;
+        }
+      }
+      const int m = __builtin_amdgcn_readlane(m_mask, i);
+      uint32_t allowed[NV];
+#pragma unroll
+      for (int u = 0; u < NV; ++u) allowed[u] = 0xffu;
+      if (m >= 0) {
+        const uint8_t* mask = reinterpret_cast<const uint8_t*>(A.masks + (int64_t)m * A.mask_stride) + n0 / kG;
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+          if (WHOLE || (uint32_t)(g0 + u * kWave) * kG < left) allowed[u] = mask[(uint32_t)(g0 + u * kWave)];
+      }
+      auto wave_bits = [&](int u) { return (any[u / 4] >> (8 * (u % 4))) & 0xffu; };
+      auto lane_bits = [&](int u) { return (bits[u / 4] >> (8 * (u % 4))) & 0xffu; };
+      // group u of this row, and the next row's on its way
+      auto take = [&](int u, float fill, float (&v)[kG]) {
+        if (full(u))
+          unpack_group<E>(q[u], v);
+        else
+          tail(MODE == kApplyGrad ? dyr : xr, u, fill, v);
+        if (read_next) issue(next, u);
+      };
+      if constexpr (MODE == kFwd) {
+        float v[NV][kG], none[kG];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          take(u, -INFINITY, v[u]);
+          if (wave_bits(u) != 0) special<false>(v[u], none, wave_bits(u), lane_bits(u), words + u * kU, S);
+          if (m >= 0) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e) v[u][e] = (allowed[u] >> e) & 1u ? v[u][e] : -INFINITY;
+          }
+          if (u == tu) {
+            float t = v[u][0];
+#pragma unroll
+            for (int e = 1; e < kG; ++e) t = e == te ? v[u][e] : t;
+            if (lane == tlane) P.xt[b * P.R + r0 + i] = t;
           }
 #pragma unroll
-          for (int e = 0; e < kG; ++e) v[u][e] = (allowed[u] >> e) & 1u ? v[u][e] * slope[e] : 0.f;
-        } else {
-          if (__ballot(sp != 0)) special<false>(v[u], slope, sp, s_word + (g0 + u * kWave) * kG, S);
-#pragma unroll
-          for (int e = 0; e < kG; ++e) v[u][e] = (allowed[u] >> e) & 1u ? v[u][e] * S.inv_t : -INFINITY;
+          for (int e = 0; e < kG; ++e) mx = fmaxf(mx, v[u][e]);
         }
-        store_group<E>(yr, c, V, v[u]);
+        // sums of 2^(y c - fl(M c)) with c = log2(e) / T, M the wave's maximum
+        const float c = kLog2e * S.inv_t;
+        const float M = wave_fold(mx, -INFINITY, [](float x, float y) { return fmaxf(x, y); });
+        const float off = M * c;
+        const bool in_range = fabsf(off) < INFINITY;
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+        if (in_range) {
+#pragma unroll
+          for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < kG; ++e) s4[e & 3] += fast_exp2(fmaf(v[u][e], c, -off));
+        } else if (M != -INFINITY) {  // a row of nothing but the type's lowest values, or of an infinity
+#pragma unroll
+          for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < kG; ++e) s4[e & 3] += fast_exp2((v[u][e] - M) * c);
+        } else {  // -inf, and NaN, which a maximum does not show
+#pragma unroll
+          for (int u = 0; u < NV; ++u)
+#pragma unroll
+            for (int e = 0; e < kG; ++e) s4[e & 3] = v[u][e] != v[u][e] ? v[u][e] : s4[e & 3];
+        }
+        float s = wave_fold((s4[0] + s4[1]) + (s4[2] + s4[3]), 0.f, [](float x, float y) { return x + y; });
+        if (in_range) s *= fast_exp2(-fmaf(M, c, -off));  // the offset's rounding undone
+        if (lane == 0)
+          reinterpret_cast<float2*>(P.part)[(b * P.R + r0 + i) * (P.slices * kWaves) + slice * kWaves + wave] = float2{M, s};
+      } else if constexpr (MODE == kBwd) {
+        if (g_now == 0.f) {
+          const float z[kG] = {};
+#pragma unroll
+          for (int u = 0; u < NV; ++u) {
+            put(u, z);
+            if (read_next) issue(next, u);
+          }
+        } else {
+          const float c = kLog2e * S.inv_t, ls = ls_now * kLog2e, gt = g_now * S.inv_t;
+#pragma unroll
+          for (int u = 0; u < NV; ++u) {
+            float v[kG], o[kG], slope[kG];
+            take(u, 0.f, v);
+#pragma unroll
+            for (int e = 0; e < kG; ++e) slope[e] = 1.f;
+            if (wave_bits(u) != 0) special<true>(v, slope, wave_bits(u), lane_bits(u), words + u * kU, S);
+#pragma unroll
+            for (int e = 0; e < kG; ++e) o[e] = fast_exp2(fmaf(v[e] - M_now, c, -ls)) * -gt;
+            if (u == tu) {
+#pragma unroll
+              for (int e = 0; e < kG; ++e)
+                o[e] = lane == tlane && e == te ? (1.f - fast_exp2(fmaf(v[e] - M_now, c, -ls))) * gt : o[e];
+            }
+            if (wave_bits(u) != 0) {
+#pragma unroll
+              for (int e = 0; e < kG; ++e) o[e] *= slope[e];
+            }
+            if (m >= 0) {
+#pragma unroll
+              for (int e = 0; e < kG; ++e) o[e] = (allowed[u] >> e) & 1u ? o[e] : 0.f;
+            }
+            put(u, o);
+          }
+        }
+      } else if constexpr (MODE == kApply) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          float v[kG], none[kG];
+          take(u, 0.f, v);
+          if (wave_bits(u) != 0) special<false>(v, none, wave_bits(u), lane_bits(u), words + u * kU, S);
+#pragma unroll
+          for (int e = 0; e < kG; ++e) v[e] *= S.inv_t;
+          if (m >= 0) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] : -INFINITY;
+          }
+          put(u, v);
+        }
+      } else {
+        // these read the logits of some groups only
+        auto logits_of = [&](int u, float (&v)[kG]) {
+          if (full(u)) {
+            vu4 w[kP<E>];
+            load_group<E>(xr, at(u), w);
+            unpack_group<E>(w, v);
+          } else {
+            tail(xr, u, 0.f, v);
+          }
+        };
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          float v[kG], slope[kG];
+          if constexpr (MODE == kInPlace) {
+            const bool mine = dense || lane_bits(u) != 0 || allowed[u] != 0xffu;
+            if (mine) {
+              logits_of(u, v);
+              special<false>(v, slope, 0xffu, lane_bits(u), words + u * kU, S);
+#pragma unroll
+              for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] * S.inv_t : -INFINITY;
+              put(u, v);
+            }
+          } else {
+            take(u, 0.f, v);
+#pragma unroll
+            for (int e = 0; e < kG; ++e) slope[e] = S.inv_t;
+            if (wave_bits(u) != 0 && lane_bits(u) != 0) {
+              float x[kG];
+              logits_of(u, x);
+              special<true>(x, slope, wave_bits(u), lane_bits(u), words + u * kU, S);
+            }
+#pragma unroll
+            for (int e = 0; e < kG; ++e) v[e] *= slope[e];
+            if (m >= 0) {
+#pragma unroll
+              for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] : 0.f;
+            }
+            put(u, v);
+          }
+        }
       }
+      read = read_next;
+      xr += P.xsr;
+      if (MODE == kApplyGrad) dyr += P.gsr;
+      if (MODE != kFwd) yr += P.ysr;
     }
-  }
+  };
+  if (left == kSlice)
+    rows(std::true_type{});
+  else
+    rows(std::false_type{});
 }
 
 // Per row, one wave: the slices' partials joined, the next token's logprob.
