@@ -994,7 +994,7 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
  * (bias_stride_b apart; 0: the same for all); of two entries of one id the later holds.  masks
  * holds n_masks rows of at least ceil(V / 32) words, mask_stride words apart, token v being
  * bit v % 32 of word v / 32 (1: allowed); mask_rows[b, r] names a row's mask, numbers
- * outside [0, n_masks) none (n_masks 0: no masks, mask_rows not read).
+ * outside [0, n_masks) none (n_masks 0: no masks, mask_rows not read).  V is at most 2^24.
  */
 typedef struct mirl_logit_processors {
   const int64_t* ids;
@@ -1017,6 +1017,15 @@ typedef struct mirl_logit_processors {
 } mirl_logit_processors;
 
 /*
+ * The samples' tokens and biases sorted by column, for calls with R rows of V columns and the
+ * same `processors` (a backward takes its forward's): table holds
+ * mirl_logit_processors_table_elems(B, V, n_ids, n_bias) words.
+ */
+int64_t mirl_logit_processors_table_elems(int64_t B, int64_t V, int64_t n_ids, int64_t n_bias);
+int mirl_logit_processors_table(const mirl_logit_processors* processors, int64_t B, int64_t R,
+                                int64_t V, uint32_t* table, void* stream);
+
+/*
  * out[b, r] ([B, R] contiguous) = log_softmax(y[b, r]) at the token behind row r, ids[b, n]:
  * 0 without one (n >= n_ids, or an id outside the columns), -inf in a row that allows
  * nothing or not that token.  y is never written.  stats ([B, R, 2], or NULL) is
@@ -1025,7 +1034,8 @@ typedef struct mirl_logit_processors {
 int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V);
 int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                                int64_t stride_b, int64_t stride_r,
-                               const mirl_logit_processors* processors, float* out,
+                               const mirl_logit_processors* processors,
+                               const uint32_t* table, float* out,
                                float* stats, float* workspace, void* stream);
 
 /*
@@ -1035,7 +1045,8 @@ int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t
  */
 int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t Rt,
                                int64_t V, int64_t stride_b, int64_t stride_r,
-                               const mirl_logit_processors* processors, const float* stats,
+                               const mirl_logit_processors* processors,
+                               const uint32_t* table, const float* stats,
                                const float* grad_out, int64_t g_stride_b, int64_t g_stride_r,
                                void* grad_in, int64_t gi_stride_b, int64_t gi_stride_r,
                                void* stream);
@@ -1048,11 +1059,13 @@ int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t
  */
 int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                         int64_t stride_b, int64_t stride_r,
-                        const mirl_logit_processors* processors, void* out,
+                        const mirl_logit_processors* processors,
+                               const uint32_t* table, void* out,
                         int64_t o_stride_b, int64_t o_stride_r, void* stream);
 int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                             int64_t stride_b, int64_t stride_r,
-                            const mirl_logit_processors* processors, const void* grad_out,
+                            const mirl_logit_processors* processors,
+                               const uint32_t* table, const void* grad_out,
                             int64_t g_stride_b, int64_t g_stride_r, void* grad_in,
                             int64_t gi_stride_b, int64_t gi_stride_r, void* stream);
 

@@ -331,12 +331,14 @@ SIGNATURES = {
          _P, _I64, _P, ctypes.c_double, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P],
     ),
     "mirl_processed_logprob_workspace_elems": (_I64, [_I64, _I64, _I64]),
-    "mirl_processed_logprob_fwd": (_I, [_P, _I] + [_I64] * 5 + [_P] * 5),
+    "mirl_logit_processors_table_elems": (_I64, [_I64] * 4),
+    "mirl_logit_processors_table": (_I, [_P, _I64, _I64, _I64, _P, _P]),
+    "mirl_processed_logprob_fwd": (_I, [_P, _I] + [_I64] * 5 + [_P] * 6),
     "mirl_processed_logprob_bwd": (
-        _I, [_P, _I] + [_I64] * 6 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
-    "mirl_process_logits": (_I, [_P, _I] + [_I64] * 5 + [_P] * 2 + [_I64] * 2 + [_P]),
+        _I, [_P, _I] + [_I64] * 6 + [_P] * 4 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
+    "mirl_process_logits": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P]),
     "mirl_process_logits_bwd": (
-        _I, [_P, _I] + [_I64] * 5 + [_P] * 2 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
+        _I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
@@ -1272,7 +1274,18 @@ def processor_args(ids: torch.Tensor, tensors: dict, scalars: dict, vocab: tuple
     return A
 
 
-def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs, want_stats: bool):
+def processor_table(logits: torch.Tensor, R: int, args: LogitProcessorArgs) -> torch.Tensor:
+    """The samples' tokens and biases by column, for the calls below (see mirl_logit_processors_table)."""
+    dev = logits.device
+    B, V = logits.shape[0], logits.shape[2]
+    lib = _lib if _lib is not None else load()
+    table = torch.empty(max(1, lib.mirl_logit_processors_table_elems(B, V, args.n_ids, args.n_bias)), dtype=torch.int32, device=dev)
+    st = _launch("mirl_logit_processors_table", dev, ctypes.byref(args), B, R, V, table.data_ptr(), _stream(dev))
+    _check(st, "mirl_logit_processors_table")
+    return table
+
+
+def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs, table: torch.Tensor, want_stats: bool):
     """(logprobs [B, R] fp32, stats [B, R, 2] or None) of the first R rows (see mirl_processed_logprob_fwd)."""
     dev = logits.device
     B, _, V = logits.shape
@@ -1281,12 +1294,12 @@ def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs
     lib = _lib if _lib is not None else load()
     ws = torch.empty(max(1, lib.mirl_processed_logprob_workspace_elems(B, R, V)), dtype=torch.float32, device=dev)
     st = _launch("mirl_processed_logprob_fwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), out.data_ptr(), _ptr(stats), ws.data_ptr(), _stream(dev))
+                 logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), _ptr(stats), ws.data_ptr(), _stream(dev))
     _check(st, "mirl_processed_logprob_fwd")
     return out, stats
 
 
-def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, stats: torch.Tensor,
+def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, stats: torch.Tensor,
                           grad_out: torch.Tensor) -> torch.Tensor:
     """The gradient of the logits, a new contiguous tensor (see mirl_processed_logprob_bwd)."""
     dev = _require_gpu(logits, stats, grad_out)
@@ -1295,24 +1308,24 @@ def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, stats:
     _require(grad_out.dtype == torch.float32 and tuple(grad_out.shape) == (B, R), "an fp32 gradient [B, R]")
     grad = torch.empty((B, Rt, V), dtype=logits.dtype, device=dev)
     st = _launch("mirl_processed_logprob_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, Rt, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), stats.data_ptr(), grad_out.data_ptr(), grad_out.stride(0),
+                 logits.stride(1), ctypes.byref(args), table.data_ptr(), stats.data_ptr(), grad_out.data_ptr(), grad_out.stride(0),
                  grad_out.stride(1), grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
     _check(st, "mirl_processed_logprob_bwd")
     return grad
 
 
-def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool) -> torch.Tensor:
+def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, inplace: bool) -> torch.Tensor:
     """Processed logits, in place or as a new contiguous tensor (see mirl_process_logits)."""
     dev = logits.device
     B, R, V = logits.shape
     out = logits if inplace else torch.empty((B, R, V), dtype=logits.dtype, device=dev)
     st = _launch("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
+                 logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
     _check(st, "mirl_process_logits")
     return out
 
 
-def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, grad_out: torch.Tensor) -> torch.Tensor:
+def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, grad_out: torch.Tensor) -> torch.Tensor:
     """The gradient of the logits, a new contiguous tensor (see mirl_process_logits_bwd)."""
     dev = _require_gpu(logits, grad_out)
     B, R, V = logits.shape
@@ -1321,7 +1334,7 @@ def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, grad_out:
         grad_out = grad_out.contiguous()
     grad = torch.empty((B, R, V), dtype=logits.dtype, device=dev)
     st = _launch("mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
+                 logits.stride(1), ctypes.byref(args), table.data_ptr(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
                  grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
     _check(st, "mirl_process_logits_bwd")
     return grad

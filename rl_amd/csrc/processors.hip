@@ -8,15 +8,17 @@
 //   logprob_t = (y_t - M) - log(sum_j exp(y_j - M)),   dx_j = slope_j (onehot_j - p_j) g
 // with y never written; slope is what z multiplies x by, over T, 0 where the grammar forbids j.
 //
-// A workgroup owns a slice of the vocabulary for a run of rows of one sample, and each lane the same
-// groups of eight tokens in all of them: it counts the tokens ahead of its first row with LDS atomics
-// (whole numbers: their order does not matter), and from then on a row's new token concerns the one
-// lane that owns it.  No barrier, sort or table in memory follows the counting, and nothing of size
+// A first launch puts each sample's tokens and biases into buckets by 2048 columns (processors_table_kernel).
+// A workgroup then owns a slice of the vocabulary, one or more buckets, for a run of rows of one sample,
+// and each lane the same groups of eight tokens in all of them: it counts the bucket's tokens ahead of its
+// first row with LDS atomics (whole numbers: their order does not matter), and from then on a row's
+// new token concerns the one lane that owns it.  No barrier follows the counting, and nothing of size
 // [rows, V] is held.  A word per token holds its count, whether it occurred and its bias; a bit per
 // token in the lane's registers says whether the word is anything but 0, so that ordinary tokens
 // cost one test for a group of eight.
 
 #include "common.h"
+#include <cstdlib>
 
 #pragma clang fp contract(off)
 
@@ -32,6 +34,17 @@ constexpr uint32_t kCountBits = 20, kInPrompt = 1u << kCountBits, kCount = kInPr
 constexpr int kBiasShift = kCountBits + 1;
 constexpr int64_t kMaxTokens = kCount, kMaxBias = (int64_t(1) << (32 - kBiasShift)) - 1;
 
+// The table of a call: per sample what holds for all its rows (kHead words) and where each bucket begins
+// (buckets + 1 numbers), then all samples' entries: a token's column in its bucket and its place, or
+// with the top bit a bias's column and number.
+constexpr int kHead = 8;
+constexpr int kBucketBits = 11, kBucket = 1 << kBucketBits;
+constexpr uint32_t kIsBias = 1u << 31;
+constexpr int64_t kMaxBuckets = 8192;
+constexpr int kTableThreads = 1024;
+static_assert(kBucket == kThreads * kG, "a slice is a whole number of buckets");
+static_assert(kCountBits + kBucketBits <= 31, "an entry holds a token's place and column");
+
 enum Mode { kFwd, kBwd, kApply, kInPlace, kApplyGrad };
 
 struct Params {
@@ -40,7 +53,8 @@ struct Params {
   int64_t xsb, xsr;
   int64_t B, R, Rt, V;   // rows with a result; rows of the gradient (those past R: zeros)
   int64_t n_vocab;       // ids vs .. vs + n_vocab - 1 stand for the columns
-  int64_t slices, chunks;
+  int64_t slices, chunks, buckets;
+  const uint32_t* table;
   int rows;              // rows of a workgroup
   void* y;               // processed logits, or a gradient
   int64_t ysb, ysr;
@@ -105,42 +119,161 @@ __device__ __forceinline__ float wave_fold(float v, float none, F&& f) {
 }
 __device__ __forceinline__ float of_row(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
 
-// What holds for all rows of a sample.
+// What holds for all rows of a sample, as the table's first words hold it.
 struct Sample {
   float rp, inv_rp, pres, freq, inv_t;
-  const float* bias;
+  int n;       // tokens that row 0 follows
+  int prompt;  // tokens of the prompt
+  int unused;
 };
+static_assert(sizeof(Sample) == kHead * 4, "the table's head");
+__device__ __forceinline__ const uint32_t* head_of(const Params& P, int64_t b) { return P.table + b * (kHead + P.buckets + 1); }
+
+// v where bit e of `keep` is set, else `other`; as bits, whatever v holds.
+__device__ __forceinline__ float keep_if(float v, uint32_t keep, int e, float other) {
+  const uint32_t t = (uint32_t)__builtin_amdgcn_sbfe((int)keep, e, 1);
+  return __uint_as_float((__float_as_uint(v) & t) | (__float_as_uint(other) & ~t));
+}
+
+// Bias and penalties of one logit under its word.
+__device__ __forceinline__ float penalized(float z, uint32_t w, const Sample& S, uint32_t& how) {
+  how = 0;
+  if (w & (kInPrompt | kCount)) {
+    how = z > 0.f ? 1u : 256u;
+    z *= z > 0.f ? S.inv_rp : S.rp;
+  }
+  const uint32_t n = w & kCount;
+  z -= S.freq * (float)n;
+  z -= n != 0 ? S.pres : 0.f;
+  return z;
+}
 
 // Bias and penalties of a group's tokens: those of any lane of the wave (`any`, a scalar), in the
-// lanes that have them (`bits`); with SLOPE what each x was multiplied by.
-template <bool SLOPE>
-__device__ __forceinline__ void special(float (&v)[kG], float (&slope)[kG], uint32_t any, uint32_t bits, const vu4* words,
-                                        const Sample& S) {
+// lanes that have them (`bits`).  Returns which were divided by the repetition penalty (bits 0 .. 7) and
+// which multiplied (8 .. 15).
+template <class F>
+__device__ __forceinline__ uint32_t special(float (&v)[kG], uint32_t any, uint32_t bits, const vu4* words, F&& bias_of,
+                                            const Sample& S) {
+  uint32_t how = 0;
 #pragma unroll
   for (int e = 0; e < kG; ++e) {
     if ((any & (1u << e)) == 0) continue;
     if ((bits >> e) & 1u) {
       const uint32_t w = words[e / 4][e % 4];
-      float z = v[e];
-      if (w >> kBiasShift) z += S.bias[(w >> kBiasShift) - 1];
-      if (w & (kInPrompt | kCount)) {
-        const float f = z > 0.f ? S.inv_rp : S.rp;
-        z *= f;
-        if constexpr (SLOPE) slope[e] *= f;
-      }
-      const uint32_t n = w & kCount;
-      z -= S.freq * (float)n;
-      z -= n != 0 ? S.pres : 0.f;
-      v[e] = z;
+      uint32_t h;
+      v[e] = penalized(w >> kBiasShift ? v[e] + bias_of(w, e) : v[e], w, S, h);
+      how |= h << e;
     }
+  }
+  return how;
+}
+// What the repetition penalty makes of a gradient.
+__device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t how, const Sample& S) {
+#pragma unroll
+  for (int e = 0; e < kG; ++e) {
+    if ((any & (1u << e)) == 0) continue;
+    o[e] *= (how >> e) & 1u ? S.inv_rp : (how >> e) & 256u ? S.rp : 1.f;
   }
 }
 
-template <class E, int MODE, int NV>
+// Buckets of one sample's tokens (those that any of the R rows follows) and biases.  An entry's place
+// in its bucket comes from an atomic: the order differs from run to run, what is counted does not.
+__global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t B, int64_t R,
+                                                                         int64_t n_vocab, int buckets, uint32_t* table) {
+  __shared__ uint32_t s_at[kMaxBuckets];
+  __shared__ int s_bias[kMaxBias];
+  __shared__ uint32_t s_wave[kTableThreads / kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t b = blockIdx.x;
+  const int64_t* ids = A.ids + b * A.ids_stride_b;
+  const int64_t* bias_ids = A.bias_ids + b * A.bias_stride_b;
+  const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1;
+  const int n = (int)min(max(n_b + R - 1, int64_t(0)), A.n_ids), n_bias = (int)A.n_bias;
+  uint32_t* const head = table + b * (kHead + buckets + 1);
+  uint32_t* const begins = head + kHead;
+  uint32_t* const entries = table + B * (kHead + buckets + 1) + b * (A.n_ids + A.n_bias);
+  if (tid == 0) {
+    Sample S;
+    S.rp = A.repetition != nullptr ? A.repetition[b] : A.repetition_all;
+    S.inv_rp = 1.f / S.rp;
+    S.pres = A.presence != nullptr ? A.presence[b] : A.presence_all;
+    S.freq = A.frequency != nullptr ? A.frequency[b] : A.frequency_all;
+    S.inv_t = 1.f / (A.temperature != nullptr ? A.temperature[b] : A.temperature_all);
+    S.n = (int)min(max(n_b, -(int64_t(1) << 30)), A.n_ids);
+    S.prompt = A.prompt_lengths != nullptr ? (int)min(max(A.prompt_lengths[b], int64_t(0)), A.n_ids) : 0;
+    S.unused = 0;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&S);
+    for (int k = 0; k < kHead; ++k) head[k] = w[k];
+  }
+  auto column = [&](int64_t id) {
+    const uint64_t c = (uint64_t)id - (uint64_t)A.vocab_start;
+    return c < (uint64_t)n_vocab ? (int)c : -1;
+  };
+  for (int k = tid; k < buckets; k += kTableThreads) s_at[k] = 0;
+  for (int k = tid; k < n_bias; k += kTableThreads) s_bias[k] = column(bias_ids[k]);
+  __syncthreads();
+#pragma unroll 4
+  for (int p = tid; p < n; p += kTableThreads) {
+    const int c = column(ids[p * A.ids_stride_s]);
+    if (c >= 0) atomicAdd(&s_at[c >> kBucketBits], 1u);
+  }
+  // a bias holds if no later one of its sample names the same token
+  int own[(kMaxBias + kTableThreads - 1) / kTableThreads];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+    const int k = i * kTableThreads + tid;
+    own[i] = k < n_bias ? s_bias[k] : -1;
+    for (int j = k + 1; j < n_bias; ++j) own[i] = s_bias[j] == own[i] ? -1 : own[i];
+    if (own[i] >= 0) atomicAdd(&s_at[own[i] >> kBucketBits], 1u);
+  }
+  __syncthreads();
+  // the sizes' running sum: a few buckets a thread, the threads' sums over waves and the workgroup
+  const int per = (buckets + kTableThreads - 1) / kTableThreads, k0 = min(tid * per, buckets), k1 = min(k0 + per, buckets);
+  uint32_t mine = 0;
+  for (int k = k0; k < k1; ++k) mine += s_at[k];
+  uint32_t upto = mine;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)upto, off, kWave);
+    upto += lane >= off ? o : 0;
+  }
+  if (lane == kWave - 1) s_wave[wave] = upto;
+  __syncthreads();
+  uint32_t at = upto - mine;
+  for (int w = 0; w < wave; ++w) at += s_wave[w];
+  for (int k = k0; k < k1; ++k) {
+    const uint32_t size = s_at[k];
+    s_at[k] = at;
+    begins[k] = at;
+    at += size;
+  }
+  if (tid == kTableThreads - 1) begins[buckets] = at;
+  __syncthreads();
+#pragma unroll 4
+  for (int p = tid; p < n; p += kTableThreads) {
+    const int c = column(ids[p * A.ids_stride_s]);
+    if (c >= 0) entries[atomicAdd(&s_at[c >> kBucketBits], 1u)] = (uint32_t)p << kBucketBits | (uint32_t)(c & (kBucket - 1));
+  }
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+    if (own[i] >= 0)
+      entries[atomicAdd(&s_at[own[i] >> kBucketBits], 1u)] =
+          kIsBias | (uint32_t)(i * kTableThreads + tid) << kBucketBits | (uint32_t)(own[i] & (kBucket - 1));
+  }
+}
+
+// MASKED: there are grammar masks.
+template <class E, int MODE, int NV, bool MASKED>
 __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   using raw = typename E::raw;
   constexpr int kWaveCols = kWave * NV * kG, kSlice = kWaves * kWaveCols;
+  constexpr int kPacks = (NV + 3) / 4;  // four groups' bytes in a word
   __shared__ __align__(16) uint32_t s_word[kSlice];
+  // kFwd: up to 64 of a wave's tokens with a word are held by a lane each
+  constexpr bool kLists = MODE == kFwd;
+  __shared__ uint16_t s_list[kLists ? kWaves : 1][kWave];
+  // the other modes: biases by column (a gather in the middle of a row would wait for the next row's loads)
+  __shared__ float s_bias[kLists ? 1 : kSlice];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slices = (uint32_t)P.slices, chunks = (uint32_t)P.chunks;
@@ -150,212 +283,316 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   const int64_t r0 = (int64_t)chunk * P.rows;
   const int n_rows = (int)min((int64_t)P.rows, P.Rt - r0);
   const mirl_logit_processors& A = P.A;
-  const int64_t L = A.n_ids;
-  const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1;
-  const int64_t prompt = A.prompt_lengths != nullptr ? A.prompt_lengths[b] : 0;
+  const uint32_t* head = head_of(P, b);
+  const Sample S = *reinterpret_cast<const Sample*>(head);
   const int64_t* ids = A.ids + b * A.ids_stride_b;
+  const float* bias = A.bias + b * A.bias_stride_b;
 
-  Sample S;
-  S.rp = A.repetition != nullptr ? A.repetition[b] : A.repetition_all;
-  S.inv_rp = 1.f / S.rp;
-  S.pres = A.presence != nullptr ? A.presence[b] : A.presence_all;
-  S.freq = A.frequency != nullptr ? A.frequency[b] : A.frequency_all;
-  S.inv_t = 1.f / (A.temperature != nullptr ? A.temperature[b] : A.temperature_all);
-  S.bias = A.bias + b * A.bias_stride_b;
-
-  // ---- the tokens ahead of row r0 ----
-#pragma unroll
-  for (int i = 0; i < kSlice / 4 / kThreads; ++i)
-    reinterpret_cast<vu4*>(s_word)[i * kThreads + tid] = vu4{0u, 0u, 0u, 0u};
-  // an id's column in this slice, or -1
-  const int64_t first_id = A.vocab_start + n0;
-  const uint32_t here = (uint32_t)max(int64_t(0), min((int64_t)kSlice, P.n_vocab - n0));
-  auto column = [&](int64_t id) {
-    const uint64_t c = (uint64_t)id - (uint64_t)first_id;
-    return c < here ? (int)c : -1;
-  };
-  __syncthreads();
-  if (A.n_bias > 0) {  // of two entries of a token the later holds
-    for (int64_t k = tid; k < A.n_bias; k += kThreads) {
-      const int c = column(A.bias_ids[b * A.bias_stride_b + k]);
-      if (c >= 0) atomicMax(&s_word[c], (uint32_t)(k + 1) << kBiasShift);
-    }
-    __syncthreads();
-  }
-  const int ahead = (int)min(max(n_b + r0, int64_t(0)), L);
-  const int in_prompt = (int)min(max(prompt, int64_t(0)), L);
-#pragma unroll 4
-  for (int p = tid; p < ahead; p += kThreads) {
-    const int c = column(ids[p * A.ids_stride_s]);
-    if (c >= 0) {
-      if (p < in_prompt)
-        atomicOr(&s_word[c], kInPrompt);
-      else
-        atomicAdd(&s_word[c], 1u);
-    }
-  }
-  // What the rows need, row r0 + l in lane l: the token that is new ahead of it and the one behind it
-  // (columns of this wave, or -1), its mask, its gradient and statistics.
-  int m_new = -1, m_next = -1, m_mask = -1;
-  float m_g = 0.f, m_M = 0.f, m_ls = 0.f;
-  if (lane < n_rows) {
-    const int64_t r = r0 + lane, at = n_b + r;
-    auto of_wave = [&](int c) { return c >= 0 && c / kWaveCols == wave ? c - wave * kWaveCols : -1; };
-    if (lane > 0 && at > 0 && at <= L) {
-      m_new = of_wave(column(ids[(at - 1) * A.ids_stride_s]));
-      if (m_new >= 0 && at - 1 < prompt) m_new |= 1 << 30;
-    }
-    if constexpr (MODE == kFwd || MODE == kBwd) {
-      if (at >= 0 && at < L) m_next = of_wave(column(ids[at * A.ids_stride_s]));
-    }
-    if (A.n_masks > 0 && (MODE != kBwd || r < P.R)) {
-      const int64_t m = A.mask_rows[b * A.mask_rows_stride_b + r * A.mask_rows_stride_r];
-      m_mask = m >= 0 && m < A.n_masks ? (int)m : -1;
-    }
-    if constexpr (MODE == kBwd) {
-      if (r < P.R) {
-        m_g = P.g[b * P.gsb + r * P.gsr];
-        m_M = P.stats[(b * P.R + r) * 2];
-        m_ls = P.stats[(b * P.R + r) * 2 + 1];
-        if (m_M == -INFINITY && m_ls == -INFINITY) m_g = 0.f;  // nothing was left in the row
-      }
-    }
-  }
-  __syncthreads();
-
-  // ---- from here on each wave by itself ----
   const int g0 = wave * NV * kWave + lane;  // group u of the lane: g0 + 64 u
-  const vu4* words = reinterpret_cast<const vu4*>(s_word) + g0 * (kG / 4);
-  constexpr int kU = kWave * (kG / 4);  // between the lane's groups
-  uint32_t bits[(NV + 3) / 4] = {}, any[(NV + 3) / 4] = {};  // a byte per group: the lane's, the wave's
-#pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    const vu4 lo = words[u * kU], hi = words[u * kU + 1];
-#pragma unroll
-    for (int e = 0; e < kG; ++e) {
-      const bool set = (e < 4 ? lo[e & 3] : hi[e & 3]) != 0;
-      bits[u / 4] |= set ? 1u << (8 * (u % 4) + e) : 0u;
-      any[u / 4] |= __ballot(set) != 0 ? 1u << (8 * (u % 4) + e) : 0u;
-    }
-  }
   const raw* xr = static_cast<const raw*>(P.x) + b * P.xsb + r0 * P.xsr + n0;
   const raw* dyr = MODE == kApplyGrad ? static_cast<const raw*>(P.dy) + b * P.gsb + r0 * P.gsr + n0 : nullptr;
   raw* yr = MODE == kFwd ? nullptr : static_cast<raw*>(P.y) + b * P.ysb + r0 * P.ysr + n0;
   const uint32_t left = (uint32_t)min((int64_t)kSlice, P.V - n0);  // columns of the slice
   const uint32_t at0 = g0 * kGroupBytes<E>;
-  const bool dense = S.inv_t != 1.f;  // kInPlace: every value changes
+  auto col = [&](int u) { return (uint32_t)(g0 + u * kWave) * kG; };
+  auto put = [&](raw* row, int u, const float (&v)[kG], bool whole) __attribute__((always_inline)) {
+    if (whole || col(u) + kG <= left) {
+      store_group<E>(row, at0 + u * kWave * kGroupBytes<E>, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kG; ++e)
+        if (col(u) + e < left) row[col(u) + e] = E::from_float(v[e]);
+    }
+  };
 
-  // WHOLE: the slice lies inside the row
-  auto rows = [&](auto whole_c) __attribute__((always_inline)) {
-    constexpr bool WHOLE = decltype(whole_c)::value;
-    constexpr bool kStreams = MODE != kInPlace;  // every group of a row is read
-    auto full = [&](int u) { return WHOLE || (uint32_t)(g0 + u * kWave + 1) * kG <= left; };
-    auto at = [&](int u) { return at0 + u * kWave * kGroupBytes<E>; };
-    auto tail = [&](const raw* row, int u, float fill, float (&v)[kG]) {
+  // What the rows need, row r0 + l in lane l.  kBwd: its gradient and statistics; rows without a gradient
+  // are zeros and not read.
+  uint64_t todo = n_rows == 64 ? ~0ull : (1ull << n_rows) - 1;
+  float m_g = 0.f, m_M = 0.f, m_ls = 0.f;
+  if constexpr (MODE == kBwd) {
+    const int64_t r = r0 + lane;
+    if (lane < n_rows && r < P.R) {
+      m_g = P.g[b * P.gsb + r * P.gsr];
+      m_M = P.stats[(b * P.R + r) * 2];
+      m_ls = P.stats[(b * P.R + r) * 2 + 1];
+      if (m_M == -INFINITY && m_ls == -INFINITY) m_g = 0.f;  // nothing was left in the row
+    }
+    uint64_t zeros = todo;
+    todo = __ballot(m_g != 0.f);
+    zeros &= ~todo;
+    const float z[kG] = {};
+    for (; zeros != 0; zeros &= zeros - 1) {
+      raw* row = yr + __builtin_ctzll(zeros) * P.ysr;
+#pragma unroll
+      for (int u = 0; u < NV; ++u) put(row, u, z, false);
+    }
+    if (todo == 0) return;  // (the same in all waves)
+  }
+  // The first row's values are on their way while the tokens are counted.
+  vu4 q[NV][kP<E>];
+  auto issue = [&](int i, int u, bool whole) __attribute__((always_inline)) {
+    const raw* row = MODE == kApplyGrad ? dyr + i * P.gsr : xr + i * P.xsr;
+    if (whole || col(u) + kG <= left) load_group<E>(row, at0 + u * kWave * kGroupBytes<E>, q[u]);
+  };
+  const int first = __builtin_ctzll(todo);
+  if constexpr (MODE != kInPlace) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) issue(first, u, false);
+  }
+
+  // ---- the tokens ahead of row r0, and the biases ----
+#pragma unroll
+  for (int i = 0; i < kSlice / 4 / kThreads; ++i)
+    reinterpret_cast<vu4*>(s_word)[i * kThreads + tid] = vu4{0u, 0u, 0u, 0u};
+  // an id's column in this wave, or -1
+  const int64_t first_id = A.vocab_start + n0 + wave * kWaveCols;
+  const uint32_t here = (uint32_t)max(int64_t(0), min((int64_t)kWaveCols, P.n_vocab - n0 - wave * kWaveCols));
+  auto column = [&](int64_t id) {
+    const uint64_t c = (uint64_t)id - (uint64_t)first_id;
+    return c < here ? (int)c : -1;
+  };
+  const uint32_t buckets = (uint32_t)P.buckets, bucket0 = slice * NV;
+  const uint32_t* begins = head + kHead;
+  const uint32_t* entries = P.table + P.B * (kHead + buckets + 1) + b * (A.n_ids + A.n_bias);
+  uint32_t begin[NV + 1];
+#pragma unroll
+  for (int u = 0; u <= NV; ++u) begin[u] = begins[min(bucket0 + u, buckets)];
+  const uint32_t ahead = (uint32_t)max(S.n + r0, int64_t(0)), in_prompt = (uint32_t)S.prompt;
+  // The token that is new ahead of a row and the one behind it (columns of this wave, or -1), its mask.
+  constexpr int kOfPrompt = 1 << 30;
+  int m_new = -1, m_next = -1, m_mask = -1;
+  if (lane < n_rows) {
+    const int64_t r = r0 + lane, at = S.n + r;
+    if (lane > 0 && at > 0 && at <= A.n_ids) {
+      m_new = column(ids[(at - 1) * A.ids_stride_s]);
+      if (m_new >= 0 && at - 1 < S.prompt) m_new |= kOfPrompt;
+    }
+    if constexpr (MODE == kFwd || MODE == kBwd) {
+      if (at >= 0 && at < A.n_ids) m_next = column(ids[at * A.ids_stride_s]);
+    }
+    if (MASKED && (MODE != kBwd || r < P.R)) {
+      const int64_t m = A.mask_rows[b * A.mask_rows_stride_b + r * A.mask_rows_stride_r];
+      m_mask = m >= 0 && m < A.n_masks ? (int)m : -1;
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = begin[0] + tid; i < begin[NV]; i += kThreads) {
+    const uint32_t w = entries[i], at = (w & ~kIsBias) >> kBucketBits;
+    uint32_t c = w & (kBucket - 1);
+#pragma unroll
+    for (int u = 1; u < NV; ++u) c += i >= begin[u] ? kBucket : 0;
+    if (w & kIsBias) {
+      atomicAdd(&s_word[c], (at + 1) << kBiasShift);
+      if constexpr (!kLists) s_bias[c] = bias[at];
+    } else if (at < ahead && at < in_prompt) {
+      atomicOr(&s_word[c], kInPrompt);
+    } else if (at < ahead) {
+      atomicAdd(&s_word[c], 1u);
+    }
+  }
+  const uint64_t new_rows = __ballot(m_new >= 0);
+  __syncthreads();
+
+  // ---- from here on each wave by itself ----
+  const vu4* words = reinterpret_cast<const vu4*>(s_word) + g0 * (kG / 4);
+  constexpr int kU = kWave * (kG / 4);  // between the lane's groups
+  auto bias_of = [&](uint32_t w, int u, int e) { return kLists ? bias[(w >> kBiasShift) - 1] : s_bias[kLists ? 0 : col(u) + e]; };
+  // Tokens with a word other than 0: a byte per group of the lane's and of any lane's.
+  uint32_t bits[kPacks] = {}, any[kPacks] = {};
+  // kFwd: the listed tokens (column, word, bias of the lane's), which are formed all at once and left out
+  // of the groups (out: the lane's, out_any: any lane's); the others as in every mode.
+  uint32_t out[kPacks] = {}, out_any[kPacks] = {};
+  int listed = 0, h_col = -1;
+  uint32_t h_word = 0;
+  float h_bias = 0.f;
+  if (begin[NV] != begin[0]) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const vu4 lo = words[u * kU], hi = words[u * kU + 1];
 #pragma unroll
       for (int e = 0; e < kG; ++e) {
-        const uint32_t c = (uint32_t)(g0 + u * kWave) * kG + e;
-        v[e] = c < left ? E::load(row + c) : fill;
-      }
-    };
-    auto put = [&](int u, const float (&v)[kG]) {
-      if (full(u)) {
-        store_group<E>(yr, at(u), v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kG; ++e) {
-          const uint32_t c = (uint32_t)(g0 + u * kWave) * kG + e;
-          if (c < left) yr[c] = E::from_float(v[e]);
+        const bool set = (e < 4 ? lo[e & 3] : hi[e & 3]) != 0;
+        const uint64_t all = __ballot(set);
+        if (all == 0) continue;
+        const uint32_t bit = 1u << (8 * (u % 4) + e);
+        bool in_list = false;
+        if constexpr (kLists) {
+          const int at = listed + (int)__popcll(all & ((1ull << lane) - 1));
+          in_list = set && at < kWave;
+          if (in_list) s_list[wave][at] = (uint16_t)((u * kWave + lane) * kG + e);
+          const int n = (int)__popcll(all);
+          if (listed < kWave) out_any[u / 4] |= bit;
+          if (listed + n > kWave) any[u / 4] |= bit;
+          listed = min(listed + n, kWave);
+        } else {
+          any[u / 4] |= bit;
         }
+        if (set) (in_list ? out : bits)[u / 4] |= bit;
       }
-    };
-    vu4 q[NV][kP<E>];
-    auto issue = [&](const raw* row, int u) {
-      if (full(u)) load_group<E>(row, at(u), q[u]);
-    };
-    bool read = true;  // whether this row's values are on their way
-    if constexpr (MODE == kBwd) read = of_row(m_g, 0) != 0.f;
-    if (kStreams && read) {
-#pragma unroll
-      for (int u = 0; u < NV; ++u) issue(MODE == kApplyGrad ? dyr : xr, u);
     }
-    for (int i = 0; i < n_rows; ++i) {
-      if (i > 0) {  // the token ahead of this row
-        const int t = __builtin_amdgcn_readlane(m_new, i);
-        if (t >= 0) {
-          const uint32_t c = (uint32_t)t & ((1u << 30) - 1), group = c / kG, e = c % kG;
-          const uint32_t bit = 1u << e;
-          if ((int)(group % kWave) == lane) {
-            uint32_t& w = s_word[wave * kWaveCols + c];
-            w = (uint32_t)t >> 30 ? w | kInPrompt : w + 1;
-          }
+    if constexpr (kLists) {
+      __builtin_amdgcn_wave_barrier();
+      if (lane < listed) {
+        h_col = s_list[wave][lane];
+        h_word = s_word[wave * kWaveCols + h_col];
+        if (h_word >> kBiasShift) h_bias = bias[(h_word >> kBiasShift) - 1];
+      }
+    }
+  }
+  // the token that is new ahead of row i
+  auto add_token = [&](int i) __attribute__((always_inline)) {
+    const int t = __builtin_amdgcn_readlane(m_new, i);
+    const int c = t & (kOfPrompt - 1), group = c / kG;
+    const uint32_t bit = 1u << (c % kG);
+    auto more_of = [&](uint32_t w) { return t & kOfPrompt ? w | kInPrompt : w + 1; };
+    const bool mine = group % kWave == lane;
+    bool lists = false;
+    if constexpr (kLists) {
+      const bool held = h_col == c;
+      if (__ballot(held) != 0) {
+        if (held) h_word = more_of(h_word);
+        return;
+      }
+      bool counted = false;  // one that is not listed
 #pragma unroll
-          for (int u = 0; u < NV; ++u)
-            if ((int)(group / kWave) == u) {
-              any[u / 4] |= bit << (8 * (u % 4));
-              if ((int)(group % kWave) == lane) bits[u / 4] |= bit << (8 * (u % 4));
-            }
+      for (int u = 0; u < NV; ++u)
+        if (group / kWave == u) counted = __ballot(mine && ((bits[u / 4] >> (8 * (u % 4))) & bit)) != 0;
+      lists = !counted && listed < kWave;
+      if (lists) {
+        if (lane == listed) {
+          h_col = c;
+          h_word = more_of(0);
         }
+        ++listed;
       }
-      const bool more = i + 1 < n_rows;
-      const raw* next = MODE == kApplyGrad ? dyr + P.gsr : xr + P.xsr;
-      float g_now = 0.f, M_now = 0.f, ls_now = 0.f;
-      bool read_next = more;
-      if constexpr (MODE == kBwd) {
-        g_now = of_row(m_g, i);
-        M_now = of_row(m_M, i);
-        ls_now = of_row(m_ls, i);
-        read_next = more && of_row(m_g, more ? i + 1 : i) != 0.f;
+    }
+    if (mine && !lists) {
+      uint32_t& w = s_word[wave * kWaveCols + c];
+      w = more_of(w);
+    }
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      if (group / kWave != u) continue;
+      const uint32_t b8 = bit << (8 * (u % 4));
+      (lists ? out_any : any)[u / 4] |= b8;
+      if (mine) (lists ? out : bits)[u / 4] |= b8;
+    }
+  };
+  auto add_tokens = [&](int from, int to) __attribute__((always_inline)) {  // ahead of rows from + 1 .. to
+    uint64_t some = new_rows & (~0ull << from << 1) & (~0ull >> (63 - to));
+    for (; some != 0; some &= some - 1) add_token(__builtin_ctzll(some));
+  };
+  add_tokens(0, first);
+  auto wave_bits = [&](int u) { return (any[u / 4] >> (8 * (u % 4))) & 0xffu; };
+  auto lane_bits = [&](int u) { return (bits[u / 4] >> (8 * (u % 4))) & 0xffu; };
+
+  // WHOLE: the slice lies inside the row.  Its loads are then issued in every row alike (a last row's once
+  // more in place of a next one's, lanes that need nothing the slice's first column): the compiler counts
+  // what is in flight, and a row waits for its own values only.
+  auto rows = [&](auto whole_c) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole_c)::value;
+    auto tail = [&](const raw* row, int u, float fill, float (&v)[kG]) {
+#pragma unroll
+      for (int e = 0; e < kG; ++e) v[e] = col(u) + e < left ? E::load(row + col(u) + e) : fill;
+    };
+    auto full = [&](int u) { return WHOLE || col(u) + kG <= left; };
+    // a row's mask bytes; kFwd: its listed tokens' logits and mask bytes; kApplyGrad: the logits of groups with
+    // a word (all as they come: what converts them would wait here)
+    uint8_t mk[NV], h_mk = 0xff;
+    raw h_x = raw();
+    vu4 qx[MODE == kApplyGrad ? NV : 1][kP<E>];
+    auto mask_of = [&](int i) {
+      const int m = __builtin_amdgcn_readlane(m_mask, i);
+      return reinterpret_cast<const uint8_t*>(A.masks + (int64_t)max(m, 0) * A.mask_stride) + n0 / kG;
+    };
+    auto issue_mask = [&](int i, int u) __attribute__((always_inline)) {
+      if constexpr (MASKED) {
+        if (WHOLE || col(u) < left) mk[u] = mask_of(i)[g0 + u * kWave];
       }
+    };
+    auto issue_words = [&](int i) __attribute__((always_inline)) {
+      if constexpr (kLists) {
+        const uint32_t c = h_col < 0 ? 0 : wave * kWaveCols + h_col;
+        h_x = xr[i * P.xsr + c];
+        if (MASKED) h_mk = mask_of(i)[c / kG];
+      }
+      if constexpr (MODE == kApplyGrad) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+          if (full(u)) load_group<E>(xr + i * P.xsr, lane_bits(u) != 0 ? at0 + u * kWave * kGroupBytes<E> : 0, qx[u]);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < NV; ++u) issue_mask(first, u);
+    issue_words(first);
+
+    for (int i = first;;) {
+      todo &= todo - 1;
+      const bool more = todo != 0;
+      const int next = more ? __builtin_ctzll(todo) : i;
+      const bool masked = MASKED && __builtin_amdgcn_readlane(m_mask, i) >= 0;
+      const raw* row = MODE == kApplyGrad ? dyr + i * P.gsr : xr + i * P.xsr;
+      raw* y_row = MODE == kFwd ? nullptr : yr + i * P.ysr;
+      uint32_t allowed[NV];
+      // group u of this row, and the next row's on its way
+      auto take = [&](int u, float fill, float (&v)[kG]) __attribute__((always_inline)) {
+        if (full(u))
+          unpack_group<E>(q[u], v);
+        else
+          tail(row, u, fill, v);
+        allowed[u] = masked ? mk[u] : 0xffu;
+        issue(next, u, WHOLE);
+        issue_mask(next, u);
+      };
       // the next token's group of the lane, and which of its eight
-      int tu = -1, tlane = -1, te = -1;
+      int t = -1, tu = -1, tlane = -1, te = -1;
       if constexpr (MODE == kFwd || MODE == kBwd) {
-        const int t = __builtin_amdgcn_readlane(m_next, i);
+        t = __builtin_amdgcn_readlane(m_next, i);
         if (t >= 0) {
           tu = t / (kG * kWave);
           tlane = t / kG % kWave;
           te = t % kG;
         }
       }
-      const int m = __builtin_amdgcn_readlane(m_mask, i);
-      uint32_t allowed[NV];
-#pragma unroll
-      for (int u = 0; u < NV; ++u) allowed[u] = 0xffu;
-      if (m >= 0) {
-        const uint8_t* mask = reinterpret_cast<const uint8_t*>(A.masks + (int64_t)m * A.mask_stride) + n0 / kG;
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (WHOLE || (uint32_t)(g0 + u * kWave) * kG < left) allowed[u] = mask[(uint32_t)(g0 + u * kWave)];
-      }
-      auto wave_bits = [&](int u) { return (any[u / 4] >> (8 * (u % 4))) & 0xffu; };
-      auto lane_bits = [&](int u) { return (bits[u / 4] >> (8 * (u % 4))) & 0xffu; };
-      // group u of this row, and the next row's on its way
-      auto take = [&](int u, float fill, float (&v)[kG]) {
-        if (full(u))
-          unpack_group<E>(q[u], v);
-        else
-          tail(MODE == kApplyGrad ? dyr : xr, u, fill, v);
-        if (read_next) issue(next, u);
-      };
       if constexpr (MODE == kFwd) {
-        float v[NV][kG], none[kG];
+        float v[NV][kG];
         float mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           take(u, -INFINITY, v[u]);
-          if (wave_bits(u) != 0) special<false>(v[u], none, wave_bits(u), lane_bits(u), words + u * kU, S);
-          if (m >= 0) {
+          const uint32_t gone = (out_any[u / 4] >> (8 * (u % 4))) & 0xffu;
+          if (gone != 0) {
+            const uint32_t mine = out[u / 4] >> (8 * (u % 4));
 #pragma unroll
-            for (int e = 0; e < kG; ++e) v[u][e] = (allowed[u] >> e) & 1u ? v[u][e] : -INFINITY;
+            for (int e = 0; e < kG; ++e)
+              if (gone & (1u << e)) v[u][e] = keep_if(-INFINITY, mine, e, v[u][e]);
           }
-          if (u == tu) {
-            float t = v[u][0];
+          if (wave_bits(u) != 0)
+            special(v[u], wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+          if (masked) {
 #pragma unroll
-            for (int e = 1; e < kG; ++e) t = e == te ? v[u][e] : t;
-            if (lane == tlane) P.xt[b * P.R + r0 + i] = t;
+            for (int e = 0; e < kG; ++e) v[u][e] = keep_if(v[u][e], allowed[u], e, -INFINITY);
           }
 #pragma unroll
           for (int e = 0; e < kG; ++e) mx = fmaxf(mx, v[u][e]);
+        }
+        float h_y = -INFINITY;
+        if (listed > 0) {
+          uint32_t how;
+          h_y = penalized(E::load_raw(h_x) + h_bias, h_word, S, how);
+          h_y = h_col >= 0 && (!masked || (h_mk >> (h_col % kG) & 1)) ? h_y : -INFINITY;
+          mx = fmaxf(mx, h_y);
+        }
+        if (t >= 0) {
+          const bool held = h_col == t;
+          float xt = h_y;
+          if (__ballot(held) == 0) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+              for (int e = 0; e < kG; ++e) xt = u == tu && e == te ? v[u][e] : xt;
+          }
+          if (__ballot(held) != 0 ? held : lane == tlane) P.xt[b * P.R + r0 + i] = xt;
         }
         // sums of 2^(y c - fl(M c)) with c = log2(e) / T, M the wave's maximum
         const float c = kLog2e * S.inv_t;
@@ -379,105 +616,100 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 #pragma unroll
             for (int e = 0; e < kG; ++e) s4[e & 3] = v[u][e] != v[u][e] ? v[u][e] : s4[e & 3];
         }
+        if (listed > 0) {
+          // (a lane without one: 2^-inf, or nothing under a maximum that is not there)
+          s4[0] += in_range ? fast_exp2(fmaf(h_y, c, -off)) : M != -INFINITY ? fast_exp2((h_y - M) * c) : h_y != h_y ? h_y : 0.f;
+        }
         float s = wave_fold((s4[0] + s4[1]) + (s4[2] + s4[3]), 0.f, [](float x, float y) { return x + y; });
         if (in_range) s *= fast_exp2(-fmaf(M, c, -off));  // the offset's rounding undone
         if (lane == 0)
           reinterpret_cast<float2*>(P.part)[(b * P.R + r0 + i) * (P.slices * kWaves) + slice * kWaves + wave] = float2{M, s};
       } else if constexpr (MODE == kBwd) {
-        if (g_now == 0.f) {
-          const float z[kG] = {};
+        const float M = of_row(m_M, i), c = kLog2e * S.inv_t, ls = of_row(m_ls, i) * kLog2e, gt = of_row(m_g, i) * S.inv_t;
 #pragma unroll
-          for (int u = 0; u < NV; ++u) {
-            put(u, z);
-            if (read_next) issue(next, u);
+        for (int u = 0; u < NV; ++u) {
+          float v[kG], o[kG];
+          take(u, 0.f, v);
+          uint32_t how = 0;
+          if (wave_bits(u) != 0)
+            how = special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+#pragma unroll
+          for (int e = 0; e < kG; ++e) o[e] = fast_exp2(fmaf(v[e] - M, c, -ls)) * -gt;
+          if (u == tu) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e)
+              o[e] = lane == tlane && e == te ? (1.f - fast_exp2(fmaf(v[e] - M, c, -ls))) * gt : o[e];
           }
-        } else {
-          const float c = kLog2e * S.inv_t, ls = ls_now * kLog2e, gt = g_now * S.inv_t;
+          if (wave_bits(u) != 0) through(o, wave_bits(u), how, S);
+          if (masked) {
 #pragma unroll
-          for (int u = 0; u < NV; ++u) {
-            float v[kG], o[kG], slope[kG];
-            take(u, 0.f, v);
-#pragma unroll
-            for (int e = 0; e < kG; ++e) slope[e] = 1.f;
-            if (wave_bits(u) != 0) special<true>(v, slope, wave_bits(u), lane_bits(u), words + u * kU, S);
-#pragma unroll
-            for (int e = 0; e < kG; ++e) o[e] = fast_exp2(fmaf(v[e] - M_now, c, -ls)) * -gt;
-            if (u == tu) {
-#pragma unroll
-              for (int e = 0; e < kG; ++e)
-                o[e] = lane == tlane && e == te ? (1.f - fast_exp2(fmaf(v[e] - M_now, c, -ls))) * gt : o[e];
-            }
-            if (wave_bits(u) != 0) {
-#pragma unroll
-              for (int e = 0; e < kG; ++e) o[e] *= slope[e];
-            }
-            if (m >= 0) {
-#pragma unroll
-              for (int e = 0; e < kG; ++e) o[e] = (allowed[u] >> e) & 1u ? o[e] : 0.f;
-            }
-            put(u, o);
+            for (int e = 0; e < kG; ++e) o[e] = keep_if(o[e], allowed[u], e, 0.f);
           }
+          put(y_row, u, o, WHOLE);
         }
       } else if constexpr (MODE == kApply) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-          float v[kG], none[kG];
+          float v[kG];
           take(u, 0.f, v);
-          if (wave_bits(u) != 0) special<false>(v, none, wave_bits(u), lane_bits(u), words + u * kU, S);
+          if (wave_bits(u) != 0)
+            special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
           for (int e = 0; e < kG; ++e) v[e] *= S.inv_t;
-          if (m >= 0) {
+          if (masked) {
 #pragma unroll
-            for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] : -INFINITY;
+            for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e], allowed[u], e, -INFINITY);
           }
-          put(u, v);
+          put(y_row, u, v, WHOLE);
         }
-      } else {
-        // these read the logits of some groups only
-        auto logits_of = [&](int u, float (&v)[kG]) {
-          if (full(u)) {
-            vu4 w[kP<E>];
-            load_group<E>(xr, at(u), w);
-            unpack_group<E>(w, v);
-          } else {
-            tail(xr, u, 0.f, v);
-          }
-        };
+      } else if constexpr (MODE == kApplyGrad) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-          float v[kG], slope[kG];
-          if constexpr (MODE == kInPlace) {
-            const bool mine = dense || lane_bits(u) != 0 || allowed[u] != 0xffu;
-            if (mine) {
-              logits_of(u, v);
-              special<false>(v, slope, 0xffu, lane_bits(u), words + u * kU, S);
+          float v[kG];
+          take(u, 0.f, v);
 #pragma unroll
-              for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] * S.inv_t : -INFINITY;
-              put(u, v);
-            }
-          } else {
-            take(u, 0.f, v);
-#pragma unroll
-            for (int e = 0; e < kG; ++e) slope[e] = S.inv_t;
-            if (wave_bits(u) != 0 && lane_bits(u) != 0) {
-              float x[kG];
-              logits_of(u, x);
-              special<true>(x, slope, wave_bits(u), lane_bits(u), words + u * kU, S);
-            }
-#pragma unroll
-            for (int e = 0; e < kG; ++e) v[e] *= slope[e];
-            if (m >= 0) {
-#pragma unroll
-              for (int e = 0; e < kG; ++e) v[e] = (allowed[u] >> e) & 1u ? v[e] : 0.f;
-            }
-            put(u, v);
+          for (int e = 0; e < kG; ++e) v[e] *= S.inv_t;
+          if (wave_bits(u) != 0) {
+            float x[kG];
+            if (full(u))
+              unpack_group<E>(qx[u], x);
+            else
+              tail(xr + i * P.xsr, u, 0.f, x);
+            const uint32_t how =
+                special(x, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+            through(v, wave_bits(u), how, S);
           }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e], allowed[u], e, 0.f);
+          }
+          put(y_row, u, v, WHOLE);
+        }
+      } else {  // kInPlace: what changes
+        const bool dense = S.inv_t != 1.f;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          allowed[u] = masked ? mk[u] : 0xffu;
+          issue_mask(next, u);
+          if (!(WHOLE || col(u) < left) || !(dense || lane_bits(u) != 0 || allowed[u] != 0xffu)) continue;
+          float v[kG];
+          if (full(u)) {
+            vu4 w[kP<E>];
+            load_group<E>(row, at0 + u * kWave * kGroupBytes<E>, w);
+            unpack_group<E>(w, v);
+          } else {
+            tail(row, u, 0.f, v);
+          }
+          special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+#pragma unroll
+          for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e] * S.inv_t, allowed[u], e, -INFINITY);
+          put(y_row, u, v, WHOLE);
         }
       }
-      read = read_next;
-      xr += P.xsr;
-      if (MODE == kApplyGrad) dyr += P.gsr;
-      if (MODE != kFwd) yr += P.ysr;
+      if (more) add_tokens(i, next);  // (this row is done with the words)
+      issue_words(next);
+      if (!more) break;
+      i = next;
     }
   };
   if (left == kSlice)
@@ -493,7 +725,8 @@ __global__ __launch_bounds__(kThreads) void processors_join_kernel(Params P, flo
   if (row >= P.B * P.R) return;
   const int64_t b = row / P.R, r = row - b * P.R, n = P.slices * kWaves;
   const mirl_logit_processors& A = P.A;
-  const float inv_t = 1.f / (A.temperature != nullptr ? A.temperature[b] : A.temperature_all), c = kLog2e * inv_t;
+  const Sample S = *reinterpret_cast<const Sample*>(head_of(P, b));
+  const float inv_t = S.inv_t, c = kLog2e * inv_t;
   const float* p = P.part + row * n * 2;
   float M = -INFINITY, s = 0.f;
   for (int64_t j = lane; j < n; j += kWave) M = fmaxf(M, p[2 * j]);
@@ -508,7 +741,7 @@ __global__ __launch_bounds__(kThreads) void processors_join_kernel(Params P, flo
   }
   s = wave_sum(s);
   if (lane != 0) return;
-  const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1, at = n_b + r;
+  const int64_t at = S.n + r;
   const int64_t t = at >= 0 && at < A.n_ids ? A.ids[b * A.ids_stride_b + at * A.ids_stride_s] - A.vocab_start : -1;
   const float logsum = logf(s);
   float lp = 0.f;
@@ -527,37 +760,49 @@ struct Plan {
   int nv;
   int64_t slices, rows, chunks;
 };
-Plan plan_of(int64_t B, int64_t R, int64_t V) {
+Plan plan_of(int mode, int64_t B, int64_t R, int64_t V) {
   Plan p;
-  p.nv = B * R * ceil_div(V, kThreads * kG) >= 4 * 4096 ? 4 : 1;
-  p.slices = ceil_div(V, kThreads * kG * p.nv);
-  p.rows = 32;
+  const int64_t wide = ceil_div(V, kBucket);
+  p.nv = mode == kFwd && B * R * wide >= 4 * 4096 ? 4 : 1;
+  if (getenv("T_NV") && mode == kFwd) p.nv = atoi(getenv("T_NV"));
+  p.slices = ceil_div(V, kBucket * p.nv);
+  p.rows = mode == kFwd ? 32 : 8;
   while (p.rows > 1 && B * ceil_div(R, p.rows) * p.slices < 2048) p.rows /= 2;
-  while (B * ceil_div(R, p.rows) * p.slices >= (int64_t(1) << 24)) p.rows *= 2;
+  if (getenv("T_ROWS")) p.rows = atoi(getenv("T_ROWS"));
+  while (B * ceil_div(R, p.rows) * p.slices >= (int64_t(1) << 24) && p.rows < kWave) p.rows *= 2;
   p.chunks = ceil_div(R, p.rows);
   return p;
 }
 
 template <int MODE>
 int launch(Params& P, int dtype, int64_t rows, const char* what, hipStream_t st) {
-  const Plan p = plan_of(P.B, rows, P.V);
+  const Plan p = plan_of(MODE, P.B, rows, P.V);
   P.slices = p.slices;
   P.chunks = p.chunks;
   P.rows = (int)p.rows;
   const dim3 grid((unsigned)(P.B * p.chunks * p.slices)), block(kThreads);
-  auto go = [&](auto e) {
-    using E = decltype(e);
-    if (p.nv == 4)
-      hipLaunchKernelGGL((processors_kernel<E, MODE, 4>), grid, block, 0, st, P);
+  auto go = [&](auto e, auto nv, auto masked) {
+    hipLaunchKernelGGL((processors_kernel<decltype(e), MODE, decltype(nv)::value, decltype(masked)::value>), grid, block, 0, st, P);
+  };
+  auto go_masked = [&](auto e, auto nv) {
+    if (P.A.n_masks > 0)
+      go(e, nv, std::true_type{});
     else
-      hipLaunchKernelGGL((processors_kernel<E, MODE, 1>), grid, block, 0, st, P);
+      go(e, nv, std::false_type{});
+  };
+  auto go_type = [&](auto e) {
+    if constexpr (MODE == kFwd) {
+      if (p.nv == 4) return go_masked(e, std::integral_constant<int, 4>{});
+      if (p.nv == 2) return go_masked(e, std::integral_constant<int, 2>{});
+    }
+    go_masked(e, std::integral_constant<int, 1>{});
   };
   if (dtype == MIRL_DTYPE_F32)
-    go(F32{});
+    go_type(F32{});
   else if (dtype == MIRL_DTYPE_BF16)
-    go(BF16{});
+    go_type(BF16{});
   else
-    go(F16{});
+    go_type(F16{});
   return check_launch(what);
 }
 
@@ -566,7 +811,8 @@ int check_args(const mirl_logit_processors* A, int dtype, int64_t B, int64_t R, 
                "unsupported logits dtype code %d", dtype);
   MIRL_REQUIRE(A != nullptr, "null pointer argument");
   MIRL_REQUIRE(B >= 0 && R >= 0 && V > 0, "invalid shape B=%lld R=%lld V=%lld", (long long)B, (long long)R, (long long)V);
-  MIRL_REQUIRE(V < (int64_t(1) << 31) && B * R < (int64_t(1) << 31), "sizes exceed 2^31-1");
+  MIRL_REQUIRE(V <= kMaxBuckets * kBucket, "a vocabulary of %lld exceeds %lld", (long long)V, (long long)(kMaxBuckets * kBucket));
+  MIRL_REQUIRE(B < (int64_t(1) << 22) && B * R < (int64_t(1) << 31), "sizes exceed 2^31-1");
   MIRL_REQUIRE(A->n_ids >= 0 && A->n_ids <= kMaxTokens, "%lld tokens of a sample, at most %lld are counted",
                (long long)A->n_ids, (long long)kMaxTokens);
   MIRL_REQUIRE(A->n_bias >= 0 && A->n_bias <= kMaxBias, "%lld biases of a sample, at most %lld are held",
@@ -580,7 +826,7 @@ int check_args(const mirl_logit_processors* A, int dtype, int64_t B, int64_t R, 
   return MIRL_OK;
 }
 
-Params params_of(const mirl_logit_processors* A, const void* x, int64_t B, int64_t R, int64_t Rt, int64_t V, int64_t xsb,
+Params params_of(const mirl_logit_processors* A, const uint32_t* table, const void* x, int64_t B, int64_t R, int64_t Rt, int64_t V, int64_t xsb,
                  int64_t xsr) {
   Params P{};
   P.A = *A;
@@ -592,7 +838,9 @@ Params params_of(const mirl_logit_processors* A, const void* x, int64_t B, int64
   P.xsb = xsb;
   P.xsr = xsr;
   const int64_t n = A->vocab_end - A->vocab_start;
-  P.n_vocab = n < V ? n : V;
+  P.n_vocab = n < 0 ? 0 : n < V ? n : V;
+  P.buckets = ceil_div(V, kBucket);
+  P.table = table;
   return P;
 }
 
@@ -601,37 +849,54 @@ Params params_of(const mirl_logit_processors* A, const void* x, int64_t B, int64
 
 using namespace mirl;
 
+extern "C" int64_t mirl_logit_processors_table_elems(int64_t B, int64_t V, int64_t n_ids, int64_t n_bias) {
+  if (B <= 0 || V <= 0 || n_ids < 0 || n_bias < 0) return 0;
+  return B * (kHead + ceil_div(V, kBucket) + 1 + n_ids + n_bias);
+}
+
+extern "C" int mirl_logit_processors_table(const mirl_logit_processors* processors, int64_t B, int64_t R, int64_t V,
+                                           uint32_t* table, void* stream) {
+  clear_error();
+  if (int e = check_args(processors, MIRL_DTYPE_F32, B, R, V)) return e;
+  if (B * R == 0) return MIRL_OK;
+  MIRL_REQUIRE(table != nullptr, "null pointer argument");
+  const Params P = params_of(processors, nullptr, nullptr, B, R, R, V, 0, 0);
+  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)B), dim3(kTableThreads), 0, static_cast<hipStream_t>(stream), *processors, B, R,
+                     P.n_vocab, (int)P.buckets, table);
+  return check_launch("mirl_logit_processors_table");
+}
+
 extern "C" int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V) {
   if (B <= 0 || R <= 0 || V <= 0) return 0;
-  return B * R * (plan_of(B, R, V).slices * kWaves * 2 + 1);
+  return B * R * (plan_of(kFwd, B, R, V).slices * kWaves * 2 + 1);
 }
 
 extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                          int64_t stride_r, const mirl_logit_processors* processors, float* out,
+                                          int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, float* out,
                                           float* stats, float* workspace, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
-  MIRL_REQUIRE(logits && out && workspace, "null pointer argument");
-  Params P = params_of(processors, logits, B, R, R, V, stride_b, stride_r);
+  MIRL_REQUIRE(table && logits && out && workspace, "null pointer argument");
+  Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   hipStream_t st = static_cast<hipStream_t>(stream);
   P.part = workspace;
-  P.xt = workspace + B * R * plan_of(B, R, V).slices * kWaves * 2;
+  P.xt = workspace + B * R * plan_of(kFwd, B, R, V).slices * kWaves * 2;
   if (int e = launch<kFwd>(P, dtype, R, "mirl_processed_logprob_fwd", st)) return e;
   hipLaunchKernelGGL(processors_join_kernel, dim3((unsigned)ceil_div(B * R, kWaves)), dim3(kThreads), 0, st, P, out, stats);
   return check_launch("mirl_processed_logprob_fwd");
 }
 
 extern "C" int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t Rt, int64_t V,
-                                          int64_t stride_b, int64_t stride_r, const mirl_logit_processors* processors,
+                                          int64_t stride_b, int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table,
                                           const float* stats, const float* grad_out, int64_t g_stride_b, int64_t g_stride_r,
                                           void* grad_in, int64_t gi_stride_b, int64_t gi_stride_r, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, Rt, V)) return e;
   MIRL_REQUIRE(R >= 0 && R <= Rt, "invalid shape R=%lld of %lld rows", (long long)R, (long long)Rt);
   if (B * Rt == 0) return MIRL_OK;
-  MIRL_REQUIRE(logits && grad_in && (R == 0 || (stats && grad_out)), "null pointer argument");
-  Params P = params_of(processors, logits, B, R, Rt, V, stride_b, stride_r);
+  MIRL_REQUIRE(table && logits && grad_in && (R == 0 || (stats && grad_out)), "null pointer argument");
+  Params P = params_of(processors, table, logits, B, R, Rt, V, stride_b, stride_r);
   P.stats = stats;
   P.g = grad_out;
   P.gsb = g_stride_b;
@@ -643,14 +908,14 @@ extern "C" int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t
 }
 
 extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                   int64_t stride_r, const mirl_logit_processors* processors, void* out,
+                                   int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, void* out,
                                    int64_t o_stride_b, int64_t o_stride_r, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
-  MIRL_REQUIRE(logits && out, "null pointer argument");
+  MIRL_REQUIRE(table && logits && out, "null pointer argument");
   MIRL_REQUIRE(out != logits || (o_stride_b == stride_b && o_stride_r == stride_r), "in place, the strides are those of the logits");
-  Params P = params_of(processors, logits, B, R, R, V, stride_b, stride_r);
+  Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   P.y = out;
   P.ysb = o_stride_b;
   P.ysr = o_stride_r;
@@ -660,14 +925,14 @@ extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int
 }
 
 extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                       int64_t stride_r, const mirl_logit_processors* processors, const void* grad_out,
+                                       int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, const void* grad_out,
                                        int64_t g_stride_b, int64_t g_stride_r, void* grad_in, int64_t gi_stride_b,
                                        int64_t gi_stride_r, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
-  MIRL_REQUIRE(logits && grad_out && grad_in, "null pointer argument");
-  Params P = params_of(processors, logits, B, R, R, V, stride_b, stride_r);
+  MIRL_REQUIRE(table && logits && grad_out && grad_in, "null pointer argument");
+  Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   P.dy = grad_out;
   P.gsb = g_stride_b;
   P.gsr = g_stride_r;

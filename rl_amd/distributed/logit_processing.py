@@ -139,16 +139,18 @@ class _ProcessedLogprob(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, R: int, call: _Call) -> torch.Tensor:  # type: ignore[override]
-        out, stats = _C.processed_logprob_fwd(logits, R, call.args(), True)
-        ctx.save_for_backward(logits, stats, *call.saved())
+        args = call.args()
+        table = _C.processor_table(logits, R, args)
+        out, stats = _C.processed_logprob_fwd(logits, R, args, table, True)
+        ctx.save_for_backward(logits, stats, table, *call.saved())
         ctx.call = call
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):  # type: ignore[override]
-        logits, stats, *saved = ctx.saved_tensors
-        return _C.processed_logprob_bwd(logits, ctx.call.args_of_saved(saved), stats, grad.float()), None, None
+        logits, stats, table, *saved = ctx.saved_tensors
+        return _C.processed_logprob_bwd(logits, ctx.call.args_of_saved(saved), table, stats, grad.float()), None, None
 
 
 class _ProcessLogits(torch.autograd.Function):
@@ -156,15 +158,17 @@ class _ProcessLogits(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, call: _Call) -> torch.Tensor:  # type: ignore[override]
-        ctx.save_for_backward(logits, *call.saved())
+        args = call.args()
+        table = _C.processor_table(logits, logits.shape[1], args)
+        ctx.save_for_backward(logits, table, *call.saved())
         ctx.call = call
-        return _C.process_logits(logits, call.args(), False)
+        return _C.process_logits(logits, args, table, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):  # type: ignore[override]
-        logits, *saved = ctx.saved_tensors
-        return _C.process_logits_bwd(logits, ctx.call.args_of_saved(saved), grad), None
+        logits, table, *saved = ctx.saved_tensors
+        return _C.process_logits_bwd(logits, ctx.call.args_of_saved(saved), table, grad), None
 
 
 def _grad_needed(logits: torch.Tensor) -> bool:
@@ -198,7 +202,8 @@ def processed_next_token_logprobs(
     end = vocab_start_index + logits.shape[2] if vocab_end_index is None else vocab_end_index
     call = _Call(logits, input_ids, processors, history_lengths, R, (int(vocab_start_index), int(end)))
     if inference_only or not _grad_needed(logits):
-        return _C.processed_logprob_fwd(logits, R, call.args(), False)[0]
+        args = call.args()
+        return _C.processed_logprob_fwd(logits, R, args, _C.processor_table(logits, R, args), False)[0]
     return _ProcessedLogprob.apply(logits, R, call)
 
 
@@ -225,9 +230,12 @@ def process_logits(
     elif x.stride(2) != 1:
         x = x.contiguous()
     call = _Call(x, input_ids, processors, history_lengths, x.shape[1], (0, x.shape[2]))
+    if not inplace and _grad_needed(logits):
+        y = _ProcessLogits.apply(x, call)
+        return y if logits.dim() == 3 else y.squeeze(1)
+    args = call.args()
+    y = _C.process_logits(x, args, _C.processor_table(x, x.shape[1], args), inplace)
     if inplace:
-        _C.process_logits(x, call.args(), True)
         torch.autograd.graph.increment_version(logits)
         return logits
-    y = _ProcessLogits.apply(x, call) if _grad_needed(logits) else _C.process_logits(x, call.args(), False)
     return y if logits.dim() == 3 else y.squeeze(1)
