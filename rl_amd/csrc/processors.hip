@@ -18,7 +18,6 @@
 // cost one test for a group of eight.
 
 #include "common.h"
-#include <cstdlib>
 
 #pragma clang fp contract(off)
 
@@ -102,19 +101,33 @@ __device__ __forceinline__ void store_group(typename E::raw* slice, uint32_t at,
   }
 }
 
-// The maximum and the sum over a wave by lane permutes within the VALU (64 lanes; in lane 63, given to all).
-template <int CTRL>
-__device__ __forceinline__ float from_lane(float other, float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, 0xf, 0xf, false));
+// The maximum and the sum over a wave within the VALU: each row of 16 lanes into its last, rows into the
+// next, lanes 0 .. 31 into the others; the result in lane 63, given to all.  (A lane that nothing is
+// permuted to keeps its own.  In asm: the compiler makes four instructions of a maximum's step; it knows
+// nothing of the two wait states ahead of a permuted operand, hence the s_nops.)
+__device__ __forceinline__ float wave_max_all(float v) {
+  asm volatile(
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n\t"
+      "s_nop 1"
+      : "+v"(v));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
-template <class F>
-__device__ __forceinline__ float wave_fold(float v, float none, F&& f) {
-  v = f(v, from_lane<0x111>(none, v));  // row_shr 1, 2, 4, 8
-  v = f(v, from_lane<0x112>(none, v));
-  v = f(v, from_lane<0x114>(none, v));
-  v = f(v, from_lane<0x118>(none, v));
-  v = f(v, from_lane<0x142>(none, v));  // row_bcast 15, 31
-  v = f(v, from_lane<0x143>(none, v));
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float wave_sum_all(float v) {
+  v += from_lane<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += from_lane<0x112>(v);
+  v += from_lane<0x114>(v);
+  v += from_lane<0x118>(v);
+  v += from_lane<0x142>(v);  // row_bcast 15, 31
+  v += from_lane<0x143>(v);
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ float of_row(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
@@ -131,7 +144,8 @@ __device__ __forceinline__ const uint32_t* head_of(const Params& P, int64_t b) {
 
 // v where bit e of `keep` is set, else `other`; as bits, whatever v holds.
 __device__ __forceinline__ float keep_if(float v, uint32_t keep, int e, float other) {
-  const uint32_t t = (uint32_t)__builtin_amdgcn_sbfe((int)keep, e, 1);
+  uint32_t t = (uint32_t)__builtin_amdgcn_sbfe((int)keep, e, 1);
+  asm("" : "+v"(t));  // (two instructions, where a compare and a select take three)
   return __uint_as_float((__float_as_uint(v) & t) | (__float_as_uint(other) & ~t));
 }
 
@@ -158,6 +172,7 @@ __device__ __forceinline__ uint32_t special(float (&v)[kG], uint32_t any, uint32
 #pragma unroll
   for (int e = 0; e < kG; ++e) {
     if ((any & (1u << e)) == 0) continue;
+    asm volatile("");  // (a branch of its own: the test of the lanes' bits is not worth making for nothing)
     if ((bits >> e) & 1u) {
       const uint32_t w = words[e / 4][e % 4];
       uint32_t h;
@@ -172,6 +187,7 @@ __device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t h
 #pragma unroll
   for (int e = 0; e < kG; ++e) {
     if ((any & (1u << e)) == 0) continue;
+    asm volatile("");
     o[e] *= (how >> e) & 1u ? S.inv_rp : (how >> e) & 256u ? S.rp : 1.f;
   }
 }
@@ -272,6 +288,11 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   // kFwd: up to 64 of a wave's tokens with a word are held by a lane each
   constexpr bool kLists = MODE == kFwd;
   __shared__ uint16_t s_list[kLists ? kWaves : 1][kWave];
+  __shared__ __align__(16) raw s_row[kLists ? kSlice : 8];  // a row's values and mask bytes, for those lanes
+  __shared__ uint8_t s_mask[kLists && MASKED ? kSlice / kG : 1];
+  // kFwd: what a mask's byte (fp32: half of one) leaves of a 16-byte piece's words
+  constexpr int kLut = kLists && MASKED ? 1 << E::kVec : 1;
+  __shared__ vu4 s_lut[kLut];
   // the other modes: biases by column (a gather in the middle of a row would wait for the next row's loads)
   __shared__ float s_bias[kLists ? 1 : kSlice];
 
@@ -330,20 +351,33 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   }
   // The first row's values are on their way while the tokens are counted.
   vu4 q[NV][kP<E>];
-  auto issue = [&](int i, int u, bool whole) __attribute__((always_inline)) {
+  auto issue = [&](int i, int u, bool whole, uint32_t keep) __attribute__((always_inline)) {
     const raw* row = MODE == kApplyGrad ? dyr + i * P.gsr : xr + i * P.xsr;
-    if (whole || col(u) + kG <= left) load_group<E>(row, at0 + u * kWave * kGroupBytes<E>, q[u]);
+    if (whole || col(u) + kG <= left) load_group<E>(row, (at0 + u * kWave * kGroupBytes<E>) & keep, q[u]);
   };
   const int first = __builtin_ctzll(todo);
   if constexpr (MODE != kInPlace) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) issue(first, u, false);
+    for (int u = 0; u < NV; ++u) issue(first, u, false, ~0u);
   }
 
   // ---- the tokens ahead of row r0, and the biases ----
 #pragma unroll
   for (int i = 0; i < kSlice / 4 / kThreads; ++i)
     reinterpret_cast<vu4*>(s_word)[i * kThreads + tid] = vu4{0u, 0u, 0u, 0u};
+  if constexpr (kLists && MASKED) {
+    if (tid < kLut) {
+      vu4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (E::kVec == 8)
+          w[k] = (tid >> (2 * k) & 1 ? 0xffffu : 0u) | (tid >> (2 * k + 1) & 1 ? 0xffff0000u : 0u);
+        else
+          w[k] = tid >> k & 1 ? ~0u : 0u;
+      }
+      s_lut[tid] = w;
+    }
+  }
   // an id's column in this wave, or -1
   const int64_t first_id = A.vocab_start + n0 + wave * kWaveCols;
   const uint32_t here = (uint32_t)max(int64_t(0), min((int64_t)kWaveCols, P.n_vocab - n0 - wave * kWaveCols));
@@ -400,8 +434,12 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   // Tokens with a word other than 0: a byte per group of the lane's and of any lane's.
   uint32_t bits[kPacks] = {}, any[kPacks] = {};
   // kFwd: the listed tokens (column, word, bias of the lane's), which are formed all at once and left out
-  // of the groups (out: the lane's, out_any: any lane's); the others as in every mode.
-  uint32_t out[kPacks] = {}, out_any[kPacks] = {};
+  // of the groups (`gone` masks the lane's in the words of a group as it is read); the others as in every mode.
+  constexpr int kRawWords = kLists ? kP<E> * 4 : 1, kPerWord = kG / (kP<E> * 4);
+  uint32_t gone[kLists ? NV : 1][kRawWords] = {};
+  auto mark_gone = [&](int u, int e) __attribute__((always_inline)) {  // (u and e constant)
+    if constexpr (kLists) gone[u][e / kPerWord] |= kPerWord == 1 ? ~0u : 0xffffu << (16 * (e % kPerWord));
+  };
   int listed = 0, h_col = -1;
   uint32_t h_word = 0;
   float h_bias = 0.f;
@@ -421,13 +459,13 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           in_list = set && at < kWave;
           if (in_list) s_list[wave][at] = (uint16_t)((u * kWave + lane) * kG + e);
           const int n = (int)__popcll(all);
-          if (listed < kWave) out_any[u / 4] |= bit;
+          if (in_list) mark_gone(u, e);
           if (listed + n > kWave) any[u / 4] |= bit;
           listed = min(listed + n, kWave);
         } else {
           any[u / 4] |= bit;
         }
-        if (set) (in_list ? out : bits)[u / 4] |= bit;
+        if (set && !in_list) bits[u / 4] |= bit;
       }
     }
     if constexpr (kLists) {
@@ -466,7 +504,15 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
         ++listed;
       }
     }
-    if (mine && !lists) {
+    if (lists) {
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int e = 0; e < kG; ++e)
+          if (mine && group / kWave == u && c % kG == e) mark_gone(u, e);
+      return;
+    }
+    if (mine) {
       uint32_t& w = s_word[wave * kWaveCols + c];
       w = more_of(w);
     }
@@ -474,8 +520,8 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
     for (int u = 0; u < NV; ++u) {
       if (group / kWave != u) continue;
       const uint32_t b8 = bit << (8 * (u % 4));
-      (lists ? out_any : any)[u / 4] |= b8;
-      if (mine) (lists ? out : bits)[u / 4] |= b8;
+      any[u / 4] |= b8;
+      if (mine) bits[u / 4] |= b8;
     }
   };
   auto add_tokens = [&](int from, int to) __attribute__((always_inline)) {  // ahead of rows from + 1 .. to
@@ -486,9 +532,9 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   auto wave_bits = [&](int u) { return (any[u / 4] >> (8 * (u % 4))) & 0xffu; };
   auto lane_bits = [&](int u) { return (bits[u / 4] >> (8 * (u % 4))) & 0xffu; };
 
-  // WHOLE: the slice lies inside the row.  Its loads are then issued in every row alike (a last row's once
-  // more in place of a next one's, lanes that need nothing the slice's first column): the compiler counts
-  // what is in flight, and a row waits for its own values only.
+  // WHOLE: the slice lies inside the row.  Its loads are then issued in every row alike (behind the last
+  // one, and in lanes that need nothing, of the slice's first columns): the compiler counts what is in flight,
+  // and a row waits for its own values only.
   auto rows = [&](auto whole_c) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole_c)::value;
     auto tail = [&](const raw* row, int u, float fill, float (&v)[kG]) {
@@ -496,10 +542,9 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       for (int e = 0; e < kG; ++e) v[e] = col(u) + e < left ? E::load(row + col(u) + e) : fill;
     };
     auto full = [&](int u) { return WHOLE || col(u) + kG <= left; };
-    // a row's mask bytes; kFwd: its listed tokens' logits and mask bytes; kApplyGrad: the logits of groups with
-    // a word (all as they come: what converts them would wait here)
-    uint8_t mk[NV], h_mk = 0xff;
-    raw h_x = raw();
+    // a row's mask bytes; kApplyGrad: the logits of groups with a word (as they come: what converts them would
+    // wait here)
+    uint8_t mk[NV];
     vu4 qx[MODE == kApplyGrad ? NV : 1][kP<E>];
     auto mask_of = [&](int i) {
       const int m = __builtin_amdgcn_readlane(m_mask, i);
@@ -511,11 +556,6 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       }
     };
     auto issue_words = [&](int i) __attribute__((always_inline)) {
-      if constexpr (kLists) {
-        const uint32_t c = h_col < 0 ? 0 : wave * kWaveCols + h_col;
-        h_x = xr[i * P.xsr + c];
-        if (MASKED) h_mk = mask_of(i)[c / kG];
-      }
       if constexpr (MODE == kApplyGrad) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
@@ -536,12 +576,37 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       uint32_t allowed[NV];
       // group u of this row, and the next row's on its way
       auto take = [&](int u, float fill, float (&v)[kG]) __attribute__((always_inline)) {
-        if (full(u))
+        if (full(u)) {
+          if constexpr (kLists) {
+            if (listed > 0) {
+#pragma unroll
+              for (int k = 0; k < kP<E>; ++k) reinterpret_cast<vu4*>(s_row + col(u))[k] = q[u][k];
+            }
+            // (a masked token's bias and penalties leave it at -inf)
+#pragma unroll
+            for (int k = 0; k < kP<E>; ++k) {
+              vu4 lost = {gone[u][4 * k], gone[u][4 * k + 1], gone[u][4 * k + 2], gone[u][4 * k + 3]};
+              if (masked) lost |= ~s_lut[mk[u] >> (k * E::kVec) & (kLut - 1)];
+              q[u][k] = (q[u][k] & ~lost) | (E::kNegInf2 & lost);
+            }
+          }
           unpack_group<E>(q[u], v);
-        else
+        } else {
           tail(row, u, fill, v);
+          if constexpr (kLists) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e) s_row[col(u) + e] = E::from_float(v[e]);  // (exact)
+#pragma unroll
+            for (int e = 0; e < kG; ++e)
+              v[e] = (gone[u][e / kPerWord] >> (kPerWord == 1 ? 0 : 16 * (e % kPerWord)) & 1u) ||
+                             (masked && !(mk[u] >> e & 1))
+                         ? -INFINITY
+                         : v[e];
+          }
+        }
         allowed[u] = masked ? mk[u] : 0xffu;
-        issue(next, u, WHOLE);
+        if (kLists && masked && listed > 0) s_mask[kLists && MASKED ? g0 + u * kWave : 0] = (uint8_t)allowed[u];
+        issue(next, u, WHOLE, more ? ~0u : 0u);
         issue_mask(next, u);
       };
       // the next token's group of the lane, and which of its eight
@@ -560,27 +625,18 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           take(u, -INFINITY, v[u]);
-          const uint32_t gone = (out_any[u / 4] >> (8 * (u % 4))) & 0xffu;
-          if (gone != 0) {
-            const uint32_t mine = out[u / 4] >> (8 * (u % 4));
-#pragma unroll
-            for (int e = 0; e < kG; ++e)
-              if (gone & (1u << e)) v[u][e] = keep_if(-INFINITY, mine, e, v[u][e]);
-          }
           if (wave_bits(u) != 0)
             special(v[u], wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < kG; ++e) v[u][e] = keep_if(v[u][e], allowed[u], e, -INFINITY);
-          }
 #pragma unroll
           for (int e = 0; e < kG; ++e) mx = fmaxf(mx, v[u][e]);
         }
         float h_y = -INFINITY;
         if (listed > 0) {
           uint32_t how;
-          h_y = penalized(E::load_raw(h_x) + h_bias, h_word, S, how);
-          h_y = h_col >= 0 && (!masked || (h_mk >> (h_col % kG) & 1)) ? h_y : -INFINITY;
+          const int c = wave * kWaveCols + max(h_col, 0);
+          h_y = penalized(E::load(s_row + (kLists ? c : 0)) + h_bias, h_word, S, how);
+          const uint32_t m = masked ? s_mask[kLists && MASKED ? c / kG : 0] : 0xffu;
+          h_y = h_col >= 0 && (m >> (c % kG) & 1u) ? h_y : -INFINITY;
           mx = fmaxf(mx, h_y);
         }
         if (t >= 0) {
@@ -596,7 +652,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
         }
         // sums of 2^(y c - fl(M c)) with c = log2(e) / T, M the wave's maximum
         const float c = kLog2e * S.inv_t;
-        const float M = wave_fold(mx, -INFINITY, [](float x, float y) { return fmaxf(x, y); });
+        const float M = wave_max_all(mx);
         const float off = M * c;
         const bool in_range = fabsf(off) < INFINITY;
         float s4[4] = {0.f, 0.f, 0.f, 0.f};
@@ -620,7 +676,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           // (a lane without one: 2^-inf, or nothing under a maximum that is not there)
           s4[0] += in_range ? fast_exp2(fmaf(h_y, c, -off)) : M != -INFINITY ? fast_exp2((h_y - M) * c) : h_y != h_y ? h_y : 0.f;
         }
-        float s = wave_fold((s4[0] + s4[1]) + (s4[2] + s4[3]), 0.f, [](float x, float y) { return x + y; });
+        float s = wave_sum_all((s4[0] + s4[1]) + (s4[2] + s4[3]));
         if (in_range) s *= fast_exp2(-fmaf(M, c, -off));  // the offset's rounding undone
         if (lane == 0)
           reinterpret_cast<float2*>(P.part)[(b * P.R + r0 + i) * (P.slices * kWaves) + slice * kWaves + wave] = float2{M, s};
@@ -760,15 +816,13 @@ struct Plan {
   int nv;
   int64_t slices, rows, chunks;
 };
-Plan plan_of(int mode, int64_t B, int64_t R, int64_t V) {
+Plan plan_of(int mode, int dtype, int64_t B, int64_t R, int64_t V) {
   Plan p;
   const int64_t wide = ceil_div(V, kBucket);
-  p.nv = mode == kFwd && B * R * wide >= 4 * 4096 ? 4 : 1;
-  if (getenv("T_NV") && mode == kFwd) p.nv = atoi(getenv("T_NV"));
+  p.nv = mode == kFwd && dtype != MIRL_DTYPE_F32 && B * R * wide >= 4096 ? 2 : 1;
   p.slices = ceil_div(V, kBucket * p.nv);
-  p.rows = mode == kFwd ? 32 : 8;
-  while (p.rows > 1 && B * ceil_div(R, p.rows) * p.slices < 2048) p.rows /= 2;
-  if (getenv("T_ROWS")) p.rows = atoi(getenv("T_ROWS"));
+  p.rows = mode == kFwd ? 32 : 4;
+  while (p.rows > 1 && B * ceil_div(R, p.rows) * p.slices < (mode == kFwd ? 1024 : 2048)) p.rows /= 2;
   while (B * ceil_div(R, p.rows) * p.slices >= (int64_t(1) << 24) && p.rows < kWave) p.rows *= 2;
   p.chunks = ceil_div(R, p.rows);
   return p;
@@ -776,10 +830,11 @@ Plan plan_of(int mode, int64_t B, int64_t R, int64_t V) {
 
 template <int MODE>
 int launch(Params& P, int dtype, int64_t rows, const char* what, hipStream_t st) {
-  const Plan p = plan_of(MODE, P.B, rows, P.V);
+  const Plan p = plan_of(MODE, dtype, P.B, rows, P.V);
   P.slices = p.slices;
   P.chunks = p.chunks;
   P.rows = (int)p.rows;
+  MIRL_REQUIRE(P.B * p.chunks * p.slices < (int64_t(1) << 24), "too many rows of %lld columns", (long long)P.V);
   const dim3 grid((unsigned)(P.B * p.chunks * p.slices)), block(kThreads);
   auto go = [&](auto e, auto nv, auto masked) {
     hipLaunchKernelGGL((processors_kernel<decltype(e), MODE, decltype(nv)::value, decltype(masked)::value>), grid, block, 0, st, P);
@@ -792,8 +847,9 @@ int launch(Params& P, int dtype, int64_t rows, const char* what, hipStream_t st)
   };
   auto go_type = [&](auto e) {
     if constexpr (MODE == kFwd) {
-      if (p.nv == 4) return go_masked(e, std::integral_constant<int, 4>{});
-      if (p.nv == 2) return go_masked(e, std::integral_constant<int, 2>{});
+      if constexpr (!std::is_same<decltype(e), F32>::value) {
+        if (p.nv == 2) return go_masked(e, std::integral_constant<int, 2>{});
+      }
     }
     go_masked(e, std::integral_constant<int, 1>{});
   };
@@ -868,7 +924,7 @@ extern "C" int mirl_logit_processors_table(const mirl_logit_processors* processo
 
 extern "C" int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V) {
   if (B <= 0 || R <= 0 || V <= 0) return 0;
-  return B * R * (plan_of(kFwd, B, R, V).slices * kWaves * 2 + 1);
+  return B * R * (plan_of(kFwd, MIRL_DTYPE_F32, B, R, V).slices * kWaves * 2 + 1);
 }
 
 extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
@@ -881,7 +937,7 @@ extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t
   Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   hipStream_t st = static_cast<hipStream_t>(stream);
   P.part = workspace;
-  P.xt = workspace + B * R * plan_of(kFwd, B, R, V).slices * kWaves * 2;
+  P.xt = workspace + B * R * plan_of(kFwd, dtype, B, R, V).slices * kWaves * 2;
   if (int e = launch<kFwd>(P, dtype, R, "mirl_processed_logprob_fwd", st)) return e;
   hipLaunchKernelGGL(processors_join_kernel, dim3((unsigned)ceil_div(B * R, kWaves)), dim3(kThreads), 0, st, P, out, stats);
   return check_launch("mirl_processed_logprob_fwd");
