@@ -924,6 +924,16 @@ int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* r
                           float* y_scale, float* rstd, void* stream);
 
 /*
+ * The same with y in 8-bit integers: s = max|y| / 127 (at least 2^-126; 1 for a row of zeros),
+ * y8 = y * (1 / s) to the nearest (ties to even); a row that holds a NaN or an infinity has a
+ * scale that is none and 0 in those places.
+ */
+int mirl_add_rms_norm_int8_fwd(const void* x, int x_dtype, int64_t ldx, const void* residual,
+                               int res_dtype, int64_t ldr, const void* weight, int w_dtype,
+                               int64_t R, int64_t H, double eps, void* h, int8_t* y,
+                               float* y_scale, void* stream);
+
+/*
  * Its backward, from the stored h and rstd: with n = h * rstd,
  *   dh = rstd * (w dy - n * mean(w dy n)) + dh_out,   dw = sum over rows of dy * n.
  * dh_out (the gradient of the returned h, of h_dtype) may be NULL.  dx (x_dtype)
@@ -945,6 +955,9 @@ int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, const void*
  */
 int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, void* y,
                        float* scale, void* stream);
+/* The same in 8-bit integers, as mirl_add_rms_norm_int8_fwd makes them. */
+int mirl_quantize_rows_int8(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H,
+                            int8_t* y, float* scale, void* stream);
 
 /*
  * Dropout of n contiguous elements (F32, BF16 or F16): element i takes the
@@ -978,6 +991,23 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
                             int64_t vocab_start, int64_t vocab_end, float* out,
                             int64_t o_stride_b, int64_t o_stride_s, float* workspace,
                             void* stream);
+
+/*
+ * The same from 8-bit integers (mirl_add_rms_norm_int8_fwd, mirl_quantize_rows_int8):
+ *   x[r, v] = (float(sum_k hidden8[r, k] weight8[v, k]) * weight_scale[v]) * hidden_scale[r]
+ * with exact sums, Hd at most 2^17 - 256.  And these logits written out: out [T, V], rows ldo apart, in
+ * fp32, bf16 or fp16, each rounded once from fp32.
+ */
+int mirl_linear_ce_int8_fwd(const int8_t* hidden8, const float* hidden_scale, int64_t T,
+                            int64_t Hd, int64_t ldh, const int8_t* weight8,
+                            const float* weight_scale, int64_t V, int64_t ldw, int64_t bsz,
+                            const int64_t* target, int64_t t_stride_b, int64_t t_stride_s,
+                            int64_t vocab_start, int64_t vocab_end, float* out,
+                            int64_t o_stride_b, int64_t o_stride_s, float* workspace,
+                            void* stream);
+int mirl_int8_logits(const int8_t* hidden8, const float* hidden_scale, int64_t T, int64_t Hd,
+                     int64_t ldh, const int8_t* weight8, const float* weight_scale, int64_t V,
+                     int64_t ldw, void* out, int out_dtype, int64_t ldo, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* What a sampler does to logits ahead of top-k and top-p                   */

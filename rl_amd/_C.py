@@ -292,6 +292,14 @@ SIGNATURES = {
     "mirl_add_rms_norm_fwd": (
         _I, [_P, _I, _I64, _P, _I, _I64, _P, _I, _I64, _I64, ctypes.c_double, _P, _P, _P, _P, _P]
     ),
+    "mirl_add_rms_norm_int8_fwd": (
+        _I, [_P, _I, _I64, _P, _I, _I64, _P, _I, _I64, _I64, ctypes.c_double, _P, _P, _P, _P]
+    ),
+    "mirl_quantize_rows_int8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "mirl_linear_ce_int8_fwd": (
+        _I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P]
+    ),
+    "mirl_int8_logits": (_I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _I64, _P]),
     "mirl_add_rms_norm_bwd_workspace_elems": (_I64, [_I64, _I64]),
     "mirl_add_rms_norm_bwd": (
         _I, [_P, _I, _I64, _P, _I64, _P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P]
@@ -1670,9 +1678,11 @@ def _direct(dev: torch.device) -> bool:
 
 
 def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
-                     want_rstd: bool, out8: bool):
-    """(y, h, rstd [R] or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd); h is x
-    itself without a residual, scale has a row's shape.  Shapes and types are the caller's to check."""
+                     want_rstd: bool, out8: Optional[torch.dtype]):
+    """(y, h, rstd [R] or None, scale or None) of ``x [..., H]`` (see mirl_add_rms_norm_fwd and, with
+    ``out8`` of int8, mirl_add_rms_norm_int8_fwd, which keeps no rstd); ``out8`` is y's type where it is
+    one of 8 bits, else None; h is x itself without a residual, scale has a row's shape.  Shapes and types
+    are the caller's to check."""
     dev = x.device
     if not x.is_cuda or weight.device != dev or (residual is not None and residual.device != dev):
         _require_gpu(x, residual, weight)
@@ -1682,10 +1692,10 @@ def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     code = DTYPE_CODES[dtype]
     if x.is_contiguous():
         x2, ldx = x, H
-        y = torch.empty_like(x, dtype=torch.float8_e4m3fn) if out8 else torch.empty_like(x)
+        y = torch.empty_like(x) if out8 is None else torch.empty_like(x, dtype=out8)
     else:
         x2, ldx = _rows2(x)
-        y = x.new_empty(shape, dtype=torch.float8_e4m3fn if out8 else dtype)
+        y = x.new_empty(shape, dtype=dtype if out8 is None else out8)
     if not weight.is_contiguous():
         weight = weight.contiguous()
     if residual is None:
@@ -1697,11 +1707,13 @@ def add_rms_norm_fwd(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
             r2, ldr = _rows2(residual)
             h = residual.new_empty(shape)
         r_ptr, h_ptr, h_code = r2.data_ptr(), h.data_ptr(), DTYPE_CODES[residual.dtype]
-    scale = x.new_empty(shape[:-1], dtype=torch.float32) if out8 else None
+    scale = None if out8 is None else x.new_empty(shape[:-1], dtype=torch.float32)
     rstd = torch.empty(R, dtype=torch.float32, device=dev) if want_rstd else None
     args = (x2.data_ptr(), code, ldx, r_ptr, h_code, ldr, weight.data_ptr(), DTYPE_CODES[weight.dtype], R, H, eps, h_ptr,
             y.data_ptr(), None if scale is None else scale.data_ptr(), None if rstd is None else rstd.data_ptr())
-    if _direct(dev):
+    if out8 == torch.int8:
+        st = _launch("mirl_add_rms_norm_int8_fwd", dev, *args[:-1], _stream(dev))
+    elif _direct(dev):
         st = _lib.mirl_add_rms_norm_fwd(*args, _raw_stream(dev.index))
     else:
         st = _launch("mirl_add_rms_norm_fwd", dev, *args, _stream(dev))
@@ -1759,14 +1771,14 @@ def add_rms_norm_bwd(dy: torch.Tensor, dh_out: Optional[torch.Tensor], h: torch.
     return dx, (dx if one else dres), dw
 
 
-def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(e4m3 rows, fp32 scales) of ``x [..., H]`` (see mirl_quantize_rows)."""
+def quantize_rows(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 or int8 rows, fp32 scales) of ``x [..., H]`` (see mirl_quantize_rows, mirl_quantize_rows_int8)."""
     dev = _require_gpu(x)
     H = x.shape[-1]
     x2, ldx = _rows2(x)
-    y = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    y = x.new_empty(x.shape, dtype=dtype)
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    st = _launch("mirl_quantize_rows", dev, x2.data_ptr(), _dtype_code(x), ldx, x.numel() // H, H, y.data_ptr(),
+    st = _launch("mirl_quantize_rows_int8" if dtype == torch.int8 else "mirl_quantize_rows", dev, x2.data_ptr(), _dtype_code(x), ldx, x.numel() // H, H, y.data_ptr(),
                  scale.data_ptr(), _stream(dev))
     _check(st, "mirl_quantize_rows")
     return y, scale
@@ -1805,34 +1817,55 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int) -> torch.Tensor:
     return y
 
 
-def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight8: torch.Tensor,
-                       weight_scale: torch.Tensor, bsz: int, target: torch.Tensor, vocab_start: int,
-                       vocab_end: int, out: torch.Tensor) -> None:
-    """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd).
-
-    hidden8 [T, >= H] and weight8 [V, H] e4m3 (H and row strides multiples of 16, or a contiguous weight with H a
-    multiple of 4; the hidden rows are zero past H,
-    up to a multiple of 256), scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
-    dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
-    T = hidden8.shape[0]
-    V, H = weight8.shape
-    _require(hidden8.dtype == torch.float8_e4m3fn and weight8.dtype == torch.float8_e4m3fn, "e4m3 operands")
+def _check_8bit(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight8: torch.Tensor, weight_scale: torch.Tensor) -> int:
+    """Checks 8-bit operands as the kernels read them; the weight's row stride."""
+    T, (V, H) = hidden8.shape[0], weight8.shape
+    _require(hidden8.dtype == weight8.dtype and hidden8.dtype in (torch.float8_e4m3fn, torch.int8), "e4m3 or int8 operands")
     _require(hidden8.stride(-1) == 1 and weight8.stride(-1) == 1 and hidden8.shape[1] == -(-H // 256) * 256,
              "hidden rows padded to 256 elements, with unit stride")
     _require(hidden_scale.is_contiguous() and hidden_scale.numel() == T and hidden_scale.dtype == torch.float32
              and weight_scale.is_contiguous() and weight_scale.numel() == V and weight_scale.dtype == torch.float32,
              "a contiguous fp32 scale per row")
+    return H if weight8.is_contiguous() else weight8.stride(0)
+
+
+def linear_ce_8bit_fwd(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight8: torch.Tensor,
+                       weight_scale: torch.Tensor, bsz: int, target: torch.Tensor, vocab_start: int,
+                       vocab_end: int, out: torch.Tensor) -> None:
+    """out[b, s] = log_softmax of row s * bsz + b of the 8-bit product (see mirl_linear_ce_8bit_fwd and
+    mirl_linear_ce_int8_fwd).
+
+    hidden8 [T, >= H] and weight8 [V, H] both e4m3 or both int8 (H and row strides multiples of 16, or a contiguous
+    weight with H a multiple of 4; the hidden rows are zero past H,
+    up to a multiple of 256), scales [T] and [V] fp32, target and out [bsz, T / bsz] int64 and fp32."""
+    dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, target, out)
+    T = hidden8.shape[0]
+    V, H = weight8.shape
+    ldw = _check_8bit(hidden8, hidden_scale, weight8, weight_scale)
     _require(target.dtype == torch.int64 and out.dtype == torch.float32
              and tuple(target.shape) == tuple(out.shape) == (bsz, T // bsz), "int64 targets and fp32 logprobs [B, S]")
     lib = _lib if _lib is not None else load()
     ws = torch.empty(max(1, int(lib.mirl_lce_x_workspace_elems(T, V))), dtype=torch.float32, device=dev)
+    name = "mirl_linear_ce_int8_fwd" if hidden8.dtype == torch.int8 else "mirl_linear_ce_8bit_fwd"
     st = _launch(
-        "mirl_linear_ce_8bit_fwd", dev, hidden8.data_ptr(), hidden_scale.data_ptr(), T, H, hidden8.stride(0),
-        weight8.data_ptr(), weight_scale.data_ptr(), V, H if weight8.is_contiguous() else weight8.stride(0), int(bsz), target.data_ptr(), target.stride(0),
+        name, dev, hidden8.data_ptr(), hidden_scale.data_ptr(), T, H, hidden8.stride(0),
+        weight8.data_ptr(), weight_scale.data_ptr(), V, ldw, int(bsz), target.data_ptr(), target.stride(0),
         target.stride(1), int(vocab_start), int(vocab_end), out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr(),
         _stream(dev),
     )
-    _check(st, "mirl_linear_ce_8bit_fwd")
+    _check(st, name)
+
+
+def int8_logits(hidden8: torch.Tensor, hidden_scale: torch.Tensor, weight8: torch.Tensor, weight_scale: torch.Tensor,
+                out: torch.Tensor) -> None:
+    """out [T, V] = the logits of int8 rows (see mirl_int8_logits), operands as for linear_ce_8bit_fwd."""
+    dev = _require_gpu(hidden8, hidden_scale, weight8, weight_scale, out)
+    V, H = weight8.shape
+    ldw = _check_8bit(hidden8, hidden_scale, weight8, weight_scale)
+    _require(hidden8.dtype == torch.int8 and tuple(out.shape) == (hidden8.shape[0], V) and out.stride(1) == 1, "int8 rows and logits [T, V]")
+    st = _launch("mirl_int8_logits", dev, hidden8.data_ptr(), hidden_scale.data_ptr(), hidden8.shape[0], H, hidden8.stride(0),
+                 weight8.data_ptr(), weight_scale.data_ptr(), V, ldw, out.data_ptr(), _dtype_code(out), out.stride(0), _stream(dev))
+    _check(st, "mirl_int8_logits")
 
 
 # ---------------------------------------------------------------------------

@@ -35,6 +35,7 @@ SOURCES = [
     "norm.hip",
     "dropout.hip",
     "linear_ce_8bit.hip",
+    "linear_ce_int8.hip",
     "linear_ce_adapters.hip",
     "processors.hip",
 ]

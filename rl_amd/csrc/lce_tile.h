@@ -15,6 +15,8 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // Operand dtype of the tile loop: its fragment (16 bytes of a row per lane), the
 // MFMA tile of kT x kT outputs and its accumulator.  run(w, h, c) forms
@@ -85,6 +87,22 @@ struct Mma<F8> {
   static constexpr int kT = 32;
   __device__ __forceinline__ static f32x16 run(frag w, frag h, f32x16 c) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, h, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+  }
+};
+
+// 8-bit integers: two v_mfma_i32_32x32x32_i8 (a lane's first 16 bytes, then the others), the rate of e4m3;
+// the sums are exact in 32 bits.
+struct I8 {
+  using raw = int8_t;
+};
+template <>
+struct Mma<I8> {
+  typedef int frag __attribute__((ext_vector_type(8)));
+  typedef i32x16 acc_t;
+  static constexpr int kT = 32;
+  __device__ __forceinline__ static i32x16 run(frag w, frag h, i32x16 c) {
+    c = __builtin_amdgcn_mfma_i32_32x32x32_i8(i32x4{w[0], w[1], w[2], w[3]}, i32x4{h[0], h[1], h[2], h[3]}, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(i32x4{w[4], w[5], w[6], w[7]}, i32x4{h[4], h[5], h[6], h[7]}, c, 0, 0, 0);
   }
 };
 
@@ -231,8 +249,9 @@ __device__ __forceinline__ auto u_f32(T* U, int64_t row, int r8) {
 }
 
 // kFwd, kGrad: logits rounded to the operand type.  kFwdX, kGradX: logits kept in fp32, with
-// adapters (16-bit operands) or row and column scales (e4m3, forward).
-enum LceMode { kFwd = 0, kGrad = 1, kGemm = 2, kFwdX = 3, kGradX = 4 };
+// adapters (16-bit operands) or row and column scales (8-bit ones, forward).  kLogits: the logits of 8-bit
+// operands, written out.
+enum LceMode { kFwd = 0, kGrad = 1, kGemm = 2, kFwdX = 3, kGradX = 4, kLogits = 5 };
 
 struct LceParams {
   const void* h;  // [T, Hd] of the kernel's E (bf16, fp16; fp32 for the plain GEMM), row stride ldh
@@ -288,12 +307,13 @@ struct LceParams {
   float g_scale;
   // kFwdX and kGradX: W's rows hold Hw elements (whole 16-byte chunks), H's Hd, zeros past Hw
   int64_t Hw;
-  // kFwdX of e4m3: logits = products * col_scale[col] * row_scale[row]
+  // kFwdX and kLogits of 8-bit operands: logits = products * col_scale[col] * row_scale[row], kLogits into C
+  // (fp32) or Cb
   const float* row_scale;
   const float* col_scale;
 };
 
-// RAGGED (kFwdX, kGradX): Hw is not a whole number of stage pairs.  What lies past a row of W is then
+// RAGGED (kFwdX, kGradX, kLogits): Hw is not a whole number of stage pairs.  What lies past a row of W is then
 // masked in the last two stages' loads: it is the next row's beginning, or no part of W, and an
 // infinity or a NaN there must not meet the zeros of H's rows.
 template <int MODE, class E, bool RAGGED = false>
@@ -304,8 +324,9 @@ void lce_tile_kernel(LceParams P) {
   constexpr int kT = Mma<E>::kT, kTM = kWM / kT, kTN = kWN / kT, kAV = kT * kT / kWave;
   constexpr int kKK = kRowBytes / (kWave / kT * (int)sizeof(frag));  // fragment steps (MFMA blocks) per stage
   constexpr int kES = (int)sizeof(typename E::raw);  // bytes per element
-  static_assert(MODE == kGemm ? kES != 1 : MODE == kFwdX ? kES <= 2 : kES == 2,
-                "fp32 operands: plain GEMM only; e4m3: forward only");
+  static_assert(MODE == kGemm ? kES != 1 : MODE == kFwdX ? kES <= 2 : MODE == kLogits ? kES == 1 : kES == 2,
+                "fp32 operands: plain GEMM only; 8-bit ones: forward and logits only");
+  constexpr bool kScales = (MODE == kFwdX || MODE == kLogits) && kES == 1;
   constexpr bool kIsGrad = MODE == kGrad || MODE == kGradX;
   constexpr bool kAdapters = (MODE == kFwdX || MODE == kGradX) && kES == 2;
   constexpr int kSKE = kRowBytes / kES;              // hidden elements per stage
@@ -314,7 +335,7 @@ void lce_tile_kernel(LceParams P) {
   __shared__ __align__(1024) unsigned char st0[kStageBytes];
   __shared__ __align__(1024) unsigned char st1[kStageBytes];
   __shared__ int s_tcol[kBM];
-  __shared__ __align__(16) float s_m[kBM], s_ls[kBM], s_g[kBM], s_rs[MODE == kFwdX && kES == 1 ? kBM : 1];
+  __shared__ __align__(16) float s_m[kBM], s_ls[kBM], s_g[kBM], s_rs[kScales ? kBM : 1];
   __shared__ int s_ord[kAdapters ? kBM : 1], s_seg[kAdapters ? kBM : 1], s_bad[kAdapters ? kBM : 1],
       s_heads[kWaves];
   constexpr bool kF16 = kAdapters && std::is_same<E, F16>::value;
@@ -384,7 +405,7 @@ void lce_tile_kernel(LceParams P) {
     const int64_t r = m0 + tid;
     int tc = -1;
     float lm = 0.f, ll = 0.f;
-    if (r < row_end) {
+    if (MODE != kLogits && r < row_end) {
       const int64_t s = r / P.bsz, b = r - s * P.bsz;
       const int64_t t = P.target[b * P.tsb + s * P.tss];
       const bool tmask = (t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V);
@@ -404,7 +425,7 @@ void lce_tile_kernel(LceParams P) {
       s_m[tid] = lm;
       s_ls[tid] = ll;
     }
-    if constexpr (MODE == kFwdX && kES == 1) {
+    if constexpr (kScales) {
       s_rs[tid] = r < row_end ? P.row_scale[r] : 0.f;
       s_ls[tid] = n0 + tid < P.V ? P.col_scale[n0 + tid] : 0.f;
     }
@@ -601,7 +622,7 @@ void lce_tile_kernel(LceParams P) {
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int v = 0; v < kAV; ++v) acc[i][j][v] = 0.f;
+        for (int v = 0; v < kAV; ++v) acc[i][j][v] = 0;
   };
   clear_acc();
   auto mfma = [&](int set, int q) __attribute__((always_inline)) {
@@ -1089,7 +1110,7 @@ void lce_tile_kernel(LceParams P) {
             c4[3] = cs.w;
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[j][4 * g + e] = kES == 1 ? acc[i][j][4 * g + e] * c4[e] : acc[i][j][4 * g + e];
+          for (int e = 0; e < 4; ++e) y[j][4 * g + e] = kES == 1 ? (float)acc[i][j][4 * g + e] * c4[e] : acc[i][j][4 * g + e];
         }
       if (negative) {
 #pragma unroll
@@ -1162,6 +1183,79 @@ void lce_tile_kernel(LceParams P) {
         float* dst = P.part + ((r - P.row0) * P.n_nt + nt) * 2;
         dst[0] = M;
         dst[1] = sum;
+      }
+    }
+  } else if constexpr (MODE == kLogits) {
+    // ---- the logits, written out ----
+    //
+    // 16-bit ones go through LDS (laid out as below), a row's 512 bytes by 32 threads; fp32 ones as each lane's
+    // four columns, 16 bytes.
+    wait_vm_barrier<0>();
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) asm volatile("" : "+a"(acc[i][j]));  // (as for kFwdX)
+    const int col_lane = lane / kT * 4;
+    auto each = [&](auto&& put) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kTM; ++i) {
+        const int rl = wm * kWM + i * kT + frow;
+        const float rs = s_rs[rl];
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int g = 0; g < kAV / 4; ++g) {
+            const int cl = wn * kWN + j * kT + g * 8 + col_lane;
+            const float4 cs = *reinterpret_cast<const float4*>(s_ls + cl);
+            const float c4[4] = {cs.x, cs.y, cs.z, cs.w};
+            f32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = ((float)acc[i][j][4 * g + e] * c4[e]) * rs;
+            put(rl, cl, o);
+          }
+      }
+    };
+    if (P.C != nullptr) {
+      const bool vec = (reinterpret_cast<uintptr_t>(P.C) & 15u) == 0 && P.ldc % 4 == 0;
+      each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
+        if (m0 + rl >= row_end) return;
+        float* dst = P.C + (m0 + rl) * P.ldc + n0 + cl;
+        if (vec && n0 + cl + 4 <= P.V) {
+          *reinterpret_cast<f32x4*>(dst) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + cl + e < P.V) dst[e] = o[e];
+        }
+      });
+      return;
+    }
+    uint16_t* const xq = reinterpret_cast<uint16_t*>(stage_ptr(wave_u >> 1));
+    if (P.cb_f16)
+      each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
+        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<F16>(o);
+      });
+    else
+      each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
+        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<BF16>(o);
+      });
+    __syncthreads();
+    const int c = tid & 31;
+    const int64_t col0 = n0 + c * 8;
+#pragma unroll 4
+    for (int k = 0; k < kBM / 8; ++k) {
+      const int rl = (tid >> 5) + 8 * k;
+      const int64_t r = m0 + rl;
+      if (r >= row_end || col0 >= P.V) continue;
+      const uint16_t* xs = reinterpret_cast<const uint16_t*>(stage_ptr(rl / kEpiRows));
+      const vu4 q = reinterpret_cast<const vu4*>(xs + (rl & (kEpiRows - 1)) * kBN)[c ^ xs_swizzle(rl)];
+      uint16_t* dst = P.Cb + r * P.ldcb + col0;
+      if (col0 + 8 <= P.V) {  // (at any multiple of 2 bytes)
+        *reinterpret_cast<Piece<2>::type*>(dst) = q;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col0 + e < P.V) dst[e] = (uint16_t)(q[e >> 1] >> ((e & 1) * 16));
       }
     }
   } else {
@@ -1334,7 +1428,7 @@ constexpr int kRStageBytes = (kRM + kRN) * kRowBytes;          // 24 KB: the H r
 constexpr int kRLoadsA = kRM / kDmaRows / kWaves, kRLoadsB = kRN / kDmaRows / kWaves;  // per wave and stage
 static_assert(kRLoadsB % 2 == 0 && kDmaPerWave % 2 == 0, "a load's parity among the wave's is that of its rows' eights");
 
-template <class E, bool RAGGED>
+template <class E, bool RAGGED, int MODE = kFwdX>
 __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
   using frag = typename Mma<E>::frag;
   using acc_t = typename Mma<E>::acc_t;
@@ -1371,11 +1465,13 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
     const int64_t r = m0 + lane;
     int tc = -1, a = -1, before = -1;
     if (lane < a_rows) {
-      const int64_t s = r / P.bsz, b = r - s * P.bsz;
-      const int64_t t = P.target[b * P.tsb + s * P.tss];
-      if (!((t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V))) {
-        const int64_t c = t - P.vs - n0;
-        if (c >= 0 && c < kRN) tc = (int)c;
+      if constexpr (MODE == kFwdX) {
+        const int64_t s = r / P.bsz, b = r - s * P.bsz;
+        const int64_t t = P.target[b * P.tsb + s * P.tss];
+        if (!((t < P.vs) || (t >= P.ve) || (t - P.vs >= P.V))) {
+          const int64_t c = t - P.vs - n0;
+          if (c >= 0 && c < kRN) tc = (int)c;
+        }
       }
       if constexpr (kAdapters) {
         a = P.aid[r];
@@ -1487,7 +1583,7 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
 #pragma unroll
     for (int j = 0; j < kTN; ++j)
 #pragma unroll
-      for (int v = 0; v < kAV; ++v) acc[i][j][v] = 0.f;
+      for (int v = 0; v < kAV; ++v) acc[i][j][v] = 0;
   auto fread = [&](const unsigned char* base, int kk) __attribute__((always_inline)) {
     if constexpr (kFC == 1) {
       return *reinterpret_cast<const frag*>(base + frag_off[kk]);
@@ -1585,20 +1681,61 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
 
   // ---- epilogue: the rows reduced in the registers, the four waves joined through LDS ----
   const int col_lane = lane / kT * 4;
+  if constexpr (MODE == kLogits) {  // the logits, written out: each lane four columns at a time
+    const bool vec = P.C != nullptr ? (reinterpret_cast<uintptr_t>(P.C) & 15u) == 0 && P.ldc % 4 == 0
+                                    : (reinterpret_cast<uintptr_t>(P.Cb) & 7u) == 0 && P.ldcb % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+      const int rl = i * kT + frow;
+      if (rl >= a_rows) continue;
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+#pragma unroll
+        for (int g = 0; g < kAV / 4; ++g) {
+          const int cl = wave * (kRN / kWaves) + j * kT + g * 8 + col_lane;
+          f32x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = ((float)acc[i][j][4 * g + e] * s_cs[kES == 1 ? cl + e : 0]) * s_rs[rl];
+          const bool whole = vec && cl + 4 <= b_rows;
+          if (P.C != nullptr) {
+            float* dst = P.C + (m0 + rl) * P.ldc + n0 + cl;
+            if (whole) {
+              *reinterpret_cast<f32x4*>(dst) = o;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (cl + e < b_rows) dst[e] = o[e];
+            }
+          } else {
+            uint16_t* dst = P.Cb + (m0 + rl) * P.ldcb + n0 + cl;
+            const uint2 w = P.cb_f16 ? pack4<F16>(o) : pack4<BF16>(o);
+            if (whole) {
+              *reinterpret_cast<uint2*>(dst) = w;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (cl + e < b_rows) dst[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
+            }
+          }
+        }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kTM; ++i) {
     const int rl = i * kT + frow, tc = s_tcol[rl] - wave * (kRN / kWaves);
+    float y[kTN][kAV];
     float M = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kTN; ++j)
 #pragma unroll
       for (int v = 0; v < kAV; ++v) {
         const int c = j * kT + v / 4 * 8 + col_lane + v % 4;
-        float x = acc[i][j][v];
+        float x = (float)acc[i][j][v];
         if constexpr (kES == 1) x = (x * s_cs[wave * (kRN / kWaves) + c]) * s_rs[rl];
         if (wave * (kRN / kWaves) + c >= b_rows) x = -INFINITY;
         if (c == tc) P.xt[m0 + rl] = x;
-        acc[i][j][v] = x;
+        y[j][v] = x;
         M = fmaxf(M, x);
       }
 #pragma unroll
@@ -1608,12 +1745,12 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int v = 0; v < kAV; ++v) sum += fast_exp2((acc[i][j][v] - M) * kLog2e);
+        for (int v = 0; v < kAV; ++v) sum += fast_exp2((y[j][v] - M) * kLog2e);
     } else {  // (see lce_tile_kernel)
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int v = 0; v < kAV; ++v) sum = acc[i][j][v] != acc[i][j][v] ? acc[i][j][v] : sum;
+        for (int v = 0; v < kAV; ++v) sum = y[j][v] != y[j][v] ? y[j][v] : sum;
     }
 #pragma unroll
     for (int off = kT; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
@@ -1710,23 +1847,25 @@ int64_t padded_hidden(int64_t Hw, int64_t bytes) {
 }
 
 // The forward kernel with fp32 logits for T rows (P.part, P.xt not set yet: `workspace` holds
-// mirl_lce_x_workspace_elems(T, V) floats).  Returns the number of tiles.
+// mirl_lce_x_workspace_elems(T, V) floats), or (kLogits, no workspace) the one that writes them.  Returns the number of tiles.
 // Rows up to which lce_rows_kernel is taken.  Whole calls over [151936, 4096], 64-row tiles
 // against 256-row ones, us: 64 rows 255 and 355 in bf16, 130 and 193 in e4m3; 128 rows 349 and
 // 365, 171 and 186; 192 rows 434 and 394, 215 and 192.
 constexpr int64_t kFewRows = 128;
-template <class E>
+template <class E, int MODE = kFwdX>
 int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
   const bool few = P.nrows <= kFewRows;
   P.n_mt = ceil_div(P.nrows, few ? kRM : kBM);
   P.n_nt = ceil_div(P.V, few ? kRN : kBN);
-  P.part = workspace;
-  P.xt = workspace + P.nrows * P.n_nt * 2;
+  if constexpr (MODE == kFwdX) {
+    P.part = workspace;
+    P.xt = workspace + P.nrows * P.n_nt * 2;
+  }
   const int64_t grid = ceil_div(P.n_mt * P.n_nt, kXcds) * kXcds;
   if (grid >= (int64_t(1) << 24)) return grid;  // a launch holds fewer than 2^32 threads
   const bool ragged = P.Hw != P.Hd;
-  const auto kernel = few ? ragged ? lce_rows_kernel<E, true> : lce_rows_kernel<E, false>
-                          : ragged ? lce_tile_kernel<kFwdX, E, true> : lce_tile_kernel<kFwdX, E, false>;
+  const auto kernel = few ? ragged ? lce_rows_kernel<E, true, MODE> : lce_rows_kernel<E, false, MODE>
+                          : ragged ? lce_tile_kernel<MODE, E, true> : lce_tile_kernel<MODE, E, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, P);
   return grid;
 }

@@ -3,7 +3,8 @@
 //
 //   h    = EH(x + res)                       the stream as it is stored (h = x without res)
 //   n    = h * rstd,  rstd = 1 / sqrt(mean(h^2) + eps)
-//   y    = EX(n * w)                         or, in 8 bits, e4m3(y * (1 / s)) with s = max|y| / 448
+//   y    = EX(n * w)                         or, in 8 bits, e4m3(y * (1 / s)) with s = max|y| / 448,
+//                                            or int8 of it, to the nearest, with s = max|y| / 127
 //   dh   = rstd * (w dy - n * mean(w dy n)) + dh_out,   dw = sum over rows of dy * n
 //
 // Every sum is fp32; y, h, dx, dres and dw are rounded once, to the types of the tensors that
@@ -99,11 +100,27 @@ __device__ __forceinline__ uint2 pack_e4m3(const float (&v)[kV]) {
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
   return uint2{(uint32_t)lo, (uint32_t)hi};
 }
+// Eight values of at most 127 to the nearest whole number (ties to the even one; NaN becomes 0).
+__device__ __forceinline__ uint2 pack_int8(const float (&v)[kV]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = (uint32_t)(int)rintf(v[4 * i + e]);
+    w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u),
+                                 0x05040100u);
+  }
+  return uint2{w[0], w[1]};
+}
 struct __attribute__((packed, aligned(1))) Bytes8 {
   uint32_t lo, hi;
 };
-__device__ __forceinline__ void store_e4m3(uint8_t* row, int64_t c, int64_t H, const float (&v)[kV]) {
-  const uint2 q = pack_e4m3(v);
+// What the rows become: the type of the input, or 8 bits with a scale.
+enum Out { kSame = 0, kE4m3 = 1, kInt8 = 2 };
+template <int OUT>
+__device__ __forceinline__ void store_8bit(uint8_t* row, int64_t c, int64_t H, const float (&v)[kV]) {
+  const uint2 q = OUT == kInt8 ? pack_int8(v) : pack_e4m3(v);
   if (c + kV <= H) {
     *reinterpret_cast<Bytes8*>(row + c) = Bytes8{q.x, q.y};
   } else {
@@ -113,15 +130,16 @@ __device__ __forceinline__ void store_e4m3(uint8_t* row, int64_t c, int64_t H, c
   }
 }
 
-constexpr float kE4m3Max = 448.f;
+constexpr float kE4m3Max = 448.f, kInt8Max = 127.f;
 constexpr uint32_t kAbs = 0x7fffffffu;
-// The scale of a row whose largest magnitude has these bits: amax / 448, not below the
+// The scale of a row whose largest magnitude has these bits: amax / 448 (int8: 127), not below the
 // smallest normal number (so that its reciprocal is finite), 1 for a row of zeros.  The
 // magnitudes are compared as integers: a NaN is then the largest and makes the row NaN.
+template <int OUT>
 __device__ __forceinline__ float row_scale(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits);
   if (amax_bits == 0) return 1.f;
-  const float s = amax / kE4m3Max;
+  const float s = amax / (OUT == kInt8 ? kInt8Max : kE4m3Max);
   return s < 0x1p-126f ? 0x1p-126f : s;
 }
 
@@ -182,7 +200,7 @@ struct NormFwd {
 
 // Rows of up to 64 * NW * kV * NV elements, in registers: NW waves a row (4 / NW rows a
 // workgroup where NW < 4).
-template <class EX, class EH, int NW, int NV, bool OUT8>
+template <class EX, class EH, int NW, int NV, int OUT>
 __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_fwd_kernel(NormFwd P) {
   constexpr int kRowsPerWg = NW < 4 ? 4 / NW : 1;
   static_assert(NW == 1 || NW >= 4, "one wave or the workgroup per row");
@@ -226,7 +244,7 @@ __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_fwd_kernel(NormFw
       load_weight<EX>(P.w, c, P.H, w);
 #pragma unroll
       for (int e = 0; e < kV; ++e) h[k][e] = (h[k][e] * rstd) * w[e];
-      if constexpr (OUT8) {
+      if constexpr (OUT != kSame) {
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
           // past the row's end h is 0 and w is 0; a NaN rstd must not reach those
@@ -237,9 +255,9 @@ __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_fwd_kernel(NormFw
         store8_to<EX>(static_cast<typename EX::raw*>(P.y) + r * P.H, c, P.H, h[k]);
       }
     }
-    if constexpr (OUT8) {
+    if constexpr (OUT != kSame) {
       amax = row_umax<NW>(amax, s);
-      const float sc = row_scale(amax), inv = 1.f / sc;
+      const float sc = row_scale<OUT>(amax), inv = 1.f / sc;
       if (t == 0) P.scale[r] = sc;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -247,7 +265,7 @@ __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_fwd_kernel(NormFw
         if (c >= P.H) continue;
 #pragma unroll
         for (int e = 0; e < kV; ++e) h[k][e] *= inv;
-        store_e4m3(static_cast<uint8_t*>(P.y) + r * P.H, c, P.H, h[k]);
+        store_8bit<OUT>(static_cast<uint8_t*>(P.y) + r * P.H, c, P.H, h[k]);
       }
     }
   }
@@ -257,7 +275,7 @@ __global__ __launch_bounds__(NW < 4 ? 256 : 64 * NW) void norm_fwd_kernel(NormFw
 // h), again for the output (from h, which this workgroup wrote: each thread reads what it
 // wrote itself), and for an 8-bit output once more.
 constexpr int kLongThreads = 1024;
-template <class EX, class EH, bool OUT8>
+template <class EX, class EH, int OUT>
 __global__ __launch_bounds__(kLongThreads) void norm_fwd_long_kernel(NormFwd P) {
   constexpr int NW = kLongThreads / kWave;
   __shared__ float s[NW];
@@ -293,7 +311,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_fwd_long_kernel(NormFwd P) 
       for (int e = 0; e < kV; ++e) y[e] = (y[e] * rstd) * w[e];
     };
     float inv = 1.f;
-    if constexpr (OUT8) {
+    if constexpr (OUT != kSame) {
       uint32_t amax = 0;
       for (int64_t c = (int64_t)threadIdx.x * kV; c < P.H; c += kLongThreads * kV) {
         float y[kV];
@@ -305,17 +323,17 @@ __global__ __launch_bounds__(kLongThreads) void norm_fwd_long_kernel(NormFwd P) 
         }
       }
       amax = row_umax<NW>(amax, s);
-      const float sc = row_scale(amax);
+      const float sc = row_scale<OUT>(amax);
       inv = 1.f / sc;
       if (threadIdx.x == 0) P.scale[r] = sc;
     }
     for (int64_t c = (int64_t)threadIdx.x * kV; c < P.H; c += kLongThreads * kV) {
       float y[kV];
       value(c, y);
-      if constexpr (OUT8) {
+      if constexpr (OUT != kSame) {
 #pragma unroll
         for (int e = 0; e < kV; ++e) y[e] *= inv;
-        store_e4m3(static_cast<uint8_t*>(P.y) + r * P.H, c, P.H, y);
+        store_8bit<OUT>(static_cast<uint8_t*>(P.y) + r * P.H, c, P.H, y);
       } else {
         store8_to<EX>(static_cast<typename EX::raw*>(P.y) + r * P.H, c, P.H, y);
       }
@@ -327,7 +345,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_fwd_long_kernel(NormFwd P) 
 // second time from the cache for rows of ordinary length).  [151936, 4096] bf16 499 us, once per
 // set of weights: 3.7 TB/s with each element read and written once, 6.4 being what streams reach;
 // a workgroup's second pass waits for the row's maximum.
-template <class EX>
+template <class EX, int OUT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename EX::raw* __restrict__ x, int64_t ldx,
                                                             int64_t R, int64_t H, uint8_t* __restrict__ y,
                                                             float* __restrict__ scale) {
@@ -345,14 +363,14 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const typename EX::r
       }
     }
     amax = row_umax<4>(amax, s);
-    const float sc = row_scale(amax), inv = 1.f / sc;
+    const float sc = row_scale<OUT>(amax), inv = 1.f / sc;
     if (threadIdx.x == 0) scale[r] = sc;
     for (int64_t c = (int64_t)threadIdx.x * kV; c < H; c += 256 * kV) {
       float v[kV];
       load8_to<EX>(xr, c, H, v);
 #pragma unroll
       for (int e = 0; e < kV; ++e) v[e] *= inv;
-      store_e4m3(y + r * H, c, H, v);
+      store_8bit<OUT>(y + r * H, c, H, v);
     }
   }
 }
@@ -644,9 +662,11 @@ unsigned row_grid(int64_t n) { return (unsigned)(n < kMaxGrid ? n : kMaxGrid); }
 
 using namespace mirl;
 
-extern "C" int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* residual, int res_dtype,
-                                     int64_t ldr, const void* weight, int w_dtype, int64_t R, int64_t H, double eps,
-                                     void* h, void* y, float* y_scale, float* rstd, void* stream) {
+namespace mirl {
+namespace {
+int norm_fwd(int out, const void* x, int x_dtype, int64_t ldx, const void* residual, int res_dtype, int64_t ldr,
+             const void* weight, int w_dtype, int64_t R, int64_t H, double eps, void* h, void* y, float* y_scale,
+             float* rstd, void* stream) {
   clear_error();
   MIRL_REQUIRE(R >= 0 && H > 0 && R < kMaxSide && H < kMaxWidth, "invalid shape R=%lld H=%lld", (long long)R, (long long)H);
   MIRL_REQUIRE(eps >= 0, "eps %g is negative", eps);
@@ -663,22 +683,42 @@ extern "C" int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, co
     hipStream_t st = static_cast<hipStream_t>(stream);
     return with_layout(H, [&](auto layout) -> int {
       using L = decltype(layout);
-      if constexpr (L::kNW == 0) {
-        if (y_scale != nullptr)
-          hipLaunchKernelGGL((norm_fwd_long_kernel<EX, EH, true>), dim3(row_grid(R)), dim3(kLongThreads), 0, st, P);
-        else
-          hipLaunchKernelGGL((norm_fwd_long_kernel<EX, EH, false>), dim3(row_grid(R)), dim3(kLongThreads), 0, st, P);
-      } else {
-        constexpr int per = L::kNW == 1 ? 4 : 1;
-        const dim3 grid(row_grid(ceil_div(R, per))), block(L::kNW == 1 ? 256 : 64 * L::kNW);
-        if (y_scale != nullptr)
-          hipLaunchKernelGGL((norm_fwd_kernel<EX, EH, L::kNW, L::kNV, true>), grid, block, 0, st, P);
-        else
-          hipLaunchKernelGGL((norm_fwd_kernel<EX, EH, L::kNW, L::kNV, false>), grid, block, 0, st, P);
-      }
+      auto go = [&](auto out_c) {
+        constexpr int OUT = decltype(out_c)::value;
+        if constexpr (L::kNW == 0) {
+          hipLaunchKernelGGL((norm_fwd_long_kernel<EX, EH, OUT>), dim3(row_grid(R)), dim3(kLongThreads), 0, st, P);
+        } else {
+          constexpr int per = L::kNW == 1 ? 4 : 1;
+          hipLaunchKernelGGL((norm_fwd_kernel<EX, EH, L::kNW, L::kNV, OUT>), dim3(row_grid(ceil_div(R, per))),
+                             dim3(L::kNW == 1 ? 256 : 64 * L::kNW), 0, st, P);
+        }
+      };
+      if (out == kInt8)
+        go(std::integral_constant<int, kInt8>{});
+      else if (out == kE4m3)
+        go(std::integral_constant<int, kE4m3>{});
+      else
+        go(std::integral_constant<int, kSame>{});
       return check_launch("mirl_add_rms_norm_fwd");
     });
   });
+}
+}  // namespace
+}  // namespace mirl
+
+extern "C" int mirl_add_rms_norm_fwd(const void* x, int x_dtype, int64_t ldx, const void* residual, int res_dtype,
+                                     int64_t ldr, const void* weight, int w_dtype, int64_t R, int64_t H, double eps,
+                                     void* h, void* y, float* y_scale, float* rstd, void* stream) {
+  return norm_fwd(y_scale != nullptr ? kE4m3 : kSame, x, x_dtype, ldx, residual, res_dtype, ldr, weight, w_dtype, R, H, eps,
+                  h, y, y_scale, rstd, stream);
+}
+
+extern "C" int mirl_add_rms_norm_int8_fwd(const void* x, int x_dtype, int64_t ldx, const void* residual, int res_dtype,
+                                          int64_t ldr, const void* weight, int w_dtype, int64_t R, int64_t H, double eps,
+                                          void* h, int8_t* y, float* y_scale, void* stream) {
+  clear_error();
+  MIRL_REQUIRE(R <= 0 || y_scale != nullptr, "null pointer argument");
+  return norm_fwd(kInt8, x, x_dtype, ldx, residual, res_dtype, ldr, weight, w_dtype, R, H, eps, h, y, y_scale, nullptr, stream);
 }
 
 extern "C" int64_t mirl_add_rms_norm_bwd_workspace_elems(int64_t R, int64_t H) {
@@ -743,8 +783,10 @@ extern "C" int mirl_add_rms_norm_bwd(const void* dy, int x_dtype, int64_t lddy, 
   });
 }
 
-extern "C" int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, void* y, float* scale,
-                                  void* stream) {
+namespace mirl {
+namespace {
+template <int OUT>
+int quantize(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, void* y, float* scale, void* stream) {
   clear_error();
   MIRL_REQUIRE(R >= 0 && H > 0 && R < kMaxSide && H < kMaxWidth, "invalid shape R=%lld H=%lld", (long long)R, (long long)H);
   return with_types(dtype, dtype, [&](auto ex, auto) -> int {
@@ -752,8 +794,20 @@ extern "C" int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t
     if (R == 0) return MIRL_OK;
     MIRL_REQUIRE(x && y && scale, "null pointer argument");
     MIRL_REQUIRE(R == 1 || ldx >= H, "row stride %lld is below H=%lld", (long long)ldx, (long long)H);
-    hipLaunchKernelGGL(quantize_rows_kernel<EX>, dim3(row_grid(R)), dim3(256), 0, static_cast<hipStream_t>(stream),
+    hipLaunchKernelGGL((quantize_rows_kernel<EX, OUT>), dim3(row_grid(R)), dim3(256), 0, static_cast<hipStream_t>(stream),
                        static_cast<const typename EX::raw*>(x), ldx, R, H, static_cast<uint8_t*>(y), scale);
     return check_launch("mirl_quantize_rows");
   });
+}
+}  // namespace
+}  // namespace mirl
+
+extern "C" int mirl_quantize_rows(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, void* y, float* scale,
+                                  void* stream) {
+  return quantize<kE4m3>(x, dtype, ldx, R, H, y, scale, stream);
+}
+
+extern "C" int mirl_quantize_rows_int8(const void* x, int dtype, int64_t ldx, int64_t R, int64_t H, int8_t* y, float* scale,
+                                       void* stream) {
+  return quantize<kInt8>(x, dtype, ldx, R, H, y, scale, stream);
 }

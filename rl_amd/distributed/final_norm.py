@@ -2,8 +2,8 @@
 
 What a policy does with its residual stream before the hidden-state logprobs
 (:mod:`rl_amd.distributed.linear_ce`): ``h = x + residual``, ``y = h / rms(h) * weight``.
-:func:`add_rms_norm` is differentiable; :func:`add_rms_norm_8bit` writes the rows in e4m3
-with one scale each, as :func:`~rl_amd.distributed.linear_ce_8bit.from_parallel_8bit_hidden_states_to_logprobs`
+:func:`add_rms_norm` is differentiable; :func:`add_rms_norm_8bit` writes the rows in e4m3 or in
+8-bit integers with one scale each, as :func:`~rl_amd.distributed.linear_ce_8bit.from_parallel_8bit_hidden_states_to_logprobs`
 reads them, for passes that need no gradient (the previous or the reference policy's
 logprobs); :func:`quantize_rows_8bit` does the same to an output weight, once.
 
@@ -25,6 +25,7 @@ from rl_amd import _C
 __all__ = ["add_rms_norm", "add_rms_norm_8bit", "quantize_rows_8bit", "rms_norm"]
 
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_8BIT_DTYPES = (torch.float8_e4m3fn, torch.int8)
 
 
 def _check(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float) -> None:
@@ -52,7 +53,7 @@ class _AddRmsNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, x, residual, weight, eps):  # type: ignore[override]
-        y, h, rstd, _ = _C.add_rms_norm_fwd(x, residual, weight, eps, True, False)
+        y, h, rstd, _ = _C.add_rms_norm_fwd(x, residual, weight, eps, True, None)
         ctx.save_for_backward(h, rstd, weight)
         ctx.set_materialize_grads(False)
         ctx.x_dtype = x.dtype
@@ -80,7 +81,7 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, x, weight, eps):  # type: ignore[override]
-        y, _, rstd, _ = _C.add_rms_norm_fwd(x, None, weight, eps, True, False)
+        y, _, rstd, _ = _C.add_rms_norm_fwd(x, None, weight, eps, True, None)
         ctx.save_for_backward(x, rstd, weight)
         return y
 
@@ -108,25 +109,30 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
 
 
 def add_rms_norm_8bit(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
-                      eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``(y8, scale, h)``: as :func:`add_rms_norm`, with ``y`` in e4m3 (``float8_e4m3fn``) and one
+                      eps: float = 1e-6, dtype: torch.dtype = torch.float8_e4m3fn
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(y8, scale, h)``: as :func:`add_rms_norm`, with ``y`` in e4m3 (``float8_e4m3fn``) or ``int8`` and one
     fp32 scale per row, ``y = y8 * scale``, rounded from the fp32 ``y``.  ``residual`` may be None
     (``h`` is then ``x``).  No gradient passes through: inputs that ask for one are refused
     unless gradients are off."""
     _check(x, residual, weight, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         raise RuntimeError("an 8-bit norm has no gradient: call it under torch.no_grad() or use add_rms_norm")
-    y8, h, _, scale = _C.add_rms_norm_fwd(x, residual, weight, eps, False, True)
+    if dtype not in _8BIT_DTYPES:
+        raise TypeError(f"8-bit rows are float8_e4m3fn or int8, got {dtype}")
+    y8, h, _, scale = _C.add_rms_norm_fwd(x, residual, weight, eps, False, dtype)
     return y8, scale, h
 
 
-def quantize_rows_8bit(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(x8, scale)``: rows ``[..., H]`` in e4m3 with one fp32 scale each, ``x = x8 * scale``:
-    ``scale = max|x| / 448``.  For an output weight, once per set of weights."""
+def quantize_rows_8bit(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(x8, scale)``: rows ``[..., H]`` in e4m3 or ``int8`` with one fp32 scale each, ``x = x8 * scale``:
+    ``scale = max|x| / 448`` (int8: 127).  For an output weight, once per set of weights."""
+    if dtype not in _8BIT_DTYPES:
+        raise TypeError(f"8-bit rows are float8_e4m3fn or int8, got {dtype}")
     if x.dtype not in _ROW_DTYPES:
         raise TypeError(f"8-bit rows are made of fp32, bf16 or fp16, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"expected rows [..., H], got {tuple(x.shape)}")
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("8-bit rows have no gradient: call this under torch.no_grad()")
-    return _C.quantize_rows(x)
+    return _C.quantize_rows(x, dtype)

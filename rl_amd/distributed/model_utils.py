@@ -45,6 +45,7 @@ __all__ = [
     "distributed_vocab_topk",
     "DistributedLogprobWithSampling",
     "dropout",
+    "from_int8_hidden_states_to_logits",
     "from_parallel_8bit_hidden_states_to_logprobs",
     "from_parallel_hidden_states_to_logprobs",
     "from_parallel_hidden_states_to_logprobs_with_adapters",
@@ -88,7 +89,7 @@ def __getattr__(name: str):
         from rl_amd.distributed import final_norm
 
         return getattr(final_norm, name)
-    if name == "from_parallel_8bit_hidden_states_to_logprobs":
+    if name in ("from_int8_hidden_states_to_logits", "from_parallel_8bit_hidden_states_to_logprobs"):
         from rl_amd.distributed import linear_ce_8bit
 
         return getattr(linear_ce_8bit, name)
