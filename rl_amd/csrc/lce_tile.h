@@ -16,7 +16,6 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // Operand dtype of the tile loop: its fragment (16 bytes of a row per lane), the
 // MFMA tile of kT x kT outputs and its accumulator.  run(w, h, c) forms
@@ -90,19 +89,18 @@ struct Mma<F8> {
   }
 };
 
-// 8-bit integers: two v_mfma_i32_32x32x32_i8 (a lane's first 16 bytes, then the others), the rate of e4m3;
-// the sums are exact in 32 bits.
+// 8-bit integers: v_mfma_i32_16x16x64_i8, the rate of e4m3; a fragment is 16 bytes of a row per lane, the
+// accumulator is laid out as for 16-bit operands and its sums are exact in 32 bits.
 struct I8 {
   using raw = int8_t;
 };
 template <>
 struct Mma<I8> {
-  typedef int frag __attribute__((ext_vector_type(8)));
-  typedef i32x16 acc_t;
-  static constexpr int kT = 32;
-  __device__ __forceinline__ static i32x16 run(frag w, frag h, i32x16 c) {
-    c = __builtin_amdgcn_mfma_i32_32x32x32_i8(i32x4{w[0], w[1], w[2], w[3]}, i32x4{h[0], h[1], h[2], h[3]}, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_i32_32x32x32_i8(i32x4{w[4], w[5], w[6], w[7]}, i32x4{h[4], h[5], h[6], h[7]}, c, 0, 0, 0);
+  typedef i32x4 frag;
+  typedef i32x4 acc_t;
+  static constexpr int kT = 16;
+  __device__ __forceinline__ static i32x4 run(frag w, frag h, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, h, c, 0, 0, 0);
   }
 };
 
@@ -316,7 +314,8 @@ struct LceParams {
 // RAGGED (kFwdX, kGradX, kLogits): Hw is not a whole number of stage pairs.  What lies past a row of W is then
 // masked in the last two stages' loads: it is the next row's beginning, or no part of W, and an
 // infinity or a NaN there must not meet the zeros of H's rows.
-template <int MODE, class E, bool RAGGED = false>
+// EO (kLogits): the logits' type.
+template <int MODE, class E, bool RAGGED = false, class EO = BF16>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void lce_tile_kernel(LceParams P) {
   using frag = typename Mma<E>::frag;
@@ -783,6 +782,7 @@ void lce_tile_kernel(LceParams P) {
     for (int idx = 0; idx < kTM + kTN; ++idx) fread(0, st0, 0, idx);
     int t = 0;
     for (; t < nst - (RAGGED ? 2 : 1) * kStages; t += kStages) {
+      if constexpr (MODE == kLogits && !RAGGED) keep_acc();  // (or 56 of them are moved in every pass)
       step(t, S0{}, T_{}, T_{});
       step(t + 1, S1{}, T_{}, T_{});
     }
@@ -1195,11 +1195,14 @@ void lce_tile_kernel(LceParams P) {
     for (int i = 0; i < kTM; ++i)
 #pragma unroll
       for (int j = 0; j < kTN; ++j) asm volatile("" : "+a"(acc[i][j]));  // (as for kFwdX)
-    const int col_lane = lane / kT * 4;
+    __builtin_amdgcn_sched_barrier(0);
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (see prepare)
+    const int col_lane = ln / kT * 4, row_lane = ln & (kT - 1);
     auto each = [&](auto&& put) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kTM; ++i) {
-        const int rl = wm * kWM + i * kT + frow;
+        const int rl = wm * kWM + i * kT + row_lane;
         const float rs = s_rs[rl];
 #pragma unroll
         for (int j = 0; j < kTN; ++j)
@@ -1213,9 +1216,10 @@ void lce_tile_kernel(LceParams P) {
             for (int e = 0; e < 4; ++e) o[e] = ((float)acc[i][j][4 * g + e] * c4[e]) * rs;
             put(rl, cl, o);
           }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    if (P.C != nullptr) {
+    if constexpr (std::is_same<EO, F32>::value) {
       const bool vec = (reinterpret_cast<uintptr_t>(P.C) & 15u) == 0 && P.ldc % 4 == 0;
       each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
         if (m0 + rl >= row_end) return;
@@ -1228,34 +1232,43 @@ void lce_tile_kernel(LceParams P) {
             if (n0 + cl + e < P.V) dst[e] = o[e];
         }
       });
-      return;
-    }
-    uint16_t* const xq = reinterpret_cast<uint16_t*>(stage_ptr(wave_u >> 1));
-    if (P.cb_f16)
+    } else {
+      uint16_t* const xq = reinterpret_cast<uint16_t*>(stage_ptr(wave_u >> 1));
       each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
-        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<F16>(o);
+        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<EO>(o);
       });
-    else
-      each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
-        *reinterpret_cast<uint2*>(xq + xs_index(rl, cl)) = pack4<BF16>(o);
-      });
-    __syncthreads();
-    const int c = tid & 31;
-    const int64_t col0 = n0 + c * 8;
-#pragma unroll 4
-    for (int k = 0; k < kBM / 8; ++k) {
-      const int rl = (tid >> 5) + 8 * k;
-      const int64_t r = m0 + rl;
-      if (r >= row_end || col0 >= P.V) continue;
-      const uint16_t* xs = reinterpret_cast<const uint16_t*>(stage_ptr(rl / kEpiRows));
-      const vu4 q = reinterpret_cast<const vu4*>(xs + (rl & (kEpiRows - 1)) * kBN)[c ^ xs_swizzle(rl)];
-      uint16_t* dst = P.Cb + r * P.ldcb + col0;
-      if (col0 + 8 <= P.V) {  // (at any multiple of 2 bytes)
-        *reinterpret_cast<Piece<2>::type*>(dst) = q;
-      } else {
+      __syncthreads();
+      const int c = ln & 31, r0 = wave * 2 + (ln >> 5);  // row r0 + 8 k, chunk c
+      auto chunk = [&](int k) __attribute__((always_inline)) {
+        const int rl = r0 + 8 * k;
+        const uint16_t* xs = reinterpret_cast<const uint16_t*>(stage_ptr(k / (kEpiRows / 8)));
+        return reinterpret_cast<const vu4*>(xs + (rl & (kEpiRows - 1)) * kBN)[c ^ xs_swizzle(rl)];
+      };
+      uint16_t* dst = P.Cb + (m0 + r0) * P.ldcb + n0 + c * 8;
+      if (m0 + kBM <= row_end && n0 + kBN <= P.V) {
+        // eight rows' pieces in flight (at any multiple of 2 bytes)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col0 + e < P.V) dst[e] = (uint16_t)(q[e >> 1] >> ((e & 1) * 16));
+        for (int k = 0; k < kBM / 8; k += 8) {
+          vu4 q[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[i] = chunk(k + i);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            __builtin_nontemporal_store((Piece<2>::type)q[i], reinterpret_cast<Piece<2>::type*>(dst + (k + i) * 8 * P.ldcb));
+        }
+      } else {
+        const int64_t left = P.V - n0 - c * 8;
+        for (int k = 0; k < kBM / 8; ++k, dst += 8 * P.ldcb) {
+          if (m0 + r0 + 8 * k >= row_end) break;
+          const vu4 q = chunk(k);
+          if (left >= 8) {
+            *reinterpret_cast<Piece<2>::type*>(dst) = q;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e < left) dst[e] = (uint16_t)(q[e >> 1] >> ((e & 1) * 16));
+          }
+        }
       }
     }
   } else {
@@ -1681,43 +1694,58 @@ __global__ __launch_bounds__(kThreads, 2) void lce_rows_kernel(LceParams P) {
 
   // ---- epilogue: the rows reduced in the registers, the four waves joined through LDS ----
   const int col_lane = lane / kT * 4;
-  if constexpr (MODE == kLogits) {  // the logits, written out: each lane four columns at a time
-    const bool vec = P.C != nullptr ? (reinterpret_cast<uintptr_t>(P.C) & 15u) == 0 && P.ldc % 4 == 0
-                                    : (reinterpret_cast<uintptr_t>(P.Cb) & 7u) == 0 && P.ldcb % 4 == 0;
+  if constexpr (MODE == kLogits) {
+    // The logits, written out: 16-bit ones through the first stage array (rows of 256 bytes, 16-byte chunks
+    // XOR-ed with the row), a row by 16 threads; fp32 ones as each lane's four columns.
+    auto each = [&](auto&& put) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kTM; ++i) {
-      const int rl = i * kT + frow;
-      if (rl >= a_rows) continue;
+      for (int i = 0; i < kTM; ++i) {
+        const int rl = i * kT + frow;
 #pragma unroll
-      for (int j = 0; j < kTN; ++j)
+        for (int j = 0; j < kTN; ++j)
 #pragma unroll
-        for (int g = 0; g < kAV / 4; ++g) {
-          const int cl = wave * (kRN / kWaves) + j * kT + g * 8 + col_lane;
-          f32x4 o;
+          for (int g = 0; g < kAV / 4; ++g) {
+            const int cl = wave * (kRN / kWaves) + j * kT + g * 8 + col_lane;
+            f32x4 o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = ((float)acc[i][j][4 * g + e] * s_cs[kES == 1 ? cl + e : 0]) * s_rs[rl];
-          const bool whole = vec && cl + 4 <= b_rows;
-          if (P.C != nullptr) {
-            float* dst = P.C + (m0 + rl) * P.ldc + n0 + cl;
-            if (whole) {
-              *reinterpret_cast<f32x4*>(dst) = o;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (cl + e < b_rows) dst[e] = o[e];
-            }
-          } else {
-            uint16_t* dst = P.Cb + (m0 + rl) * P.ldcb + n0 + cl;
-            const uint2 w = P.cb_f16 ? pack4<F16>(o) : pack4<BF16>(o);
-            if (whole) {
-              *reinterpret_cast<uint2*>(dst) = w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (cl + e < b_rows) dst[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
-            }
+            for (int e = 0; e < 4; ++e) o[e] = ((float)acc[i][j][4 * g + e] * s_cs[kES == 1 ? cl + e : 0]) * s_rs[rl];
+            put(rl, cl, o);
           }
+      }
+    };
+    if (P.C != nullptr) {
+      const bool vec = (reinterpret_cast<uintptr_t>(P.C) & 15u) == 0 && P.ldc % 4 == 0;
+      each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
+        if (rl >= a_rows) return;
+        float* dst = P.C + (m0 + rl) * P.ldc + n0 + cl;
+        if (vec && cl + 4 <= b_rows) {
+          *reinterpret_cast<f32x4*>(dst) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (cl + e < b_rows) dst[e] = o[e];
         }
+      });
+      return;
+    }
+    __syncthreads();  // (every wave's last fragments are read)
+    auto place = [](int rl, int c) { return (rl * (kRN / 8) + (c ^ (rl & 15))) * 16; };  // chunk c of row rl, bytes
+    static_assert(kRN / 8 == 16 && kRM * kRN * 2 <= kRStageBytes, "the tile fits the stage array");
+    each([&](int rl, int cl, f32x4 o) __attribute__((always_inline)) {
+      *reinterpret_cast<uint2*>(st0 + place(rl, cl / 8) + cl % 8 * 2) = P.cb_f16 ? pack4<F16>(o) : pack4<BF16>(o);
+    });
+    __syncthreads();
+    const int c = tid & 15;
+    for (int rl = tid >> 4; rl < a_rows; rl += kThreads / 16) {
+      const vu4 q = *reinterpret_cast<const vu4*>(st0 + place(rl, c));
+      uint16_t* dst = P.Cb + (m0 + rl) * P.ldcb + n0 + c * 8;
+      if (c * 8 + 8 <= b_rows) {  // (at any multiple of 2 bytes)
+        __builtin_nontemporal_store((Piece<2>::type)q, reinterpret_cast<Piece<2>::type*>(dst));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c * 8 + e < b_rows) dst[e] = (uint16_t)(q[e >> 1] >> ((e & 1) * 16));
+      }
     }
     return;
   }
@@ -1852,7 +1880,7 @@ int64_t padded_hidden(int64_t Hw, int64_t bytes) {
 // against 256-row ones, us: 64 rows 255 and 355 in bf16, 130 and 193 in e4m3; 128 rows 349 and
 // 365, 171 and 186; 192 rows 434 and 394, 215 and 192.
 constexpr int64_t kFewRows = 128;
-template <class E, int MODE = kFwdX>
+template <class E, int MODE = kFwdX, class EO = BF16>
 int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
   const bool few = P.nrows <= kFewRows;
   P.n_mt = ceil_div(P.nrows, few ? kRM : kBM);
@@ -1865,7 +1893,7 @@ int64_t launch_fwd_x(LceParams& P, float* workspace, hipStream_t st) {
   if (grid >= (int64_t(1) << 24)) return grid;  // a launch holds fewer than 2^32 threads
   const bool ragged = P.Hw != P.Hd;
   const auto kernel = few ? ragged ? lce_rows_kernel<E, true, MODE> : lce_rows_kernel<E, false, MODE>
-                          : ragged ? lce_tile_kernel<MODE, E, true> : lce_tile_kernel<MODE, E, false>;
+                          : ragged ? lce_tile_kernel<MODE, E, true, EO> : lce_tile_kernel<MODE, E, false, EO>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, st, P);
   return grid;
 }

@@ -107,7 +107,10 @@ extern "C" int mirl_int8_logits(const int8_t* hidden8, const float* hidden_scale
     P.cb_f16 = out_dtype == MIRL_DTYPE_F16;
     P.ldcb = ldo;
   }
-  const int64_t tiles = launch_fwd_x<I8, kLogits>(P, nullptr, static_cast<hipStream_t>(stream));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t tiles = out_dtype == MIRL_DTYPE_F32    ? launch_fwd_x<I8, kLogits, F32>(P, nullptr, st)
+                        : out_dtype == MIRL_DTYPE_BF16 ? launch_fwd_x<I8, kLogits, BF16>(P, nullptr, st)
+                                                       : launch_fwd_x<I8, kLogits, F16>(P, nullptr, st);
   MIRL_REQUIRE(tiles < (int64_t(1) << 24), "too many tiles");
   return check_launch("mirl_int8_logits");
 }
