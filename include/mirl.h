@@ -1046,14 +1046,9 @@ typedef struct mirl_logit_processors {
   float repetition_all, presence_all, frequency_all, temperature_all;
 } mirl_logit_processors;
 
-/*
- * The samples' tokens and biases sorted by column, for calls with R rows of V columns and the
- * same `processors` (a backward takes its forward's): table holds
- * mirl_logit_processors_table_elems(B, V, n_ids, n_bias) words.
- */
+/* The size of `table`, in words: a forward leaves there what its backward reads again (with the
+ * same processors). */
 int64_t mirl_logit_processors_table_elems(int64_t B, int64_t V, int64_t n_ids, int64_t n_bias);
-int mirl_logit_processors_table(const mirl_logit_processors* processors, int64_t B, int64_t R,
-                                int64_t V, uint32_t* table, void* stream);
 
 /*
  * out[b, r] ([B, R] contiguous) = log_softmax(y[b, r]) at the token behind row r, ids[b, n]:
@@ -1065,7 +1060,7 @@ int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V);
 int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                                int64_t stride_b, int64_t stride_r,
                                const mirl_logit_processors* processors,
-                               const uint32_t* table, float* out,
+                               uint32_t* table, float* out,
                                float* stats, float* workspace, void* stream);
 
 /*
@@ -1090,7 +1085,7 @@ int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t
 int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                         int64_t stride_b, int64_t stride_r,
                         const mirl_logit_processors* processors,
-                               const uint32_t* table, void* out,
+                               uint32_t* table, void* out,
                         int64_t o_stride_b, int64_t o_stride_r, void* stream);
 int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                             int64_t stride_b, int64_t stride_r,

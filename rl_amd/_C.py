@@ -340,7 +340,6 @@ SIGNATURES = {
     ),
     "mirl_processed_logprob_workspace_elems": (_I64, [_I64, _I64, _I64]),
     "mirl_logit_processors_table_elems": (_I64, [_I64] * 4),
-    "mirl_logit_processors_table": (_I, [_P, _I64, _I64, _I64, _P, _P]),
     "mirl_processed_logprob_fwd": (_I, [_P, _I] + [_I64] * 5 + [_P] * 6),
     "mirl_processed_logprob_bwd": (
         _I, [_P, _I] + [_I64] * 6 + [_P] * 4 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
@@ -1257,54 +1256,68 @@ def top_k_top_p_mask(x2d: torch.Tensor, top_k: int, top_p: float,
 # ---------------------------------------------------------------------------
 # penalties, biases and grammar masks on logits
 # ---------------------------------------------------------------------------
-def processor_args(ids: torch.Tensor, tensors: dict, scalars: dict, vocab: tuple) -> LogitProcessorArgs:
-    """The C struct of one call.  ``ids`` [B, n_ids] int64; ``tensors``: lengths and prompt_lengths
-    [B] int64, repetition, presence, frequency and temperature [B] fp32, bias_ids and bias [K] or [B, K]
-    (int64, fp32), masks [M, W] int32, mask_rows [B, R] int64, each contiguous in its last dimension or
-    None; ``scalars``: the value of each of the four that is None; ``vocab``: (start, end).  Sizes are
-    the caller's to check."""
-    A = LogitProcessorArgs()
-    A.ids, A.n_ids, A.ids_stride_b, A.ids_stride_s = ids.data_ptr(), ids.shape[1], ids.stride(0), ids.stride(1)
-    for name in ("lengths", "prompt_lengths", "repetition", "presence", "frequency", "temperature", "bias_ids", "bias", "masks", "mask_rows"):
-        t = tensors.get(name)
-        if t is not None:
-            setattr(A, name, t.data_ptr())
-    for name, value in scalars.items():
-        setattr(A, name + "_all", value)
-    bias = tensors.get("bias")
+_PROCESSOR_TENSORS = ("lengths", "prompt_lengths", "repetition", "presence", "frequency", "temperature", "bias_ids", "bias", "masks",
+                      "mask_rows")
+
+
+def processor_args(ids: torch.Tensor, tensors: tuple, scalars: tuple, vocab: tuple) -> LogitProcessorArgs:
+    """The C struct of one call.  ``ids`` [B, n_ids] int64; ``tensors`` in the order of _PROCESSOR_TENSORS: lengths
+    and prompt_lengths [B] int64, repetition, presence, frequency and temperature [B] fp32, bias_ids and bias [K]
+    or [B, K] (int64, fp32), masks [M, W] int32, mask_rows [B, R] int64, contiguous (masks: in the last
+    dimension; mask_rows: by strides), or None; ``scalars``: the value of each of the four that is None;
+    ``vocab``: (start, end).  Sizes are the caller's to check."""
+    bias, masks, rows = tensors[7], tensors[8], tensors[9]
+    n_bias = n_masks = bias_sb = mask_stride = rows_sb = rows_sr = 0
     if bias is not None:
-        A.n_bias, A.bias_stride_b = bias.shape[-1], bias.shape[-1] if bias.dim() == 2 else 0
-    masks, rows = tensors.get("masks"), tensors.get("mask_rows")
+        n_bias = bias.shape[-1]
+        bias_sb = n_bias if bias.dim() == 2 else 0
     if masks is not None:
-        A.n_masks, A.mask_stride = masks.shape[0], masks.stride(0)
-        A.mask_rows_stride_b, A.mask_rows_stride_r = rows.stride(0), rows.stride(1)
-    A.vocab_start, A.vocab_end = vocab
-    return A
+        n_masks, mask_stride = masks.shape[0], masks.stride(0)
+        rows_sb, rows_sr = rows.stride()
+    p = [None if t is None else t.data_ptr() for t in tensors]
+    sb, ss = ids.stride()
+    return LogitProcessorArgs(ids.data_ptr(), ids.shape[1], sb, ss, *p[:8], n_bias, bias_sb, p[8], n_masks, mask_stride, p[9],
+                              rows_sb, rows_sr, vocab[0], vocab[1], *scalars)
 
 
-def processor_table(logits: torch.Tensor, R: int, args: LogitProcessorArgs) -> torch.Tensor:
-    """The samples' tokens and biases by column, for the calls below (see mirl_logit_processors_table)."""
-    dev = logits.device
-    B, V = logits.shape[0], logits.shape[2]
-    lib = _lib if _lib is not None else load()
-    table = torch.empty(max(1, lib.mirl_logit_processors_table_elems(B, V, args.n_ids, args.n_bias)), dtype=torch.int32, device=dev)
-    st = _launch("mirl_logit_processors_table", dev, ctypes.byref(args), B, R, V, table.data_ptr(), _stream(dev))
-    _check(st, "mirl_logit_processors_table")
-    return table
+@functools.lru_cache(maxsize=256)
+def _processor_elems(B: int, R: int, V: int, n_ids: int, n_bias: int) -> tuple[int, int]:
+    lib = load()
+    return (lib.mirl_processed_logprob_workspace_elems(B, R, V),
+            max(1, lib.mirl_logit_processors_table_elems(B, V, n_ids, n_bias)))
 
 
-def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs, table: torch.Tensor, want_stats: bool):
-    """(logprobs [B, R] fp32, stats [B, R, 2] or None) of the first R rows (see mirl_processed_logprob_fwd)."""
+def _processors(name: str, dev: torch.device, *args) -> None:
+    """A launch of the processors' kernels (small calls are host work, see _direct)."""
+    if _direct(dev):
+        st = getattr(_lib, name)(*args, _raw_stream(dev.index))
+    else:
+        st = _launch(name, dev, *args, _stream(dev))
+    if st != 0:
+        _check(st, name)
+
+
+def processed_logprob_fwd(logits: torch.Tensor, R: int, args: LogitProcessorArgs, want_stats: bool):
+    """(logprobs [B, R] fp32, stats [B, R, 2] or None, table) of the first R rows (see
+    mirl_processed_logprob_fwd); stats and table are the backward's."""
     dev = logits.device
     B, _, V = logits.shape
+    sb, sr, _ = logits.stride()
+    n, m = _processor_elems(B, R, V, args.n_ids, args.n_bias)
     out = torch.empty((B, R), dtype=torch.float32, device=dev)
-    stats = torch.empty((B, R, 2), dtype=torch.float32, device=dev) if want_stats else None
-    lib = _lib if _lib is not None else load()
-    ws = torch.empty(max(1, lib.mirl_processed_logprob_workspace_elems(B, R, V)), dtype=torch.float32, device=dev)
-    st = _launch("mirl_processed_logprob_fwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), _ptr(stats), ws.data_ptr(), _stream(dev))
-    _check(st, "mirl_processed_logprob_fwd")
-    return out, stats
+    stats = table = None
+    if want_stats:
+        stats = torch.empty((B, R, 2), dtype=torch.float32, device=dev)
+        table = torch.empty(m, dtype=torch.int32, device=dev)
+        ws = torch.empty(n, dtype=torch.float32, device=dev).data_ptr()
+        at = table.data_ptr()
+    else:
+        both = torch.empty(n + m, dtype=torch.float32, device=dev)
+        ws = both.data_ptr()
+        at = ws + 4 * n
+    _processors("mirl_processed_logprob_fwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, sb, sr, ctypes.byref(args), at,
+                out.data_ptr(), _ptr(stats), ws)
+    return out, stats, table
 
 
 def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, stats: torch.Tensor,
@@ -1315,22 +1328,21 @@ def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table:
     R = stats.shape[1]
     _require(grad_out.dtype == torch.float32 and tuple(grad_out.shape) == (B, R), "an fp32 gradient [B, R]")
     grad = torch.empty((B, Rt, V), dtype=logits.dtype, device=dev)
-    st = _launch("mirl_processed_logprob_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, Rt, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), table.data_ptr(), stats.data_ptr(), grad_out.data_ptr(), grad_out.stride(0),
-                 grad_out.stride(1), grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
-    _check(st, "mirl_processed_logprob_bwd")
+    _processors("mirl_processed_logprob_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, Rt, V, logits.stride(0),
+                logits.stride(1), ctypes.byref(args), table.data_ptr(), stats.data_ptr(), grad_out.data_ptr(),
+                grad_out.stride(0), grad_out.stride(1), grad.data_ptr(), grad.stride(0), grad.stride(1))
     return grad
 
 
-def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, inplace: bool) -> torch.Tensor:
-    """Processed logits, in place or as a new contiguous tensor (see mirl_process_logits)."""
+def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """(processed logits, table): in place or as a new contiguous tensor (see mirl_process_logits)."""
     dev = logits.device
     B, R, V = logits.shape
     out = logits if inplace else torch.empty((B, R, V), dtype=logits.dtype, device=dev)
-    st = _launch("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
-    _check(st, "mirl_process_logits")
-    return out
+    table = torch.empty(_processor_elems(B, R, V, args.n_ids, args.n_bias)[1], dtype=torch.int32, device=dev)
+    _processors("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
+                ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1))
+    return out, table
 
 
 def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, grad_out: torch.Tensor) -> torch.Tensor:
@@ -1341,10 +1353,9 @@ def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: to
     if grad_out.stride(-1) != 1:
         grad_out = grad_out.contiguous()
     grad = torch.empty((B, R, V), dtype=logits.dtype, device=dev)
-    st = _launch("mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0),
-                 logits.stride(1), ctypes.byref(args), table.data_ptr(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
-                 grad.data_ptr(), grad.stride(0), grad.stride(1), _stream(dev))
-    _check(st, "mirl_process_logits_bwd")
+    _processors("mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
+                ctypes.byref(args), table.data_ptr(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
+                grad.data_ptr(), grad.stride(0), grad.stride(1))
     return grad
 
 

@@ -62,8 +62,8 @@ extern "C" int mirl_linear_ce_int8_fwd(const int8_t* hidden8, const float* hidde
   clear_error();
   LceParams P{};
   MIRL_REQUIRE(bsz > 0, "invalid batch size %lld", (long long)bsz);
-  if (int e = operands(P, hidden8, hidden_scale, T, Hd, ldh, weight8, weight_scale, V, ldw)) return e;
   MIRL_REQUIRE(T % bsz == 0, "row count %lld is not a multiple of the batch size %lld", (long long)T, (long long)bsz);
+  if (int e = operands(P, hidden8, hidden_scale, T, Hd, ldh, weight8, weight_scale, V, ldw)) return e;
   if (T == 0) return MIRL_OK;
   MIRL_REQUIRE(target && out && workspace, "null pointer argument");
   P.bsz = bsz;

@@ -900,6 +900,12 @@ Params params_of(const mirl_logit_processors* A, const uint32_t* table, const vo
   return P;
 }
 
+int make_table(const Params& P, int64_t rows, uint32_t* table, const char* what, hipStream_t st) {
+  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)P.B), dim3(kTableThreads), 0, st, P.A, P.B, rows, P.n_vocab,
+                     (int)P.buckets, table);
+  return check_launch(what);
+}
+
 }  // namespace
 }  // namespace mirl
 
@@ -910,25 +916,13 @@ extern "C" int64_t mirl_logit_processors_table_elems(int64_t B, int64_t V, int64
   return B * (kHead + ceil_div(V, kBucket) + 1 + n_ids + n_bias);
 }
 
-extern "C" int mirl_logit_processors_table(const mirl_logit_processors* processors, int64_t B, int64_t R, int64_t V,
-                                           uint32_t* table, void* stream) {
-  clear_error();
-  if (int e = check_args(processors, MIRL_DTYPE_F32, B, R, V)) return e;
-  if (B * R == 0) return MIRL_OK;
-  MIRL_REQUIRE(table != nullptr, "null pointer argument");
-  const Params P = params_of(processors, nullptr, nullptr, B, R, R, V, 0, 0);
-  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)B), dim3(kTableThreads), 0, static_cast<hipStream_t>(stream), *processors, B, R,
-                     P.n_vocab, (int)P.buckets, table);
-  return check_launch("mirl_logit_processors_table");
-}
-
 extern "C" int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V) {
   if (B <= 0 || R <= 0 || V <= 0) return 0;
   return B * R * (plan_of(kFwd, MIRL_DTYPE_F32, B, R, V).slices * kWaves * 2 + 1);
 }
 
 extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                          int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, float* out,
+                                          int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, float* out,
                                           float* stats, float* workspace, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
@@ -938,6 +932,7 @@ extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t
   hipStream_t st = static_cast<hipStream_t>(stream);
   P.part = workspace;
   P.xt = workspace + B * R * plan_of(kFwd, dtype, B, R, V).slices * kWaves * 2;
+  if (int e = make_table(P, R, table, "mirl_processed_logprob_fwd", st)) return e;
   if (int e = launch<kFwd>(P, dtype, R, "mirl_processed_logprob_fwd", st)) return e;
   hipLaunchKernelGGL(processors_join_kernel, dim3((unsigned)ceil_div(B * R, kWaves)), dim3(kThreads), 0, st, P, out, stats);
   return check_launch("mirl_processed_logprob_fwd");
@@ -964,7 +959,7 @@ extern "C" int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t
 }
 
 extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                   int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, void* out,
+                                   int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, void* out,
                                    int64_t o_stride_b, int64_t o_stride_r, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
@@ -976,6 +971,7 @@ extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int
   P.ysb = o_stride_b;
   P.ysr = o_stride_r;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (int e = make_table(P, R, table, "mirl_process_logits", st)) return e;
   return out == logits ? launch<kInPlace>(P, dtype, R, "mirl_process_logits", st)
                        : launch<kApply>(P, dtype, R, "mirl_process_logits", st);
 }

@@ -21,7 +21,7 @@ in fp32, rounded once where it is written.  A masked logit may hold anything.
 from __future__ import annotations
 
 import math
-from typing import Any, Optional, Union
+from typing import Any, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -31,10 +31,9 @@ from rl_amd import _C
 __all__ = ["process_logits", "processed_next_token_logprobs"]
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_MAX_TOKENS, _MAX_BIAS = (1 << 20) - 1, 2047  # what the kernels' words hold
-# the settings with one value per sample: name in the kernels' arguments, field, least value (excluded)
-_PER_SAMPLE = (("repetition", "repetition_penalty", 0.0), ("presence", "presence_penalty", None),
-               ("frequency", "frequency_penalty", None), ("temperature", "temperature", 0.0))
+_MAX_TOKENS, _MAX_BIAS, _MAX_VOCAB = (1 << 20) - 1, 2047, 1 << 24  # what the kernels' words and tables hold
+# the settings with one value per sample, in the kernels' order: field, least value (excluded)
+_PER_SAMPLE = (("repetition_penalty", 0.0), ("presence_penalty", None), ("frequency_penalty", None), ("temperature", 0.0))
 
 
 def _int64(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -45,49 +44,68 @@ def _int64(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.long()
 
 
-class _Call:
-    """The checked settings of one call: the tensors that the kernels read and the numbers."""
+def _per_sample(t: Any, name: str, B: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != (B,):
+        raise ValueError(f"{name} is a tensor [{B}], got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    t = _int64(t, name)
+    return t if t.is_contiguous() else t.contiguous()
 
-    names = ("lengths", "prompt_lengths", "repetition", "presence", "frequency", "temperature", "bias_ids", "bias", "masks",
-             "mask_rows")
+
+def _f32(t: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _no_grad(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"no gradient passes to {name}: detach it")
+
+
+class _Call:
+    """The checked settings of one call: the tensors that the kernels read, in their order, and the numbers."""
+
+    __slots__ = ("ids", "tensors", "scalars", "vocab")
 
     def __init__(self, logits: torch.Tensor, input_ids: torch.Tensor, P: Any, history_lengths: Optional[torch.Tensor],
                  R: int, vocab: tuple[int, int]):
         dev, (B, _, V) = logits.device, logits.shape
         if logits.dtype not in _DTYPES:
             raise TypeError(f"logit processors take fp32, bf16 or fp16 logits, got {logits.dtype}")
-        if V == 0:
-            raise ValueError("the vocabulary is empty")
+        if not 0 < V <= _MAX_VOCAB:
+            raise ValueError(f"a vocabulary of {V} tokens: 1 to {_MAX_VOCAB} are taken")
         if input_ids.dim() != 2 or input_ids.shape[0] != B:
             raise ValueError(f"expected input_ids [B, L] of {B} samples, got {tuple(input_ids.shape)}")
-        ids = _int64(input_ids, "input_ids")
+        self.ids = ids = _int64(input_ids, "input_ids")
         L = ids.shape[1]
         if L > _MAX_TOKENS:
             raise ValueError(f"{L} tokens of a sample: at most {_MAX_TOKENS} are counted")
-        t: dict = {}
+        lengths = prompts = bias_ids = bias = masks = rows = None
         if history_lengths is not None:
-            t["lengths"] = self._per_sample(history_lengths, "history_lengths", B)
+            lengths = _per_sample(history_lengths, "history_lengths", B)
         elif L < R:
             raise ValueError(f"{R} rows of logits for {L} tokens: give history_lengths for rows behind a history")
         if P.prompt_lengths is not None:
-            t["prompt_lengths"] = self._per_sample(P.prompt_lengths, "prompt_lengths", B)
-        scalars = {}
-        for name, field, least in _PER_SAMPLE:
+            prompts = _per_sample(P.prompt_lengths, "prompt_lengths", B)
+        penalties, scalars = [], []
+        for field, least in _PER_SAMPLE:
             value = getattr(P, field)
             if isinstance(value, torch.Tensor):
-                self._no_grad(value, field)
+                _no_grad(value, field)
                 if tuple(value.shape) != (B,) or not value.dtype.is_floating_point:
                     raise ValueError(f"{field} is a number or a floating tensor [{B}], got {value.dtype} {tuple(value.shape)}")
-                t[name] = value.to(torch.float32).contiguous()
+                penalties.append(_f32(value))
+                scalars.append(1.0)
             else:
                 value = float(value)
                 if not math.isfinite(value) or (least is not None and value <= least):
                     raise ValueError(f"{field} must be finite{'' if least is None else ' and positive'}, got {value}")
-                scalars[name] = value
+                penalties.append(None)
+                scalars.append(value)
         if (P.bias_ids is None) != (P.bias is None):
             raise ValueError("bias_ids and bias come together")
         if P.bias is not None:
-            self._no_grad(P.bias, "bias")
+            _no_grad(P.bias, "bias")
             shape = tuple(P.bias.shape)
             if tuple(P.bias_ids.shape) != shape or len(shape) not in (1, 2) or (len(shape) == 2 and shape[0] != B):
                 raise ValueError(f"bias_ids and bias are [K] or [{B}, K], got {tuple(P.bias_ids.shape)} and {shape}")
@@ -96,8 +114,7 @@ class _Call:
             if shape[-1] > _MAX_BIAS:
                 raise ValueError(f"{shape[-1]} biases of a sample: at most {_MAX_BIAS} are held (a grammar mask rules out any number)")
             if shape[-1]:
-                t["bias_ids"] = _int64(P.bias_ids, "bias_ids").contiguous()
-                t["bias"] = P.bias.to(torch.float32).contiguous()
+                bias_ids, bias = _int64(P.bias_ids, "bias_ids").contiguous(), _f32(P.bias)
         if (P.grammar_masks is None) != (P.grammar_rows is None):
             raise ValueError("grammar_masks and grammar_rows come together")
         if P.grammar_masks is not None:
@@ -106,31 +123,24 @@ class _Call:
                 raise ValueError(f"grammar_masks are int32 [M, W] with W >= {-(-V // 32)} words for {V} tokens, got {masks.dtype} {tuple(masks.shape)}")
             if rows.dim() != 2 or rows.shape[0] != B or rows.shape[1] < R:
                 raise ValueError(f"grammar_rows name the masks of {B} x {R} rows, got {tuple(rows.shape)}")
-            if masks.shape[0]:
-                t["masks"] = masks if masks.stride(1) == 1 and (masks.stride(0) >= masks.shape[1] or masks.shape[0] == 1) else masks.contiguous()
-                t["mask_rows"] = rows
-        _C._require_gpu(logits, ids, *t.values())
-        self.ids, self.tensors, self.scalars, self.vocab = ids, t, scalars, vocab
-
-    @staticmethod
-    def _no_grad(t: torch.Tensor, name: str) -> None:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"no gradient passes to {name}: detach it")
-
-    @staticmethod
-    def _per_sample(t: Any, name: str, B: int) -> torch.Tensor:
-        if not isinstance(t, torch.Tensor) or tuple(t.shape) != (B,):
-            raise ValueError(f"{name} is a tensor [{B}], got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
-        return _int64(t, name).contiguous()
+            if not masks.shape[0]:
+                masks = rows = None
+            elif masks.stride(1) != 1 or (masks.stride(0) < masks.shape[1] and masks.shape[0] > 1):
+                masks = masks.contiguous()
+        self.tensors = (lengths, prompts, *penalties, bias_ids, bias, masks, rows)
+        self.scalars, self.vocab = tuple(scalars), vocab
+        for t in (logits, ids, *self.tensors):
+            if t is not None and (not t.is_cuda or t.device != dev):
+                _C._require_gpu(logits, ids, *self.tensors)
 
     def args(self) -> "_C.LogitProcessorArgs":
         return _C.processor_args(self.ids, self.tensors, self.scalars, self.vocab)
 
     def saved(self) -> tuple:
-        return (self.ids, *(self.tensors.get(n) for n in self.names))
+        return (self.ids, *self.tensors)
 
-    def args_of_saved(self, saved: tuple) -> "_C.LogitProcessorArgs":
-        return _C.processor_args(saved[0], dict(zip(self.names, saved[1:])), self.scalars, self.vocab)
+    def args_of_saved(self, saved: Any) -> "_C.LogitProcessorArgs":
+        return _C.processor_args(saved[0], tuple(saved[1:]), self.scalars, self.vocab)
 
 
 class _ProcessedLogprob(torch.autograd.Function):
@@ -139,18 +149,22 @@ class _ProcessedLogprob(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, R: int, call: _Call) -> torch.Tensor:  # type: ignore[override]
-        args = call.args()
-        table = _C.processor_table(logits, R, args)
-        out, stats = _C.processed_logprob_fwd(logits, R, args, table, True)
+        out, stats, table = _C.processed_logprob_fwd(logits, R, call.args(), True)
         ctx.save_for_backward(logits, stats, table, *call.saved())
         ctx.call = call
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):  # type: ignore[override]
+        # the decorator only where a graph of the backward is asked for: it costs a small call 4 us
+        return (_ProcessedLogprob._once if torch.is_grad_enabled() else _ProcessedLogprob._grads)(ctx, grad)
+
+    @staticmethod
+    def _grads(ctx: Any, grad: torch.Tensor):
         logits, stats, table, *saved = ctx.saved_tensors
         return _C.processed_logprob_bwd(logits, ctx.call.args_of_saved(saved), table, stats, grad.float()), None, None
+
+    _once = staticmethod(once_differentiable(_grads.__func__))
 
 
 class _ProcessLogits(torch.autograd.Function):
@@ -158,17 +172,21 @@ class _ProcessLogits(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, call: _Call) -> torch.Tensor:  # type: ignore[override]
-        args = call.args()
-        table = _C.processor_table(logits, logits.shape[1], args)
+        out, table = _C.process_logits(logits, call.args(), False)
         ctx.save_for_backward(logits, table, *call.saved())
         ctx.call = call
-        return _C.process_logits(logits, args, table, False)
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):  # type: ignore[override]
+        return (_ProcessLogits._once if torch.is_grad_enabled() else _ProcessLogits._grads)(ctx, grad)
+
+    @staticmethod
+    def _grads(ctx: Any, grad: torch.Tensor):
         logits, table, *saved = ctx.saved_tensors
         return _C.process_logits_bwd(logits, ctx.call.args_of_saved(saved), table, grad), None
+
+    _once = staticmethod(once_differentiable(_grads.__func__))
 
 
 def _grad_needed(logits: torch.Tensor) -> bool:
@@ -202,8 +220,7 @@ def processed_next_token_logprobs(
     end = vocab_start_index + logits.shape[2] if vocab_end_index is None else vocab_end_index
     call = _Call(logits, input_ids, processors, history_lengths, R, (int(vocab_start_index), int(end)))
     if inference_only or not _grad_needed(logits):
-        args = call.args()
-        return _C.processed_logprob_fwd(logits, R, args, _C.processor_table(logits, R, args), False)[0]
+        return _C.processed_logprob_fwd(logits, R, call.args(), False)[0]
     return _ProcessedLogprob.apply(logits, R, call)
 
 
@@ -233,8 +250,7 @@ def process_logits(
     if not inplace and _grad_needed(logits):
         y = _ProcessLogits.apply(x, call)
         return y if logits.dim() == 3 else y.squeeze(1)
-    args = call.args()
-    y = _C.process_logits(x, args, _C.processor_table(x, x.shape[1], args), inplace)
+    y, _ = _C.process_logits(x, call.args(), inplace)
     if inplace:
         torch.autograd.graph.increment_version(logits)
         return logits
