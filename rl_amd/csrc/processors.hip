@@ -142,6 +142,14 @@ struct Sample {
 static_assert(sizeof(Sample) == kHead * 4, "the table's head");
 __device__ __forceinline__ const uint32_t* head_of(const Params& P, int64_t b) { return P.table + b * (kHead + P.buckets + 1); }
 
+// The bits of a where `mask` has them, else those of b.  (In asm: from the shifts and masks that follow, the
+// compiler makes three instructions of it.)
+__device__ __forceinline__ uint32_t either(uint32_t mask, uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(mask), "s"(a), "v"(b));
+  return r;
+}
+
 // v where bit e of `keep` is set, else `other`; as bits, whatever v holds.
 __device__ __forceinline__ float keep_if(float v, uint32_t keep, int e, float other) {
   uint32_t t = (uint32_t)__builtin_amdgcn_sbfe((int)keep, e, 1);
@@ -585,9 +593,10 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
             // (a masked token's bias and penalties leave it at -inf)
 #pragma unroll
             for (int k = 0; k < kP<E>; ++k) {
-              vu4 lost = {gone[u][4 * k], gone[u][4 * k + 1], gone[u][4 * k + 2], gone[u][4 * k + 3]};
-              if (masked) lost |= ~s_lut[mk[u] >> (k * E::kVec) & (kLut - 1)];
-              q[u][k] = (q[u][k] & ~lost) | (E::kNegInf2 & lost);
+              vu4 left_out = {gone[u][4 * k], gone[u][4 * k + 1], gone[u][4 * k + 2], gone[u][4 * k + 3]};
+              if (masked) left_out |= ~s_lut[mk[u] >> (k * E::kVec) & (kLut - 1)];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) q[u][k][j] = either(left_out[j], E::kNegInf2, q[u][k][j]);
             }
           }
           unpack_group<E>(q[u], v);
@@ -822,8 +831,10 @@ Plan plan_of(int mode, int dtype, int64_t B, int64_t R, int64_t V) {
   p.nv = mode == kFwd && dtype != MIRL_DTYPE_F32 && B * R * wide >= 4096 ? 2 : 1;
   p.slices = ceil_div(V, kBucket * p.nv);
   p.rows = mode == kFwd ? 32 : 4;
-  while (p.rows > 1 && B * ceil_div(R, p.rows) * p.slices < (mode == kFwd ? 1024 : 2048)) p.rows /= 2;
-  while (B * ceil_div(R, p.rows) * p.slices >= (int64_t(1) << 24) && p.rows < kWave) p.rows *= 2;
+  auto workgroups = [&] { return B * ceil_div(R, p.rows) * p.slices; };
+  while (p.rows > 8 && workgroups() < 8192) p.rows /= 2;
+  while (p.rows > 1 && workgroups() < (mode == kFwd ? 1024 : 2048)) p.rows /= 2;
+  while (workgroups() >= (int64_t(1) << 24) && p.rows < kWave) p.rows *= 2;
   p.chunks = ceil_div(R, p.rows);
   return p;
 }
