@@ -1272,7 +1272,8 @@ def processor_args(ids: torch.Tensor, tensors: tuple, scalars: tuple, vocab: tup
         n_bias = bias.shape[-1]
         bias_sb = n_bias if bias.dim() == 2 else 0
     if masks is not None:
-        n_masks, mask_stride = masks.shape[0], masks.stride(0)
+        n_masks = masks.shape[0]
+        mask_stride = masks.stride(0) if n_masks > 1 else masks.shape[1]
         rows_sb, rows_sr = rows.stride()
     p = [None if t is None else t.data_ptr() for t in tensors]
     sb, ss = ids.stride()

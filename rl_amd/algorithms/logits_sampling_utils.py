@@ -85,7 +85,8 @@ class LogitProcessors:
     multiplied; 1.0: off); one of the response, the positions from ``prompt_lengths [B]`` on (None: all),
     loses ``frequency_penalty`` for each occurrence and ``presence_penalty`` once.  ``bias_ids`` and ``bias``
     (``[K]`` or ``[B, K]``, at most 2047 entries, unused ones with an id of -1; of two entries of one id the
-    later holds) are added to single tokens' logits ahead of the penalties; -inf rules a token out.
+    later holds) are added to single tokens' logits ahead of the penalties; each is finite, or -inf, which rules a
+    token out.
     ``grammar_masks [M, W]`` (int32; token v is bit ``v % 32`` of word ``v // 32``, 1 allowed) holds the distinct
     masks and ``grammar_rows [B, R]`` each row's, -1 for a row under no grammar.  ``temperature`` comes last:
     with it here ``apply_temperature_scaling`` is not called as well.

@@ -135,7 +135,8 @@ def from_int8_hidden_states_to_logits(
         _C._require_gpu(h8, w8, out)
         return out
     rows = _operand8(h8.reshape(-1, H), True)
-    torch.autograd.graph.increment_version(out)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     _C.int8_logits(rows, hidden_scales.reshape(-1).contiguous(), _operand8(w8, False), output_weight_scales.contiguous(),
                    out.view(-1, V))
     return out

@@ -136,12 +136,6 @@ class _Call:
     def args(self) -> "_C.LogitProcessorArgs":
         return _C.processor_args(self.ids, self.tensors, self.scalars, self.vocab)
 
-    def saved(self) -> tuple:
-        return (self.ids, *self.tensors)
-
-    def args_of_saved(self, saved: Any) -> "_C.LogitProcessorArgs":
-        return _C.processor_args(saved[0], tuple(saved[1:]), self.scalars, self.vocab)
-
 
 class _ProcessedLogprob(torch.autograd.Function):
     """Logprobs [B, R] of the tokens behind the first R rows.  Kept for the backward: the logits, eight
@@ -150,8 +144,8 @@ class _ProcessedLogprob(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, R: int, call: _Call) -> torch.Tensor:  # type: ignore[override]
         out, stats, table = _C.processed_logprob_fwd(logits, R, call.args(), True)
-        ctx.save_for_backward(logits, stats, table, *call.saved())
-        ctx.call = call
+        ctx.save_for_backward(logits, stats, table, call.ids, *call.tensors)
+        ctx.numbers = (call.scalars, call.vocab)
         return out
 
     @staticmethod
@@ -161,8 +155,9 @@ class _ProcessedLogprob(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx: Any, grad: torch.Tensor):
-        logits, stats, table, *saved = ctx.saved_tensors
-        return _C.processed_logprob_bwd(logits, ctx.call.args_of_saved(saved), table, stats, grad.float()), None, None
+        logits, stats, table, ids, *tensors = ctx.saved_tensors
+        args = _C.processor_args(ids, tuple(tensors), *ctx.numbers)
+        return _C.processed_logprob_bwd(logits, args, table, stats, grad.float()), None, None
 
     _once = staticmethod(once_differentiable(_grads.__func__))
 
@@ -173,8 +168,8 @@ class _ProcessLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, logits: torch.Tensor, call: _Call) -> torch.Tensor:  # type: ignore[override]
         out, table = _C.process_logits(logits, call.args(), False)
-        ctx.save_for_backward(logits, table, *call.saved())
-        ctx.call = call
+        ctx.save_for_backward(logits, table, call.ids, *call.tensors)
+        ctx.numbers = (call.scalars, call.vocab)
         return out
 
     @staticmethod
@@ -183,8 +178,8 @@ class _ProcessLogits(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx: Any, grad: torch.Tensor):
-        logits, table, *saved = ctx.saved_tensors
-        return _C.process_logits_bwd(logits, ctx.call.args_of_saved(saved), table, grad), None
+        logits, table, ids, *tensors = ctx.saved_tensors
+        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad), None
 
     _once = staticmethod(once_differentiable(_grads.__func__))
 
@@ -252,6 +247,7 @@ def process_logits(
         return y if logits.dim() == 3 else y.squeeze(1)
     y, _ = _C.process_logits(x, call.args(), inplace)
     if inplace:
-        torch.autograd.graph.increment_version(logits)
+        if not logits.is_inference():
+            torch.autograd.graph.increment_version(logits)
         return logits
     return y if logits.dim() == 3 else y.squeeze(1)

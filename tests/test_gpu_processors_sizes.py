@@ -178,3 +178,27 @@ def test_no_masks_in_the_table():
     wide = torch.cat([pack_masks(allowed), torch.zeros(2, 5, dtype=torch.int32)], 1)  # wider than the vocabulary
     W = dataclasses.replace(P, grammar_masks=wide, grammar_rows=torch.tensor([[0, 1, 7]]))  # 7: no such mask
     assert torch.equal(apply_logit_processors(x.cuda(), ids.cuda(), cuda(P)), apply_logit_processors(x.cuda(), ids.cuda(), cuda(W)))
+
+
+def test_one_mask_of_any_stride_and_inference_mode():
+    x, ids, P, _ = make(2, 3, 3, 70, torch.float32, seed=6, K=2)
+    mask = pack_masks(torch.rand(1, 70, generator=torch.Generator().manual_seed(3)) < 0.7)
+    P = dataclasses.replace(P, grammar_masks=mask, grammar_rows=torch.zeros(2, 3, dtype=torch.int64))
+    want = apply_logit_processors(x.cuda(), ids.cuda(), cuda(P))
+    odd = dataclasses.replace(cuda(P), grammar_masks=mask.cuda().as_strided((1, 3), (1, 1)))
+    assert torch.equal(apply_logit_processors(x.cuda(), ids.cuda(), odd), want)
+    with torch.inference_mode():
+        place = x.cuda()
+        apply_logit_processors(place, ids.cuda(), cuda(P), inplace=True)
+        assert torch.equal(place, want)
+        lp = from_parallel_logits_to_logprobs(x.cuda(), ids.cuda(), 0, 70, None, logit_processors=cuda(P))
+    assert torch.equal(lp, from_parallel_logits_to_logprobs(x.cuda(), ids.cuda(), 0, 70, None, logit_processors=cuda(P)))
+
+
+def test_saved_tensor_hooks_may_move_what_is_kept():
+    x, ids, P, _ = make(2, 5, 5, 900, torch.float32, seed=7, K=3, M=3)
+    g = torch.ones(2, 4)
+    _, want = gradient(x, ids, P, g)
+    with torch.autograd.graph.save_on_cpu():
+        _, got = gradient(x, ids, P, g)
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))

@@ -21,6 +21,12 @@ from rl_amd.distributed.model_utils import (
 B, R, V = 2, 3, 40
 
 
+@pytest.fixture(autouse=True)
+def no_message_left():
+    yield
+    assert _C.load().mirl_dropout(None, 0, 0, 0.5, 0, None, 0, None, None) == 0  # (a call that succeeds clears it)
+
+
 def logits(**kw):
     return torch.zeros(B, R, V, **kw)
 
