@@ -16,6 +16,14 @@
 // [rows, V] is held.  A word per token holds its count, whether it occurred and its bias; a bit per
 // token in the lane's registers says whether the word is anything but 0, so that ordinary tokens
 // cost one test for a group of eight.
+//
+// Bound by memory but for the logprobs' forward, which the vector units share (some 60 instructions for eight
+// ordinary values of bf16).  bf16 [8, 2048, 151936] with the penalties and biases of a GRPO step, half of the rows without
+// a gradient: forward 920 us (4.98 GB, 5.4 TB/s; 860 where no token of the rows occurs, logprob.hip's of untouched
+// logits 730), backward 1.36 to 1.43 ms (7.4 GB, 5.3 TB/s; logprob.hip's 1.22).  [2, 2048, 151936]: written out
+// 412 us (2.49 GB, 6.0 TB/s), its backward 495 (5.0; the logits of tokens that occur are read as well).  One token of
+// each of 64 requests behind up to 2048 tokens: table 8 us, logprobs 13 and 4 to join, written out 15: the
+// latency of a few loads that wait for each other.
 
 #include "common.h"
 
@@ -306,10 +314,12 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slices = (uint32_t)P.slices, chunks = (uint32_t)P.chunks;
-  // Neighbouring workgroups take neighbouring slices.  The first slice moves on from run to run of rows: workgroups
-  // go to the eight dies in turn, and with a number of slices that eight divides a die would always have the
-  // same columns ([4, 1024, 131072] bf16 under masks, 32 slices: 229 us, without 301).
-  const uint32_t rest = blockIdx.x / slices, slice = (blockIdx.x + rest) % slices;
+  // Neighbouring workgroups take neighbouring slices, from the first one on; where eight divides their number,
+  // from another one in each run of rows: workgroups go to the eight dies in turn, and a die would always have
+  // the same columns ([4, 1024, 131072] bf16 under masks, 32 slices: forward 229 us, without 301; the gradient of
+  // written-out logits 435 and 483, of the logprobs, whose zero rows differ from run to run, 1.36 ms and 1.24).
+  const uint32_t rest = blockIdx.x / slices;
+  const uint32_t slice = (blockIdx.x + (MODE != kBwd && slices % 8 == 0 ? rest : 0)) % slices;
   const uint32_t chunk = rest % chunks, b = rest / chunks;
   const int64_t n0 = (int64_t)slice * kSlice;
   const int64_t r0 = (int64_t)chunk * P.rows;
@@ -823,7 +833,15 @@ __global__ __launch_bounds__(kThreads) void processors_join_kernel(Params P, flo
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Groups of a lane and rows of a workgroup.
+// Groups of a lane and rows of a workgroup.  The forward of 16-bit rows takes two groups (16 bytes each) where there
+// are workgroups enough ([8, 2048, 151936] bf16, 16 rows, at an early stage: 1174 us, with one 1420, with four 1281;
+// with 32 rows now 929 and 1006 with four), one where there are not; fp32 one of 32 bytes ([3, 256, 32003], 8 rows:
+// 24 us, with two 26).  The others take one: narrow slices keep what is read and written close together (backward of
+// the large rows 1.41 ms with one, 1.53 with two).  In the forward many rows share the count of the tokens ahead of
+// them (929 us with 32, 959 with 16); where rows are written, few at a time reach across less memory: written out
+// [2, 2048, 151936] 412 us with 4, 446 with 8, 465 with 2; the backward 1.36 ms with 4, 1.39 with 8, 1.57 with 2.  Fewer
+// rows where there would be less than some rounds of workgroups (the fp32 forward 24 us with 8, 29 with 16, 44 with
+// 32; its backward 41 with 4, 45 with 8).
 struct Plan {
   int nv;
   int64_t slices, rows, chunks;
