@@ -184,6 +184,18 @@ class _ProcessLogits(torch.autograd.Function):
     _once = staticmethod(once_differentiable(_grads.__func__))
 
 
+def _rows_meet(x: torch.Tensor) -> bool:
+    """Whether two rows of ``x [B, R, V]`` (unit stride in V) have an element in common."""
+    (n, s), (m, t) = sorted(zip(x.shape[:2], x.stride()[:2]), key=lambda d: d[1])  # the lesser stride first
+    V = x.shape[2]
+    if (n > 1 and s < V) or (m > 1 and t < V):
+        return True
+    if n <= 1 or m <= 1 or t >= (n - 1) * s + V:
+        return False
+    # rows that are i of the one stride and j of the other apart
+    return any(abs(i * t - j * s) < V for i in range(1, m) for j in (i * t // s, i * t // s + 1) if j < n)
+
+
 def _grad_needed(logits: torch.Tensor) -> bool:
     return logits.requires_grad and torch.is_grad_enabled()
 
@@ -237,7 +249,7 @@ def process_logits(
             raise RuntimeError("in place there is no gradient: the backward needs the logits as they were")
         if x.stride(2) != 1 and x.shape[2] > 1:
             raise ValueError("in place, the vocabulary has unit stride")
-        if any(n > 1 and abs(s) < x.shape[2] for n, s in zip(x.shape[:2], x.stride()[:2])):
+        if _rows_meet(x):
             raise ValueError("in place, no two rows share memory")
     elif x.stride(2) != 1:
         x = x.contiguous()

@@ -113,6 +113,15 @@ def test_in_place():
         apply_logit_processors(torch.zeros(1, R, V).expand(B, R, V), ids(), P, inplace=True)
 
 
+@pytest.mark.parametrize("strides", [(V, V), (R * V, V), (V, B * V), (R * V - 1, V), (5 * V, 2 * V), (2 * V, 5 * V), (4 * V, 2 * V)])
+def test_in_place_rows_that_nest(strides):
+    x = torch.zeros(40 * V).as_strided((B, R, V), (*strides, 1))
+    places = {i * strides[0] + j * strides[1] + v for i in range(B) for j in range(R) for v in range(V)}
+    shared = len(places) < B * R * V
+    with pytest.raises(ValueError if shared else _C.MirlError, match="share memory" if shared else None):
+        apply_logit_processors(x, ids(), LogitProcessors(repetition_penalty=1.1), inplace=True)
+
+
 def test_valid_calls_end_at_the_device():
     P = LogitProcessors(repetition_penalty=torch.full((B,), 1.1), bias_ids=torch.zeros(3, dtype=torch.int64), bias=torch.zeros(3),
                         grammar_masks=MASK, grammar_rows=ROWS)
