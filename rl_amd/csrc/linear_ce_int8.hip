@@ -6,9 +6,10 @@
 // of a row and whose accumulators are 32-bit integers: the sum is exact and its rounding to fp32 (above
 // 2^24) is the first one.  The target's logit is therefore the tile's own.
 //
-// Bound by the matrix cores and what feeds them, few rows by the weight's bytes.  [16376, 4096] x [151936, 4096]: logprobs
-// 7.56 to 7.75 ms, 2.63 to 2.7 POP/s (e4m3 on the same loop 7.44; a library product 2.13).  Logits of [2048, 4096] x [151936, 4096] in bf16, 622 MB of them:
-// 1.07 ms, 2.39 POP/s.  Of 64 rows: logits 131 us, logprobs 124 us, 4.9 and 5.0 TB/s.
+// Bound by the matrix cores and what feeds them, few rows by the weight's bytes.  [16376, 4096] x [151936, 4096]:
+// logprobs 7.56 to 7.75 ms, 2.63 to 2.70 POP/s (e4m3 on the same loop 7.44; a library product alone 2.13 POP/s).  Logits
+// of [2048, 4096] x [151936, 4096] in bf16, 622 MB of them: 1.07 ms, 2.39 POP/s.  Of 64 rows: logits 131 us,
+// logprobs 124 us, 4.9 and 5.0 TB/s.
 
 #include "lce_tile.h"
 
