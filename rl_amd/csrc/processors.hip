@@ -49,6 +49,8 @@ constexpr int kBucketBits = 11, kBucket = 1 << kBucketBits;
 constexpr uint32_t kIsBias = 1u << 31;
 constexpr int64_t kMaxBuckets = 8192;
 constexpr int kTableThreads = 1024;
+constexpr int kBiasSlots = 4096;
+static_assert(2 * kBiasSlots <= kMaxBuckets && kMaxBias < kBiasSlots, "the biases' columns find a place");
 static_assert(kBucket == kThreads * kG, "a slice is a whole number of buckets");
 static_assert(kCountBits + kBucketBits <= 31, "an entry holds a token's place and column");
 
@@ -213,7 +215,6 @@ __device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t h
 __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t B, int64_t R,
                                                                          int64_t n_vocab, int buckets, uint32_t* table) {
   __shared__ uint32_t s_at[kMaxBuckets];
-  __shared__ int s_bias[kMaxBias];
   __shared__ uint32_t s_wave[kTableThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t b = blockIdx.x;
@@ -241,21 +242,46 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     const uint64_t c = (uint64_t)id - (uint64_t)A.vocab_start;
     return c < (uint64_t)n_vocab ? (int)c : -1;
   };
+  // A bias holds if no later one of its sample names the same token: each column finds a slot of its own (open
+  // addressing, less than half of the slots taken), which keeps the largest number that came by.
+  int own[(kMaxBias + kTableThreads - 1) / kTableThreads];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+    const int k = i * kTableThreads + tid;
+    own[i] = k < n_bias ? column(bias_ids[k]) : -1;
+  }
+  if (n_bias > 1) {
+    uint32_t* const s_column = s_at;
+    uint32_t* const s_last = s_at + kBiasSlots;
+    for (int k = tid; k < 2 * kBiasSlots; k += kTableThreads) s_at[k] = 0;
+    __syncthreads();
+    uint32_t slot[sizeof(own) / sizeof(int)];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+      if (own[i] < 0) continue;
+      uint32_t h = (uint32_t)own[i] * 0x9e3779b1u >> 20;
+      for (;; h = (h + 1) % kBiasSlots) {
+        const uint32_t was = atomicCAS(&s_column[h], 0u, (uint32_t)own[i] + 1);
+        if (was == 0 || was == (uint32_t)own[i] + 1) break;
+      }
+      slot[i] = h;
+      atomicMax(&s_last[h], (uint32_t)(i * kTableThreads + tid));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i)
+      if (own[i] >= 0 && s_last[slot[i]] != (uint32_t)(i * kTableThreads + tid)) own[i] = -1;
+    __syncthreads();
+  }
   for (int k = tid; k < buckets; k += kTableThreads) s_at[k] = 0;
-  for (int k = tid; k < n_bias; k += kTableThreads) s_bias[k] = column(bias_ids[k]);
   __syncthreads();
 #pragma unroll 4
   for (int p = tid; p < n; p += kTableThreads) {
     const int c = column(ids[p * A.ids_stride_s]);
     if (c >= 0) atomicAdd(&s_at[c >> kBucketBits], 1u);
   }
-  // a bias holds if no later one of its sample names the same token
-  int own[(kMaxBias + kTableThreads - 1) / kTableThreads];
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
-    const int k = i * kTableThreads + tid;
-    own[i] = k < n_bias ? s_bias[k] : -1;
-    for (int j = k + 1; j < n_bias; ++j) own[i] = s_bias[j] == own[i] ? -1 : own[i];
     if (own[i] >= 0) atomicAdd(&s_at[own[i] >> kBucketBits], 1u);
   }
   __syncthreads();
