@@ -41,15 +41,16 @@ constexpr uint32_t kCountBits = 20, kInPrompt = 1u << kCountBits, kCount = kInPr
 constexpr int kBiasShift = kCountBits + 1;
 constexpr int64_t kMaxTokens = kCount, kMaxBias = (int64_t(1) << (32 - kBiasShift)) - 1;
 
-// The table of a call: per sample what holds for all its rows (kHead words) and where each bucket begins
-// (buckets + 1 numbers), then all samples' entries: a token's column in its bucket and its place, or
-// with the top bit a bias's column and number.
+// The table of a call: per sample what holds for all its rows (kHead words) and for each of its lists (kList tokens
+// each, and one of biases) where each bucket begins (buckets + 1 numbers), then all samples' entries: a token's
+// column in its bucket and its place, or with the top bit a bias's column and number.
 constexpr int kHead = 8;
 constexpr int kBucketBits = 11, kBucket = 1 << kBucketBits;
 constexpr uint32_t kIsBias = 1u << 31;
 constexpr int64_t kMaxBuckets = 8192;
 constexpr int kTableThreads = 1024;
 constexpr int kBiasSlots = 4096;
+constexpr int64_t kList = 4096;
 static_assert(2 * kBiasSlots <= kMaxBuckets && kMaxBias < kBiasSlots, "the biases' columns find a place");
 static_assert(kBucket == kThreads * kG, "a slice is a whole number of buckets");
 static_assert(kCountBits + kBucketBits <= 31, "an entry holds a token's place and column");
@@ -63,6 +64,7 @@ struct Params {
   int64_t B, R, Rt, V;   // rows with a result; rows of the gradient (those past R: zeros)
   int64_t n_vocab;       // ids vs .. vs + n_vocab - 1 stand for the columns
   int64_t slices, chunks, buckets;
+  int64_t lists;         // of a sample: of tokens, and one of biases if there are any
   const uint32_t* table;
   int rows;              // rows of a workgroup
   void* y;               // processed logits, or a gradient
@@ -150,7 +152,10 @@ struct Sample {
   int unused;
 };
 static_assert(sizeof(Sample) == kHead * 4, "the table's head");
-__device__ __forceinline__ const uint32_t* head_of(const Params& P, int64_t b) { return P.table + b * (kHead + P.buckets + 1); }
+__host__ __device__ __forceinline__ int64_t token_lists(int64_t n_ids) { return n_ids > kList ? (n_ids + kList - 1) / kList : 1; }
+// Words of a sample ahead of all samples' entries.
+__host__ __device__ __forceinline__ int64_t head_words(int64_t lists, int64_t buckets) { return kHead + lists * (buckets + 1); }
+__device__ __forceinline__ const uint32_t* head_of(const Params& P, int64_t b) { return P.table + b * head_words(P.lists, P.buckets); }
 
 // The bits of a where `mask` has them, else those of b.  (In asm: from the shifts and masks that follow, the
 // compiler makes three instructions of it.)
@@ -210,22 +215,24 @@ __device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t h
   }
 }
 
-// Buckets of one sample's tokens (those that any of the R rows follows) and biases.  An entry's place
-// in its bucket comes from an atomic: the order differs from run to run, what is counted does not.
-__global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t B, int64_t R,
-                                                                         int64_t n_vocab, int buckets, uint32_t* table) {
+// Buckets of a list of one sample's tokens (those that any of the R rows follows), or of its biases.  An entry's place
+// in its bucket comes from an atomic: the order differs from run to run, what is counted does not.  A workgroup
+// has kList tokens, so that a long history is spread over the chip (one row behind 131072 tokens, written out: 16 us with even ones, 57 with
+// Zipf-like ones, of which one slice has most; by one workgroup 94 and 206).
+__global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t R, int64_t n_vocab,
+                                                                         int64_t lists, int buckets, uint32_t* table) {
   __shared__ uint32_t s_at[kMaxBuckets];
   __shared__ uint32_t s_wave[kTableThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t b = blockIdx.x;
+  const int64_t b = blockIdx.x / lists, list = blockIdx.x - b * lists, B = gridDim.x / lists;
+  const bool biases = list == token_lists(A.n_ids);
   const int64_t* ids = A.ids + b * A.ids_stride_b;
   const int64_t* bias_ids = A.bias_ids + b * A.bias_stride_b;
   const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1;
-  const int n = (int)min(max(n_b + R - 1, int64_t(0)), A.n_ids), n_bias = (int)A.n_bias;
-  uint32_t* const head = table + b * (kHead + buckets + 1);
-  uint32_t* const begins = head + kHead;
-  uint32_t* const entries = table + B * (kHead + buckets + 1) + b * (A.n_ids + A.n_bias);
-  if (tid == 0) {
+  uint32_t* const head = table + b * head_words(lists, buckets);
+  uint32_t* const begins = head + kHead + list * (buckets + 1);
+  uint32_t* const entries = table + B * head_words(lists, buckets) + b * (A.n_ids + A.n_bias);
+  if (list == 0 && tid == 0) {
     Sample S;
     S.rp = A.repetition != nullptr ? A.repetition[b] : A.repetition_all;
     S.inv_rp = 1.f / S.rp;
@@ -242,22 +249,27 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     const uint64_t c = (uint64_t)id - (uint64_t)A.vocab_start;
     return c < (uint64_t)n_vocab ? (int)c : -1;
   };
-  // A bias holds if no later one of its sample names the same token: each column finds a slot of its own (open
-  // addressing, less than half of the slots taken), which keeps the largest number that came by.
-  int own[(kMaxBias + kTableThreads - 1) / kTableThreads];
+  // the list's tokens (place, column), or biases (number, column), of this thread
+  constexpr int kOwn = kList / kTableThreads;
+  static_assert(kList % kTableThreads == 0 && kMaxBias <= kList, "a thread holds its part of a list");
+  const int64_t from = biases ? 0 : list * kList;
+  const int n = biases ? (int)A.n_bias : (int)min(max(min(n_b + R - 1, A.n_ids) - from, int64_t(0)), kList);
+  int own[kOwn];
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+  for (int i = 0; i < kOwn; ++i) {
     const int k = i * kTableThreads + tid;
-    own[i] = k < n_bias ? column(bias_ids[k]) : -1;
+    own[i] = k < n ? column(biases ? bias_ids[k] : ids[(from + k) * A.ids_stride_s]) : -1;
   }
-  if (n_bias > 1) {
+  // A bias holds if no later one of its sample names the same token: each column finds a slot of its own (open
+  // addressing, at most half of the slots taken), which keeps the largest number that came by.
+  if (biases && n > 1) {
     uint32_t* const s_column = s_at;
     uint32_t* const s_last = s_at + kBiasSlots;
     for (int k = tid; k < 2 * kBiasSlots; k += kTableThreads) s_at[k] = 0;
     __syncthreads();
-    uint32_t slot[sizeof(own) / sizeof(int)];
+    uint32_t slot[kOwn];
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+    for (int i = 0; i < kOwn; ++i) {
       if (own[i] < 0) continue;
       uint32_t h = (uint32_t)own[i] * 0x9e3779b1u >> 20;
       for (;; h = (h + 1) % kBiasSlots) {
@@ -269,21 +281,17 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i)
+    for (int i = 0; i < kOwn; ++i)
       if (own[i] >= 0 && s_last[slot[i]] != (uint32_t)(i * kTableThreads + tid)) own[i] = -1;
     __syncthreads();
   }
   for (int k = tid; k < buckets; k += kTableThreads) s_at[k] = 0;
   __syncthreads();
-#pragma unroll 4
-  for (int p = tid; p < n; p += kTableThreads) {
-    const int c = column(ids[p * A.ids_stride_s]);
-    if (c >= 0) atomicAdd(&s_at[c >> kBucketBits], 1u);
-  }
+  // An atomic for each; its result is the entry's place in its bucket.
+  uint32_t place[kOwn];
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
-    if (own[i] >= 0) atomicAdd(&s_at[own[i] >> kBucketBits], 1u);
-  }
+  for (int i = 0; i < kOwn; ++i)
+    if (own[i] >= 0) place[i] = atomicAdd(&s_at[own[i] >> kBucketBits], 1u);
   __syncthreads();
   // the sizes' running sum: a few buckets a thread, the threads' sums over waves and the workgroup
   const int per = (buckets + kTableThreads - 1) / kTableThreads, k0 = min(tid * per, buckets), k1 = min(k0 + per, buckets);
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
   }
   if (lane == kWave - 1) s_wave[wave] = upto;
   __syncthreads();
-  uint32_t at = upto - mine;
+  uint32_t at = (uint32_t)(biases ? A.n_ids : from) + upto - mine;
   for (int w = 0; w < wave; ++w) at += s_wave[w];
   for (int k = k0; k < k1; ++k) {
     const uint32_t size = s_at[k];
@@ -307,16 +315,12 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
   }
   if (tid == kTableThreads - 1) begins[buckets] = at;
   __syncthreads();
-#pragma unroll 4
-  for (int p = tid; p < n; p += kTableThreads) {
-    const int c = column(ids[p * A.ids_stride_s]);
-    if (c >= 0) entries[atomicAdd(&s_at[c >> kBucketBits], 1u)] = (uint32_t)p << kBucketBits | (uint32_t)(c & (kBucket - 1));
-  }
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(own) / sizeof(int)); ++i) {
+  for (int i = 0; i < kOwn; ++i) {
     if (own[i] >= 0)
-      entries[atomicAdd(&s_at[own[i] >> kBucketBits], 1u)] =
-          kIsBias | (uint32_t)(i * kTableThreads + tid) << kBucketBits | (uint32_t)(own[i] & (kBucket - 1));
+      entries[s_at[own[i] >> kBucketBits] + place[i]] = (biases ? kIsBias : 0u) |
+                                                        (uint32_t)(from + i * kTableThreads + tid) << kBucketBits |
+                                                        (uint32_t)(own[i] & (kBucket - 1));
   }
 }
 
@@ -432,12 +436,19 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
     const uint64_t c = (uint64_t)id - (uint64_t)first_id;
     return c < here ? (int)c : -1;
   };
-  const uint32_t buckets = (uint32_t)P.buckets, bucket0 = slice * NV;
-  const uint32_t* begins = head + kHead;
-  const uint32_t* entries = P.table + P.B * (kHead + buckets + 1) + b * (A.n_ids + A.n_bias);
-  uint32_t begin[NV + 1];
-#pragma unroll
-  for (int u = 0; u <= NV; ++u) begin[u] = begins[min(bucket0 + u, buckets)];
+  const uint32_t buckets = (uint32_t)P.buckets, bucket0 = slice * NV, lists = (uint32_t)P.lists;
+  const uint32_t* entries = P.table + P.B * head_words(P.lists, P.buckets) + b * (A.n_ids + A.n_bias);
+  // where the slice's entries of a list begin, those of its second bucket, and where they end
+  struct Span {
+    uint32_t from, mid, to;
+  };
+  auto span_of = [&](uint32_t l) {
+    const uint32_t* begins = head + kHead + (int64_t)l * (buckets + 1) + bucket0;
+    const uint32_t mid = begins[1];
+    return Span{begins[0], mid, NV > 1 ? begins[min(2u, buckets - bucket0)] : mid};
+  };
+  const bool few = lists <= 2;
+  const Span first_span = few ? span_of(0) : Span{}, second_span = few && lists == 2 ? span_of(1) : Span{};
   const uint32_t ahead = (uint32_t)max(S.n + r0, int64_t(0)), in_prompt = (uint32_t)S.prompt;
   // The token that is new ahead of a row and the one behind it (columns of this wave, or -1), its mask.
   constexpr int kOfPrompt = 1 << 30;
@@ -456,12 +467,10 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       m_mask = m >= 0 && m < A.n_masks ? (int)m : -1;
     }
   }
-  __syncthreads();
-  for (uint32_t i = begin[0] + tid; i < begin[NV]; i += kThreads) {
-    const uint32_t w = entries[i], at = (w & ~kIsBias) >> kBucketBits;
-    uint32_t c = w & (kBucket - 1);
-#pragma unroll
-    for (int u = 1; u < NV; ++u) c += i >= begin[u] ? kBucket : 0;
+  // entry w, number i of the table; from `mid` on a list's entries are those of the second bucket
+  auto count = [&](uint32_t w, uint32_t i, uint32_t mid) __attribute__((always_inline)) {
+    const uint32_t at = (w & ~kIsBias) >> kBucketBits;
+    const uint32_t c = (w & (kBucket - 1)) + (NV > 1 && i >= mid ? kBucket : 0);
     if (w & kIsBias) {
       atomicAdd(&s_word[c], (at + 1) << kBiasShift);
       if constexpr (!kLists) s_bias[c] = bias[at];
@@ -469,6 +478,36 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       atomicOr(&s_word[c], kInPrompt);
     } else if (at < ahead) {
       atomicAdd(&s_word[c], 1u);
+    }
+  };
+  __syncthreads();
+  bool some = false;
+  if (few) {  // one after the other; what leads to them is loaded by scalars, ahead of all this
+    const uint32_t n = first_span.to - first_span.from, all = n + second_span.to - second_span.from;
+    some = all != 0;
+    for (uint32_t k = tid; k < all; k += kThreads) {
+      const uint32_t i = k + (k < n ? first_span.from : second_span.from - n);
+      count(entries[i], i, k < n ? first_span.mid : second_span.mid);
+    }
+  } else {  // each wave a list, those behind the first row left out, with some loads under way at a time
+    constexpr int kDeep = 8;
+    for (uint32_t l0 = 0; l0 < lists; l0 += kWave) {
+      const uint32_t l = l0 + lane, n_lists = min(lists - l0, (uint32_t)kWave);
+      Span at{};
+      if (l < lists && (l * kList < ahead || l == (uint32_t)token_lists(A.n_ids))) at = span_of(l);
+      some |= __ballot(at.from != at.to) != 0;
+      for (uint32_t k = wave; k < n_lists; k += kWaves) {
+        const uint32_t k_from = __builtin_amdgcn_readlane(at.from, k), k_mid = __builtin_amdgcn_readlane(at.mid, k),
+                       k_to = __builtin_amdgcn_readlane(at.to, k);
+        for (uint32_t i = k_from; i < k_to; i += kDeep * kWave) {
+          uint32_t w[kDeep];
+#pragma unroll
+          for (int d = 0; d < kDeep; ++d) w[d] = entries[min(i + d * kWave + lane, k_to - 1)];
+#pragma unroll
+          for (int d = 0; d < kDeep; ++d)
+            if (i + d * kWave + lane < k_to) count(w[d], i + d * kWave + lane, k_mid);
+        }
+      }
     }
   }
   const uint64_t new_rows = __ballot(m_new >= 0);
@@ -490,7 +529,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   int listed = 0, h_col = -1;
   uint32_t h_word = 0;
   float h_bias = 0.f;
-  if (begin[NV] != begin[0]) {
+  if (some) {
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const vu4 lo = words[u * kU], hi = words[u * kU + 1];
@@ -954,13 +993,14 @@ Params params_of(const mirl_logit_processors* A, const uint32_t* table, const vo
   const int64_t n = A->vocab_end - A->vocab_start;
   P.n_vocab = n < 0 ? 0 : n < V ? n : V;
   P.buckets = ceil_div(V, kBucket);
+  P.lists = token_lists(A->n_ids) + (A->n_bias > 0);
   P.table = table;
   return P;
 }
 
 int make_table(const Params& P, int64_t rows, uint32_t* table, const char* what, hipStream_t st) {
-  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)P.B), dim3(kTableThreads), 0, st, P.A, P.B, rows, P.n_vocab,
-                     (int)P.buckets, table);
+  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)(P.B * P.lists)), dim3(kTableThreads), 0, st, P.A, rows, P.n_vocab,
+                     P.lists, (int)P.buckets, table);
   return check_launch(what);
 }
 
@@ -971,7 +1011,7 @@ using namespace mirl;
 
 extern "C" int64_t mirl_logit_processors_table_elems(int64_t B, int64_t V, int64_t n_ids, int64_t n_bias) {
   if (B <= 0 || V <= 0 || n_ids < 0 || n_bias < 0) return 0;
-  return B * (kHead + ceil_div(V, kBucket) + 1 + n_ids + n_bias);
+  return B * (head_words(token_lists(n_ids) + (n_bias > 0), ceil_div(V, kBucket)) + n_ids + n_bias);
 }
 
 extern "C" int64_t mirl_processed_logprob_workspace_elems(int64_t B, int64_t R, int64_t V) {

@@ -202,3 +202,41 @@ def test_saved_tensor_hooks_may_move_what_is_kept():
     with torch.autograd.graph.save_on_cpu():
         _, got = gradient(x, ids, P, g)
     assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+# histories of several lists of tokens, rows that cross from one to the next, and one that ends with it
+@pytest.mark.parametrize("dtype,V,R,K,M", [(torch.float32, 700, 3, 0, 0), (torch.bfloat16, 5003, 3, 9, 3), (torch.float16, 2049, 1, 300, 0),
+                                           (torch.bfloat16, 141001, 30, 40, 0), (torch.float16, 141001, 30, 0, 3)])
+def test_histories_of_several_lists(dtype, V, R, K, M):
+    lengths = torch.tensor([8191, 12290] if V > 100000 else [0, 4095, 4096, 4097, 8190, 8193, 12290])
+    B, L = len(lengths), 12291 + R
+    x, ids, P, _ = make(B, R, L, V, dtype, seed=V + K, K=K, M=M)
+    h = torch.Generator().manual_seed(8)
+    some = torch.randint(0, V, (120,), generator=h)  # (the oracle takes one token at a time)
+    ids = torch.where(torch.rand(B, L, generator=h) < 0.4, some[torch.randint(0, 120, (B, L), generator=h)], ids % 7 + V // 2)
+    if K:
+        P.bias_ids[:, K // 2:] = P.bias_ids[:, : K - K // 2]  # of two of one token the later holds
+    P.prompt_lengths = (lengths - 4200).clamp(min=1)
+    A, T = magnitude(x, P, L), least_t(P)
+    want = oracle.process(x, ids, P, lengths)
+    args = (ids.cuda(), cuda(P), lengths.cuda())
+    check_values(apply_logit_processors(x.cuda(), *args), want, A, T, dtype)
+    check_values(apply_logit_processors(x.cuda(), *args, inplace=True), want, A, T, dtype)
+    t = x.cuda().requires_grad_(True)
+    lp = processed_next_token_logprobs(t, *args)
+    xo = x.double().requires_grad_(True)
+    lpo = oracle.logprobs(xo, ids, P, lengths)
+    check_logprobs(lp.detach(), lpo.detach(), A, T)
+    g = torch.where(lpo.detach().isfinite(), torch.randn(B, R, generator=torch.Generator().manual_seed(2)), torch.zeros(()))
+    (dx,) = torch.autograd.grad([lp], [t], [g.cuda()])
+    (dxo,) = torch.autograd.grad([torch.where(g != 0, lpo, torch.zeros_like(lpo)).mul(g.double()).sum()], [xo])
+    check_grad(dx, dxo.nan_to_num(0.0), A, T, dtype, g, P.repetition_penalty.max().item() / T)
+    y = apply_logit_processors(t, *args)
+    dy = torch.randn(x.shape, generator=torch.Generator().manual_seed(3)).to(dtype)
+    (da,) = torch.autograd.grad([y], [t], [dy.cuda()])
+    yo = oracle.process(xo, ids, P, lengths)
+    (dao,) = torch.autograd.grad([torch.where(yo.isfinite(), yo, torch.zeros_like(yo)).mul(dy.double()).sum()], [xo])
+    # dy times two factors, three roundings in fp32 and one to the type
+    fine = yo.detach().isfinite()
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((da.double().cpu() - dao).abs() <= dao.abs() * (half + 2**-21) + torch.finfo(dtype).smallest_normal)[fine].all())
