@@ -8,7 +8,8 @@
 //   logprob_t = (y_t - M) - log(sum_j exp(y_j - M)),   dx_j = slope_j (onehot_j - p_j) g
 // with y never written; slope is what z multiplies x by, over T, 0 where the grammar forbids j.
 //
-// A first launch puts each sample's tokens and biases into buckets by 2048 columns (processors_table_kernel).
+// A first launch puts each sample's tokens, 4096 at a time, and its biases into buckets by 2048 columns
+// (processors_table_kernel).
 // A workgroup then owns a slice of the vocabulary, one or more buckets, for a run of rows of one sample,
 // and each lane the same groups of eight tokens in all of them: it counts the bucket's tokens ahead of its
 // first row with LDS atomics (whole numbers: their order does not matter), and from then on a row's
@@ -22,7 +23,7 @@
 // a gradient: forward 920 us (4.98 GB, 5.4 TB/s; 860 where no token of the rows occurs, logprob.hip's of untouched
 // logits 730), backward 1.36 to 1.43 ms (7.4 GB, 5.3 TB/s; logprob.hip's 1.22).  [2, 2048, 151936]: written out
 // 412 us (2.49 GB, 6.0 TB/s), its backward 495 (5.0; the logits of tokens that occur are read as well).  One token of
-// each of 64 requests behind up to 2048 tokens: table 8 us, logprobs 13 and 4 to join, written out 15: the
+// each of 64 requests behind up to 2048 tokens: table 7 us, logprobs 14 and 4 to join, written out 16: the
 // latency of a few loads that wait for each other.
 
 #include "common.h"
@@ -217,8 +218,9 @@ __device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t h
 
 // Buckets of a list of one sample's tokens (those that any of the R rows follows), or of its biases.  An entry's place
 // in its bucket comes from an atomic: the order differs from run to run, what is counted does not.  A workgroup
-// has kList tokens, so that a long history is spread over the chip (one row behind 131072 tokens, written out: 16 us with even ones, 57 with
-// Zipf-like ones, of which one slice has most; by one workgroup 94 and 206).
+// has kList tokens, so that a long history is spread over the chip: one row of 151936 logits behind 131072 tokens,
+// written out, takes 16 us where they are spread evenly and 56 where they follow Zipf's law (most in one slice, which
+// one workgroup counts); with one workgroup for all of them 94 and 206.
 __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t R, int64_t n_vocab,
                                                                          int64_t lists, int buckets, uint32_t* table) {
   __shared__ uint32_t s_at[kMaxBuckets];
@@ -482,15 +484,24 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   };
   __syncthreads();
   bool some = false;
+  // Loads under way at a time (one row behind 8192 tokens, of which one slice has most: 14.5 us with four for a
+  // thread, 16.6 with one; behind 131072 with eight 56, with four 65).
+  constexpr int kFew = 4, kMany = 8;
   if (few) {  // one after the other; what leads to them is loaded by scalars, ahead of all this
     const uint32_t n = first_span.to - first_span.from, all = n + second_span.to - second_span.from;
     some = all != 0;
-    for (uint32_t k = tid; k < all; k += kThreads) {
-      const uint32_t i = k + (k < n ? first_span.from : second_span.from - n);
-      count(entries[i], i, k < n ? first_span.mid : second_span.mid);
+    auto place = [&](uint32_t k) { return k + (k < n ? first_span.from : second_span.from - n); };
+    for (uint32_t k0 = 0; k0 < all; k0 += kFew * kThreads) {
+      uint32_t w[kFew];
+#pragma unroll
+      for (int d = 0; d < kFew; ++d) w[d] = entries[place(min(k0 + d * kThreads + tid, all - 1))];
+#pragma unroll
+      for (int d = 0; d < kFew; ++d) {
+        const uint32_t k = k0 + d * kThreads + tid;
+        if (k < all) count(w[d], place(k), k < n ? first_span.mid : second_span.mid);
+      }
     }
-  } else {  // each wave a list, those behind the first row left out, with some loads under way at a time
-    constexpr int kDeep = 8;
+  } else {  // each wave a list, those behind the first row left out
     for (uint32_t l0 = 0; l0 < lists; l0 += kWave) {
       const uint32_t l = l0 + lane, n_lists = min(lists - l0, (uint32_t)kWave);
       Span at{};
@@ -499,12 +510,12 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       for (uint32_t k = wave; k < n_lists; k += kWaves) {
         const uint32_t k_from = __builtin_amdgcn_readlane(at.from, k), k_mid = __builtin_amdgcn_readlane(at.mid, k),
                        k_to = __builtin_amdgcn_readlane(at.to, k);
-        for (uint32_t i = k_from; i < k_to; i += kDeep * kWave) {
-          uint32_t w[kDeep];
+        for (uint32_t i = k_from; i < k_to; i += kMany * kWave) {
+          uint32_t w[kMany];
 #pragma unroll
-          for (int d = 0; d < kDeep; ++d) w[d] = entries[min(i + d * kWave + lane, k_to - 1)];
+          for (int d = 0; d < kMany; ++d) w[d] = entries[min(i + d * kWave + lane, k_to - 1)];
 #pragma unroll
-          for (int d = 0; d < kDeep; ++d)
+          for (int d = 0; d < kMany; ++d)
             if (i + d * kWave + lane < k_to) count(w[d], i + d * kWave + lane, k_mid);
         }
       }
