@@ -158,7 +158,10 @@ def test_the_c_entry_points():
     assert lib.mirl_process_logits(one, 0, 2, 1, V, V, V, ctypes.byref(_C.LogitProcessorArgs()), one, one, V + 1, V, None) != 0
     assert "in place" in lib.mirl_last_error().decode()
     assert lib.mirl_processed_logprob_bwd(None, 0, 1, 3, 2, V, V, V, ctypes.byref(_C.LogitProcessorArgs()), *none[:3], 1, 1, None, V, V, None) != 0
-    assert lib.mirl_logit_processors_table_elems(2, 5000, 10, 3) == 2 * (8 + 3 + 1 + 10 + 3)
+    # a sample's head, where the three buckets of each list begin and the last ends (tokens, 4096 a list; biases), the entries
+    assert lib.mirl_logit_processors_table_elems(2, 5000, 10, 3) == 2 * (8 + 2 * (3 + 1) + 10 + 3)
+    assert lib.mirl_logit_processors_table_elems(2, 5000, 0, 0) == 2 * (8 + 3 + 1)
+    assert lib.mirl_logit_processors_table_elems(1, 5000, 4097, 0) == 8 + 2 * (3 + 1) + 4097
 
 
 # ---------------------------------------------------------------------------
