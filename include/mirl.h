@@ -1065,8 +1065,9 @@ int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t B, int64_t
 
 /*
  * Its backward: grad_in [B, Rt, V] in the logits' type, zeros in rows R .. Rt - 1, in rows
- * whose upstream gradient (grad_out [B, R] by strides) is zero and in rows that allow
- * nothing; those rows' logits are not read.
+ * whose upstream gradient (grad_out [B, R] by strides) is zero, in rows that allow nothing
+ * and in rows without a token (their result is the constant 0); those rows' logits are not
+ * read.
  */
 int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t Rt,
                                int64_t V, int64_t stride_b, int64_t stride_r,

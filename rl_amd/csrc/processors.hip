@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       m_g = P.g[b * P.gsb + r * P.gsr];
       m_M = P.stats[(b * P.R + r) * 2];
       m_ls = P.stats[(b * P.R + r) * 2 + 1];
-      if (m_M == -INFINITY && m_ls == -INFINITY) m_g = 0.f;  // nothing was left in the row
+      if (m_M == -INFINITY && m_ls == -INFINITY) m_g = 0.f;  // nothing was left in the row, or it has no next token
     }
     uint64_t zeros = todo;
     todo = __ballot(m_g != 0.f);
@@ -898,12 +898,11 @@ __global__ __launch_bounds__(kThreads) void processors_join_kernel(Params P, flo
   const int64_t at = S.n + r;
   const int64_t t = at >= 0 && at < A.n_ids ? A.ids[b * A.ids_stride_b + at * A.ids_stride_s] - A.vocab_start : -1;
   const float logsum = logf(s);
-  float lp = 0.f;
-  if (t >= 0 && t < P.n_vocab) lp = M == -INFINITY && s == 0.f ? -INFINITY : (P.xt[row] - M) * inv_t - logsum;
-  out[row] = lp;
-  if (stats != nullptr) {
-    stats[2 * row] = M;
-    stats[2 * row + 1] = logsum;
+  const bool scored = t >= 0 && t < P.n_vocab;
+  out[row] = !scored ? 0.f : M == -INFINITY && s == 0.f ? -INFINITY : (P.xt[row] - M) * inv_t - logsum;
+  if (stats != nullptr) {  // (a constant 0 has no gradient, as a row in which nothing is left)
+    stats[2 * row] = scored ? M : -INFINITY;
+    stats[2 * row + 1] = scored ? logsum : -INFINITY;
   }
 }
 

@@ -215,8 +215,9 @@ def processed_next_token_logprobs(
     ``input_ids[:, r + 1]``, and there are ``min(R, L - 1)`` results.  With ``history_lengths [B]`` row r
     follows the first ``history_lengths[b] + r`` tokens and is scored against the token behind them; a
     row whose token ``input_ids`` does not hold gives 0, as does a token outside ``[vocab_start_index,
-    vocab_end_index)``.  A token that its row does not allow gives -inf, and a row that allows nothing has no
-    gradient."""
+    vocab_end_index)``: a constant, without a gradient (the logprobs of unprocessed logits, whose ranges may be the
+    parts of a sharded vocabulary, leave the probabilities' gradient there).  A token that its row does not
+    allow gives -inf, and a row that allows nothing has no gradient."""
     if logits.dim() != 3:
         raise ValueError(f"expected logits of shape [B, R, V], got {tuple(logits.shape)}")
     R = logits.shape[1]
