@@ -1095,6 +1095,22 @@ int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R,
                             int64_t g_stride_b, int64_t g_stride_r, void* grad_in,
                             int64_t gi_stride_b, int64_t gi_stride_r, void* stream);
 
+/*
+ * The same with y, and the gradient that comes back, in fp32 whatever the logits' type (grad_in
+ * has the logits' type): what top-k and top-p read next.  out is not the logits.
+ */
+int mirl_process_logits_f32(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
+                            int64_t stride_b, int64_t stride_r,
+                            const mirl_logit_processors* processors,
+                            uint32_t* table, float* out,
+                            int64_t o_stride_b, int64_t o_stride_r, void* stream);
+int mirl_process_logits_f32_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
+                                int64_t stride_b, int64_t stride_r,
+                                const mirl_logit_processors* processors,
+                                const uint32_t* table, const float* grad_out,
+                                int64_t g_stride_b, int64_t g_stride_r, void* grad_in,
+                                int64_t gi_stride_b, int64_t gi_stride_r, void* stream);
+
 /* ---------------------------------------------------------------------- */
 /* Logprobs from hidden states with low-rank adapters beside the weight     */
 /* ---------------------------------------------------------------------- */

@@ -346,6 +346,9 @@ SIGNATURES = {
     "mirl_process_logits": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P]),
     "mirl_process_logits_bwd": (
         _I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
+    "mirl_process_logits_f32": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P]),
+    "mirl_process_logits_f32_bwd": (
+        _I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
 }
 
@@ -1335,28 +1338,31 @@ def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table:
     return grad
 
 
-def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """(processed logits, table): in place or as a new contiguous tensor (see mirl_process_logits)."""
+def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool, f32: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """(processed logits, table): in place, or as a new contiguous tensor of the logits' type or with ``f32`` of fp32
+    (see mirl_process_logits and mirl_process_logits_f32)."""
     dev = logits.device
     B, R, V = logits.shape
-    out = logits if inplace else torch.empty((B, R, V), dtype=logits.dtype, device=dev)
+    out = logits if inplace else torch.empty((B, R, V), dtype=torch.float32 if f32 else logits.dtype, device=dev)
     table = torch.empty(_processor_elems(B, R, V, args.n_ids, args.n_bias)[1], dtype=torch.int32, device=dev)
-    _processors("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
-                ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1))
+    _processors("mirl_process_logits_f32" if f32 else "mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V,
+                logits.stride(0), logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1))
     return out, table
 
 
-def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, grad_out: torch.Tensor) -> torch.Tensor:
-    """The gradient of the logits, a new contiguous tensor (see mirl_process_logits_bwd)."""
+def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, grad_out: torch.Tensor,
+                       f32: bool = False) -> torch.Tensor:
+    """The gradient of the logits, a new contiguous tensor (see mirl_process_logits_bwd and, with ``f32``,
+    mirl_process_logits_f32_bwd)."""
     dev = _require_gpu(logits, grad_out)
     B, R, V = logits.shape
-    _require(grad_out.dtype == logits.dtype and grad_out.shape == logits.shape, "a gradient like the logits")
+    _require(grad_out.dtype == (torch.float32 if f32 else logits.dtype) and grad_out.shape == logits.shape, "a gradient like the processed logits")
     if grad_out.stride(-1) != 1:
         grad_out = grad_out.contiguous()
     grad = torch.empty((B, R, V), dtype=logits.dtype, device=dev)
-    _processors("mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
-                ctypes.byref(args), table.data_ptr(), grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1),
-                grad.data_ptr(), grad.stride(0), grad.stride(1))
+    _processors("mirl_process_logits_f32_bwd" if f32 else "mirl_process_logits_bwd", dev, logits.data_ptr(), _dtype_code(logits), B, R, V,
+                logits.stride(0), logits.stride(1), ctypes.byref(args), table.data_ptr(), grad_out.data_ptr(), grad_out.stride(0),
+                grad_out.stride(1), grad.data_ptr(), grad.stride(0), grad.stride(1))
     return grad
 
 

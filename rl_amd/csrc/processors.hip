@@ -56,7 +56,8 @@ static_assert(2 * kBiasSlots <= kMaxBuckets && kMaxBias < kBiasSlots, "the biase
 static_assert(kBucket == kThreads * kG, "a slice is a whole number of buckets");
 static_assert(kCountBits + kBucketBits <= 31, "an entry holds a token's place and column");
 
-enum Mode { kFwd, kBwd, kApply, kInPlace, kApplyGrad };
+// kWide, kWideGrad: y, and its gradient, in fp32 whatever the logits' type (a filter reads them next).
+enum Mode { kFwd, kBwd, kApply, kInPlace, kApplyGrad, kWide, kWideGrad };
 
 struct Params {
   mirl_logit_processors A;
@@ -70,7 +71,7 @@ struct Params {
   int rows;              // rows of a workgroup
   void* y;               // processed logits, or a gradient
   int64_t ysb, ysr;
-  const void* dy;        // kApplyGrad
+  const void* dy;        // kApplyGrad, kWideGrad
   int64_t gsb, gsr;      // strides of g, or of dy
   const float* g;        // kBwd [B, R]
   const float* stats;    // kBwd [B, R, 2]
@@ -330,6 +331,10 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
 template <class E, int MODE, int NV, bool MASKED>
 __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   using raw = typename E::raw;
+  constexpr bool kWritten = MODE == kApply || MODE == kWide, kGradOfY = MODE == kApplyGrad || MODE == kWideGrad;
+  using EY = std::conditional_t<MODE == kWide || MODE == kWideGrad, F32, E>;  // of y and its gradient
+  using EI = std::conditional_t<kGradOfY, EY, E>;                             // of the values a row is read as: logits, or y's gradient
+  using EO = std::conditional_t<MODE == kWide, F32, E>;                       // of what is written
   constexpr int kWaveCols = kWave * NV * kG, kSlice = kWaves * kWaveCols;
   constexpr int kPacks = (NV + 3) / 4;  // four groups' bytes in a word
   __shared__ __align__(16) uint32_t s_word[kSlice];
@@ -364,18 +369,25 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 
   const int g0 = wave * NV * kWave + lane;  // group u of the lane: g0 + 64 u
   const raw* xr = static_cast<const raw*>(P.x) + b * P.xsb + r0 * P.xsr + n0;
-  const raw* dyr = MODE == kApplyGrad ? static_cast<const raw*>(P.dy) + b * P.gsb + r0 * P.gsr + n0 : nullptr;
-  raw* yr = MODE == kFwd ? nullptr : static_cast<raw*>(P.y) + b * P.ysb + r0 * P.ysr + n0;
+  const typename EY::raw* dyr = kGradOfY ? static_cast<const typename EY::raw*>(P.dy) + b * P.gsb + r0 * P.gsr + n0 : nullptr;
+  typename EO::raw* yr = MODE == kFwd ? nullptr : static_cast<typename EO::raw*>(P.y) + b * P.ysb + r0 * P.ysr + n0;
   const uint32_t left = (uint32_t)min((int64_t)kSlice, P.V - n0);  // columns of the slice
-  const uint32_t at0 = g0 * kGroupBytes<E>;
   auto col = [&](int u) { return (uint32_t)(g0 + u * kWave) * kG; };
-  auto put = [&](raw* row, int u, const float (&v)[kG], bool whole) __attribute__((always_inline)) {
+  const uint32_t at0 = g0 * kGroupBytes<E>;
+  auto group_at = [&](auto t, int u) -> uint32_t {  // of t's elements, in bytes
+    constexpr uint32_t bytes = kGroupBytes<decltype(t)>;
+    if constexpr (bytes == kGroupBytes<E>)
+      return at0 + u * kWave * bytes;
+    else
+      return (uint32_t)(g0 + u * kWave) * bytes;
+  };
+  auto put = [&](typename EO::raw* row, int u, const float (&v)[kG], bool whole) __attribute__((always_inline)) {
     if (whole || col(u) + kG <= left) {
-      store_group<E>(row, at0 + u * kWave * kGroupBytes<E>, v);
+      store_group<EO>(row, group_at(EO{}, u), v);
     } else {
 #pragma unroll
       for (int e = 0; e < kG; ++e)
-        if (col(u) + e < left) row[col(u) + e] = E::from_float(v[e]);
+        if (col(u) + e < left) row[col(u) + e] = EO::from_float(v[e]);
     }
   };
 
@@ -396,17 +408,21 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
     zeros &= ~todo;
     const float z[kG] = {};
     for (; zeros != 0; zeros &= zeros - 1) {
-      raw* row = yr + __builtin_ctzll(zeros) * P.ysr;
+      typename EO::raw* row = yr + __builtin_ctzll(zeros) * P.ysr;
 #pragma unroll
       for (int u = 0; u < NV; ++u) put(row, u, z, false);
     }
     if (todo == 0) return;  // (the same in all waves)
   }
   // The first row's values are on their way while the tokens are counted.
-  vu4 q[NV][kP<E>];
+  vu4 q[NV][kP<EI>];
   auto issue = [&](int i, int u, bool whole, uint32_t keep) __attribute__((always_inline)) {
-    const raw* row = MODE == kApplyGrad ? dyr + i * P.gsr : xr + i * P.xsr;
-    if (whole || col(u) + kG <= left) load_group<E>(row, (at0 + u * kWave * kGroupBytes<E>) & keep, q[u]);
+    const typename EI::raw* row;
+    if constexpr (kGradOfY)
+      row = dyr + i * P.gsr;
+    else
+      row = xr + i * P.xsr;
+    if (whole || col(u) + kG <= left) load_group<EI>(row, group_at(EI{}, u) & keep, q[u]);
   };
   const int first = __builtin_ctzll(todo);
   if constexpr (MODE != kInPlace) {
@@ -634,15 +650,15 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   // and a row waits for its own values only.
   auto rows = [&](auto whole_c) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole_c)::value;
-    auto tail = [&](const raw* row, int u, float fill, float (&v)[kG]) {
+    auto tail = [&](auto et, const auto* row, int u, float fill, float (&v)[kG]) {
 #pragma unroll
-      for (int e = 0; e < kG; ++e) v[e] = col(u) + e < left ? E::load(row + col(u) + e) : fill;
+      for (int e = 0; e < kG; ++e) v[e] = col(u) + e < left ? decltype(et)::load(row + col(u) + e) : fill;
     };
     auto full = [&](int u) { return WHOLE || col(u) + kG <= left; };
-    // a row's mask bytes; kApplyGrad: the logits of groups with a word (as they come: what converts them would
+    // a row's mask bytes; with y's gradient, the logits of groups with a word (as they come: what converts them would
     // wait here)
     uint8_t mk[NV];
-    vu4 qx[MODE == kApplyGrad ? NV : 1][kP<E>];
+    vu4 qx[kGradOfY ? NV : 1][kP<E>];
     auto mask_of = [&](int i) {
       const int m = __builtin_amdgcn_readlane(m_mask, i);
       return reinterpret_cast<const uint8_t*>(A.masks + (int64_t)max(m, 0) * A.mask_stride) + n0 / kG;
@@ -653,10 +669,10 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       }
     };
     auto issue_words = [&](int i) __attribute__((always_inline)) {
-      if constexpr (MODE == kApplyGrad) {
+      if constexpr (kGradOfY) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
-          if (full(u)) load_group<E>(xr + i * P.xsr, lane_bits(u) != 0 ? at0 + u * kWave * kGroupBytes<E> : 0, qx[u]);
+          if (full(u)) load_group<E>(xr + i * P.xsr, lane_bits(u) != 0 ? group_at(E{}, u) : 0, qx[u]);
       }
     };
 #pragma unroll
@@ -668,8 +684,12 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
       const bool more = todo != 0;
       const int next = more ? __builtin_ctzll(todo) : i;
       const bool masked = MASKED && __builtin_amdgcn_readlane(m_mask, i) >= 0;
-      const raw* row = MODE == kApplyGrad ? dyr + i * P.gsr : xr + i * P.xsr;
-      raw* y_row = MODE == kFwd ? nullptr : yr + i * P.ysr;
+      const typename EI::raw* row;
+      if constexpr (kGradOfY)
+        row = dyr + i * P.gsr;
+      else
+        row = xr + i * P.xsr;
+      typename EO::raw* y_row = MODE == kFwd ? nullptr : yr + i * P.ysr;
       uint32_t allowed[NV];
       // group u of this row, and the next row's on its way
       auto take = [&](int u, float fill, float (&v)[kG]) __attribute__((always_inline)) {
@@ -688,9 +708,9 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
               for (int j = 0; j < 4; ++j) q[u][k][j] = either(left_out[j], E::kNegInf2, q[u][k][j]);
             }
           }
-          unpack_group<E>(q[u], v);
+          unpack_group<EI>(q[u], v);
         } else {
-          tail(row, u, fill, v);
+          tail(EI{}, row, u, fill, v);
           if constexpr (kLists) {
 #pragma unroll
             for (int e = 0; e < kG; ++e) s_row[col(u) + e] = E::from_float(v[e]);  // (exact)
@@ -801,7 +821,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           }
           put(y_row, u, o, WHOLE);
         }
-      } else if constexpr (MODE == kApply) {
+      } else if constexpr (kWritten) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           float v[kG];
@@ -816,7 +836,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           }
           put(y_row, u, v, WHOLE);
         }
-      } else if constexpr (MODE == kApplyGrad) {
+      } else if constexpr (kGradOfY) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           float v[kG];
@@ -828,7 +848,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
             if (full(u))
               unpack_group<E>(qx[u], x);
             else
-              tail(xr + i * P.xsr, u, 0.f, x);
+              tail(E{}, xr + i * P.xsr, u, 0.f, x);
             const uint32_t how =
                 special(x, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
             through(v, wave_bits(u), how, S);
@@ -849,10 +869,10 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           float v[kG];
           if (full(u)) {
             vu4 w[kP<E>];
-            load_group<E>(row, at0 + u * kWave * kGroupBytes<E>, w);
+            load_group<E>(row, group_at(E{}, u), w);
             unpack_group<E>(w, v);
           } else {
-            tail(row, u, 0.f, v);
+            tail(E{}, row, u, 0.f, v);
           }
           special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
@@ -1066,28 +1086,35 @@ extern "C" int mirl_processed_logprob_bwd(const void* logits, int dtype, int64_t
   return launch<kBwd>(P, dtype, Rt, "mirl_processed_logprob_bwd", static_cast<hipStream_t>(stream));
 }
 
-extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                   int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, void* out,
-                                   int64_t o_stride_b, int64_t o_stride_r, void* stream) {
+namespace mirl {
+namespace {
+// MODE: kApply (which becomes kInPlace where out is the logits) or kWide.
+template <int MODE>
+int write_processed(const char* what, const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b, int64_t stride_r,
+                    const mirl_logit_processors* processors, uint32_t* table, void* out, int64_t o_stride_b, int64_t o_stride_r,
+                    void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
   MIRL_REQUIRE(table && logits && out, "null pointer argument");
-  MIRL_REQUIRE(out != logits || (o_stride_b == stride_b && o_stride_r == stride_r), "in place, the strides are those of the logits");
+  MIRL_REQUIRE(MODE == kApply ? out != logits || (o_stride_b == stride_b && o_stride_r == stride_r) : out != logits,
+               MODE == kApply ? "in place, the strides are those of the logits" : "fp32 values are not written in place");
   Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   P.y = out;
   P.ysb = o_stride_b;
   P.ysr = o_stride_r;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int e = make_table(P, R, table, "mirl_process_logits", st)) return e;
-  return out == logits ? launch<kInPlace>(P, dtype, R, "mirl_process_logits", st)
-                       : launch<kApply>(P, dtype, R, "mirl_process_logits", st);
+  if (int e = make_table(P, R, table, what, st)) return e;
+  if constexpr (MODE == kApply) {
+    if (out == logits) return launch<kInPlace>(P, dtype, R, what, st);
+  }
+  return launch<MODE>(P, dtype, R, what, st);
 }
 
-extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
-                                       int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, const void* grad_out,
-                                       int64_t g_stride_b, int64_t g_stride_r, void* grad_in, int64_t gi_stride_b,
-                                       int64_t gi_stride_r, void* stream) {
+template <int MODE>
+int write_gradient(const char* what, const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b, int64_t stride_r,
+                   const mirl_logit_processors* processors, const uint32_t* table, const void* grad_out, int64_t g_stride_b,
+                   int64_t g_stride_r, void* grad_in, int64_t gi_stride_b, int64_t gi_stride_r, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
@@ -1099,5 +1126,37 @@ extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B,
   P.y = grad_in;
   P.ysb = gi_stride_b;
   P.ysr = gi_stride_r;
-  return launch<kApplyGrad>(P, dtype, R, "mirl_process_logits_bwd", static_cast<hipStream_t>(stream));
+  return launch<MODE>(P, dtype, R, what, static_cast<hipStream_t>(stream));
+}
+}  // namespace
+}  // namespace mirl
+
+extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
+                                   int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, void* out,
+                                   int64_t o_stride_b, int64_t o_stride_r, void* stream) {
+  return write_processed<kApply>("mirl_process_logits", logits, dtype, B, R, V, stride_b, stride_r, processors, table, out,
+                                 o_stride_b, o_stride_r, stream);
+}
+
+extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
+                                       int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table, const void* grad_out,
+                                       int64_t g_stride_b, int64_t g_stride_r, void* grad_in, int64_t gi_stride_b,
+                                       int64_t gi_stride_r, void* stream) {
+  return write_gradient<kApplyGrad>("mirl_process_logits_bwd", logits, dtype, B, R, V, stride_b, stride_r, processors, table, grad_out,
+                                    g_stride_b, g_stride_r, grad_in, gi_stride_b, gi_stride_r, stream);
+}
+
+extern "C" int mirl_process_logits_f32(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
+                                       int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, float* out,
+                                       int64_t o_stride_b, int64_t o_stride_r, void* stream) {
+  return write_processed<kWide>("mirl_process_logits_f32", logits, dtype, B, R, V, stride_b, stride_r, processors, table, out,
+                                o_stride_b, o_stride_r, stream);
+}
+
+extern "C" int mirl_process_logits_f32_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
+                                           int64_t stride_r, const mirl_logit_processors* processors, const uint32_t* table,
+                                           const float* grad_out, int64_t g_stride_b, int64_t g_stride_r, void* grad_in,
+                                           int64_t gi_stride_b, int64_t gi_stride_r, void* stream) {
+  return write_gradient<kWideGrad>("mirl_process_logits_f32_bwd", logits, dtype, B, R, V, stride_b, stride_r, processors, table,
+                                   grad_out, g_stride_b, g_stride_r, grad_in, gi_stride_b, gi_stride_r, stream);
 }

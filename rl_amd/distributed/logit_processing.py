@@ -163,13 +163,14 @@ class _ProcessedLogprob(torch.autograd.Function):
 
 
 class _ProcessLogits(torch.autograd.Function):
-    """Processed logits as a new tensor.  The backward reads the logits of the tokens that occur."""
+    """Processed logits as a new tensor, of their type or in fp32.  The backward reads the logits of the tokens that occur."""
 
     @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, call: _Call) -> torch.Tensor:  # type: ignore[override]
-        out, table = _C.process_logits(logits, call.args(), False)
+    def forward(ctx: Any, logits: torch.Tensor, call: _Call, f32: bool) -> torch.Tensor:  # type: ignore[override]
+        out, table = _C.process_logits(logits, call.args(), False, f32)
         ctx.save_for_backward(logits, table, call.ids, *call.tensors)
         ctx.numbers = (call.scalars, call.vocab)
+        ctx.f32 = f32
         return out
 
     @staticmethod
@@ -179,7 +180,7 @@ class _ProcessLogits(torch.autograd.Function):
     @staticmethod
     def _grads(ctx: Any, grad: torch.Tensor):
         logits, table, ids, *tensors = ctx.saved_tensors
-        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad), None
+        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad, ctx.f32), None, None
 
     _once = staticmethod(once_differentiable(_grads.__func__))
 
@@ -232,6 +233,31 @@ def processed_next_token_logprobs(
     return _ProcessedLogprob.apply(logits, R, call)
 
 
+def filtered_processed_logprobs(
+    logits: torch.Tensor,
+    target: torch.Tensor,
+    processors: Any,
+    top_k: Optional[int],
+    top_p: Optional[float],
+    inference_only: bool,
+) -> torch.Tensor:
+    """fp32 logprobs ``[B, S - 1]`` of the next tokens of ``target [B, S]`` under the processors and the filter behind
+    them, from ``logits [B, >= S, V]``.
+
+    The processed logits are written once, in fp32 whatever the type of the logits: what is held in 16 bits between the two would
+    be off by half a step there (2^-4 at 16), and the cut would be decided on that.  Top-p is therefore
+    decided in fp32, as a sampler decides it."""
+    from rl_amd.distributed.sampling import filtered_row_logprobs
+
+    x = logits[:, : max(target.shape[1] - 1, 0)]
+    call = _Call(x, target, processors, None, x.shape[1], (0, x.shape[2]))
+    if inference_only or not _grad_needed(logits):
+        y, _ = _C.process_logits(x, call.args(), False, True)
+    else:
+        y = _ProcessLogits.apply(x, call, True)
+    return filtered_row_logprobs(y, target[:, 1:], top_k, top_p, inference_only=inference_only)
+
+
 def process_logits(
     logits: torch.Tensor,
     input_ids: torch.Tensor,
@@ -256,7 +282,7 @@ def process_logits(
         x = x.contiguous()
     call = _Call(x, input_ids, processors, history_lengths, x.shape[1], (0, x.shape[2]))
     if not inplace and _grad_needed(logits):
-        y = _ProcessLogits.apply(x, call)
+        y = _ProcessLogits.apply(x, call, False)
         return y if logits.dim() == 3 else y.squeeze(1)
     y, _ = _C.process_logits(x, call.args(), inplace)
     if inplace:

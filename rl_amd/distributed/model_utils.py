@@ -449,7 +449,8 @@ def from_parallel_logits_to_logprobs(
     the reference's DistributedLogprobWithSampling does on this tensor.
     ``logit_processors`` (an extension: penalties, biases, grammar masks and temperature of the
     sampler) come ahead of the filter; ``target`` is also the history that they count.  Without
-    a filter the processed logits are never written, with one they are, in the logits' type.
+    a filter the processed logits are never written, with one they are, in fp32, and top-p is decided
+    in fp32.
     """
     return _next_token_logprobs(vocab_parallel_logits, target, vocab_start_index,
                                 vocab_end_index, tp_group, inference_only, cp_group, chunk_size,
@@ -463,20 +464,14 @@ def _next_token_logprobs(logits, target, vocab_start_index, vocab_end_index, tp_
     _check_chunk_size(chunk_size)
     logits = _check_logits(logits)
     if logit_processors is not None:
-        from rl_amd.distributed.logit_processing import process_logits, processed_next_token_logprobs
+        from rl_amd.distributed.logit_processing import filtered_processed_logprobs, processed_next_token_logprobs
 
-        tgt = _next_token_targets(target, logits.shape[1])  # (the checks of the plain path)
+        _next_token_targets(target, logits.shape[1])  # (the checks of the plain path)
         if not need_top_k_or_top_p_filtering(sampling_params):
             return processed_next_token_logprobs(
                 logits, target, logit_processors, None, inference_only, vocab_start_index, vocab_end_index)
-        from rl_amd.distributed.sampling import filtered_row_logprobs
-
-        with torch.set_grad_enabled(torch.is_grad_enabled() and not inference_only):
-            rows = process_logits(logits[:, : tgt.shape[1]], target, logit_processors)
-        return filtered_row_logprobs(
-            rows, tgt, sampling_params.top_k, sampling_params.top_p,  # type: ignore[union-attr]
-            inference_only=inference_only, decision_dtype=decision_dtype,
-        )
+        return filtered_processed_logprobs(
+            logits, target, logit_processors, sampling_params.top_k, sampling_params.top_p, inference_only)  # type: ignore[union-attr]
     if need_top_k_or_top_p_filtering(sampling_params):
         from rl_amd.distributed.sampling import filtered_next_token_logprobs
 

@@ -1,0 +1,106 @@
+"""Logit processors ahead of top-k and top-p against the 64-bit oracle.
+
+Bounds.  The processed logits stay in fp32 between the two (8 A / T 2^-24, see test_gpu_processors.py); the filter's
+log-sum-exp adds what the unfiltered one adds: 32 A / T 2^-24 + 2^-18 in all.  The kept sets are the oracle's: the
+inputs leave the threshold and the cut a margin wider than that, or an exact tie, which both sides see."""
+
+import pytest
+import torch
+
+from oracle import processors as oracle
+from rl_amd.algorithms.logits_sampling_utils import TrainingSamplingParams
+from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs, get_next_token_logprobs_from_logits
+from tests.test_gpu_processors import DTYPES, INF, check_grad, check_logprobs, cuda, least_t, magnitude, make
+
+pytestmark = pytest.mark.gpu
+FILTERS = [(20, 1.0), (None, 0.8), (50, 0.9)]
+
+
+def sampled(x, ids, start=0):
+    """The logits with most next tokens likely, as those of sampled ones are."""
+    B, S, V = x.shape
+    for b in range(B):
+        for r in range(S - 1):
+            if r % 4 and start <= ids[b, r + 1] < start + V:
+                x[b, r, ids[b, r + 1] - start] += 9
+    return x
+
+
+def kept(y, top_k, top_p):
+    """bool [V] of one row y (float64): top-k with its ties, then of those the tokens whose cumulative probability, from
+    the least on (ties by index), passes 1 - top_p."""
+    keep = torch.ones_like(y, dtype=torch.bool)
+    if top_k:
+        kth = y.topk(min(top_k, y.numel())).values[-1]
+        keep = y >= kth
+        if kth > -INF and not bool(keep.all()):
+            assert kth - y[~keep].max() > 1e-4, "no margin at the threshold"
+    if top_p < 1.0:
+        z = torch.where(keep, y, torch.full_like(y, -INF))
+        v, order = z.sort(stable=True)
+        cum = torch.softmax(v, -1).cumsum(-1)
+        past = cum > 1.0 - top_p
+        cut = int(past.nonzero()[0]) if bool(past.any()) else y.numel() - 1
+        assert (cum - (1.0 - top_p)).abs().min() > 1e-5, "no margin at the cut"
+        for a, b in ((cut - 1, cut), (cut, cut + 1)):
+            if 0 <= a and b < y.numel() and v[a] > -INF:
+                assert v[b] == v[a] or v[b] - v[a] > 2e-6, "no margin between the tokens at the cut"
+        keep = torch.zeros_like(keep)
+        keep[order[cut:]] = True
+    return keep
+
+
+def filtered(x, ids, P, top_k, top_p, vocab_start=0, vocab_end=None):
+    """Logprobs [B, S - 1] (float64, differentiable) of the next tokens among the kept ones: -inf for one that is not among them
+    and in a row with nothing left, which has no gradient."""
+    B, S, V = x.shape
+    end = vocab_start + V if vocab_end is None else vocab_end
+    y = oracle.process(x[:, : S - 1], ids, P, vocab_start=vocab_start, vocab_end=vocab_end)
+    out = []
+    for b in range(B):
+        for r in range(S - 1):
+            t, row = int(ids[b, r + 1]), y[b, r]
+            if bool((row == -INF).all()):
+                out.append(row.new_full((), -INF))
+                continue
+            keep = kept(row.detach(), top_k, top_p)
+            fine = keep & (row > -INF)
+            total = torch.logsumexp(row[fine], 0)
+            inside = vocab_start <= t < end and bool(fine[t - vocab_start])
+            out.append(row[t - vocab_start] - total if inside else -INF - 0.0 * total)
+    return torch.stack(out).view(B, S - 1)
+
+
+def compare(x, ids, P, top_k, top_p, dtype, start=0, end=None):
+    B, S, V = x.shape
+    end = V if end is None else end
+    A, T = magnitude(x, P, S), least_t(P)
+    t, xo = x.cuda().requires_grad_(True), x.double().requires_grad_(True)
+    F = TrainingSamplingParams(top_k=top_k, top_p=top_p)
+    want = filtered(xo, ids, P, top_k, top_p, start, end)
+    assert bool(want.isfinite().any()) and bool((want == -INF).any())
+    lp = from_parallel_logits_to_logprobs(t, ids.cuda(), start, end, None, sampling_params=F, logit_processors=cuda(P))
+    check_logprobs(lp.detach(), want.detach(), A, T)
+    with torch.no_grad():
+        again = from_parallel_logits_to_logprobs(x.cuda(), ids.cuda(), start, end, None, sampling_params=F, logit_processors=cuda(P))
+        assert torch.equal(again, lp)
+        if (start, end) == (0, V):
+            assert torch.equal(get_next_token_logprobs_from_logits(ids.cuda(), x.cuda(), sampling_params=F, logit_processors=cuda(P)), lp)
+    g = torch.randn(B, S - 1, generator=torch.Generator().manual_seed(1))
+    (dx,) = torch.autograd.grad([lp], [t], [g.cuda()])
+    fine = want.detach().isfinite()
+    (dxo,) = torch.autograd.grad([torch.where(fine, want, torch.zeros_like(want)).mul(g.double()).sum()], [xo])
+    assert dx.dtype == dtype and not dx[:, -1].any() and not dx.isnan().any()
+    # (rows whose token is not kept have the probabilities' gradient, as without processors: compared where it is)
+    check_grad(dx[:, :-1].cpu()[fine][None], dxo[:, :-1][fine][None].nan_to_num(0.0), A, T, dtype, g[fine][None], P.repetition_penalty.max().item() / T)
+    nothing = (oracle.process(x[:, : S - 1], ids, P, vocab_start=start, vocab_end=end) == -INF).all(-1)
+    assert not dx[:, :-1].cpu()[nothing].any()
+    return nothing
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top_k,top_p", FILTERS)
+def test_processed_logits_stay_in_fp32(dtype, top_k, top_p):
+    x, ids, P, _ = make(2, 17, 17, 3001, dtype, seed=5, K=3)
+    x = sampled(x, ids)
+    assert not compare(x, ids, P, top_k, top_p, dtype).any()
