@@ -1097,13 +1097,16 @@ int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R,
 
 /*
  * The same with y, and the gradient that comes back, in fp32 whatever the logits' type (grad_in
- * has the logits' type): what top-k and top-p read next.  out is not the logits.
+ * has the logits' type): what top-k and top-p read next.  out is not the logits.  left
+ * ([B, R]) is 1 for rows in which anything but -inf is left; the others hold finite values that
+ * stand for nothing, so that a filter of them has a result.
  */
 int mirl_process_logits_f32(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                             int64_t stride_b, int64_t stride_r,
                             const mirl_logit_processors* processors,
                             uint32_t* table, float* out,
-                            int64_t o_stride_b, int64_t o_stride_r, void* stream);
+                            int64_t o_stride_b, int64_t o_stride_r, int32_t* left,
+                            void* stream);
 int mirl_process_logits_f32_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V,
                                 int64_t stride_b, int64_t stride_r,
                                 const mirl_logit_processors* processors,

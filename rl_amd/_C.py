@@ -346,7 +346,7 @@ SIGNATURES = {
     "mirl_process_logits": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P]),
     "mirl_process_logits_bwd": (
         _I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
-    "mirl_process_logits_f32": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P]),
+    "mirl_process_logits_f32": (_I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] * 2),
     "mirl_process_logits_f32_bwd": (
         _I, [_P, _I] + [_I64] * 5 + [_P] * 3 + [_I64] * 2 + [_P] + [_I64] * 2 + [_P]),
     "mirl_dropout": (_I, [_P, _I, _I64, ctypes.c_double, _I64, _P, _I64, _P, _P]),
@@ -1338,16 +1338,27 @@ def processed_logprob_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table:
     return grad
 
 
-def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool, f32: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
-    """(processed logits, table): in place, or as a new contiguous tensor of the logits' type or with ``f32`` of fp32
-    (see mirl_process_logits and mirl_process_logits_f32)."""
+def process_logits(logits: torch.Tensor, args: LogitProcessorArgs, inplace: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """(processed logits, table): in place or as a new contiguous tensor (see mirl_process_logits)."""
     dev = logits.device
     B, R, V = logits.shape
-    out = logits if inplace else torch.empty((B, R, V), dtype=torch.float32 if f32 else logits.dtype, device=dev)
+    out = logits if inplace else torch.empty((B, R, V), dtype=logits.dtype, device=dev)
     table = torch.empty(_processor_elems(B, R, V, args.n_ids, args.n_bias)[1], dtype=torch.int32, device=dev)
-    _processors("mirl_process_logits_f32" if f32 else "mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V,
-                logits.stride(0), logits.stride(1), ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1))
+    _processors("mirl_process_logits", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
+                ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1))
     return out, table
+
+
+def process_logits_f32(logits: torch.Tensor, args: LogitProcessorArgs) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(processed logits in fp32, left [B, R] int32, table), see mirl_process_logits_f32."""
+    dev = logits.device
+    B, R, V = logits.shape
+    out = torch.empty((B, R, V), dtype=torch.float32, device=dev)
+    left = torch.empty((B, R), dtype=torch.int32, device=dev)
+    table = torch.empty(_processor_elems(B, R, V, args.n_ids, args.n_bias)[1], dtype=torch.int32, device=dev)
+    _processors("mirl_process_logits_f32", dev, logits.data_ptr(), _dtype_code(logits), B, R, V, logits.stride(0), logits.stride(1),
+                ctypes.byref(args), table.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), left.data_ptr())
+    return out, left, table
 
 
 def process_logits_bwd(logits: torch.Tensor, args: LogitProcessorArgs, table: torch.Tensor, grad_out: torch.Tensor,

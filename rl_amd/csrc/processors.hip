@@ -69,6 +69,7 @@ struct Params {
   int64_t lists;         // of a sample: of tokens, and one of biases if there are any
   const uint32_t* table;
   int rows;              // rows of a workgroup
+  int32_t* left;         // kWide [B, R]: whether anything is left in a row
   void* y;               // processed logits, or a gradient
   int64_t ysb, ysr;
   const void* dy;        // kApplyGrad, kWideGrad
@@ -222,8 +223,9 @@ __device__ __forceinline__ void through(float (&o)[kG], uint32_t any, uint32_t h
 // has kList tokens, so that a long history is spread over the chip: one row of 151936 logits behind 131072 tokens,
 // written out, takes 16 us where they are spread evenly and 56 where they follow Zipf's law (most in one slice, which
 // one workgroup counts); with one workgroup for all of them 94 and 206.
+// (And the flags that kWide's rows set, if there are any, begin as 0.)
 __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_logit_processors A, int64_t R, int64_t n_vocab,
-                                                                         int64_t lists, int buckets, uint32_t* table) {
+                                                                         int64_t lists, int buckets, uint32_t* table, int32_t* left) {
   __shared__ uint32_t s_at[kMaxBuckets];
   __shared__ uint32_t s_wave[kTableThreads / kWave];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -248,6 +250,8 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&S);
     for (int k = 0; k < kHead; ++k) head[k] = w[k];
   }
+  if (left != nullptr && list == 0)
+    for (int64_t r = tid; r < R; r += kTableThreads) left[b * R + r] = 0;
   auto column = [&](int64_t id) {
     const uint64_t c = (uint64_t)id - (uint64_t)A.vocab_start;
     return c < (uint64_t)n_vocab ? (int)c : -1;
@@ -822,6 +826,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           put(y_row, u, o, WHOLE);
         }
       } else if constexpr (kWritten) {
+        bool some_left = false;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           float v[kG];
@@ -834,7 +839,14 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 #pragma unroll
             for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e], allowed[u], e, -INFINITY);
           }
+          if constexpr (MODE == kWide) {
+#pragma unroll
+            for (int e = 0; e < kG; ++e) some_left |= v[e] != -INFINITY && (WHOLE || col(u) + e < left);
+          }
           put(y_row, u, v, WHOLE);
+        }
+        if constexpr (MODE == kWide) {  // (any wave of any workgroup: all write the same)
+          if (__ballot(some_left) != 0 && lane == 0) P.left[b * P.R + r0 + i] = 1;
         }
       } else if constexpr (kGradOfY) {
 #pragma unroll
@@ -925,6 +937,18 @@ __global__ __launch_bounds__(kThreads) void processors_join_kernel(Params P, flo
     stats[2 * row + 1] = scored ? logsum : -INFINITY;
   }
 }
+
+// Rows of kWide in which nothing is left become a finite ramp, which any filter cuts as ordinary logits (of a row of -inf it
+// forms (-inf) - (-inf)); what it makes of them is not used.
+__global__ __launch_bounds__(kThreads) void processors_ramp_kernel(Params P) {
+  const float step = -256.f / (float)P.V;
+  for (int64_t row = blockIdx.x; row < P.B * P.R; row += gridDim.x) {
+    if (P.left[row] != 0) continue;
+    float* y = static_cast<float*>(P.y) + row / P.R * P.ysb + row % P.R * P.ysr;
+    for (int64_t j = threadIdx.x; j < P.V; j += kThreads) y[j] = step * (float)j;
+  }
+}
+constexpr int64_t kRampGrid = 4096;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -1030,7 +1054,7 @@ Params params_of(const mirl_logit_processors* A, const uint32_t* table, const vo
 
 int make_table(const Params& P, int64_t rows, uint32_t* table, const char* what, hipStream_t st) {
   hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)(P.B * P.lists)), dim3(kTableThreads), 0, st, P.A, rows, P.n_vocab,
-                     P.lists, (int)P.buckets, table);
+                     P.lists, (int)P.buckets, table, P.left);
   return check_launch(what);
 }
 
@@ -1092,23 +1116,27 @@ namespace {
 template <int MODE>
 int write_processed(const char* what, const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b, int64_t stride_r,
                     const mirl_logit_processors* processors, uint32_t* table, void* out, int64_t o_stride_b, int64_t o_stride_r,
-                    void* stream) {
+                    int32_t* left, void* stream) {
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
-  MIRL_REQUIRE(table && logits && out, "null pointer argument");
+  MIRL_REQUIRE(table && logits && out && (MODE == kApply || left), "null pointer argument");
   MIRL_REQUIRE(MODE == kApply ? out != logits || (o_stride_b == stride_b && o_stride_r == stride_r) : out != logits,
                MODE == kApply ? "in place, the strides are those of the logits" : "fp32 values are not written in place");
   Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   P.y = out;
   P.ysb = o_stride_b;
   P.ysr = o_stride_r;
+  P.left = left;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (int e = make_table(P, R, table, what, st)) return e;
   if constexpr (MODE == kApply) {
-    if (out == logits) return launch<kInPlace>(P, dtype, R, what, st);
+    return out == logits ? launch<kInPlace>(P, dtype, R, what, st) : launch<kApply>(P, dtype, R, what, st);
+  } else {
+    if (int e = launch<kWide>(P, dtype, R, what, st)) return e;
+    hipLaunchKernelGGL(processors_ramp_kernel, dim3((unsigned)(B * R < kRampGrid ? B * R : kRampGrid)), dim3(kThreads), 0, st, P);
+    return check_launch(what);
   }
-  return launch<MODE>(P, dtype, R, what, st);
 }
 
 template <int MODE>
@@ -1135,7 +1163,7 @@ extern "C" int mirl_process_logits(const void* logits, int dtype, int64_t B, int
                                    int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, void* out,
                                    int64_t o_stride_b, int64_t o_stride_r, void* stream) {
   return write_processed<kApply>("mirl_process_logits", logits, dtype, B, R, V, stride_b, stride_r, processors, table, out,
-                                 o_stride_b, o_stride_r, stream);
+                                 o_stride_b, o_stride_r, nullptr, stream);
 }
 
 extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
@@ -1148,9 +1176,9 @@ extern "C" int mirl_process_logits_bwd(const void* logits, int dtype, int64_t B,
 
 extern "C" int mirl_process_logits_f32(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,
                                        int64_t stride_r, const mirl_logit_processors* processors, uint32_t* table, float* out,
-                                       int64_t o_stride_b, int64_t o_stride_r, void* stream) {
+                                       int64_t o_stride_b, int64_t o_stride_r, int32_t* left, void* stream) {
   return write_processed<kWide>("mirl_process_logits_f32", logits, dtype, B, R, V, stride_b, stride_r, processors, table, out,
-                                o_stride_b, o_stride_r, stream);
+                                o_stride_b, o_stride_r, left, stream);
 }
 
 extern "C" int mirl_process_logits_f32_bwd(const void* logits, int dtype, int64_t B, int64_t R, int64_t V, int64_t stride_b,

@@ -163,14 +163,13 @@ class _ProcessedLogprob(torch.autograd.Function):
 
 
 class _ProcessLogits(torch.autograd.Function):
-    """Processed logits as a new tensor, of their type or in fp32.  The backward reads the logits of the tokens that occur."""
+    """Processed logits as a new tensor.  The backward reads the logits of the tokens that occur."""
 
     @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, call: _Call, f32: bool) -> torch.Tensor:  # type: ignore[override]
-        out, table = _C.process_logits(logits, call.args(), False, f32)
+    def forward(ctx: Any, logits: torch.Tensor, call: _Call) -> torch.Tensor:  # type: ignore[override]
+        out, table = _C.process_logits(logits, call.args(), False)
         ctx.save_for_backward(logits, table, call.ids, *call.tensors)
         ctx.numbers = (call.scalars, call.vocab)
-        ctx.f32 = f32
         return out
 
     @staticmethod
@@ -180,9 +179,30 @@ class _ProcessLogits(torch.autograd.Function):
     @staticmethod
     def _grads(ctx: Any, grad: torch.Tensor):
         logits, table, ids, *tensors = ctx.saved_tensors
-        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad, ctx.f32), None, None
+        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad), None
 
     _once = staticmethod(once_differentiable(_grads.__func__))
+
+
+class _ProcessLogitsF32(torch.autograd.Function):
+    """(processed logits in fp32, whether anything is left in a row)."""
+
+    @staticmethod
+    def forward(ctx: Any, logits: torch.Tensor, call: _Call):  # type: ignore[override]
+        out, left, table = _C.process_logits_f32(logits, call.args())
+        ctx.save_for_backward(logits, table, call.ids, *call.tensors)
+        ctx.numbers = (call.scalars, call.vocab)
+        ctx.mark_non_differentiable(left)
+        ctx.set_materialize_grads(False)
+        return out, left
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: Optional[torch.Tensor], _: Any):  # type: ignore[override]
+        if grad is None:
+            return None, None
+        logits, table, ids, *tensors = ctx.saved_tensors
+        return _C.process_logits_bwd(logits, _C.processor_args(ids, tuple(tensors), *ctx.numbers), table, grad, True), None
 
 
 def _rows_meet(x: torch.Tensor) -> bool:
@@ -246,16 +266,17 @@ def filtered_processed_logprobs(
 
     The processed logits are written once, in fp32 whatever the type of the logits: what is held in 16 bits between the two would
     be off by half a step there (2^-4 at 16), and the cut would be decided on that.  Top-p is therefore
-    decided in fp32, as a sampler decides it."""
+    decided in fp32, as a sampler decides it.  A row in which nothing is left gives -inf and has no gradient."""
     from rl_amd.distributed.sampling import filtered_row_logprobs
 
     x = logits[:, : max(target.shape[1] - 1, 0)]
     call = _Call(x, target, processors, None, x.shape[1], (0, x.shape[2]))
     if inference_only or not _grad_needed(logits):
-        y, _ = _C.process_logits(x, call.args(), False, True)
+        y, left, _ = _C.process_logits_f32(x, call.args())
     else:
-        y = _ProcessLogits.apply(x, call, True)
-    return filtered_row_logprobs(y, target[:, 1:], top_k, top_p, inference_only=inference_only)
+        y, left = _ProcessLogitsF32.apply(x, call)
+    logprobs = filtered_row_logprobs(y, target[:, 1:], top_k, top_p, inference_only=inference_only)
+    return logprobs.masked_fill(left == 0, -math.inf)
 
 
 def process_logits(
@@ -282,7 +303,7 @@ def process_logits(
         x = x.contiguous()
     call = _Call(x, input_ids, processors, history_lengths, x.shape[1], (0, x.shape[2]))
     if not inplace and _grad_needed(logits):
-        y = _ProcessLogits.apply(x, call, False)
+        y = _ProcessLogits.apply(x, call)
         return y if logits.dim() == 3 else y.squeeze(1)
     y, _ = _C.process_logits(x, call.args(), inplace)
     if inplace:

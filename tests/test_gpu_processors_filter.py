@@ -104,3 +104,15 @@ def test_processed_logits_stay_in_fp32(dtype, top_k, top_p):
     x, ids, P, _ = make(2, 17, 17, 3001, dtype, seed=5, K=3)
     x = sampled(x, ids)
     assert not compare(x, ids, P, top_k, top_p, dtype).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top_k,top_p", FILTERS)
+@pytest.mark.parametrize("V", [61, 3001])
+def test_masks_and_rows_with_nothing_left(dtype, top_k, top_p, V):
+    x, ids, P, _ = make(3, 17, 17, V, dtype, seed=V + 5, K=3, M=4)
+    x = sampled(x, ids)
+    P.grammar_rows[0, 2], P.grammar_rows[1, 4], P.grammar_rows[2, 7] = -1, 0, 0
+    x[0, 2] = -INF  # nothing left by itself
+    x[1, 4] = float("nan")  # masked: anything
+    assert compare(x, ids, P, top_k, top_p, dtype).sum() >= 3

@@ -31,7 +31,7 @@ def refused(status, word):
 def test_the_fp32_c_entry_points():
     lib = _C.load()
     one = 16  # an address that is never read
-    fwd = lambda x=None, dtype=0, b=1, v=V, out=None: lib.mirl_process_logits_f32(x, dtype, b, 1, v, v, v, settings(), one, out, v, v, None)  # noqa: E731
+    fwd = lambda x=None, dtype=0, b=1, v=V, out=None: lib.mirl_process_logits_f32(x, dtype, b, 1, v, v, v, settings(), one, out, v, v, out, None)  # noqa: E731
     bwd = lambda x=None, dtype=0, b=1, v=V: lib.mirl_process_logits_f32_bwd(x, dtype, b, 1, v, v, v, settings(), one, None, v, v, None, v, v, None)  # noqa: E731
     for call in (fwd, bwd):
         assert refused(call(dtype=3), "dtype") and refused(call(v=0), "shape") and refused(call(b=-1), "shape") and refused(call(), "null")
