@@ -260,9 +260,12 @@ def filtered_processed_logprobs(
     top_k: Optional[int],
     top_p: Optional[float],
     inference_only: bool,
+    vocab_start_index: int,
+    vocab_end_index: Optional[int],
 ) -> torch.Tensor:
     """fp32 logprobs ``[B, S - 1]`` of the next tokens of ``target [B, S]`` under the processors and the filter behind
-    them, from ``logits [B, >= S, V]``.
+    them, from ``logits [B, >= S, V]``.  Ids count from ``vocab_start_index``, for the processors and for the next tokens; one
+    that is no column is not among those kept: -inf.
 
     The processed logits are written once, in fp32 whatever the type of the logits: what is held in 16 bits between the two would
     be off by half a step there (2^-4 at 16), and the cut would be decided on that.  Top-p is therefore
@@ -270,12 +273,17 @@ def filtered_processed_logprobs(
     from rl_amd.distributed.sampling import filtered_row_logprobs
 
     x = logits[:, : max(target.shape[1] - 1, 0)]
-    call = _Call(x, target, processors, None, x.shape[1], (0, x.shape[2]))
+    start = int(vocab_start_index)
+    end = start + x.shape[2] if vocab_end_index is None else int(vocab_end_index)
+    call = _Call(x, target, processors, None, x.shape[1], (start, end))
     if inference_only or not _grad_needed(logits):
         y, left, _ = _C.process_logits_f32(x, call.args())
     else:
         y, left = _ProcessLogitsF32.apply(x, call)
-    logprobs = filtered_row_logprobs(y, target[:, 1:], top_k, top_p, inference_only=inference_only)
+    tokens = call.ids[:, 1:]
+    if start != 0 or end < x.shape[2]:
+        tokens = torch.where((tokens >= start) & (tokens < end), tokens - start, -1)
+    logprobs = filtered_row_logprobs(y, tokens, top_k, top_p, inference_only=inference_only)
     return logprobs.masked_fill(left == 0, -math.inf)
 
 

@@ -450,7 +450,7 @@ def from_parallel_logits_to_logprobs(
     ``logit_processors`` (an extension: penalties, biases, grammar masks and temperature of the
     sampler) come ahead of the filter; ``target`` is also the history that they count.  Without
     a filter the processed logits are never written, with one they are, in fp32, and top-p is decided
-    in fp32.
+    in fp32; ids count from ``vocab_start_index`` in both.
     """
     return _next_token_logprobs(vocab_parallel_logits, target, vocab_start_index,
                                 vocab_end_index, tp_group, inference_only, cp_group, chunk_size,
@@ -471,7 +471,8 @@ def _next_token_logprobs(logits, target, vocab_start_index, vocab_end_index, tp_
             return processed_next_token_logprobs(
                 logits, target, logit_processors, None, inference_only, vocab_start_index, vocab_end_index)
         return filtered_processed_logprobs(
-            logits, target, logit_processors, sampling_params.top_k, sampling_params.top_p, inference_only)  # type: ignore[union-attr]
+            logits, target, logit_processors, sampling_params.top_k, sampling_params.top_p,  # type: ignore[union-attr]
+            inference_only, vocab_start_index, vocab_end_index)
     if need_top_k_or_top_p_filtering(sampling_params):
         from rl_amd.distributed.sampling import filtered_next_token_logprobs
 

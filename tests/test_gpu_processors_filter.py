@@ -116,3 +116,13 @@ def test_masks_and_rows_with_nothing_left(dtype, top_k, top_p, V):
     x[0, 2] = -INF  # nothing left by itself
     x[1, 4] = float("nan")  # masked: anything
     assert compare(x, ids, P, top_k, top_p, dtype).sum() >= 3
+
+
+@pytest.mark.parametrize("top_k,top_p", FILTERS)
+@pytest.mark.parametrize("start,end", [(1000, 1700), (1000, 1640)])
+def test_a_range_of_ids(top_k, top_p, start, end):
+    x, ids, P, _ = make(2, 17, 17, 700, torch.float32, seed=30, K=3)
+    ids, P.bias_ids = ids + start, P.bias_ids + start
+    ids[0, 5], ids[1, 9] = 3, 10**12
+    x = sampled(x, ids, start)
+    compare(x, ids, P, top_k, top_p, torch.float32, start, end)
