@@ -1025,6 +1025,8 @@ int mirl_int8_logits(const int8_t* hidden8, const float* hidden_scale, int64_t T
  * holds n_masks rows of at least ceil(V / 32) words, mask_stride words apart, token v being
  * bit v % 32 of word v / 32 (1: allowed); mask_rows[b, r] names a row's mask, numbers
  * outside [0, n_masks) none (n_masks 0: no masks, mask_rows not read).  V is at most 2^24.
+ * The samples times their lists (one for each 4096 tokens, at least one, and one of biases if there
+ * are any) are fewer than 2^22, the rows that a call scores fewer than 2^26.
  */
 typedef struct mirl_logit_processors {
   const int64_t* ids;

@@ -979,13 +979,22 @@ Plan plan_of(int mode, int dtype, int64_t B, int64_t R, int64_t V) {
   return p;
 }
 
+int make_table(const Params& P, int64_t rows, uint32_t* table, const char* what, hipStream_t st) {
+  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)(P.B * P.lists)), dim3(kTableThreads), 0, st, P.A, rows, P.n_vocab,
+                     P.lists, (int)P.buckets, table, P.left);
+  return check_launch(what);
+}
+
+// `table`: the one to make ahead of the rows (a backward has its forward's).
 template <int MODE>
-int launch(Params& P, int dtype, int64_t rows, const char* what, hipStream_t st) {
+int launch(Params& P, int dtype, int64_t rows, const char* what, hipStream_t st, uint32_t* table = nullptr) {
   const Plan p = plan_of(MODE, dtype, P.B, rows, P.V);
   P.slices = p.slices;
   P.chunks = p.chunks;
   P.rows = (int)p.rows;
   MIRL_REQUIRE(P.B * p.chunks * p.slices < (int64_t(1) << 24), "too many rows of %lld columns", (long long)P.V);
+  if (table != nullptr)
+    if (int e = make_table(P, rows, table, what, st)) return e;
   const dim3 grid((unsigned)(P.B * p.chunks * p.slices)), block(kThreads);
   auto go = [&](auto e, auto nv, auto masked) {
     hipLaunchKernelGGL((processors_kernel<decltype(e), MODE, decltype(nv)::value, decltype(masked)::value>), grid, block, 0, st, P);
@@ -1019,13 +1028,16 @@ int check_args(const mirl_logit_processors* A, int dtype, int64_t B, int64_t R, 
   MIRL_REQUIRE(A != nullptr, "null pointer argument");
   MIRL_REQUIRE(B >= 0 && R >= 0 && V > 0, "invalid shape B=%lld R=%lld V=%lld", (long long)B, (long long)R, (long long)V);
   MIRL_REQUIRE(V <= kMaxBuckets * kBucket, "a vocabulary of %lld exceeds %lld", (long long)V, (long long)(kMaxBuckets * kBucket));
-  MIRL_REQUIRE(B < (int64_t(1) << 22) && B * R < (int64_t(1) << 31), "sizes exceed 2^31-1");
+  MIRL_REQUIRE(B < (int64_t(1) << 31) && R < (int64_t(1) << 31) && B * R < (int64_t(1) << 31), "sizes exceed 2^31-1");
   MIRL_REQUIRE(A->n_ids >= 0 && A->n_ids <= kMaxTokens, "%lld tokens of a sample, at most %lld are counted",
                (long long)A->n_ids, (long long)kMaxTokens);
   MIRL_REQUIRE(A->n_bias >= 0 && A->n_bias <= kMaxBias, "%lld biases of a sample, at most %lld are held",
                (long long)A->n_bias, (long long)kMaxBias);
   MIRL_REQUIRE(A->n_masks >= 0 && (A->n_masks == 0 || A->mask_stride >= ceil_div(V, 32)),
                "grammar masks of %lld words do not cover %lld columns", (long long)A->mask_stride, (long long)V);
+  // a launch holds fewer than 2^32 threads; the table takes 1024 for each list
+  const int64_t lists = token_lists(A->n_ids) + (A->n_bias > 0);
+  MIRL_REQUIRE(B * lists < (int64_t(1) << 22), "too many samples (%lld) with %lld lists of tokens and biases each", (long long)B, (long long)lists);
   if (B * R == 0) return MIRL_OK;
   MIRL_REQUIRE((A->n_ids == 0 || A->ids != nullptr) && (A->n_bias == 0 || (A->bias_ids != nullptr && A->bias != nullptr)) &&
                    (A->n_masks == 0 || (A->masks != nullptr && A->mask_rows != nullptr)),
@@ -1052,12 +1064,6 @@ Params params_of(const mirl_logit_processors* A, const uint32_t* table, const vo
   return P;
 }
 
-int make_table(const Params& P, int64_t rows, uint32_t* table, const char* what, hipStream_t st) {
-  hipLaunchKernelGGL(processors_table_kernel, dim3((unsigned)(P.B * P.lists)), dim3(kTableThreads), 0, st, P.A, rows, P.n_vocab,
-                     P.lists, (int)P.buckets, table, P.left);
-  return check_launch(what);
-}
-
 }  // namespace
 }  // namespace mirl
 
@@ -1079,13 +1085,14 @@ extern "C" int mirl_processed_logprob_fwd(const void* logits, int dtype, int64_t
   clear_error();
   if (int e = check_args(processors, dtype, B, R, V)) return e;
   if (B * R == 0) return MIRL_OK;
+  // (a wave joins a row's parts, and a launch holds fewer than 2^32 threads)
+  MIRL_REQUIRE(B * R < (int64_t(1) << 26), "%lld rows: fewer than 2^26 are scored in a call", (long long)(B * R));
   MIRL_REQUIRE(table && logits && out && workspace, "null pointer argument");
   Params P = params_of(processors, table, logits, B, R, R, V, stride_b, stride_r);
   hipStream_t st = static_cast<hipStream_t>(stream);
   P.part = workspace;
   P.xt = workspace + B * R * plan_of(kFwd, dtype, B, R, V).slices * kWaves * 2;
-  if (int e = make_table(P, R, table, "mirl_processed_logprob_fwd", st)) return e;
-  if (int e = launch<kFwd>(P, dtype, R, "mirl_processed_logprob_fwd", st)) return e;
+  if (int e = launch<kFwd>(P, dtype, R, "mirl_processed_logprob_fwd", st, table)) return e;
   hipLaunchKernelGGL(processors_join_kernel, dim3((unsigned)ceil_div(B * R, kWaves)), dim3(kThreads), 0, st, P, out, stats);
   return check_launch("mirl_processed_logprob_fwd");
 }
@@ -1129,11 +1136,10 @@ int write_processed(const char* what, const void* logits, int dtype, int64_t B, 
   P.ysr = o_stride_r;
   P.left = left;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int e = make_table(P, R, table, what, st)) return e;
   if constexpr (MODE == kApply) {
-    return out == logits ? launch<kInPlace>(P, dtype, R, what, st) : launch<kApply>(P, dtype, R, what, st);
+    return out == logits ? launch<kInPlace>(P, dtype, R, what, st, table) : launch<kApply>(P, dtype, R, what, st, table);
   } else {
-    if (int e = launch<kWide>(P, dtype, R, what, st)) return e;
+    if (int e = launch<kWide>(P, dtype, R, what, st, table)) return e;
     hipLaunchKernelGGL(processors_ramp_kernel, dim3((unsigned)(B * R < kRampGrid ? B * R : kRampGrid)), dim3(kThreads), 0, st, P);
     return check_launch(what);
   }
