@@ -995,8 +995,8 @@ int mirl_linear_ce_8bit_fwd(const void* hidden8, const float* hidden_scale, int6
 /*
  * The same from 8-bit integers (mirl_add_rms_norm_int8_fwd, mirl_quantize_rows_int8):
  *   x[r, v] = (float(sum_k hidden8[r, k] weight8[v, k]) * weight_scale[v]) * hidden_scale[r]
- * with exact sums, Hd at most 2^17 - 256.  And these logits written out: out [T, V], rows ldo apart, in
- * fp32, bf16 or fp16, each rounded once from fp32.
+ * with exact sums, Hd at most 2^17 - 256 and T below 2^26.  And these logits written out: out [T, V],
+ * rows ldo apart, in fp32, bf16 or fp16, each rounded once from fp32.
  */
 int mirl_linear_ce_int8_fwd(const int8_t* hidden8, const float* hidden_scale, int64_t T,
                             int64_t Hd, int64_t ldh, const int8_t* weight8,

@@ -68,6 +68,8 @@ extern "C" int mirl_linear_ce_int8_fwd(const int8_t* hidden8, const float* hidde
   LceParams P{};
   MIRL_REQUIRE(bsz > 0, "invalid batch size %lld", (long long)bsz);
   MIRL_REQUIRE(T % bsz == 0, "row count %lld is not a multiple of the batch size %lld", (long long)T, (long long)bsz);
+  // (a wave merges a row's parts, and a launch holds fewer than 2^32 threads)
+  MIRL_REQUIRE(T < (int64_t(1) << 26), "%lld rows: fewer than 2^26 are scored in a call", (long long)T);
   if (int e = operands(P, hidden8, hidden_scale, T, Hd, ldh, weight8, weight_scale, V, ldw)) return e;
   if (T == 0) return MIRL_OK;
   MIRL_REQUIRE(target && out && workspace, "null pointer argument");

@@ -62,3 +62,12 @@ def test_sizes_that_no_launch_holds():
         assert refused(call(2, 1 << 62), "2^31") and refused(call(1 << 62, 4), "2^31")  # (products past 64 bits)
     assert refused(fwd(1, 1 << 26), "scored") and refused(fwd(1, (1 << 26) - 1), "null")
     assert refused(process(1, 1 << 26), "null")  # (no join)
+
+
+def test_int8_rows_that_no_launch_merges():
+    lib = _C.load()
+
+    def fwd(T):
+        return lib.mirl_linear_ce_int8_fwd(None, None, T, 256, 256, None, None, 5, 256, 1, None, 1, 1, 0, 5, None, 1, 1, None, None)
+
+    assert refused(fwd(1 << 26), "scored") and refused(fwd((1 << 26) - 1), "null")
