@@ -747,8 +747,8 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           take(u, -INFINITY, v[u]);
-          if (wave_bits(u) != 0)
-            special(v[u], wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+          if (wave_bits(u) != 0)  // (a masked token's bias must not meet the -inf that the mask left)
+            special(v[u], wave_bits(u), lane_bits(u) & allowed[u], words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
           for (int e = 0; e < kG; ++e) mx = fmaxf(mx, v[u][e]);
         }

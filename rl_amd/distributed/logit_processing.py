@@ -15,7 +15,7 @@ single new token, or several drafted ones).  With ``c`` a token's count among th
     z = z - frequency * c - presence * [c > 0]
     y = z / temperature where the row's grammar allows the token, -inf elsewhere
 
-in fp32, rounded once where it is written.  A masked logit may hold anything.
+in fp32, rounded once where it is written.  A masked logit may hold anything, and so may its bias.
 """
 
 from __future__ import annotations

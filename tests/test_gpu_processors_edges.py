@@ -1,0 +1,36 @@
+"""Edges of the logit processors.  Bounds as derived in test_gpu_processors.py."""
+
+import dataclasses
+
+import pytest
+import torch
+
+from oracle import processors as oracle
+from rl_amd.algorithms.logits_sampling_utils import apply_logit_processors
+from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs
+from tests.test_gpu_processors import DTYPES, INF, check_logprobs, cuda, least_t, magnitude, make, pack_masks
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [520, 70001])
+def test_a_masked_token_s_bias_takes_no_part(dtype, V):
+    """More biased tokens in 512 columns than a wave holds apart, half of them masked, with biases of infinity and NaN there."""
+    B, S, K = 2, 40, 400
+    x, ids, P, _ = make(B, S, S, V, dtype, seed=V)
+    v = torch.arange(V)
+    P.bias_ids = torch.arange(K)
+    P.bias = torch.randn(K, generator=torch.Generator().manual_seed(1))
+    P.grammar_masks, P.grammar_rows = pack_masks((v % 2 == 0)[None]), torch.zeros(B, S, dtype=torch.int64)
+    Q = dataclasses.replace(P, bias=torch.where(v[:K] % 2 == 0, P.bias, torch.where(v[:K] % 4 == 1, INF, float("nan"))))
+    outs = []
+    for settings in (P, Q):
+        t = x.cuda().requires_grad_(True)
+        lp = from_parallel_logits_to_logprobs(t, ids.cuda(), 0, V, None, logit_processors=cuda(settings))
+        g = torch.where(lp.detach().isfinite(), 1.0, 0.0)
+        (dx,) = torch.autograd.grad([lp], [t], [g])
+        outs.append((lp.detach(), dx, apply_logit_processors(t.detach(), ids.cuda(), cuda(settings))))
+    check_logprobs(outs[0][0], oracle.logprobs(x, ids, P, rows=S - 1), magnitude(x, P, S), least_t(P))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
