@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
   const bool biases = list == token_lists(A.n_ids);
   const int64_t* ids = A.ids + b * A.ids_stride_b;
   const int64_t* bias_ids = A.bias_ids + b * A.bias_stride_b;
-  const int64_t n_b = A.lengths != nullptr ? A.lengths[b] : 1;
+  const int64_t n_b = min(A.lengths != nullptr ? A.lengths[b] : int64_t(1), A.n_ids);  // (what is beyond counts all tokens too)
   uint32_t* const head = table + b * head_words(lists, buckets);
   uint32_t* const begins = head + kHead + list * (buckets + 1);
   uint32_t* const entries = table + B * head_words(lists, buckets) + b * (A.n_ids + A.n_bias);
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     S.pres = A.presence != nullptr ? A.presence[b] : A.presence_all;
     S.freq = A.frequency != nullptr ? A.frequency[b] : A.frequency_all;
     S.inv_t = 1.f / (A.temperature != nullptr ? A.temperature[b] : A.temperature_all);
-    S.n = (int)min(max(n_b, -(int64_t(1) << 30)), A.n_ids);
+    S.n = (int)max(n_b, -(int64_t(1) << 30));
     S.prompt = A.prompt_lengths != nullptr ? (int)min(max(A.prompt_lengths[b], int64_t(0)), A.n_ids) : 0;
     S.unused = 0;
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&S);

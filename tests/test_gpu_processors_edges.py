@@ -7,8 +7,8 @@ import torch
 
 from oracle import processors as oracle
 from rl_amd.algorithms.logits_sampling_utils import apply_logit_processors
-from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs
-from tests.test_gpu_processors import DTYPES, INF, check_logprobs, cuda, least_t, magnitude, make, pack_masks
+from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs, processed_next_token_logprobs
+from tests.test_gpu_processors import DTYPES, INF, check_logprobs, check_values, cuda, least_t, magnitude, make, pack_masks
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,13 @@ def test_a_masked_token_s_bias_takes_no_part(dtype, V):
     check_logprobs(outs[0][0], oracle.logprobs(x, ids, P, rows=S - 1), magnitude(x, P, S), least_t(P))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_lengths_at_the_end_of_their_type():
+    B, L, R, V = 4, 8, 3, 300
+    x, ids, P, _ = make(B, R, L, V, torch.float32, seed=3)
+    n = torch.tensor([2**63 - 1, 2**63 - 2, -(2**63), 5])
+    A, T = magnitude(x, P, L), least_t(P)
+    near = n.clamp(-5, L)  # (as far as a history reaches, the same)
+    check_values(apply_logit_processors(x.cuda(), ids.cuda(), cuda(P), history_lengths=n.cuda()), oracle.process(x, ids, P, near), A, T, torch.float32)
+    check_logprobs(processed_next_token_logprobs(x.cuda(), ids.cuda(), cuda(P), history_lengths=n.cuda()), oracle.logprobs(x, ids, P, near), A, T)
