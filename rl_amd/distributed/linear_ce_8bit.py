@@ -116,10 +116,7 @@ def from_int8_hidden_states_to_logits(
     or fp16).  ``out`` takes them where it is given (contiguous, of ``dtype``).  There is no gradient; operands are
     copied where :func:`from_parallel_8bit_hidden_states_to_logprobs` copies them."""
     h8, w8 = hidden_states_8bit, output_weight_8bit
-    if h8.dtype != torch.int8 or w8.dtype != torch.int8:
-        raise TypeError(f"expected int8 hidden states and weight, got {h8.dtype} and {w8.dtype}")
-    if h8.dim() < 1 or h8.shape[-1] == 0:
-        raise ValueError(f"expected hidden states [..., H], got {tuple(h8.shape)}")
+    _check_int8(h8, w8)
     if dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError(f"logits are fp32, bf16 or fp16, got {dtype}")
     V = _check_weight(h8, w8)
@@ -134,9 +131,30 @@ def from_int8_hidden_states_to_logits(
     if h8.numel() == 0:
         _C._require_gpu(h8, w8, out)
         return out
-    rows = _operand8(h8.reshape(-1, H), True)
+    operands = _int8_layout(h8, hidden_scales, w8, output_weight_scales)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
-    _C.int8_logits(rows, hidden_scales.reshape(-1).contiguous(), _operand8(w8, False), output_weight_scales.contiguous(),
-                   out.view(-1, V))
+    _C.int8_logits(*operands, out.view(-1, V))
     return out
+
+
+def _check_int8(h8: torch.Tensor, w8: torch.Tensor) -> None:
+    if h8.dtype != torch.int8 or w8.dtype != torch.int8:
+        raise TypeError(f"expected int8 hidden states and weight, got {h8.dtype} and {w8.dtype}")
+    if h8.dim() < 1 or h8.shape[-1] == 0:
+        raise ValueError(f"expected hidden states [..., H], got {tuple(h8.shape)}")
+
+
+def int8_operands(h8: torch.Tensor, hidden_scales: torch.Tensor, w8: torch.Tensor, weight_scales: torch.Tensor
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Hidden rows ``[T, H]`` with their scales and the weight with its, checked and as ``_C.int8_logits`` reads them.  Any run of rows
+    (and of their scales) is such an operand as well: a caller that takes them by blocks has them laid out once."""
+    _check_int8(h8, w8)
+    _check_scales(hidden_scales, tuple(h8.shape[:-1]), weight_scales, _check_weight(h8, w8))
+    return _int8_layout(h8, hidden_scales, w8, weight_scales)
+
+
+def _int8_layout(h8: torch.Tensor, hidden_scales: torch.Tensor, w8: torch.Tensor, weight_scales: torch.Tensor
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return (_operand8(h8.reshape(-1, h8.shape[-1]), True), hidden_scales.reshape(-1).contiguous(), _operand8(w8, False),
+            weight_scales.contiguous())

@@ -15,10 +15,11 @@ from typing import Any, Optional, Union
 
 import torch
 
+from rl_amd import _C
 from rl_amd.algorithms.logits_sampling_utils import LogitProcessors
 from rl_amd.distributed.final_norm import add_rms_norm, add_rms_norm_8bit, rms_norm
 from rl_amd.distributed.linear_ce import from_parallel_hidden_states_to_logprobs
-from rl_amd.distributed.linear_ce_8bit import from_int8_hidden_states_to_logits, from_parallel_8bit_hidden_states_to_logprobs
+from rl_amd.distributed.linear_ce_8bit import from_parallel_8bit_hidden_states_to_logprobs, int8_operands
 from rl_amd.distributed.linear_ce_adapters import from_parallel_hidden_states_to_logprobs_with_adapters
 from rl_amd.distributed.logit_processing import processed_next_token_logprobs
 from rl_amd.distributed.model_utils import _check_chunk_size, _require_single_rank
@@ -111,14 +112,16 @@ def _processed_int8(y8, scales, weight8, weight_scales, target, vocab_start, voc
     if tuple(target.shape) != (B, S):
         raise ValueError(f"target shape {tuple(target.shape)} does not match [B, S] = {(B, S)}")
     V, R = weight8.shape[0], max(S - 1, 0)
-    step = chunk_size or max(1, _CHUNK_BYTES // (4 * max(B, 1) * V))
     out = torch.empty((B, R), dtype=torch.float32, device=y8.device)
-    logits = None
+    if R * B == 0:
+        return out
+    rows, row_scales, weight, col_scales = int8_operands(y8, scales, weight8, weight_scales)
+    step, logits = chunk_size or max(1, _CHUNK_BYTES // (4 * B * V)), None
     for s0 in range(0, R, step):
         s1 = min(s0 + step, R)
         if logits is None or logits.shape[0] != s1 - s0:
             logits = torch.empty((s1 - s0, B, V), dtype=torch.float32, device=y8.device)
-        from_int8_hidden_states_to_logits(y8[s0:s1], scales[s0:s1], weight8, weight_scales, torch.float32, logits)
+        _C.int8_logits(rows[s0 * B:s1 * B], row_scales[s0 * B:s1 * B], weight, col_scales, logits.view(-1, V))
         block = processors
         if processors.grammar_rows is not None:
             block = replace(processors, grammar_rows=processors.grammar_rows[:, s0:s1])
