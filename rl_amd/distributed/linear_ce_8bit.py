@@ -49,6 +49,11 @@ def _check_weight(h8: torch.Tensor, w8: torch.Tensor) -> int:
     return w8.shape[0]
 
 
+def _no_gradient_to_scales(*scales: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in scales):
+        raise RuntimeError("no gradient passes to the scales of int8 rows: detach them")
+
+
 def _check_scales(hidden_scales: torch.Tensor, shape: tuple, weight_scales: torch.Tensor, V: int) -> None:
     for name, scale, want in (("hidden", hidden_scales, shape), ("weight", weight_scales, (V,))):
         if scale.dtype != torch.float32 or tuple(scale.shape) != want:
@@ -89,6 +94,8 @@ def from_parallel_8bit_hidden_states_to_logprobs(
     if tuple(target.shape) != (B, S):
         raise ValueError(f"target shape {tuple(target.shape)} does not match [B, S] = {(B, S)}")
     _check_scales(hidden_scales, (S, B), output_weight_scales, V)
+    if h8.dtype == torch.int8:
+        _no_gradient_to_scales(hidden_scales, output_weight_scales)
     R = max(S - 1, 0)
     out = torch.empty((B, R), dtype=torch.float32, device=h8.device)
     if R * B == 0:
@@ -113,8 +120,8 @@ def from_int8_hidden_states_to_logits(
 ) -> torch.Tensor:
     """Logits ``[..., V]`` of ``hidden [..., H] . weight [V, H]^T``, both ``int8`` with one fp32 scale per row
     (``[...]`` and ``[V]``): ``float(sum) * weight_scale * hidden_scale``, rounded once to ``dtype`` (fp32, bf16
-    or fp16).  ``out`` takes them where it is given (contiguous, of ``dtype``).  There is no gradient; operands are
-    copied where :func:`from_parallel_8bit_hidden_states_to_logprobs` copies them."""
+    or fp16).  ``out`` takes them where it is given (contiguous, of ``dtype``).  There is no gradient (scales that ask
+    for one are refused unless gradients are off); operands are copied where :func:`from_parallel_8bit_hidden_states_to_logprobs` copies them."""
     h8, w8 = hidden_states_8bit, output_weight_8bit
     _check_int8(h8, w8)
     if dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -122,6 +129,7 @@ def from_int8_hidden_states_to_logits(
     V = _check_weight(h8, w8)
     lead, H = tuple(h8.shape[:-1]), h8.shape[-1]
     _check_scales(hidden_scales, lead, output_weight_scales, V)
+    _no_gradient_to_scales(hidden_scales, output_weight_scales)
     if out is None:
         out = torch.empty((*lead, V), dtype=dtype, device=h8.device)
     elif out.dtype != dtype or tuple(out.shape) != (*lead, V) or not out.is_contiguous():
@@ -151,6 +159,7 @@ def int8_operands(h8: torch.Tensor, hidden_scales: torch.Tensor, w8: torch.Tenso
     (and of their scales) is such an operand as well: a caller that takes them by blocks has them laid out once."""
     _check_int8(h8, w8)
     _check_scales(hidden_scales, tuple(h8.shape[:-1]), weight_scales, _check_weight(h8, w8))
+    _no_gradient_to_scales(hidden_scales, weight_scales)
     return _int8_layout(h8, hidden_scales, w8, weight_scales)
 
 

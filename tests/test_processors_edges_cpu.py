@@ -4,8 +4,12 @@ anything is launched."""
 import ctypes
 
 import pytest
+import torch
 
 from rl_amd import _C
+from rl_amd.algorithms.logits_sampling_utils import LogitProcessors
+from rl_amd.distributed.model_utils import (from_int8_hidden_states_to_logits, from_parallel_8bit_hidden_states_to_logprobs,
+                                            from_residual_stream_to_logprobs)
 
 V = 40
 
@@ -71,3 +75,29 @@ def test_int8_rows_that_no_launch_merges():
         return lib.mirl_linear_ce_int8_fwd(None, None, T, 256, 256, None, None, 5, 256, 1, None, 1, 1, 0, 5, None, 1, 1, None, None)
 
     assert refused(fwd(1 << 26), "scored") and refused(fwd((1 << 26) - 1), "null")
+
+
+@pytest.mark.parametrize("which", ["hidden", "weight"])
+def test_int8_scales_take_no_gradient(which):
+    h, w = torch.zeros(2, 2, 16, dtype=torch.int8), torch.zeros(5, 16, dtype=torch.int8)
+    hs, ws = torch.ones(2, 2, requires_grad=which == "hidden"), torch.ones(5, requires_grad=which == "weight")
+    target = torch.zeros(2, 2, dtype=torch.int64)
+    calls = [lambda: from_int8_hidden_states_to_logits(h, hs, w, ws),
+             lambda: from_parallel_8bit_hidden_states_to_logprobs(h, hs, w, ws, target, 0, 5)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient passes"):
+            call()
+        with torch.no_grad(), pytest.raises(_C.MirlError):  # (no GPU here: the call is taken)
+            call()
+    e4m3 = torch.float8_e4m3fn
+    with pytest.raises(_C.MirlError):  # as before
+        from_parallel_8bit_hidden_states_to_logprobs(h.to(e4m3), hs, w.to(e4m3), ws, target, 0, 5)
+
+
+def test_int8_weight_scales_of_the_policy_head_take_no_gradient(monkeypatch):
+    w, ws = torch.zeros(5, 16, dtype=torch.int8), torch.ones(5, requires_grad=True)
+    rows = (torch.zeros(2, 1, 16, dtype=torch.int8), torch.ones(2, 1), None)
+    monkeypatch.setattr("rl_amd.distributed.policy_head.add_rms_norm_8bit", lambda *a: rows)  # (the norm needs a GPU)
+    for P in (None, LogitProcessors(temperature=0.7)):
+        with pytest.raises(RuntimeError, match="no gradient passes"):
+            from_residual_stream_to_logprobs(torch.zeros(2, 1, 16), None, torch.ones(16), (w, ws), torch.zeros(1, 2, dtype=torch.int64), 0, 5, logit_processors=P)
