@@ -16,6 +16,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().with_name("libmirl.so")
 
@@ -455,6 +456,14 @@ def _require_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
     if dev is None:
         raise MirlError("no device tensor given")
     return dev
+
+
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives end at a launch: tensors that carry one are refused, not taken without it."""
+    if forward_ad._current_level < 0:  # (none is under way: 0.1 us where looking at each tensor takes 2)
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("a tensor carries a forward-mode tangent, which this call has no derivative for")
 
 
 def start_fetch(t: torch.Tensor):

@@ -52,6 +52,7 @@ def _check_weight(h8: torch.Tensor, w8: torch.Tensor) -> int:
 def _no_gradient_to_scales(*scales: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in scales):
         raise RuntimeError("no gradient passes to the scales of int8 rows: detach them")
+    _C.refuse_tangents(*scales)
 
 
 def _check_scales(hidden_scales: torch.Tensor, shape: tuple, weight_scales: torch.Tensor, V: int) -> None:

@@ -129,6 +129,7 @@ class _Call:
                 masks = masks.contiguous()
         self.tensors = (lengths, prompts, *penalties, bias_ids, bias, masks, rows)
         self.scalars, self.vocab = tuple(scalars), vocab
+        _C.refuse_tangents(logits, *self.tensors)
         for t in (logits, ids, *self.tensors):
             if t is not None and (not t.is_cuda or t.device != dev):
                 _C._require_gpu(logits, ids, *self.tensors)

@@ -5,11 +5,13 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from rl_amd import _C
-from rl_amd.algorithms.logits_sampling_utils import LogitProcessors
+from rl_amd.algorithms.logits_sampling_utils import LogitProcessors, TrainingSamplingParams, apply_logit_processors
 from rl_amd.distributed.model_utils import (from_int8_hidden_states_to_logits, from_parallel_8bit_hidden_states_to_logprobs,
-                                            from_residual_stream_to_logprobs)
+                                            from_parallel_logits_to_logprobs, from_residual_stream_to_logprobs,
+                                            processed_next_token_logprobs)
 
 V = 40
 
@@ -101,3 +103,32 @@ def test_int8_weight_scales_of_the_policy_head_take_no_gradient(monkeypatch):
     for P in (None, LogitProcessors(temperature=0.7)):
         with pytest.raises(RuntimeError, match="no gradient passes"):
             from_residual_stream_to_logprobs(torch.zeros(2, 1, 16), None, torch.ones(16), (w, ws), torch.zeros(1, 2, dtype=torch.int64), 0, 5, logit_processors=P)
+
+
+@pytest.mark.parametrize("what", ["logits", "bias", "temperature"])
+def test_forward_mode_tangents_are_refused(what):
+    """Not taken without their tangents: neither where a graph is recorded nor where none is."""
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        x = torch.zeros(2, 3, V)
+        P = LogitProcessors(temperature=torch.ones(2), bias_ids=torch.zeros(4, dtype=torch.int64), bias=torch.zeros(4))
+        if what == "logits":
+            x = dual(x)
+        else:
+            setattr(P, what, dual(getattr(P, what)))
+        F = TrainingSamplingParams(top_k=3)
+        for call in (lambda: apply_logit_processors(x, ids, P), lambda: apply_logit_processors(x, ids, P, inplace=True),
+                     lambda: processed_next_token_logprobs(x, ids, P),
+                     lambda: from_parallel_logits_to_logprobs(x, ids, 0, V, None, logit_processors=P),
+                     lambda: from_parallel_logits_to_logprobs(x, ids, 0, V, None, sampling_params=F, logit_processors=P)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        h, w, hs, ws = torch.zeros(2, 16, dtype=torch.int8), torch.zeros(5, 16, dtype=torch.int8), torch.ones(2), torch.ones(5)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            from_int8_hidden_states_to_logits(h, dual(hs), w, ws)
+    plain = LogitProcessors(repetition_penalty=1.1)
+    with pytest.raises(_C.MirlError):  # (no GPU here: a call without a tangent is taken)
+        apply_logit_processors(torch.zeros(2, 3, V), ids, plain)
