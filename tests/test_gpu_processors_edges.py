@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import processors as oracle
-from rl_amd.algorithms.logits_sampling_utils import apply_logit_processors
+from rl_amd.algorithms.logits_sampling_utils import LogitProcessors, apply_logit_processors
 from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs, processed_next_token_logprobs
 from tests.test_gpu_processors import DTYPES, INF, check_logprobs, check_values, cuda, least_t, magnitude, make, pack_masks
 
@@ -44,3 +44,28 @@ def test_lengths_at_the_end_of_their_type():
     near = n.clamp(-5, L)  # (as far as a history reaches, the same)
     check_values(apply_logit_processors(x.cuda(), ids.cuda(), cuda(P), history_lengths=n.cuda()), oracle.process(x, ids, P, near), A, T, torch.float32)
     check_logprobs(processed_next_token_logprobs(x.cuda(), ids.cuda(), cuda(P), history_lengths=n.cuda()), oracle.logprobs(x, ids, P, near), A, T)
+
+
+@pytest.mark.parametrize("dtype,integer,signalling", [(torch.float32, torch.int32, 0x7F800001), (torch.bfloat16, torch.int16, 0x7F81),
+                                                      (torch.float16, torch.int16, 0x7C01)])
+def test_in_place_leaves_the_bits_of_what_does_not_change(dtype, integer, signalling):
+    """Signalling NaN in groups of eight tokens of which none has a penalty or a bias: arithmetic makes quiet ones of them, as
+    the written-out form does, and the call in place does not touch them."""
+    B, V = 3, 5000
+    ids = torch.randint(0, 700, (B, 40), generator=torch.Generator().manual_seed(2))
+    lengths = torch.tensor([40, 13, 0])
+    P = LogitProcessors(repetition_penalty=1.3, presence_penalty=0.5, bias_ids=torch.tensor([4999, 17, -1]), bias=torch.tensor([1.0, 2.0, 3.0]))
+    quiet = torch.ones(B, V, dtype=torch.bool)
+    for b in range(B):
+        for j in [*ids[b, : lengths[b]].tolist(), 4999, 17]:
+            quiet[b, j // 8 * 8: j // 8 * 8 + 8] = False
+    assert bool(quiet.any(1).all())
+    x = torch.randn(B, V, generator=torch.Generator().manual_seed(3)).to(dtype)
+    bits = x.view(integer).clone()
+    bits[quiet] = signalling
+    place = bits.cuda().view(dtype)
+    out = apply_logit_processors(place, ids.cuda(), cuda(P), history_lengths=lengths.cuda())
+    assert bool((out.view(integer).cpu()[quiet] != signalling).all())  # the forms can be told apart
+    apply_logit_processors(place, ids.cuda(), cuda(P), history_lengths=lengths.cuda(), inplace=True)
+    assert bool((place.view(integer).cpu()[quiet] == signalling).all())
+    assert torch.equal(place.cpu()[~quiet], out.cpu()[~quiet])

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import processors as oracle
-from rl_amd.algorithms.logits_sampling_utils import TrainingSamplingParams
+from rl_amd.algorithms.logits_sampling_utils import LogitProcessors, TrainingSamplingParams
 from rl_amd.distributed.model_utils import from_parallel_logits_to_logprobs, get_next_token_logprobs_from_logits
 from tests.test_gpu_processors import DTYPES, INF, check_grad, check_logprobs, cuda, least_t, magnitude, make
 
@@ -126,3 +126,56 @@ def test_a_range_of_ids(top_k, top_p, start, end):
     ids[0, 5], ids[1, 9] = 3, 10**12
     x = sampled(x, ids, start)
     compare(x, ids, P, top_k, top_p, torch.float32, start, end)
+
+
+@pytest.mark.parametrize("top_k,top_p", [(20, 1.0), (None, 0.8)])
+def test_captured_graphs_replay(top_k, top_p):
+    """The filtered step with its gradient, captured and replayed on other logits, histories and masks than it was captured on."""
+    B, S, V = 3, 9, 3001
+    x, ids, P, _ = make(B, S, S, V, torch.bfloat16, seed=3, K=3, M=3)
+    x, ids, P = x.cuda(), ids.cuda(), cuda(P)
+    F = TrainingSamplingParams(top_k=top_k, top_p=top_p)
+    g = torch.randn(B, S - 1, device="cuda")
+
+    def step(t):
+        t = t.detach().requires_grad_(True)
+        lp = from_parallel_logits_to_logprobs(t, ids, 0, V, None, sampling_params=F, logit_processors=P)
+        (dx,) = torch.autograd.grad([lp], [t], [g])
+        return lp.detach(), dx
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    static = x.clone()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for k in range(4):
+        fresh = (x.float() * (1 + k)).to(x.dtype)
+        static.copy_(fresh)
+        ids[:, 5] = k
+        P.grammar_rows.copy_((P.grammar_rows + 2) % 4 - 1)  # other rows are left with nothing
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step(fresh)):
+            assert torch.equal(a, b)
+
+
+def test_another_stream_and_strided_logits():
+    B, S, V = 2, 9, 1031
+    x, ids, P, _ = make(B, S, S, V, torch.float16, seed=8, K=3, M=3)
+    F = TrainingSamplingParams(top_k=30, top_p=0.9)
+    wide = torch.zeros(S, B, V + 7, dtype=torch.float16, device="cuda")
+    view = wide.transpose(0, 1)[:, :, 5:V + 5]  # [B, S, V] rows at odd places
+    view.copy_(x)
+    want = from_parallel_logits_to_logprobs(x.cuda(), ids.cuda(), 0, V, None, sampling_params=F, logit_processors=cuda(P))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = from_parallel_logits_to_logprobs(view, ids.int().cuda(), 0, V, None, sampling_params=F, logit_processors=cuda(P))
+    side.synchronize()
+    assert torch.equal(got, want)
+    one = from_parallel_logits_to_logprobs(x.cuda()[:, :1], ids.cuda()[:, :1], 0, V, None, sampling_params=F, logit_processors=LogitProcessors())
+    assert one.shape == (B, 0)  # one token has no next
