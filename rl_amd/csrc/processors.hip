@@ -152,7 +152,7 @@ struct Sample {
   float rp, inv_rp, pres, freq, inv_t;
   int n;       // tokens that row 0 follows
   int prompt;  // tokens of the prompt
-  int unused;
+  float t;     // the temperature
 };
 static_assert(sizeof(Sample) == kHead * 4, "the table's head");
 __host__ __device__ __forceinline__ int64_t token_lists(int64_t n_ids) { return n_ids > kList ? (n_ids + kList - 1) / kList : 1; }
@@ -175,12 +175,28 @@ __device__ __forceinline__ float keep_if(float v, uint32_t keep, int e, float ot
   return __uint_as_float((__float_as_uint(v) & t) | (__float_as_uint(other) & ~t));
 }
 
+// z / d to the nearest, from inv = 1 / d to the nearest: the product is off by up to an ulp and a half, and its remainder, exact in
+// one fma, gives the rest (P. Markstein, IBM J. Res. Dev. 34, 1990).  Infinities and NaN have no remainder and stay.  !EXACT: the
+// product alone, where the result is rounded to 16 bits or goes into a logprob, whose sums are off by more.  (fp32 tokens written
+// out 20.0 us either way.)
+template <bool EXACT>
+__device__ __forceinline__ float quotient(float z, float d, float inv) {
+  const float q = z * inv;
+  if constexpr (!EXACT) return q;
+  const float r = fmaf(-q, d, z);
+  return fabsf(r) < INFINITY ? fmaf(r, inv, q) : q;
+}
+
 // Bias and penalties of one logit under its word.
+template <bool EXACT>
 __device__ __forceinline__ float penalized(float z, uint32_t w, const Sample& S, uint32_t& how) {
   how = 0;
   if (w & (kInPrompt | kCount)) {
     how = z > 0.f ? 1u : 256u;
-    z *= z > 0.f ? S.inv_rp : S.rp;
+    if constexpr (EXACT)
+      z = z > 0.f ? quotient<true>(z, S.rp, S.inv_rp) : z * S.rp;
+    else
+      z *= z > 0.f ? S.inv_rp : S.rp;
   }
   const uint32_t n = w & kCount;
   z -= S.freq * (float)n;
@@ -191,7 +207,7 @@ __device__ __forceinline__ float penalized(float z, uint32_t w, const Sample& S,
 // Bias and penalties of a group's tokens: those of any lane of the wave (`any`, a scalar), in the
 // lanes that have them (`bits`).  Returns which were divided by the repetition penalty (bits 0 .. 7) and
 // which multiplied (8 .. 15).
-template <class F>
+template <bool EXACT, class F>
 __device__ __forceinline__ uint32_t special(float (&v)[kG], uint32_t any, uint32_t bits, const vu4* words, F&& bias_of,
                                             const Sample& S) {
   uint32_t how = 0;
@@ -202,7 +218,7 @@ __device__ __forceinline__ uint32_t special(float (&v)[kG], uint32_t any, uint32
     if ((bits >> e) & 1u) {
       const uint32_t w = words[e / 4][e % 4];
       uint32_t h;
-      v[e] = penalized(w >> kBiasShift ? v[e] + bias_of(w, e) : v[e], w, S, h);
+      v[e] = penalized<EXACT>(w >> kBiasShift ? v[e] + bias_of(w, e) : v[e], w, S, h);
       how |= h << e;
     }
   }
@@ -243,10 +259,10 @@ __global__ __launch_bounds__(kTableThreads) void processors_table_kernel(mirl_lo
     S.inv_rp = 1.f / S.rp;
     S.pres = A.presence != nullptr ? A.presence[b] : A.presence_all;
     S.freq = A.frequency != nullptr ? A.frequency[b] : A.frequency_all;
-    S.inv_t = 1.f / (A.temperature != nullptr ? A.temperature[b] : A.temperature_all);
+    S.t = A.temperature != nullptr ? A.temperature[b] : A.temperature_all;
+    S.inv_t = 1.f / S.t;
     S.n = (int)max(n_b, -(int64_t(1) << 30));
     S.prompt = A.prompt_lengths != nullptr ? (int)min(max(A.prompt_lengths[b], int64_t(0)), A.n_ids) : 0;
-    S.unused = 0;
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&S);
     for (int k = 0; k < kHead; ++k) head[k] = w[k];
   }
@@ -339,6 +355,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
   using EY = std::conditional_t<MODE == kWide || MODE == kWideGrad, F32, E>;  // of y and its gradient
   using EI = std::conditional_t<kGradOfY, EY, E>;                             // of the values a row is read as: logits, or y's gradient
   using EO = std::conditional_t<MODE == kWide, F32, E>;                       // of what is written
+  constexpr bool kExact = (kWritten || MODE == kInPlace) && std::is_same<EO, F32>::value;
   constexpr int kWaveCols = kWave * NV * kG, kSlice = kWaves * kWaveCols;
   constexpr int kPacks = (NV + 3) / 4;  // four groups' bytes in a word
   __shared__ __align__(16) uint32_t s_word[kSlice];
@@ -748,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
         for (int u = 0; u < NV; ++u) {
           take(u, -INFINITY, v[u]);
           if (wave_bits(u) != 0)  // (a masked token's bias must not meet the -inf that the mask left)
-            special(v[u], wave_bits(u), lane_bits(u) & allowed[u], words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+            special<kExact>(v[u], wave_bits(u), lane_bits(u) & allowed[u], words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
           for (int e = 0; e < kG; ++e) mx = fmaxf(mx, v[u][e]);
         }
@@ -756,7 +773,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
         if (listed > 0) {
           uint32_t how;
           const int c = wave * kWaveCols + max(h_col, 0);
-          h_y = penalized(E::load(s_row + (kLists ? c : 0)) + h_bias, h_word, S, how);
+          h_y = penalized<false>(E::load(s_row + (kLists ? c : 0)) + h_bias, h_word, S, how);
           const uint32_t m = masked ? s_mask[kLists && MASKED ? c / kG : 0] : 0xffu;
           h_y = h_col >= 0 && (m >> (c % kG) & 1u) ? h_y : -INFINITY;
           mx = fmaxf(mx, h_y);
@@ -810,7 +827,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           take(u, 0.f, v);
           uint32_t how = 0;
           if (wave_bits(u) != 0)
-            how = special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+            how = special<kExact>(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
           for (int e = 0; e < kG; ++e) o[e] = fast_exp2(fmaf(v[e] - M, c, -ls)) * -gt;
           if (u == tu) {
@@ -832,9 +849,9 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           float v[kG];
           take(u, 0.f, v);
           if (wave_bits(u) != 0)
-            special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+            special<kExact>(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
-          for (int e = 0; e < kG; ++e) v[e] *= S.inv_t;
+          for (int e = 0; e < kG; ++e) v[e] = quotient<kExact>(v[e], S.t, S.inv_t);
           if (masked) {
 #pragma unroll
             for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e], allowed[u], e, -INFINITY);
@@ -862,7 +879,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
             else
               tail(E{}, xr + i * P.xsr, u, 0.f, x);
             const uint32_t how =
-                special(x, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+                special<kExact>(x, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
             through(v, wave_bits(u), how, S);
           }
           if (masked) {
@@ -872,7 +889,7 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           put(y_row, u, v, WHOLE);
         }
       } else {  // kInPlace: what changes
-        const bool dense = S.inv_t != 1.f;
+        const bool dense = S.t != 1.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
           allowed[u] = masked ? mk[u] : 0xffu;
@@ -886,9 +903,9 @@ __global__ __launch_bounds__(kThreads) void processors_kernel(Params P) {
           } else {
             tail(E{}, row, u, 0.f, v);
           }
-          special(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
+          special<kExact>(v, wave_bits(u), lane_bits(u), words + u * kU, [&](uint32_t w, int e) { return bias_of(w, u, e); }, S);
 #pragma unroll
-          for (int e = 0; e < kG; ++e) v[e] = keep_if(v[e] * S.inv_t, allowed[u], e, -INFINITY);
+          for (int e = 0; e < kG; ++e) v[e] = keep_if(quotient<kExact>(v[e], S.t, S.inv_t), allowed[u], e, -INFINITY);
           put(y_row, u, v, WHOLE);
         }
       }

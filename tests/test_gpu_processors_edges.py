@@ -69,3 +69,20 @@ def test_in_place_leaves_the_bits_of_what_does_not_change(dtype, integer, signal
     apply_logit_processors(place, ids.cuda(), cuda(P), history_lengths=lengths.cuda(), inplace=True)
     assert bool((place.view(integer).cpu()[quiet] == signalling).all())
     assert torch.equal(place.cpu()[~quiet], out.cpu()[~quiet])
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_quotients_are_rounded_once(inplace):
+    """Temperature and repetition penalty divide: fp32 results are those of a division to the nearest, not of a product with the
+    rounded reciprocal (off by an ulp in a third of them)."""
+    B, V = 40, 3000
+    g = torch.Generator().manual_seed(5)
+    T, rp = 0.3 + 1.7 * torch.rand(B, generator=g), 1 + torch.rand(B, generator=g)
+    x = torch.randn(B, V, generator=g) * 5
+    x[:, 7], x[:, 8], x[:, 9] = INF, -INF, float("nan")
+    ids = torch.arange(V).expand(B, V)
+    none, all_ = torch.zeros(B, dtype=torch.int64), torch.full((B,), V)
+    for P, lengths, want in ((LogitProcessors(temperature=T), none, x / T[:, None]),
+                             (LogitProcessors(repetition_penalty=rp), all_, torch.where(x > 0, x / rp[:, None], x * rp[:, None]))):
+        got = apply_logit_processors(x.cuda(), ids.cuda(), cuda(P), history_lengths=lengths.cuda(), inplace=inplace).cpu()
+        assert torch.equal(got.nan_to_num(0.5), want.nan_to_num(0.5)) and torch.equal(got.isnan(), want.isnan())
