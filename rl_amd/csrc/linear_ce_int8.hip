@@ -7,8 +7,9 @@
 // 2^24) is the first one.  The target's logit is therefore the tile's own.
 //
 // Bound by the matrix cores and what feeds them, few rows by the weight's bytes.  [16376, 4096] x [151936, 4096]:
-// logprobs 7.56 to 7.75 ms, 2.63 to 2.70 POP/s (e4m3 on the same loop 7.44; a library product alone 2.13 POP/s).  Logits
-// of [2048, 4096] x [151936, 4096] in bf16, 622 MB of them: 1.07 ms, 2.39 POP/s.  Of 64 rows: logits 131 us,
+// logprobs 7.66 to 8.1 ms from card to card, 2.5 to 2.66 POP/s (a library product alone 2.13 POP/s).  Logits
+// of [2048, 4096] x [151936, 4096] in bf16, 622 MB of them: 1.05 to 1.10 ms, 2.3 to 2.4 POP/s; in fp32 1.17, with an odd
+// vocabulary, whose rows no 16 bytes divide, 1.54 (words stored one by one).  Of 64 rows: logits 131 us,
 // logprobs 124 us, 4.9 and 5.0 TB/s.
 
 #include "lce_tile.h"

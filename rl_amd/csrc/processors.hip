@@ -4,7 +4,8 @@
 // `seen` if it occurs at all:
 //   z = x + bias;   z = seen ? (z > 0 ? z / rp : z rp) : z;   z = z - freq c - pres [c > 0]
 //   y = allowed ? z / T : -inf
-// in three forms: y written out (with its backward), y written in place, and the next token's logprob
+// in three forms: y written out in the logits' type, or in fp32 for a filter (either with its backward), y written in
+// place, and the next token's logprob
 //   logprob_t = (y_t - M) - log(sum_j exp(y_j - M)),   dx_j = slope_j (onehot_j - p_j) g
 // with y never written; slope is what z multiplies x by, over T, 0 where the grammar forbids j.
 //
@@ -22,9 +23,9 @@
 // ordinary values of bf16).  bf16 [8, 2048, 151936] with the penalties and biases of a GRPO step, half of the rows without
 // a gradient: forward 920 us (4.98 GB, 5.4 TB/s; 860 where no token of the rows occurs, logprob.hip's of untouched
 // logits 730), backward 1.36 to 1.43 ms (7.4 GB, 5.3 TB/s; logprob.hip's 1.22).  [2, 2048, 151936]: written out
-// 412 us (2.49 GB, 6.0 TB/s), its backward 495 (5.0; the logits of tokens that occur are read as well).  One token of
-// each of 64 requests behind up to 2048 tokens: table 7 us, logprobs 14 and 4 to join, written out 16: the
-// latency of a few loads that wait for each other.
+// 412 us (2.49 GB, 6.0 TB/s), its backward 495 (5.0; the logits of tokens that occur are read as well); in fp32 810 us
+// (3.73 GB, 4.6 TB/s), its backward 733 (5.1).  One token of each of 64 requests behind up to 2048 tokens: table 7 us,
+// logprobs 14 and 4 to join, written out 16, in place 14: the latency of a few loads that wait for each other.
 
 #include "common.h"
 
