@@ -177,15 +177,16 @@ __device__ __forceinline__ float keep_if(float v, uint32_t keep, int e, float ot
 }
 
 // z / d to the nearest, from inv = 1 / d to the nearest: the product is off by up to an ulp and a half, and its remainder, exact in
-// one fma, gives the rest (P. Markstein, IBM J. Res. Dev. 34, 1990).  Infinities and NaN have no remainder and stay.  !EXACT: the
+// one fma, gives the rest (P. Markstein, IBM J. Res. Dev. 34, 1990).  Infinities and NaN have no remainder and stay, and so does
+// the sign of a zero (a remainder of 0 is +0, and is subtracted).  !EXACT: the
 // product alone, where the result is rounded to 16 bits or goes into a logprob, whose sums are off by more.  (fp32 tokens written
 // out 20.0 us either way.)
 template <bool EXACT>
 __device__ __forceinline__ float quotient(float z, float d, float inv) {
   const float q = z * inv;
   if constexpr (!EXACT) return q;
-  const float r = fmaf(-q, d, z);
-  return fabsf(r) < INFINITY ? fmaf(r, inv, q) : q;
+  const float r = fmaf(q, d, -z);
+  return fabsf(r) < INFINITY ? fmaf(-r, inv, q) : q;
 }
 
 // Bias and penalties of one logit under its word.

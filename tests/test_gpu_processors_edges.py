@@ -86,3 +86,15 @@ def test_quotients_are_rounded_once(inplace):
                              (LogitProcessors(repetition_penalty=rp), all_, torch.where(x > 0, x / rp[:, None], x * rp[:, None]))):
         got = apply_logit_processors(x.cuda(), ids.cuda(), cuda(P), history_lengths=lengths.cuda(), inplace=inplace).cpu()
         assert torch.equal(got.nan_to_num(0.5), want.nan_to_num(0.5)) and torch.equal(got.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inplace", [False, True])
+def test_zeros_keep_their_signs(dtype, inplace):
+    x = torch.zeros(2, 600)
+    x[:, ::3] = -0.0
+    P = LogitProcessors(repetition_penalty=1.3, temperature=0.7)
+    ids, lengths = torch.arange(0, 600, 2).expand(2, 300), torch.tensor([300, 0])  # zeros of tokens that occurred, and not
+    for settings in (P, LogitProcessors()):
+        got = apply_logit_processors(x.to(dtype).cuda(), ids.cuda(), settings, history_lengths=lengths.cuda(), inplace=inplace).cpu()
+        assert not got.any() and torch.equal(got.signbit(), x.signbit())
